@@ -317,6 +317,102 @@ int mvlm_attention_decode_step(mvlm_device* dev, const mvlm_buffer* qkv, mvlm_bu
 int mvlm_argmax(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
                 mvlm_buffer* out_index, mvlm_event** ev);
 
+/* ---- a step over a batch of sequences with a paged cache ----------------------
+ * The reference decodes one sequence with one contiguous cache (kv_cache_append
+ * and attention_decode, src/models/moondream2.cpp:305-316, :404-440; rope_apply,
+ * src/kernels/rope.cl:42-87).  These three serve many at once next to the M-row
+ * products (mvlm_gemm_quant_grouped, mvlm_gemm_packed) and mvlm_argmax: qkv
+ * product, mvlm_kv_append_paged, mvlm_attention_paged, ..., LM head,
+ * mvlm_logits_process, mvlm_argmax.  What changes from step to step (lengths,
+ * tables, histories, masks) is in device memory, so a plan captured once serves
+ * every step of a batch of the same shape.
+ *
+ * A cache: K and V hold num_pages pages of [kv_heads][page_size][head_dim]
+ * elements (F16 or BF16), 16-byte aligned, not overlapping; head_dim a multiple
+ * of 8, at most 128; fewer than 2^31 slots num_pages kv_heads page_size. */
+typedef struct mvlm_paged_kv {
+    mvlm_buffer* k;
+    mvlm_buffer* v;
+    int dtype;
+    int num_pages;
+    int page_size;               /* any positive number of positions */
+    int kv_heads;
+    int head_dim;
+} mvlm_paged_kv;
+/* A batch: sequence s owns rows [row_start[s], row_start[s + 1]) of the step's
+ * tensors (row_start: int32 [num_seqs + 1], not decreasing; NULL: row s alone,
+ * rows == num_seqs) and holds kv_len[s] positions, its new rows' among them: its
+ * row j is position kv_len[s] - n + j, n = its number of rows.  Position t lies in
+ * slot t % page_size of page page_table[s][t / page_size].  A place that the
+ * table does not have, or a page outside [0, num_pages), does not exist: it is
+ * neither read nor written.  A sequence with kv_len 0 is idle.  Rows of no
+ * sequence are left as they were.  At most 65536 sequences, 2^22 rows and 2^30
+ * positions in a table. */
+typedef struct mvlm_paged_batch {
+    int num_seqs;
+    int rows;
+    const mvlm_buffer* row_start;    /* int32 [num_seqs + 1] or NULL */
+    const mvlm_buffer* kv_len;       /* int32 [num_seqs] */
+    const mvlm_buffer* page_table;   /* int32 [num_seqs][table_width] */
+    int table_width;
+} mvlm_paged_batch;
+/* Rotary positions: table holds cos and sin of position p and pair i as fp32
+ * [positions][rot_dim / 2][2] (the reference's tables, moondream2.cpp:198-253;
+ * whatever scaling of frequencies a model uses is in them).  Pairs are elements
+ * (i, i + rot_dim / 2) of a head or, interleaved, (2i, 2i + 1); elements from
+ * rot_dim on are kept. */
+typedef struct mvlm_rope {
+    const mvlm_buffer* table;
+    int positions;
+    int rot_dim;
+    int interleaved;
+} mvlm_rope;
+/* Row r of qkv (F32, F16 or BF16, ld elements apart) is num_heads q heads, then
+ * kv_heads key heads, then kv_heads value heads.  q and keys are rotated to the
+ * row's position (rope NULL: not) in fp32; q goes to q_out [rows][num_heads]
+ * [head_dim] and keys and values into the cache, rounded to its type.  A row
+ * without a place (no position, no page, or past the rope table) writes zeros to
+ * q_out and nothing to the cache. */
+int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                         const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                         mvlm_buffer* q_out, const mvlm_rope* rope, mvlm_event** ev);
+/* O[r][h] = sum over t of softmax(scale Q[r][h] . K[t][h / group]) V[t][h / group],
+ * group = num_heads / kv_heads, over the positions t up to row r's own that exist
+ * (what lies in others may be anything).  Q [rows][num_heads][head_dim] in the
+ * cache's type, O the same shape in F32 or the cache's type; scale 0:
+ * 1/sqrt(head_dim).  A row that sees no position, or only scores of -inf, is 0. */
+int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
+                         const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
+                         mvlm_event** ev);
+/* What a request asks of its logits.  History: token ids of row r,
+ * history[r][0 .. history_len[r]), those from generated_from[r] on (NULL: all)
+ * generated; penalties[r] = repetition (> 0), frequency, presence.  Biases:
+ * bias_values[r][i] for token bias_ids[r][i], i < bias_len[r]; the last entry of a
+ * token counts.  allowed: one bit per token, bit t % 32 of word t / 32, 0 = masked.
+ * Lengths are taken within [0, width], ids outside [0, n) name nothing.  Each
+ * group may be absent (all its pointers NULL). */
+typedef struct mvlm_logit_controls {
+    const mvlm_buffer* history;          /* int32 [rows][history_width] */
+    const mvlm_buffer* history_len;      /* int32 [rows] */
+    const mvlm_buffer* generated_from;   /* int32 [rows] or NULL */
+    int history_width;
+    const mvlm_buffer* penalties;        /* fp32 [rows][3] */
+    const mvlm_buffer* bias_ids;         /* int32 [rows][bias_width] */
+    const mvlm_buffer* bias_values;      /* fp32 [rows][bias_width] */
+    const mvlm_buffer* bias_len;         /* int32 [rows] */
+    int bias_width;
+    const mvlm_buffer* allowed;          /* uint32 [rows][(n + 31) / 32] */
+} mvlm_logit_controls;
+/* For every token of each row (rows x n, ld elements apart, F32/F16/BF16), with c
+ * its occurrences in the history and g those generated, in fp32 and rounded once:
+ *   x = x > 0 ? x / repetition : x * repetition     if c > 0
+ *   x = x - (g * frequency + presence)              if g > 0
+ *   x = x + bias
+ *   x = -inf                                        if masked
+ * out may be x. */
+int mvlm_logits_process(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                        const mvlm_logit_controls* controls, mvlm_buffer* out, mvlm_event** ev);
+
 /* ---- synthetic inputs on the device ------------------------------------- */
 /* SplitMix64 -> Box-Muller fills (same generator as the CPU oracle, computed
  * on the GPU so multi-GB weight sets need no host staging). */
@@ -374,6 +470,13 @@ int mvlm_plan_add_attention_decode_step(mvlm_plan* plan, const mvlm_buffer* qkv,
                                         int head_dim, float scale);
 int mvlm_plan_add_argmax(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
                          mvlm_buffer* out_index);
+int mvlm_plan_add_kv_append_paged(mvlm_plan* plan, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                  const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                  mvlm_buffer* q_out, const mvlm_rope* rope);
+int mvlm_plan_add_attention_paged(mvlm_plan* plan, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
+                                  const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale);
+int mvlm_plan_add_logits_process(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                                 const mvlm_logit_controls* controls, mvlm_buffer* out);
 /* enable != 0: capture the plan into a HIP graph (now) and replay it on run. */
 int mvlm_plan_use_graph(mvlm_plan* plan, int enable);
 /* Enqueue the plan `repeats` times; `ev` (optional) spans everything enqueued. */

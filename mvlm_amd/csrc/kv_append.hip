@@ -1,0 +1,135 @@
+// New rows of q | k | v for sequences with a paged cache: rotary positions on q
+// and k, keys and values into their pages, q out, in one pass.
+//
+//   x = one row of qkv: heads q heads, then kv_heads k heads, then kv_heads v
+//   heads of D elements; p = the row's position (paged.h); (c, s) = rope[p][i]
+//   rotated pairs i < rot / 2 of a q or k head, (a, b) = (x[i], x[i + rot/2]) or,
+//   interleaved, (x[2i], x[2i + 1]):   a' = a c - b s,   b' = b c + a s
+// in fp32, rounded once (to nearest even) to the cache's type, since that is what
+// the matrix products of the attention read.
+//
+// Bytes bound it: each element is read once and written once.  A thread makes 8
+// elements of one head: a 16-byte store whatever the types are, and its partner
+// elements (a chunk further on in the same head, or its own) come from the lines
+// that its neighbours read.  One block per row, so sequence, position, page
+// and table row are found once per wave.
+#include "common.h"
+#include "device_math.h"
+#include "paged_ops.h"
+
+namespace mvlm {
+
+constexpr int APPEND_THREADS = 256;
+
+// 8 elements from x[i], fp32
+template <int XD, bool VEC>
+__device__ __forceinline__ void append_load8(const void* x, int64_t i, float (&v)[8]) {
+    if constexpr (!VEC) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = load_as_f32(x, i + e, XD);
+    } else if constexpr (XD == MVLM_F32) {
+        const f32x4* p = reinterpret_cast<const f32x4*>((const float*)x + i);
+        const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)x + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            v[e] = XD == MVLM_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
+        }
+    }
+}
+
+// XD: type of qkv; VEC: its rows are 16-byte aligned
+template <int XD, bool VEC>
+__global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppendArgs a) {
+    const int row = (int)blockIdx.x;
+    PagedSpan sp;
+    const int seq = paged_seq_of_row(a.batch, row, &sp);
+    if (seq < 0) return;                                   // behind the last sequence: left as it is
+    const int p = sp.position(row - sp.row0);
+    const PagedKv& kv = a.kv;
+    // a row without a place: no position, past the table or the rotary table, a page that does not exist
+    int slot0 = -1;                                        // slot of kv head 0
+    if (p >= 0 && p < a.batch.positions && (a.rot == 0 || p < a.rope_positions)) {
+        const int pi = kv.page.quotient(p);
+        const int page = a.batch.table[(int64_t)seq * a.batch.width + pi];
+        if (page >= 0 && page < kv.num_pages) slot0 = kv.slot(page, 0, p - pi * kv.page.div);
+    }
+    const int D = kv.D, cpr = D / 8, half = a.rot / 2;
+    const int chunks = (a.heads + 2 * kv.kv_heads) * cpr;
+    const int64_t xrow = (int64_t)row * a.ld;
+    const float* cs = a.rope + (int64_t)p * a.rot;         // [rot / 2][2], read only with a place
+    for (int c = (int)threadIdx.x; c < chunks; c += APPEND_THREADS) {
+        const int head = a.chunk.quotient(c), d = 8 * (c - head * cpr);
+        float v[8], o[8];
+        append_load8<XD, VEC>(a.qkv, xrow + (int64_t)head * D + d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[e];
+        if (d < a.rot && head < a.heads + kv.kv_heads && slot0 >= 0) {
+            const int64_t h0 = xrow + (int64_t)head * D;
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    if (d + e < a.rot) {
+                        const float co = cs[d + e], si = cs[d + e + 1];
+                        o[e] = v[e] * co - v[e + 1] * si;
+                        o[e + 1] = v[e + 1] * co + v[e] * si;
+                    }
+            } else if (half % 8 == 0) {                    // a chunk lies in one half, its partner chunk in the other
+                const bool first = d < half;
+                const int i = first ? d : d - half;
+                float w[8];
+                append_load8<XD, VEC>(a.qkv, h0 + (first ? d + half : i), w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float co = cs[2 * (i + e)], si = cs[2 * (i + e) + 1];
+                    o[e] = v[e] * co + (first ? -w[e] : w[e]) * si;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (d + e < a.rot) {
+                        const bool first = d + e < half;
+                        const int i = first ? d + e : d + e - half;
+                        const float w = load_as_f32(a.qkv, h0 + (first ? i + half : i), XD);
+                        const float co = cs[2 * i], si = cs[2 * i + 1];
+                        o[e] = v[e] * co + (first ? -w : w) * si;
+                    }
+            }
+        }
+        u32x4 out;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            out[j] = kv.dtype == MVLM_F16 ? (uint32_t)f32_to_f16_bits(o[2 * j]) | (uint32_t)f32_to_f16_bits(o[2 * j + 1]) << 16
+                                          : (uint32_t)f32_to_bf16_bits(o[2 * j]) | (uint32_t)f32_to_bf16_bits(o[2 * j + 1]) << 16;
+        if (head < a.heads) {
+            if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.heads + head) * D + d) = out;
+        } else if (slot0 >= 0) {
+            const bool key = head < a.heads + kv.kv_heads;
+            const int h = head - a.heads - (key ? 0 : kv.kv_heads);
+            const int64_t at = (int64_t)(slot0 + h * kv.page.div) * D + d;
+            *reinterpret_cast<u32x4*>((key ? kv.k : kv.v) + at) = out;
+        }
+    }
+}
+
+hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a) {
+    const size_t es = dtype_size(a.x_dtype);
+    const bool vec = ((uintptr_t)a.qkv & 15u) == 0 && (a.ld * (int64_t)es) % 16 == 0;
+    const dim3 grid((unsigned)a.batch.rows), block(APPEND_THREADS);
+    auto go = [&](auto dt) {
+        constexpr int XD = decltype(dt)::value;
+        if (vec) launch_kernel(kv_append_kernel<XD, true>, grid, block, 0, s, a);
+        else launch_kernel(kv_append_kernel<XD, false>, grid, block, 0, s, a);
+    };
+    if (a.x_dtype == MVLM_F32) go(std::integral_constant<int, MVLM_F32>{});
+    else if (a.x_dtype == MVLM_F16) go(std::integral_constant<int, MVLM_F16>{});
+    else go(std::integral_constant<int, MVLM_BF16>{});
+    return hipGetLastError();
+}
+
+}  // namespace mvlm

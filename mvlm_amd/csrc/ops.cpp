@@ -7,7 +7,10 @@
 // add time and enqueues from native code on every run, eagerly or by
 // replaying a captured HIP graph.
 #include "common.h"
+#include "logits.h"
+#include "paged_ops.h"
 
+#include <climits>
 #include <cmath>
 #include <cstdlib>
 #include <new>
@@ -18,7 +21,7 @@ using namespace mvlm;
 namespace {
 
 enum OpKind { OP_GEMM_ORDER, OP_GEMV_EXACT, OP_GEMM_MFMA, OP_GEMV_DENSE, OP_GEMV_QUANT, OP_GEMV_GROUP, OP_ATTENTION,
-              OP_ATTN_STEP, OP_ARGMAX };
+              OP_ATTN_STEP, OP_ARGMAX, OP_KV_APPEND, OP_ATTN_PAGED, OP_LOGITS };
 
 struct Op {
     OpKind kind;
@@ -45,6 +48,10 @@ struct Op {
     float scale = 0.0f;
     void* workspace = nullptr;    // attention key splits, GEMM K splits
     size_t workspace_bytes = 0;
+    // operators of a batch over a paged cache
+    KvAppendArgs append{};
+    PagedAttnArgs paged{};
+    LogitsArgs logits{};
     // plan fusion: a grouped GEMV whose launch can also compute a decode
     // attention entry next to it; 1: the entry before it (some entries read
     // its output as x), 2: the entry after it (a decode step whose q, k, v
@@ -291,6 +298,219 @@ int make_argmax(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     return MVLM_OK;
 }
 
+// ---- a batch over a paged cache ---------------------------------------------
+
+int need_ints(mvlm_device* dev, const mvlm_buffer* b, size_t count, const char* fn, const char* name) {
+    REQUIRE(b->dev == dev, "%s: %s belongs to another device", fn, name);
+    REQUIRE(((uintptr_t)b->ptr & 3u) == 0, "%s: %s does not start at a multiple of 4 bytes", fn, name);
+    return need(b, count * 4, fn, name);
+}
+
+int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, PagedKv* out) {
+    REQUIRE(in && in->k && in->v, "%s: null cache", fn);
+    REQUIRE(in->k->dev == dev && in->v->dev == dev, "%s: the cache belongs to another device", fn);
+    REQUIRE(in->dtype == MVLM_F16 || in->dtype == MVLM_BF16, "%s: cache dtype %d is not F16/BF16", fn, in->dtype);
+    REQUIRE(in->num_pages > 0 && in->page_size > 0 && in->kv_heads > 0 && in->head_dim > 0,
+            "%s: num_pages=%d page_size=%d kv_heads=%d head_dim=%d must be positive", fn, in->num_pages, in->page_size,
+            in->kv_heads, in->head_dim);
+    if (in->head_dim % 8 != 0 || in->head_dim > 128)
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: head_dim=%d must be a multiple of 8 and at most 128", fn, in->head_dim);
+    const int64_t per_head = (int64_t)in->num_pages * in->page_size;
+    if (per_head > INT_MAX / in->kv_heads)
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: %d pages of %d positions of %d heads are 2^31 slots or more", fn,
+                         in->num_pages, in->page_size, in->kv_heads);
+    const size_t bytes = (size_t)per_head * in->kv_heads * in->head_dim * 2;
+    REQUIRE(aligned16(in->k->ptr) && aligned16(in->v->ptr), "%s: K and V must be 16-byte aligned", fn);
+    NEED(in->k, bytes, "K");
+    NEED(in->v, bytes, "V");
+    REQUIRE(!overlaps(in->k->ptr, bytes, in->v->ptr, bytes), "%s: K and V overlap", fn);
+    out->k = (uint16_t*)in->k->ptr;
+    out->v = (uint16_t*)in->v->ptr;
+    out->dtype = in->dtype;
+    out->num_pages = in->num_pages;
+    out->kv_heads = in->kv_heads;
+    out->D = in->head_dim;
+    out->page = fast_div(in->page_size);
+    return MVLM_OK;
+}
+size_t kv_bytes(const PagedKv& kv) { return (size_t)kv.num_pages * kv.page.div * kv.kv_heads * kv.D * 2; }
+
+int make_paged_batch(mvlm_device* dev, const mvlm_paged_batch* in, int page_size, const char* fn, PagedSeqs* out) {
+    REQUIRE(in && in->kv_len && in->page_table, "%s: null batch", fn);
+    REQUIRE(in->num_seqs > 0 && in->rows > 0 && in->table_width > 0, "%s: num_seqs=%d rows=%d table_width=%d must be positive",
+            fn, in->num_seqs, in->rows, in->table_width);
+    REQUIRE(in->num_seqs <= 65536 && in->rows <= (1 << 22), "%s: more than 65536 sequences or 2^22 rows", fn);
+    REQUIRE(in->row_start || in->rows == in->num_seqs, "%s: rows=%d of %d sequences need row_start", fn, in->rows,
+            in->num_seqs);
+    REQUIRE((int64_t)in->table_width * page_size <= PAGED_MAX_POSITIONS, "%s: a table of %d pages of %d holds over 2^30 positions",
+            fn, in->table_width, page_size);
+    int st = need_ints(dev, in->kv_len, (size_t)in->num_seqs, fn, "kv_len");
+    if (st == MVLM_OK) st = need_ints(dev, in->page_table, (size_t)in->num_seqs * in->table_width, fn, "page_table");
+    if (st == MVLM_OK && in->row_start) st = need_ints(dev, in->row_start, (size_t)in->num_seqs + 1, fn, "row_start");
+    if (st != MVLM_OK) return st;
+    out->seqs = in->num_seqs;
+    out->rows = in->rows;
+    out->row_start = in->row_start ? (const int*)in->row_start->ptr : nullptr;
+    out->kv_len = (const int*)in->kv_len->ptr;
+    out->table = (const int*)in->page_table->ptr;
+    out->width = in->table_width;
+    out->positions = in->table_width * page_size;
+    return MVLM_OK;
+}
+
+// Whether [p, p + bytes) holds any of what the batch reads.
+bool holds_batch(const void* p, size_t bytes, const PagedSeqs& b) {
+    return overlaps(p, bytes, b.kv_len, (size_t)b.seqs * 4) || overlaps(p, bytes, b.table, (size_t)b.seqs * b.width * 4) ||
+           overlaps(p, bytes, b.row_start, ((size_t)b.seqs + 1) * 4);
+}
+
+int check_heads(int num_heads, const PagedKv& kv, const char* fn) {
+    REQUIRE(num_heads > 0 && num_heads % kv.kv_heads == 0, "%s: num_heads=%d is not a positive multiple of kv_heads=%d", fn,
+            num_heads, kv.kv_heads);
+    REQUIRE(num_heads <= 65535 && (int64_t)num_heads * kv.D <= (1 << 24), "%s: shape too large", fn);
+    return MVLM_OK;
+}
+
+int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld, const mvlm_paged_batch* batch,
+                   const mvlm_paged_kv* cache, int num_heads, mvlm_buffer* q_out, const mvlm_rope* rope, const char* fn,
+                   Op* op) {
+    REQUIRE(dev && qkv && q_out, "%s: null argument", fn);
+    REQUIRE(qkv->dev == dev && q_out->dev == dev, "%s: buffers belong to another device", fn);
+    REQUIRE(is_dense(x_dtype), "%s: qkv dtype %d is not F32/F16/BF16", fn, x_dtype);
+    KvAppendArgs& a = op->append;
+    int st = make_paged_kv(dev, cache, fn, &a.kv);
+    if (st == MVLM_OK) st = make_paged_batch(dev, batch, a.kv.page.div, fn, &a.batch);
+    if (st == MVLM_OK) st = check_heads(num_heads, a.kv, fn);
+    if (st != MVLM_OK) return st;
+    const int64_t width = ((int64_t)num_heads + 2 * a.kv.kv_heads) * a.kv.D;
+    const size_t es = dtype_size(x_dtype), rows = (size_t)a.batch.rows;
+    REQUIRE(ld >= width, "%s: ld=%lld is below the %lld elements of a row", fn, (long long)ld, (long long)width);
+    REQUIRE(ld <= ((int64_t)1 << 40), "%s: ld=%lld too large", fn, (long long)ld);
+    REQUIRE((uintptr_t)qkv->ptr % es == 0, "%s: qkv does not start at a multiple of %zu bytes", fn, es);
+    REQUIRE(aligned16(q_out->ptr), "%s: q_out must be 16-byte aligned", fn);
+    const size_t x_bytes = ((rows - 1) * (size_t)ld + (size_t)width) * es, q_bytes = rows * num_heads * a.kv.D * 2;
+    NEED(qkv, x_bytes, "qkv");
+    NEED(q_out, q_bytes, "q_out");
+    size_t rope_bytes = 0;
+    if (rope) {
+        REQUIRE(rope->rot_dim > 0 && rope->rot_dim <= a.kv.D && rope->rot_dim % 2 == 0,
+                "%s: rot_dim=%d is not a positive even number up to head_dim=%d", fn, rope->rot_dim, a.kv.D);
+        REQUIRE(rope->positions > 0, "%s: rope positions=%d must be positive", fn, rope->positions);
+        REQUIRE(rope->table && rope->table->dev == dev, "%s: rope table is null or belongs to another device", fn);
+        REQUIRE(((uintptr_t)rope->table->ptr & 3u) == 0, "%s: rope table does not start at a multiple of 4 bytes", fn);
+        rope_bytes = (size_t)rope->positions * rope->rot_dim * 4;
+        NEED(rope->table, rope_bytes, "rope table");
+        a.rope = (const float*)rope->table->ptr;
+        a.rope_positions = rope->positions;
+        a.rot = rope->rot_dim;
+        a.interleaved = rope->interleaved != 0;
+    }
+    const size_t kvb = kv_bytes(a.kv);
+    const struct { const void* p; size_t bytes; } written[3] = {{a.kv.k, kvb}, {a.kv.v, kvb}, {q_out->ptr, q_bytes}};
+    for (const auto& w : written)
+        REQUIRE(!overlaps(w.p, w.bytes, qkv->ptr, x_bytes) && !overlaps(w.p, w.bytes, a.rope, rope_bytes) &&
+                    !holds_batch(w.p, w.bytes, a.batch),
+                "%s: the cache and q_out must not overlap what is read", fn);
+    REQUIRE(!overlaps(q_out->ptr, q_bytes, a.kv.k, kvb) && !overlaps(q_out->ptr, q_bytes, a.kv.v, kvb),
+            "%s: q_out overlaps the cache", fn);
+    a.qkv = qkv->ptr;
+    a.x_dtype = x_dtype;
+    a.ld = ld;
+    a.heads = num_heads;
+    a.chunk = fast_div(a.kv.D / 8);
+    a.q_out = (uint16_t*)q_out->ptr;
+    op->kind = OP_KV_APPEND;
+    return MVLM_OK;
+}
+
+int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
+                         const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
+                         const char* fn, Op* op) {
+    REQUIRE(dev && Q && O, "%s: null argument", fn);
+    REQUIRE(Q->dev == dev && O->dev == dev, "%s: buffers belong to another device", fn);
+    PagedAttnArgs& a = op->paged;
+    int st = make_paged_kv(dev, cache, fn, &a.kv);
+    if (st == MVLM_OK) st = make_paged_batch(dev, batch, a.kv.page.div, fn, &a.batch);
+    if (st == MVLM_OK) st = check_heads(num_heads, a.kv, fn);
+    if (st != MVLM_OK) return st;
+    REQUIRE(o_dtype == MVLM_F32 || o_dtype == a.kv.dtype, "%s: output dtype %d is neither F32 nor the cache's", fn, o_dtype);
+    REQUIRE(scale >= 0.0f && scale < INFINITY, "%s: scale %g must be finite and non-negative", fn, (double)scale);
+    REQUIRE((int64_t)a.batch.rows * num_heads <= (1 << 28), "%s: shape too large", fn);
+    REQUIRE(aligned16(Q->ptr) && aligned16(O->ptr), "%s: Q and O must be 16-byte aligned", fn);
+    const size_t elems = (size_t)a.batch.rows * num_heads * a.kv.D;
+    const size_t o_bytes = elems * dtype_size(o_dtype);
+    NEED(Q, elems * 2, "Q");
+    NEED(O, o_bytes, "O");
+    REQUIRE(!overlaps(O->ptr, o_bytes, Q->ptr, elems * 2) && !overlaps(O->ptr, o_bytes, a.kv.k, kv_bytes(a.kv)) &&
+                !overlaps(O->ptr, o_bytes, a.kv.v, kv_bytes(a.kv)) && !holds_batch(O->ptr, o_bytes, a.batch),
+            "%s: O must not overlap what is read", fn);
+    a.q = (const uint16_t*)Q->ptr;
+    a.o = O->ptr;
+    a.o_dtype = o_dtype;
+    a.heads = num_heads;
+    a.group = num_heads / a.kv.kv_heads;
+    a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)a.kv.D) : scale) * 1.4426950408889634f;
+    op->workspace_bytes = plan_attention_paged(&a, dev->prop.multiProcessorCount);
+    REQUIRE((int64_t)a.items * a.kv.kv_heads <= (1 << 30), "%s: shape too large", fn);
+    st = device_scratch(dev, op->workspace_bytes, &op->workspace);
+    a.ws = (float*)op->workspace;
+    op->kind = OP_ATTN_PAGED;
+    return st;
+}
+
+int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                const mvlm_logit_controls* c, mvlm_buffer* out, const char* fn, Op* op) {
+    REQUIRE(dev && x && c && out, "%s: null argument", fn);
+    REQUIRE(x->dev == dev && out->dev == dev, "%s: buffers belong to another device", fn);
+    REQUIRE(is_dense(dtype), "%s: dtype %d is not F32/F16/BF16", fn, dtype);
+    REQUIRE(rows > 0 && n > 0 && ld >= n && ld <= ((int64_t)1 << 40), "%s: rows=%d n=%d ld=%lld", fn, rows, n, (long long)ld);
+    REQUIRE(rows <= (1 << 20) && n <= (1 << 30) && (int64_t)rows * ((n + 1023) / 1024) <= INT_MAX, "%s: shape too large", fn);
+    const size_t es = dtype_size(dtype), bytes = ((size_t)(rows - 1) * (size_t)ld + (size_t)n) * es, R = (size_t)rows;
+    NEED(x, bytes, "x");
+    NEED(out, bytes, "out");
+    REQUIRE((uintptr_t)x->ptr % es == 0 && (uintptr_t)out->ptr % es == 0, "%s: misaligned buffer", fn);
+    REQUIRE(x->ptr == out->ptr || !overlaps(x->ptr, bytes, out->ptr, bytes), "%s: out overlaps x without being x", fn);
+    LogitsArgs& a = op->logits;
+    auto ints = [&](const mvlm_buffer* b, size_t count, const char* name, const void** to) {
+        const int st = need_ints(dev, b, count, fn, name);
+        if (st != MVLM_OK) return st;
+        REQUIRE(!overlaps(out->ptr, bytes, b->ptr, count * 4), "%s: out overlaps %s", fn, name);
+        *to = b->ptr;
+        return (int)MVLM_OK;
+    };
+    int st = MVLM_OK;
+    REQUIRE(!c->penalties == !c->history && !c->history == !c->history_len && (c->history || !c->generated_from),
+            "%s: penalties, history and history_len go together, generated_from with them", fn);
+    if (c->penalties) {
+        REQUIRE(c->history_width > 0, "%s: history_width=%d must be positive", fn, c->history_width);
+        st = ints(c->penalties, 3 * R, "penalties", (const void**)&a.penalties);
+        if (st == MVLM_OK) st = ints(c->history, R * c->history_width, "history", (const void**)&a.history);
+        if (st == MVLM_OK) st = ints(c->history_len, R, "history_len", (const void**)&a.history_len);
+        if (st == MVLM_OK && c->generated_from) st = ints(c->generated_from, R, "generated_from", (const void**)&a.generated_from);
+        a.history_width = c->history_width;
+    }
+    if (st != MVLM_OK) return st;
+    REQUIRE(!c->bias_ids == !c->bias_values && !c->bias_ids == !c->bias_len, "%s: bias_ids, bias_values and bias_len go together", fn);
+    if (c->bias_ids) {
+        REQUIRE(c->bias_width > 0, "%s: bias_width=%d must be positive", fn, c->bias_width);
+        st = ints(c->bias_ids, R * c->bias_width, "bias_ids", (const void**)&a.bias_ids);
+        if (st == MVLM_OK) st = ints(c->bias_values, R * c->bias_width, "bias_values", (const void**)&a.bias_values);
+        if (st == MVLM_OK) st = ints(c->bias_len, R, "bias_len", (const void**)&a.bias_len);
+        a.bias_width = c->bias_width;
+    }
+    if (st == MVLM_OK && c->allowed) st = ints(c->allowed, R * (((size_t)n + 31) / 32), "allowed", (const void**)&a.allowed);
+    if (st != MVLM_OK) return st;
+    a.x = x->ptr;
+    a.out = out->ptr;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.n = n;
+    a.ld = ld;
+    op->num_cus = dev->prop.multiProcessorCount;
+    op->kind = OP_LOGITS;
+    return MVLM_OK;
+}
+
 // Whether a quantized weight's product with M rows of x runs on the streaming
 // kernel rather than the skinny GEMM.  The streaming kernel multiplies each
 // weight on the vector ALU once per row, the skinny GEMM pays for 16 rows
@@ -462,6 +682,12 @@ hipError_t enqueue_op(hipStream_t s, const Op& op, bool with_attn = false) {
                                     op.scale, op.num_cus, op.workspace, op.workspace_bytes);
         case OP_ATTN_STEP:
             return launch_attn_decode(s, attn_step_desc(op), op.num_cus);
+        case OP_KV_APPEND:
+            return launch_kv_append(s, op.append);
+        case OP_ATTN_PAGED:
+            return launch_attention_paged(s, op.paged);
+        case OP_LOGITS:
+            return launch_logits(s, op.logits, op.num_cus);
     }
     return hipErrorInvalidValue;
 }
@@ -649,6 +875,26 @@ extern "C" int mvlm_argmax(mvlm_device* dev, const mvlm_buffer* x, int dtype, in
                            mvlm_buffer* out_index, mvlm_event** ev) {
     const char* fn = __func__;
     RUN(make_argmax(dev, x, dtype, rows, n, ld, out_index, fn, &op));
+}
+
+extern "C" int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                    const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                    mvlm_buffer* q_out, const mvlm_rope* rope, mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_kv_append(dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, fn, &op));
+}
+
+extern "C" int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
+                                    const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
+                                    mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_attention_paged(dev, Q, batch, cache, O, o_dtype, num_heads, scale, fn, &op));
+}
+
+extern "C" int mvlm_logits_process(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                                   const mvlm_logit_controls* controls, mvlm_buffer* out, mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_logits(dev, x, dtype, rows, n, ld, controls, out, fn, &op));
 }
 
 // ---------------------------------------------------------------------------
@@ -938,6 +1184,35 @@ extern "C" int mvlm_plan_add_argmax(mvlm_plan* plan, const mvlm_buffer* x, int d
     REQUIRE(plan, "%s: null argument", fn);
     Op op{};
     int st = make_argmax(plan->dev, x, dtype, rows, n, ld, out_index, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_kv_append_paged(mvlm_plan* plan, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                             const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                             mvlm_buffer* q_out, const mvlm_rope* rope) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_kv_append(plan->dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_attention_paged(mvlm_plan* plan, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
+                                             const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads,
+                                             float scale) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_attention_paged(plan->dev, Q, batch, cache, O, o_dtype, num_heads, scale, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_logits_process(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                                            const mvlm_logit_controls* controls, mvlm_buffer* out) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_logits(plan->dev, x, dtype, rows, n, ld, controls, out, fn, &op);
     return st != MVLM_OK ? st : plan_push(plan, op);
 }
 

@@ -1,0 +1,154 @@
+// Arguments of the kernels over a paged cache, and what their wavefronts share:
+// finding a row's sequence, and dividing the attention's work.
+#pragma once
+
+#include "common.h"
+#include "paged.h"
+
+namespace mvlm {
+
+struct KvAppendArgs {
+    PagedSeqs batch;
+    PagedKv kv;
+    const void* qkv;
+    int x_dtype;
+    int64_t ld;
+    int heads;
+    FastDiv chunk;                 // by head_dim / 8
+    const float* rope;             // [rope_positions][rot / 2][2] cos, sin
+    int rope_positions, rot, interleaved;
+    uint16_t* q_out;               // [rows][heads][D], the cache's type
+};
+
+struct PagedAttnArgs {
+    PagedSeqs batch;
+    PagedKv kv;
+    const uint16_t* q;             // [rows][heads][D], the cache's type
+    void* o;                       // [rows][heads][D]
+    int o_dtype, heads, group;     // group: heads per kv head
+    float scale_log2;              // scale * log2(e)
+    // division of the work (attention_paged.hip)
+    int64_t blocks_per_head;       // blocks wanted per kv head
+    int unit_min, unit_step;       // least keys per block, and what a block's keys are a multiple of
+    int items;                     // grid: upper bound of the items per kv head
+    float* ws;                     // partial results of split tiles
+    int records;                   // room in ws, in tiles
+};
+
+hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a);
+// Fills a's division of the work for a device; returns the workspace it needs.
+size_t plan_attention_paged(PagedAttnArgs* a, int num_cus);
+hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a);
+
+#if defined(__HIPCC__)
+
+// Sequence of a row of the batch and its span, the same in all lanes; -1 for a
+// row of no sequence.  Starts are counted 64 at a time (they do not decrease, so
+// the count of those <= row, less one, is the last sequence that starts there,
+// and the sequences before it that start there too are empty).
+__device__ __forceinline__ int paged_seq_of_row(const PagedSeqs& b, int row, PagedSpan* span) {
+    if (!b.row_start) {
+        *span = paged_span(row, row + 1, b.kv_len[row], b.rows, b.positions);
+        return row;
+    }
+    const int lane = (int)(threadIdx.x & 63);
+    int count = 0;
+    for (int base = 0; base < b.seqs; base += 64) {
+        const bool before = base + lane < b.seqs && b.row_start[base + lane] <= row;
+        count += __popcll(__builtin_amdgcn_ballot_w64(before));
+    }
+    const int seq = count - 1;
+    if (seq < 0) return -1;
+    *span = paged_span(b.row_start[seq], b.row_start[seq + 1], b.kv_len[seq], b.rows, b.positions);
+    return row >= span->row0 && row < span->row0 + span->n ? seq : -1;
+}
+
+// v plus the values of the lanes before (inclusive scan over 64 lanes)
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// Tiles of the attention.  The new rows of a sequence and the heads of a group
+// are one axis, f = j group + g (j: new row, g: head in the group), cut into
+// tiles of R; the keys of a tile are cut into splits of `unit` keys, the same
+// number for every tile of a sequence.  An item is one (tile, split).
+struct PagedItem {
+    int seq;
+    PagedSpan span;
+    int tile, split;
+    int unit;
+    int record;                    // of split 0 of this tile; -1: the tile is not split
+};
+
+__device__ __forceinline__ int paged_tiles(const PagedSpan& p, int group, int R) {
+    const int64_t f = (int64_t)p.n * group;
+    return (int)((f + R - 1) / R);
+}
+
+// Keys per block: total work (tiles x keys) over the blocks wanted, at least
+// unit_min, rounded up to unit_step.
+__device__ __forceinline__ int paged_unit(const PagedAttnArgs& a, int64_t total) {
+    int64_t u = (total + a.blocks_per_head - 1) / a.blocks_per_head;
+    u = u < a.unit_min ? a.unit_min : u;
+    u = (u + a.unit_step - 1) / a.unit_step * a.unit_step;
+    return (int)(u > PAGED_MAX_POSITIONS ? PAGED_MAX_POSITIONS : u);
+}
+
+__device__ __forceinline__ PagedSpan paged_lane_span(const PagedSeqs& b, int s) {
+    if (s >= b.seqs) return PagedSpan{0, 0, 0, 0};
+    return b.row_start ? paged_span(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.rows, b.positions)
+                       : paged_span(s, s + 1, b.kv_len[s], b.rows, b.positions);
+}
+
+// The index-th item of the batch (TILES: the index-th tile, split 0), the same in
+// all lanes; false past the last one.
+template <int R, bool TILES>
+__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int index, PagedItem* out) {
+    const PagedSeqs& b = a.batch;
+    const int lane = (int)(threadIdx.x & 63);
+    PagedSpan sp = paged_lane_span(b, lane);
+    int64_t total = 0;
+    for (int base = 0; base < b.seqs; base += 64) {
+        const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
+        total += (int64_t)paged_tiles(p, a.group, R) * p.len;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+    const int unit = paged_unit(a, total);
+    int first = 0, record = 0;                             // items and records before this round of sequences
+    for (int base = 0; base < b.seqs; base += 64) {
+        if (base) sp = paged_lane_span(b, base + lane);
+        const int tiles = paged_tiles(sp, a.group, R);
+        int splits = (sp.len + unit - 1) / unit;
+        if (splits < 1) splits = 1;
+        const int items = TILES ? tiles : tiles * splits, records = splits > 1 ? tiles * splits : 0;
+        const int end = first + wave_scan(items), rec_end = record + wave_scan(records);
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(index >= end - items && index < end);
+        if (mine) {
+            const int l = __builtin_ctzll(mine);
+            auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            out->seq = base + l;
+            out->span = PagedSpan{at(sp.row0), at(sp.n), at(sp.held), at(sp.len)};
+            out->unit = unit;
+            const int ns = at(splits), r = index - at(end - items);
+            out->tile = TILES ? r : r / ns;
+            out->split = TILES ? 0 : r - out->tile * ns;
+            out->record = ns > 1 ? at(rec_end - records) + out->tile * ns : -1;
+            // a batch whose starts decrease can exceed the items and records planned for: refused here
+            return out->tile < at(tiles) && (ns == 1 || (out->record >= 0 && out->record <= a.records - ns));
+        }
+        first = __builtin_amdgcn_readlane(end, 63);
+        record = __builtin_amdgcn_readlane(rec_end, 63);
+    }
+    return false;
+}
+
+#endif
+
+}  // namespace mvlm

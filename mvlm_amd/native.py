@@ -66,6 +66,67 @@ class GemvDesc(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("x_dtype", c_int), ("W", c_void_p), ("y", c_void_p), ("y_dtype", c_int)]
 
 
+class _PagedKV(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("num_pages", c_int), ("page_size", c_int),
+                ("kv_heads", c_int), ("head_dim", c_int)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("num_seqs", c_int), ("rows", c_int), ("row_start", c_void_p), ("kv_len", c_void_p),
+                ("page_table", c_void_p), ("table_width", c_int)]
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("table", c_void_p), ("positions", c_int), ("rot_dim", c_int), ("interleaved", c_int)]
+
+
+class _LogitControls(ctypes.Structure):
+    _fields_ = [("history", c_void_p), ("history_len", c_void_p), ("generated_from", c_void_p),
+                ("history_width", c_int), ("penalties", c_void_p), ("bias_ids", c_void_p), ("bias_values", c_void_p),
+                ("bias_len", c_void_p), ("bias_width", c_int), ("allowed", c_void_p)]
+
+
+def _handle(buf):
+    return buf.handle if buf is not None else None
+
+
+class PagedKV:
+    """A paged key/value cache: k and v hold num_pages pages of [kv_heads][page_size][head_dim]."""
+
+    def __init__(self, k, v, dtype, num_pages, page_size, kv_heads, head_dim):
+        self.buffers = [k, v]
+        self.struct = _PagedKV(k.handle, v.handle, dtype, num_pages, page_size, kv_heads, head_dim)
+
+
+class PagedBatch:
+    """The sequences of a step: int32 kv_len [num_seqs], page_table [num_seqs][table_width] and, where a
+    sequence may have more rows than one, row_start [num_seqs + 1]."""
+
+    def __init__(self, num_seqs, rows, kv_len, page_table, table_width, row_start=None):
+        self.buffers = [b for b in (kv_len, page_table, row_start) if b is not None]
+        self.struct = _PagedBatch(num_seqs, rows, _handle(row_start), _handle(kv_len), _handle(page_table), table_width)
+
+
+class Rope:
+    """Rotary positions: fp32 table [positions][rot_dim / 2][2] of cos and sin."""
+
+    def __init__(self, table, positions, rot_dim, interleaved=False):
+        self.buffers = [table]
+        self.struct = _Rope(_handle(table), positions, rot_dim, 1 if interleaved else 0)
+
+
+class LogitControls:
+    """Penalties (fp32 [rows][3]) over int32 histories, biases and the mask of a batch's logits; each may be absent."""
+
+    def __init__(self, history=None, history_len=None, generated_from=None, history_width=0, penalties=None,
+                 bias_ids=None, bias_values=None, bias_len=None, bias_width=0, allowed=None):
+        self.buffers = [b for b in (history, history_len, generated_from, penalties, bias_ids, bias_values, bias_len,
+                                    allowed) if b is not None]
+        self.struct = _LogitControls(_handle(history), _handle(history_len), _handle(generated_from), history_width,
+                                     _handle(penalties), _handle(bias_ids), _handle(bias_values), _handle(bias_len),
+                                     bias_width, _handle(allowed))
+
+
 MAX_GROUP = 8
 
 _P = c_void_p
@@ -129,6 +190,15 @@ _SIGNATURES = {
     "mvlm_plan_add_attention": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float]),
     "mvlm_argmax": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, _P, _PP]),
     "mvlm_plan_add_argmax": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, _P]),
+    "mvlm_kv_append_paged": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV), c_int, _P,
+                                     POINTER(_Rope), _PP]),
+    "mvlm_attention_paged": (c_int, [_P, _P, POINTER(_PagedBatch), POINTER(_PagedKV), _P, c_int, c_int, c_float, _PP]),
+    "mvlm_logits_process": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, POINTER(_LogitControls), _P, _PP]),
+    "mvlm_plan_add_kv_append_paged": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV), c_int,
+                                              _P, POINTER(_Rope)]),
+    "mvlm_plan_add_attention_paged": (c_int, [_P, _P, POINTER(_PagedBatch), POINTER(_PagedKV), _P, c_int, c_int,
+                                              c_float]),
+    "mvlm_plan_add_logits_process": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, POINTER(_LogitControls), _P]),
     "mvlm_fill_normal": (c_int, [_P, _P, c_int, c_size_t, c_uint64, c_double]),
     "mvlm_weight_random": (c_int, [_P, c_int, c_int, c_int, c_uint64, c_double, _PP]),
     "mvlm_event_wait": (c_int, [_P]),
@@ -499,6 +569,24 @@ class Plan:
         self._keep += [x, out_index]
         return self
 
+    def add_kv_append_paged(self, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope=None):
+        _call("mvlm_plan_add_kv_append_paged", self.handle, qkv.handle, x_dtype, ld, byref(batch.struct),
+              byref(cache.struct), num_heads, q_out.handle, byref(rope.struct) if rope else None)
+        self._keep += [qkv, q_out, *batch.buffers, *cache.buffers, *(rope.buffers if rope else [])]
+        return self
+
+    def add_attention_paged(self, Q, batch, cache, O, o_dtype, num_heads, scale=0.0):
+        _call("mvlm_plan_add_attention_paged", self.handle, Q.handle, byref(batch.struct), byref(cache.struct),
+              O.handle, o_dtype, num_heads, scale)
+        self._keep += [Q, O, *batch.buffers, *cache.buffers]
+        return self
+
+    def add_logits_process(self, x, dtype, rows, n, ld, controls, out):
+        _call("mvlm_plan_add_logits_process", self.handle, x.handle, dtype, rows, n, ld, byref(controls.struct),
+              out.handle)
+        self._keep += [x, out, *controls.buffers]
+        return self
+
     def use_graph(self, enable=True):
         _call("mvlm_plan_use_graph", self.handle, 1 if enable else 0)
         return self
@@ -712,6 +800,22 @@ class Device:
     def argmax(self, x, dtype, rows, n, ld, out_index, event=False):
         """out_index[r] (int32 on the device) = first index of the largest key of row r."""
         return self._launch("mvlm_argmax", (x.handle, dtype, rows, n, ld, out_index.handle), event)
+
+    def kv_append_paged(self, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope=None, event=False):
+        """Rotate q and k of the rows of qkv (q | k | v heads), append k and v to the paged cache, write q."""
+        return self._launch("mvlm_kv_append_paged", (qkv.handle, x_dtype, ld, byref(batch.struct),
+                                                     byref(cache.struct), num_heads, q_out.handle,
+                                                     byref(rope.struct) if rope else None), event)
+
+    def attention_paged(self, Q, batch, cache, O, o_dtype, num_heads, scale=0.0, event=False):
+        """Attention of each sequence's new rows over its pages, up to their own positions."""
+        return self._launch("mvlm_attention_paged", (Q.handle, byref(batch.struct), byref(cache.struct), O.handle,
+                                                     o_dtype, num_heads, scale), event)
+
+    def logits_process(self, x, dtype, rows, n, ld, controls, out, event=False):
+        """Penalties, biases and masks on rows of logits; out may be x."""
+        return self._launch("mvlm_logits_process", (x.handle, dtype, rows, n, ld, byref(controls.struct), out.handle),
+                            event)
 
     def gemm_quant(self, X, W, Y, M, N, K, event=False):
         """Dispatch by the weight's dtype (Q8_0 or Q4_0)."""
