@@ -159,10 +159,10 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
 #pragma unroll
     for (int t = 0; t < DT; ++t) oacc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int kv0 = k_begin + PAGED_KEYS * wave; kv0 < k_end; kv0 += PAGED_KEYS * NW) {
-        const int slot = find_slot(kv0);
-        const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(slot < 0);
-        u32x4 kf[2][KS];
+    // K fragments and V chunks of a tile are asked for while the tile before is
+    // computed: K's registers are free once its scores are, V's once it is in LDS.
+    u32x4 kf[2][KS], vf[VI];
+    auto load_k = [&](int slot) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int sl = max(__shfl(slot, 16 * u + c16, 64), 0);   // a hidden key's score is replaced below
@@ -170,19 +170,32 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int d = 32 * s + 8 * g4;
-                kf[u][s] = u32x4{0u, 0u, 0u, 0u};
-                if (d < D) kf[u][s] = *reinterpret_cast<const u32x4*>(row + d);
+                kf[u][s] = *reinterpret_cast<const u32x4*>(row + (d < D ? d : 0));
             }
         }
+    };
+    auto load_v = [&](int slot) {
 #pragma unroll
         for (int i = 0; i < VI; ++i) {
-            if (vkey[i] < PAGED_KEYS) {
-                const int sl = __shfl(slot, vkey[i], 64);
-                u32x4 v = u32x4{0u, 0u, 0u, 0u};
-                if (sl >= 0) v = *reinterpret_cast<const u32x4*>(a.kv.v + (int64_t)sl * D + vdim[i]);
-                *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = v;
-            }
+            const int sl = max(__shfl(slot, vkey[i] & 31, 64), 0);
+            vf[i] = *reinterpret_cast<const u32x4*>(a.kv.v + (int64_t)sl * D + vdim[i]);
         }
+    };
+    int kv0 = k_begin + PAGED_KEYS * wave;
+    int slot = find_slot(kv0);
+    load_k(slot);
+    load_v(slot);
+    int slot_next = find_slot(kv0 + PAGED_KEYS * NW);
+    for (; kv0 < k_end; kv0 += PAGED_KEYS * NW) {
+        const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(slot < 0);
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+            if (vkey[i] < PAGED_KEYS) {
+                if (gone && ((gone >> vkey[i]) & 1u)) vf[i] = u32x4{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = vf[i];
+            }
+        slot = slot_next;
+        load_v(slot);
         asm volatile("" ::: "memory");                         // this wave's LDS: its reads follow its stores
 
         float p[8];
@@ -190,10 +203,16 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
         for (int u = 0; u < 2; ++u) {
             f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < KS; ++k) s = mfma16<BF>(kf[u][k], qf[k], s);
+            for (int k = 0; k < KS; ++k) {
+                // dims past head_dim: K's registers hold other dims there
+                if (32 * k + 32 > D && 32 * k + 8 * g4 >= D) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
+                s = mfma16<BF>(kf[u][k], qf[k], s);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) p[4 * u + r] = s[r];
         }
+        load_k(slot);
+        slot_next = find_slot(kv0 + 2 * PAGED_KEYS * NW);
         if (gone || kv0 + PAGED_KEYS > open_end) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

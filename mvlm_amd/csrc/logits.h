@@ -20,7 +20,7 @@ struct LogitsArgs {
     const int* bias_len;
     int bias_width;
     const uint32_t* allowed;       // [rows][(n + 31) / 32]; null: everything
-    int slice, slices;             // tokens per block, blocks per row (set by the launcher)
+    int slices;                    // blocks per row (set by the launcher)
 };
 hipError_t launch_logits(hipStream_t s, const LogitsArgs& a, int num_cus);
 

@@ -8,12 +8,14 @@
 // in fp32, rounded once to the logits' type.
 //
 // Reading and writing the logits once bounds it, and for one row the launch.  A
-// block owns a slice of a row's tokens and counts the history's tokens that fall
-// into it in LDS (one word per token: generated occurrences, and the top bit for
-// one in the prompt), so no count ever reaches memory; every block of a row reads
-// the row's history, from L2 after the first, which costs history / slice of the
-// logits' own traffic.  Integer counts and the maximum of entry numbers do not
-// depend on the order in which the threads arrive.
+// block owns a slice of a row's tokens, T of them per thread, and counts the
+// history's tokens that fall into it in LDS (one word per token: generated
+// occurrences, and the top bit for one in the prompt), so no count ever reaches
+// memory.  A thread asks for its logits, its mask bits and its share of the
+// history before it waits for any of them.  Every block of a row reads the row's
+// history, from L2 after the first: history / slice of the logits' own traffic.
+// Integer counts and the maximum of entry numbers do not depend on the order in
+// which the threads arrive.
 #include "common.h"
 #include "device_math.h"
 #include "logits.h"
@@ -22,112 +24,194 @@
 
 namespace mvlm {
 
-constexpr int LOGITS_THREADS = 256;
 constexpr uint32_t IN_PROMPT = 0x80000000u;
+constexpr int LOGITS_IDS = 8;          // history entries in flight per thread
 
-template <int DT>
-__device__ __forceinline__ float logit_elem(const u32x4& w, int e) {
-    if constexpr (DT == MVLM_F32) return __uint_as_float(w[e]);
-    const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-    return DT == MVLM_F16 ? f16_bits_to_f32(b) : bf16_bits_to_f32(b);
+// N consecutive logits from x[t], N of them past v1 read as 0
+template <int DT, int N, bool VEC>
+__device__ __forceinline__ void load_logits(const void* x, int64_t t, int left, float (&v)[N]) {
+    if (VEC && left >= N) {
+        if constexpr (DT == MVLM_F32) {
+            static_assert(N == 4, "16 bytes");
+            const f32x4 w = *reinterpret_cast<const f32x4*>((const float*)x + t);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = w[e];
+        } else {
+            uint32_t w[N / 2];
+            if constexpr (N == 8) {
+                const u32x4 q = *reinterpret_cast<const u32x4*>((const uint16_t*)x + t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = q[e];
+            } else {
+                const u32x2 q = *reinterpret_cast<const u32x2*>((const uint16_t*)x + t);
+                w[0] = q[0], w[1] = q[1];
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint16_t h = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+                v[e] = DT == MVLM_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < left ? load_as_f32(x, t + e, DT) : 0.0f;
 }
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const LogitsArgs a) {
-    extern __shared__ uint32_t counts[];                       // [slice] counts, then [slice] last bias entries + 1
-    constexpr int ES = DT == MVLM_F32 ? 4 : 2, EPC = VEC ? 16 / ES : 1;
+template <int DT, int N, bool VEC>
+__device__ __forceinline__ void store_logits(void* y, int64_t t, int left, const float (&v)[N]) {
+    if (VEC && left >= N) {
+        if constexpr (DT == MVLM_F32) {
+            *reinterpret_cast<f32x4*>((float*)y + t) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+            uint32_t w[N / 2];
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e)
+                w[e] = DT == MVLM_F16 ? (uint32_t)f32_to_f16_bits(v[2 * e]) | (uint32_t)f32_to_f16_bits(v[2 * e + 1]) << 16
+                                      : (uint32_t)f32_to_bf16_bits(v[2 * e]) | (uint32_t)f32_to_bf16_bits(v[2 * e + 1]) << 16;
+            if constexpr (N == 8) *reinterpret_cast<u32x4*>((uint16_t*)y + t) = u32x4{w[0], w[1], w[2], w[3]};
+            else *reinterpret_cast<u32x2*>((uint16_t*)y + t) = u32x2{w[0], w[1]};
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e < left) store_out(y, t + e, v[e], DT);
+}
+
+// A thread's share of a list, entries tid, tid + THREADS, ...: asked for LOGITS_IDS
+// at a time, the first of them before the list's length is known (its room is).
+template <int THREADS, int BATCH>
+struct ListShare {
+    int id[BATCH];
+    const int* list;
+    int room, tid;
+    __device__ __forceinline__ void ask(int base) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) id[u] = list[min(base + u * THREADS, room - 1)];
+    }
+    __device__ __forceinline__ ListShare(const int* l, int width, int t) : list(l), room(width), tid(t) {
+        if (list) ask(tid);
+    }
+    // f(i, list[i]) for the thread's entries below len
+    template <class F>
+    __device__ __forceinline__ void each(int len, F&& f) {
+        for (int base = tid; base < len; base += THREADS * BATCH) {
+            if (base != tid) ask(base);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u)
+                if (base + u * THREADS < len) f(base + u * THREADS, id[u]);
+        }
+    }
+};
+
+// T tokens per thread; VEC: rows of x and out start 16-byte aligned
+template <int DT, bool VEC, int THREADS, int T>
+__global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
+    constexpr int N = DT == MVLM_F32 || T == 4 ? 4 : 8, NV = T / N, SLICE = THREADS * T;
+    extern __shared__ __attribute__((aligned(16))) uint32_t words[];   // [SLICE] counts, then [SLICE] last bias entries + 1
+    uint32_t* counts = words;
+    uint32_t* entries = words + (a.penalties ? SLICE : 0);
     const int row = (int)(blockIdx.x / (uint32_t)a.slices);
-    const int v0 = ((int)blockIdx.x - row * a.slices) * a.slice, v1 = min(v0 + a.slice, a.n);
+    const int v0 = ((int)blockIdx.x - row * a.slices) * SLICE, size = min(SLICE, a.n - v0);
     const int tid = (int)threadIdx.x;
-    uint32_t* entries = counts + a.slice;
-    if (a.penalties)
-        for (int i = tid; i < a.slice; i += LOGITS_THREADS) counts[i] = 0u;
-    if (a.bias_ids)
-        for (int i = tid; i < a.slice; i += LOGITS_THREADS) entries[i] = 0u;
-    __syncthreads();
+    const int64_t base = (int64_t)row * a.ld + v0;
+    float v[NV][N];
+    uint32_t mask[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int t = (i * THREADS + tid) * N;
+        load_logits<DT, N, VEC>(a.x, base + t, size - t, v[i]);
+        mask[i] = 0xFFFFFFFFu;
+        if (a.allowed && t < size)
+            mask[i] = a.allowed[(int64_t)row * ((a.n + 31) / 32) + ((v0 + t) >> 5)] >> ((v0 + t) & 31);
+    }
+    ListShare<THREADS, LOGITS_IDS> history(a.penalties ? a.history + (int64_t)row * a.history_width : nullptr,
+                                           a.history_width, tid);
+    ListShare<THREADS, 1> biases(a.bias_ids ? a.bias_ids + (int64_t)row * a.bias_width : nullptr, a.bias_width, tid);
+    const int used = (a.penalties ? SLICE : 0) + (a.bias_ids ? SLICE : 0);
+    for (int i = 4 * tid; i < used; i += 4 * THREADS) *reinterpret_cast<u32x4*>(words + i) = u32x4{0u, 0u, 0u, 0u};
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    int len = 0, from = 0, bias_len = 0;
     if (a.penalties) {
         rep = a.penalties[3 * (int64_t)row];
         freq = a.penalties[3 * (int64_t)row + 1];
         pres = a.penalties[3 * (int64_t)row + 2];
-        const int len = min(max(a.history_len[row], 0), a.history_width);
-        const int from = a.generated_from ? a.generated_from[row] : 0;
-        const int* ids = a.history + (int64_t)row * a.history_width;
-        for (int i = tid; i < len; i += LOGITS_THREADS) {
-            const int id = ids[i];
-            if (id >= v0 && id < v1) {
+        len = min(max(a.history_len[row], 0), a.history_width);
+        from = a.generated_from ? a.generated_from[row] : 0;
+    }
+    if (a.bias_ids) bias_len = min(max(a.bias_len[row], 0), a.bias_width);
+    __syncthreads();
+    if (a.penalties) {
+        history.each(len, [&](int i, int id) {
+            if ((uint32_t)(id - v0) < (uint32_t)size) {
                 if (i >= from) atomicAdd(&counts[id - v0], 1u);
                 else atomicOr(&counts[id - v0], IN_PROMPT);
             }
-        }
+        });
     }
-    const float* bias = nullptr;
+    const float* bias = a.bias_values + (int64_t)row * a.bias_width;
     if (a.bias_ids) {
-        const int len = min(max(a.bias_len[row], 0), a.bias_width);
-        const int* ids = a.bias_ids + (int64_t)row * a.bias_width;
-        bias = a.bias_values + (int64_t)row * a.bias_width;
-        for (int i = tid; i < len; i += LOGITS_THREADS) {
-            const int id = ids[i];
-            if (id >= v0 && id < v1) atomicMax(&entries[id - v0], (uint32_t)i + 1u);
-        }
+        biases.each(bias_len, [&](int i, int id) {
+            if ((uint32_t)(id - v0) < (uint32_t)size) atomicMax(&entries[id - v0], (uint32_t)i + 1u);
+        });
     }
     __syncthreads();
-    const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)row * ((a.n + 31) / 32) : nullptr;
-    auto one = [&](float x, int t) {
-        if (a.penalties) {
-            const uint32_t w = counts[t - v0], g = w & ~IN_PROMPT;
-            if (w) x = x > 0.0f ? x / rep : x * rep;
-            if (g) x -= __builtin_fmaf((float)g, freq, pres);
-        }
-        if (bias) {
-            const uint32_t e = entries[t - v0];
-            if (e) x += bias[e - 1];
-        }
-        if (allowed && !((allowed[t >> 5] >> (t & 31)) & 1u)) x = -INFINITY;
-        return x;
-    };
-    const int64_t base = (int64_t)row * a.ld;
-    const uint8_t* x = (const uint8_t*)a.x + base * ES;
-    uint8_t* out = (uint8_t*)a.out + base * ES;
-    if constexpr (VEC) {
-        const int whole = v0 + (v1 - v0) / EPC * EPC;
-        for (int t = v0 + tid * EPC; t < whole; t += LOGITS_THREADS * EPC) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(x + (int64_t)t * ES);
-            u32x4 o;
-            if constexpr (DT == MVLM_F32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(one(logit_elem<DT>(w, e), t + e));
-            } else {
+    for (int i = 0; i < NV; ++i) {
+        const int t = (i * THREADS + tid) * N;
+        if (a.penalties) {
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(counts + t + q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float lo = one(logit_elem<DT>(w, 2 * e), t + 2 * e), hi = one(logit_elem<DT>(w, 2 * e + 1), t + 2 * e + 1);
-                    o[e] = DT == MVLM_F16 ? (uint32_t)f32_to_f16_bits(lo) | (uint32_t)f32_to_f16_bits(hi) << 16
-                                          : (uint32_t)f32_to_bf16_bits(lo) | (uint32_t)f32_to_bf16_bits(hi) << 16;
+                    float& x = v[i][q + e];
+                    const uint32_t g = w[e] & ~IN_PROMPT;
+                    if (w[e]) x = x > 0.0f ? x / rep : x * rep;
+                    if (g) x -= __builtin_fmaf((float)g, freq, pres);
                 }
             }
-            *reinterpret_cast<u32x4*>(out + (int64_t)t * ES) = o;
         }
-        for (int t = whole + tid; t < v1; t += LOGITS_THREADS) store_out(out, t, one(load_as_f32(x, t, DT), t), DT);
-    } else {
-        for (int t = v0 + tid; t < v1; t += LOGITS_THREADS) store_out(out, t, one(load_as_f32(x, t, DT), t), DT);
+        if (a.bias_ids) {
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(entries + t + q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (w[e]) v[i][q + e] += bias[w[e] - 1];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (!((mask[i] >> e) & 1u)) v[i][e] = -INFINITY;
+        store_logits<DT, N, VEC>(a.out, base + t, size - t, v[i]);
     }
 }
 
-hipError_t launch_logits(hipStream_t s, const LogitsArgs& in, int num_cus) {
-    LogitsArgs a = in;
-    // the largest slice that still gives every CU a block: large slices read the
-    // history less often, small ones share a row among more CUs
-    a.slice = 8192;
-    while (a.slice > 1024 && (int64_t)a.rows * ((a.n + a.slice - 1) / a.slice) < num_cus) a.slice /= 2;
-    a.slices = (a.n + a.slice - 1) / a.slice;
+template <int DT, bool VEC, int THREADS, int T>
+static void launch_slices(hipStream_t s, LogitsArgs a) {
+    constexpr int SLICE = THREADS * T;
+    a.slices = (a.n + SLICE - 1) / SLICE;
+    const uint32_t shmem = SLICE * 4u * ((a.penalties ? 1u : 0u) + (a.bias_ids ? 1u : 0u));
+    launch_kernel(logits_kernel<DT, VEC, THREADS, T>, dim3((unsigned)(a.rows * a.slices)), dim3(THREADS), shmem, s, a);
+}
+
+hipError_t launch_logits(hipStream_t s, const LogitsArgs& a, int num_cus) {
     const int es = a.dtype == MVLM_F32 ? 4 : 2;
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.out) & 15u) == 0 && (a.ld * es) % 16 == 0;
-    const uint32_t shmem = (uint32_t)a.slice * 4u * (a.bias_ids ? 2u : 1u);
-    const dim3 grid((unsigned)(a.rows * a.slices)), block(LOGITS_THREADS);
+    // slices of 4096 read the history a quarter as often as slices of 1024, which
+    // share few rows among more CUs
+    const bool large = (int64_t)a.rows * ((a.n + 4095) / 4096) >= 2 * (int64_t)num_cus;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (vec) launch_kernel(logits_kernel<DT, true>, grid, block, shmem, s, a);
-        else launch_kernel(logits_kernel<DT, false>, grid, block, shmem, s, a);
+        if (vec) {
+            if (large) launch_slices<DT, true, 512, 8>(s, a);
+            else launch_slices<DT, true, 256, 4>(s, a);
+        } else {
+            if (large) launch_slices<DT, false, 512, 8>(s, a);
+            else launch_slices<DT, false, 256, 4>(s, a);
+        }
     };
     if (a.dtype == MVLM_F32) go(std::integral_constant<int, MVLM_F32>{});
     else if (a.dtype == MVLM_F16) go(std::integral_constant<int, MVLM_F16>{});
