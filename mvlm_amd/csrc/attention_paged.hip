@@ -28,16 +28,11 @@
 //    the exp2 domain), so P stays below 2^8 and most tiles rescale nothing.
 //  * hidden keys may hold anything: their scores are replaced, not added to,
 //    and their V rows are staged as zeros.
-#include "common.h"
-#include "device_math.h"
-#include "paged_ops.h"
+#include "attention_paged.h"
 
 #include <algorithm>
 
 namespace mvlm {
-
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
 constexpr int PAGED_R = 16;        // rows per tile
 constexpr int PAGED_KEYS = 32;     // keys per wave and step
@@ -49,46 +44,6 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-
-// (lo, hi) rounded to nearest even, packed; with REST, lo and hi become what was lost
-template <bool BF, bool REST>
-__device__ __forceinline__ uint32_t round2(float& lo, float& hi) {
-    if constexpr (BF) {
-        const bf16x2v h = __builtin_convertvector(f32x2{lo, hi}, bf16x2v);
-        if constexpr (REST) lo -= (float)h[0], hi -= (float)h[1];
-        return __builtin_bit_cast(uint32_t, h);
-    } else {
-        const f16x2v h = __builtin_convertvector(f32x2{lo, hi}, f16x2v);
-        if constexpr (REST) lo -= (float)h[0], hi -= (float)h[1];
-        return __builtin_bit_cast(uint32_t, h);
-    }
-}
-
-// Workspace: per record (tile of one split and kv head) 16 rows of D floats of
-// unnormalized output, then, behind all records, 16 (max, sum) pairs each.
-__device__ __forceinline__ float* paged_ws_out(const PagedAttnArgs& a, int record, int h) {
-    return a.ws + ((int64_t)record * a.kv.kv_heads + h) * PAGED_R * a.kv.D;
-}
-__device__ __forceinline__ f32x2* paged_ws_ml(const PagedAttnArgs& a, int record, int h) {
-    return reinterpret_cast<f32x2*>(a.ws + (int64_t)a.records * a.kv.kv_heads * PAGED_R * a.kv.D) +
-           ((int64_t)record * a.kv.kv_heads + h) * PAGED_R;
-}
-
-// four outputs of row f of a tile's sequence, from dim d on
-template <bool BF>
-__device__ __forceinline__ void paged_store4(const PagedAttnArgs& a, const PagedSpan& sp, int h, int f, int d, f32x4 v) {
-    const int j = f / a.group, g = f - j * a.group;
-    const int64_t at = ((int64_t)(sp.row0 + j) * a.heads + h * a.group + g) * a.kv.D + d;
-    if (a.o_dtype == MVLM_F32)
-        *reinterpret_cast<f32x4*>((float*)a.o + at) = v;
-    else {
-        float e[4] = {v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<u32x2*>((uint16_t*)a.o + at) = u32x2{round2<BF, false>(e[0], e[1]), round2<BF, false>(e[2], e[3])};
-    }
 }
 
 // LDS of a wave: 32 V rows while it runs, 16 rows of output and their statistics
@@ -115,7 +70,7 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
     const int D = a.kv.D, index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads);
     const int h = (int)blockIdx.x - index * a.kv.kv_heads;
     PagedItem it;
-    if (!paged_find<PAGED_R, false>(a, index, &it)) return;
+    if (!paged_find<PAGED_R, false, false>(a, index, &it)) return;
     const PagedSpan sp = it.span;
 
     // this lane's row of the tile
@@ -214,6 +169,7 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
         load_k(slot);
         slot_next = find_slot(kv0 + 2 * PAGED_KEYS * NW);
         if (gone || kv0 + PAGED_KEYS > open_end) {
+            asm volatile("");                                  // a branch: few tiles need this
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int i = 16 * (e >> 2) + 4 * g4 + (e & 3);
@@ -288,83 +244,78 @@ __global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const Pa
             o += e * *reinterpret_cast<const f32x4*>(rw + r * L::OP + d);
         }
         if (it.record >= 0) {
-            *reinterpret_cast<f32x4*>(paged_ws_out(a, it.record + it.split, h) + r * D + d) = o;
-            if (d == 0) paged_ws_ml(a, it.record + it.split, h)[r] = f32x2{mx, sum};
+            *reinterpret_cast<f32x4*>(paged_ws_out<PAGED_R>(a, it.record + it.split, h) + r * D + d) = o;
+            if (d == 0) paged_ws_ml<PAGED_R, false>(a, it.record + it.split, h)[r] = f32x2{mx, sum};
             continue;
         }
         paged_store4<BF>(a, sp, h, it.tile * PAGED_R + r, d, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / sum));
     }
 }
 
-// Merges the splits of a tile, in their order.
-template <bool BF>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs a) {
-    const int D = a.kv.D, index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads);
-    const int h = (int)blockIdx.x - index * a.kv.kv_heads;
-    PagedItem it;
-    if (!paged_find<PAGED_R, true>(a, index, &it) || it.record < 0) return;
-    const PagedSpan sp = it.span;
-    const int rows_f = sp.n * a.group, last_row = min(it.tile * PAGED_R + PAGED_R - 1, rows_f - 1) / a.group;
-    const int splits = max(1, (sp.visible(last_row) + it.unit - 1) / it.unit);   // those that saw keys
-    const int d4 = D / 4;
-    for (int i = (int)threadIdx.x; i < PAGED_R * d4; i += 256) {
-        const int r = i / d4, d = 4 * (i - r * d4);
-        if (it.tile * PAGED_R + r >= rows_f) continue;
-        float mx = -INFINITY, sum = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < splits; ++s) {
-            const f32x2 ml = paged_ws_ml(a, it.record + s, h)[r];
-            const f32x4 ov = *reinterpret_cast<const f32x4*>(paged_ws_out(a, it.record + s, h) + r * D + d);
-            if (ml[0] == -INFINITY && ml[1] == 0.0f) continue;   // saw no key
-            const float mn = fmaxf(mx, ml[0]);
-            const float f0 = __builtin_amdgcn_exp2f(mx - mn), f1 = __builtin_amdgcn_exp2f(ml[0] - mn);
-            sum = sum * f0 + ml[1] * f1;
-            o = o * f0 + ov * f1;
-            mx = mn;
-        }
-        paged_store4<BF>(a, sp, h, it.tile * PAGED_R + r, d, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / sum));
-    }
+// Division of the sequences of at most (or of more than) PAGED_FEW f-rows: `blocks`
+// blocks are wanted.  The sum of ceil(len / unit) over tiles is at most total / unit
+// + tiles, and a tile is split when len > unit, so split tiles make at most
+// 2 total / unit records.
+static PagedDivision paged_divide(const PagedAttnArgs& a, int tile, int64_t blocks, int64_t tiles, int unit_step) {
+    PagedDivision d{};
+    d.tile = tile;
+    d.unit_step = unit_step;
+    d.unit_min = unit_step;
+    d.blocks_per_head = (blocks + a.kv.kv_heads - 1) / a.kv.kv_heads;
+    d.tiles = (int)tiles;
+    d.items = (int)(d.blocks_per_head + tiles);
+    d.records = (int)(2 * d.blocks_per_head);
+    return d;
 }
 
 size_t plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const PagedSeqs& b = a->batch;
-    const int64_t most = b.row_start ? (int64_t)b.rows * a->group / PAGED_R + b.seqs
-                                     : (int64_t)b.seqs * ((a->group + PAGED_R - 1) / PAGED_R);
-    a->unit_step = PAGED_KEYS * PAGED_NW;
-    a->unit_min = a->unit_step;
-    a->blocks_per_head = (4 * (int64_t)num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
-    // sum of ceil(len / unit) over tiles <= total / unit + tiles; a tile is split
-    // when len > unit, so split tiles make at most 2 total / unit records
-    a->items = (int)(a->blocks_per_head + most);
-    a->records = (int)(2 * a->blocks_per_head);
-    return (size_t)a->records * a->kv.kv_heads * PAGED_R * (a->kv.D + 2) * sizeof(float);
+    const int64_t f = (int64_t)b.rows * a->group;
+    const bool single = !b.row_start;                          // every sequence has `group` f-rows
+    a->few = a->many = PagedDivision{};
+    if (!single || a->group <= PAGED_FEW) {
+        const int64_t few = single ? (int64_t)b.seqs * ((a->group + PAGED_R - 1) / PAGED_R) : f / PAGED_R + b.seqs;
+        a->few = paged_divide(*a, PAGED_R, 4 * (int64_t)num_cus, few, PAGED_KEYS * PAGED_NW);
+    }
+    if (single ? a->group > PAGED_FEW : f > PAGED_FEW) {
+        const int rw = 1;
+        // at most one sequence in PAGED_FEW f-rows has more of them
+        a->many = paged_divide(*a, 128 * rw, (int64_t)num_cus * (rw == 1 ? 2 : 1), f / (128 * rw) + std::min<int64_t>(b.seqs, f / PAGED_FEW + 1),
+                               256);
+    }
+    size_t bytes = 0;
+    for (const PagedDivision* d : {&a->few, &a->many})
+        bytes = std::max(bytes, (size_t)d->records * a->kv.kv_heads * d->tile * (a->kv.D + 2) * sizeof(float));
+    return bytes;
 }
 
 template <int KS, bool BF, int PP>
-static void launch_paged_variant(hipStream_t s, const PagedAttnArgs& a) {
-    const dim3 grid((unsigned)(a.kv.kv_heads * a.items)), block(64 * PAGED_NW);
-    launch_kernel_part(LaunchPart::First, paged_attention_kernel<KS, BF, PP>, grid, block, 0, s, a);
-    const dim3 tiles((unsigned)(a.kv.kv_heads * (a.items - (int)a.blocks_per_head)));
-    launch_kernel_part(LaunchPart::Last, paged_combine_kernel<BF>, tiles, dim3(256), 0, s, a);
+static void launch_few(PagedLaunch& go) {
+    go(paged_attention_kernel<KS, BF, PP>, go.a.few.items);
+    go(paged_combine_kernel<BF, PAGED_R, false>, go.a.few.tiles);
 }
 
 template <int KS>
-static void launch_paged_dims(hipStream_t s, const PagedAttnArgs& a) {
-    const bool wide = a.o_dtype == MVLM_F32;
-    if (a.kv.dtype == MVLM_F16) {
-        if (wide) launch_paged_variant<KS, false, 2>(s, a);
-        else launch_paged_variant<KS, false, 1>(s, a);
+static void launch_few_dims(PagedLaunch& go) {
+    const bool wide = go.a.o_dtype == MVLM_F32;
+    if (go.a.kv.dtype == MVLM_F16) {
+        if (wide) launch_few<KS, false, 2>(go);
+        else launch_few<KS, false, 1>(go);
     } else {
-        if (wide) launch_paged_variant<KS, true, 3>(s, a);
-        else launch_paged_variant<KS, true, 1>(s, a);
+        if (wide) launch_few<KS, true, 3>(go);
+        else launch_few<KS, true, 1>(go);
     }
 }
 
 hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a) {
-    if (a.kv.D <= 32) launch_paged_dims<1>(s, a);
-    else if (a.kv.D <= 64) launch_paged_dims<2>(s, a);
-    else if (a.kv.D <= 96) launch_paged_dims<3>(s, a);
-    else launch_paged_dims<4>(s, a);
+    PagedLaunch go{s, a, (a.few.tile ? 2 : 0) + (a.many.tile ? 2 : 0)};
+    if (a.many.tile) launch_attention_paged_chunk(go);
+    if (a.few.tile) {
+        if (a.kv.D <= 32) launch_few_dims<1>(go);
+        else if (a.kv.D <= 64) launch_few_dims<2>(go);
+        else if (a.kv.D <= 96) launch_few_dims<3>(go);
+        else launch_few_dims<4>(go);
+    }
     return hipGetLastError();
 }
 

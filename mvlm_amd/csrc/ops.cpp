@@ -451,7 +451,7 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     a.group = num_heads / a.kv.kv_heads;
     a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)a.kv.D) : scale) * 1.4426950408889634f;
     op->workspace_bytes = plan_attention_paged(&a, dev->prop.multiProcessorCount);
-    REQUIRE((int64_t)a.items * a.kv.kv_heads <= (1 << 30), "%s: shape too large", fn);
+    REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads <= (1 << 30), "%s: shape too large", fn);
     st = device_scratch(dev, op->workspace_bytes, &op->workspace);
     a.ws = (float*)op->workspace;
     op->kind = OP_ATTN_PAGED;

@@ -20,6 +20,17 @@ struct KvAppendArgs {
     uint16_t* q_out;               // [rows][heads][D], the cache's type
 };
 
+// How one kernel's share of a batch is cut into blocks.
+struct PagedDivision {
+    int tile;                      // f-rows per tile; 0: no sequence is this kernel's
+    int64_t blocks_per_head;       // blocks wanted per kv head
+    int unit_min, unit_step;       // least keys per block, and what a block's keys are a multiple of
+    int items;                     // grid: upper bound of the items per kv head
+    int tiles;                     // upper bound of the tiles per kv head
+    int records;                   // room in the workspace, in tiles
+};
+constexpr int PAGED_FEW = 64;
+
 struct PagedAttnArgs {
     PagedSeqs batch;
     PagedKv kv;
@@ -27,12 +38,10 @@ struct PagedAttnArgs {
     void* o;                       // [rows][heads][D]
     int o_dtype, heads, group;     // group: heads per kv head
     float scale_log2;              // scale * log2(e)
-    // division of the work (attention_paged.hip)
-    int64_t blocks_per_head;       // blocks wanted per kv head
-    int unit_min, unit_step;       // least keys per block, and what a block's keys are a multiple of
-    int items;                     // grid: upper bound of the items per kv head
     float* ws;                     // partial results of split tiles
-    int records;                   // room in ws, in tiles
+    // division of the work (attention_paged.hip) of the sequences with few new
+    // rows, f = n group <= PAGED_FEW, and of those with more
+    PagedDivision few, many;
 };
 
 hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a);
@@ -86,14 +95,15 @@ struct PagedItem {
     int record;                    // of split 0 of this tile; -1: the tile is not split
 };
 
-__device__ __forceinline__ int paged_tiles(const PagedSpan& p, int group, int R) {
+template <int R, bool MANY>
+__device__ __forceinline__ int paged_tiles(const PagedSpan& p, int group) {
     const int64_t f = (int64_t)p.n * group;
-    return (int)((f + R - 1) / R);
+    return (f > PAGED_FEW) == MANY ? (int)((f + R - 1) / R) : 0;
 }
 
 // Keys per block: total work (tiles x keys) over the blocks wanted, at least
 // unit_min, rounded up to unit_step.
-__device__ __forceinline__ int paged_unit(const PagedAttnArgs& a, int64_t total) {
+__device__ __forceinline__ int paged_unit(const PagedDivision& a, int64_t total) {
     int64_t u = (total + a.blocks_per_head - 1) / a.blocks_per_head;
     u = u < a.unit_min ? a.unit_min : u;
     u = (u + a.unit_step - 1) / a.unit_step * a.unit_step;
@@ -108,23 +118,24 @@ __device__ __forceinline__ PagedSpan paged_lane_span(const PagedSeqs& b, int s) 
 
 // The index-th item of the batch (TILES: the index-th tile, split 0), the same in
 // all lanes; false past the last one.
-template <int R, bool TILES>
+template <int R, bool MANY, bool TILES>
 __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int index, PagedItem* out) {
     const PagedSeqs& b = a.batch;
+    const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
     PagedSpan sp = paged_lane_span(b, lane);
     int64_t total = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        total += (int64_t)paged_tiles(p, a.group, R) * p.len;
+        total += (int64_t)paged_tiles<R, MANY>(p, a.group) * p.len;
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
-    const int unit = paged_unit(a, total);
+    const int unit = paged_unit(div, total);
     int first = 0, record = 0;                             // items and records before this round of sequences
     for (int base = 0; base < b.seqs; base += 64) {
         if (base) sp = paged_lane_span(b, base + lane);
-        const int tiles = paged_tiles(sp, a.group, R);
+        const int tiles = paged_tiles<R, MANY>(sp, a.group);
         int splits = (sp.len + unit - 1) / unit;
         if (splits < 1) splits = 1;
         const int items = TILES ? tiles : tiles * splits, records = splits > 1 ? tiles * splits : 0;
@@ -141,7 +152,7 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int index, Pa
             out->split = TILES ? 0 : r - out->tile * ns;
             out->record = ns > 1 ? at(rec_end - records) + out->tile * ns : -1;
             // a batch whose starts decrease can exceed the items and records planned for: refused here
-            return out->tile < at(tiles) && (ns == 1 || (out->record >= 0 && out->record <= a.records - ns));
+            return out->tile < at(tiles) && (ns == 1 || (out->record >= 0 && out->record <= div.records - ns));
         }
         first = __builtin_amdgcn_readlane(end, 63);
         record = __builtin_amdgcn_readlane(rec_end, 63);
