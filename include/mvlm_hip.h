@@ -329,7 +329,8 @@ int mvlm_argmax(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
  *
  * A cache: K and V hold num_pages pages of [kv_heads][page_size][head_dim]
  * elements (F16 or BF16), 16-byte aligned, not overlapping; head_dim a multiple
- * of 8, at most 128; fewer than 2^31 slots num_pages kv_heads page_size. */
+ * of 8, at most 128; at most 1024 kv_heads; fewer than 2^31 slots num_pages
+ * kv_heads page_size, and K less than 64 GiB. */
 typedef struct mvlm_paged_kv {
     mvlm_buffer* k;
     mvlm_buffer* v;

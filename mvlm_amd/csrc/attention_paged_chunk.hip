@@ -1,23 +1,43 @@
-// Attention over a paged cache for sequences with many new rows (see
-// attention_paged.hip for the operator and its division into items).
+// Attention over a paged cache for batches in which some sequence may have many new
+// rows (attention_paged.hip describes the operator and its division into items).
 //
-// A block of four waves owns 128 RW f-rows of one kv head, wave w rows
-// 32 RW w .. of them, and walks the keys in tiles of 64 that all its waves share:
-// the matrix cores bound it, and each K or V fragment a wave reads from LDS serves
-// its RW products.
-//  * K and V tiles go straight from memory to LDS, two buffers each, a tile ahead
-//    (16-byte chunks, the waves' loads finding their rows through the table);
-//    a hidden key's chunks come from zeros.
+// A block of eight waves owns 256 f-rows of one kv head, wave w rows 32 w .. of
+// them, and walks the keys in tiles of 64 that all its waves share.  The matrix
+// cores and the vector ALUs bound it about equally: a tile costs a wave 32
+// matrix instructions of 32 cycles and, for its 2048 scores, about as many cycles of
+// exponentials, maxima, sums and conversions.  So the two waves of a SIMD (w and
+// w + 4) alternate: while one runs the products of its tile, O^T += V^T P^T of
+// the tile before and S^T = K Q^T, the other runs its softmax, and a barrier
+// swaps them.  Phases 2i and 2i + 1 hold the products of tile i of waves 0..3 and
+// of waves 4..7, so both use K of tile i and V of tile i - 1 there, while the tiles
+// after them are on their way into the other buffers of a ring: the blocks of one kv
+// head walk its keys in step, so each tile comes from memory once for all of them
+// and its loads have to cover that latency.
+//  * K and V tiles go straight from memory to LDS in 16-byte chunks; a hidden
+//    key's chunks and those past head_dim come from zeros.  Their rows are found through the page table for
+//    SLOT_KEYS keys at a time, kept in LDS, so that no load that a wave waits for
+//    comes between them.
 //  * LDS rows are CH chunks; chunk c of key k lies at c ^ key_swizzle(k), so that
 //    16 lanes reading one chunk of 16 keys touch all 64 banks, and c ^
 //    value_swizzle(k), so that the four keys x 64 bytes of half a transposed read do.
-//  * S^T = K Q^T and O^T = V^T P^T as above on v_mfma_f32_32x32x16: lane l's
-//    results are row l % 32 and keys 8 (r / 4) + 4 (l / 32) + r % 4.
+//  * v_mfma_f32_32x32x16: lane l's results are row l % 32 and keys
+//    8 (r / 4) + 4 (l / 32) + r % 4, which are the B operand of the second product
+//    as they stand when V^T is read in the same key order.
+//  * a tile that only some of a wave's rows see in part is checked for values that are
+//    not finite (0 x infinity would reach rows that do not see it); if it holds any,
+//    its second product is made key by key over the rows that see the key.
+// The sequences with few new rows are items of paged_few_item in the same launch,
+// behind those with many.  A block fills a CU (its LDS), so there is one per CU, and
+// they take items from queues, one per XCD: item w belongs to queue w % 8, so with a
+// multiple of 8 kv heads the tiles of a head run on one XCD and share its L2.  A
+// sequence's tiles come in order of their keys, the most first, and the blocks take
+// them in turn, from the last block to the first in every other round, so that who
+// had the longest takes the shortest next.
 #include "attention_paged.h"
 
-namespace mvlm {
+#include <algorithm>
 
-constexpr int CHUNK_KEYS = 64;
+namespace mvlm {
 
 __device__ const u32x4 paged_zeros = {0u, 0u, 0u, 0u};
 
@@ -33,249 +53,381 @@ __device__ __forceinline__ int key_swizzle(int key) { return CH == 16 ? key & 15
 template <int CH>
 __device__ __forceinline__ int value_swizzle(int key) { return CH == 16 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
 
-// KS: head_dim <= 16 KS; DT: head_dim <= 32 DT; RW: 32-row tiles per wave
-template <int KS, int DT, bool BF, int PP, int RW>
-__global__ __launch_bounds__(256, RW == 1 ? 2 : 1) void paged_chunk_kernel(const PagedAttnArgs a) {
-    constexpr int CH = DT > 2 ? 16 : 8, PB = 16 * CH, TILE = CHUNK_KEYS * PB, R = 128 * RW;
-    constexpr int NL = CHUNK_KEYS * CH / 256;                  // chunks of K (and of V) per thread and tile
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];   // K0 V0 K1 V1
-    const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+// Barrier between phases: this wave's LDS reads are complete, its direct loads
+// stay in flight, and no instruction moves to the other side.
+__device__ __forceinline__ void phase_barrier() {
+    asm_wait_lgkmcnt<0>();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
+constexpr int CHUNK_THREADS = 512;
+
+constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
+constexpr int SLOT_KEYS = 2048;                                // keys whose slots LDS holds, twice
+
+template <int DT>
+struct ChunkLayout {
+    static constexpr int CH = DT > 2 ? 16 : 8;                 // chunks per LDS row
+    static constexpr int PB = 16 * CH, TILE = CHUNK_KEYS * PB;
+    static constexpr int NB = DT > 2 ? 3 : 4;                  // tiles of the K ring, and of the V ring behind it
+    static constexpr int V = NB * TILE, SLOTS = 2 * NB * TILE, P = SLOTS + 2 * SLOT_KEYS * 4;
+    static constexpr int P_WAVE = 32 * 32 * 4;                 // 32 keys x 32 rows of probabilities (slow path)
+    static constexpr int ZEROS = P + 8 * P_WAVE, BYTES = ZEROS + TILE;   // a V tile of zeros
+};
+
+// KS: head_dim <= 16 KS; DT: head_dim <= 32 DT; PP: parts of P
+template <int KS, int DT, bool BF, int PP>
+__device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, int unit, int index, int h, uint8_t* lds) {
+    using L = ChunkLayout<DT>;
+    constexpr int CH = L::CH, PB = L::PB, TILE = L::TILE, NB = L::NB, R = CHUNK_R;
+    constexpr int NL = CHUNK_KEYS * CH / CHUNK_THREADS;        // chunks of K (and of V) per thread and tile
+    const int tid = own_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
-    const int D = a.kv.D, index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads);
-    const int h = (int)blockIdx.x - index * a.kv.kv_heads;
+    const bool second = wave >= 4;
+    const int D = a.kv.D;
     PagedItem it;
-    if (!paged_find<R, true, false>(a, index, &it)) return;
+    if (!paged_locate<R, true>(a, unit, index, &it)) return;
     const PagedSpan sp = it.span;
     const int rows_f = sp.n * a.group;
-    const int tile_f = it.tile * R, wave_f = tile_f + 32 * RW * wave;
+    const int tile_f = it.tile * R, wave_f = tile_f + 32 * wave;
     const int k_begin = it.split * it.unit;
     const int k_end = min(k_begin + it.unit, sp.visible(min(tile_f + R - 1, rows_f - 1) / a.group));
-    if (it.split > 0 && k_begin >= k_end) return;              // the combine knows (paged_combine_kernel)
+    if (it.split > 0 && k_begin >= k_end) return;              // the merge counts on it (paged_merge)
     const int wave_open = wave_f < rows_f ? sp.visible(wave_f / a.group) : 0;   // keys below it are visible to all the wave's rows
-    const int wave_end = wave_f < rows_f ? min(k_end, sp.visible(min(wave_f + 32 * RW - 1, rows_f - 1) / a.group)) : 0;
+    const int wave_end = wave_f < rows_f ? min(k_end, sp.visible(min(wave_f + 31, rows_f - 1) / a.group)) : 0;
 
-    u32x4 qf[RW][KS];
-    int last[RW];                                              // keys below it are visible to the lane's row
+    const int f = wave_f + l32, fj = f / a.group, fg = f - fj * a.group;
+    const int last = f < rows_f ? sp.visible(fj) : 0;          // keys below it are visible to the lane's row
+    u32x4 qf[KS];
 #pragma unroll
-    for (int t = 0; t < RW; ++t) {
-        const int f = wave_f + 32 * t + l32, j = f / a.group, g = f - j * a.group;
-        last[t] = f < rows_f ? sp.visible(j) : 0;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = 16 * s + 8 * h2;
-            qf[t][s] = u32x4{0u, 0u, 0u, 0u};
-            if (f < rows_f && d < D)
-                qf[t][s] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(sp.row0 + j) * a.heads + h * a.group + g) * D + d);
-        }
+    for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * h2;
+        qf[s] = u32x4{0u, 0u, 0u, 0u};
+        if (f < rows_f && d < D)
+            qf[s] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(sp.row0 + fj) * a.heads + h * a.group + fg) * D + d);
     }
-
-    // the chunks of a row past head_dim: K's are contracted with Q's zeros, and no load reaches them
-    if (D < 8 * CH) {
-        for (int i = (int)threadIdx.x; i < 4 * TILE / 16; i += 256) *reinterpret_cast<u32x4*>(lds + 16 * i) = u32x4{0u, 0u, 0u, 0u};
-        __syncthreads();
-    }
-
+    for (int i = tid; i < TILE / 16; i += CHUNK_THREADS) *reinterpret_cast<u32x4*>(lds + L::ZEROS + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    const int n = (max(k_end - k_begin, 0) + CHUNK_KEYS - 1) / CHUNK_KEYS;
+    // where the part-th SLOT_KEYS keys are, in 16-byte chunks of the cache (below 2^32, checked
+    // on the host) or NOWHERE, into their half of the buffer
     const int* table = a.batch.table + (int64_t)it.seq * a.batch.width;
-    // slot of key kv0 + lane, -1 where there is none
-    auto find_slot = [&](int kv0) {
-        const int key = kv0 + lane;
-        if (key >= k_end) return -1;
-        const int pi = a.kv.page.quotient(key), page = table[pi];
-        return page >= 0 && page < a.kv.num_pages ? a.kv.slot(page, h, key - pi * a.kv.page.div) : -1;
+    uint32_t* slots = (uint32_t*)(lds + L::SLOTS);
+    auto find_slots = [&](int part) {
+#pragma unroll
+        for (int u = 0; u < SLOT_KEYS / CHUNK_THREADS; ++u) {
+            const int i = u * CHUNK_THREADS + tid, key = k_begin + part * SLOT_KEYS + i;
+            uint32_t at = NOWHERE;
+            if (key < k_end) {
+                const int pi = a.kv.page.quotient(key), page = table[pi];
+                if (page >= 0 && page < a.kv.num_pages)
+                    at = (uint32_t)a.kv.slot(page, h, key - pi * a.kv.page.div) * (uint32_t)(D / 8);
+            }
+            slots[(part & 1) * SLOT_KEYS + i] = at;
+        }
     };
+    find_slots(0);
+    __syncthreads();
+
     const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_offset(lds));
-    auto load_tile = [&](int buf, int slot) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int first = 64 * wave + 256 * i;             // this wave's chunks first .. +63
-            const int key = (first + lane) / CH, c = (first + lane) % CH;
-            const int sl = __shfl(slot, key, 64);
-            const int ck = c ^ key_swizzle<CH>(key), cv = c ^ value_swizzle<CH>(key);
-            const uint16_t* k = sl >= 0 ? a.kv.k + (int64_t)sl * D + 8 * ck : (const uint16_t*)&paged_zeros;
-            const uint16_t* v = sl >= 0 ? a.kv.v + (int64_t)sl * D + 8 * cv : (const uint16_t*)&paged_zeros;
-            const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 2 * buf * TILE + 16 * first));
-            if (8 * ck < D) asm_global_load_lds_b128(k, to);
-            if (8 * cv < D) asm_global_load_lds_b128(v, to + TILE);
-        }
+    // this wave's l-th 64 chunks of a tile: chunk 64 wave + 512 l + lane
+    const int chunk = 64 * wave + lane, wave_lds = lds0 + 1024 * wave;
+    auto slot_of = [&](int tile, int l) {
+        return slots[(uint32_t)(tile * CHUNK_KEYS + (chunk + CHUNK_THREADS * l) / CH) % (2 * SLOT_KEYS)];
     };
+    auto load_chunks = [&](const uint16_t* from, uint32_t slot, int l, uint32_t to, bool keys) {
+        const int key = (chunk + CHUNK_THREADS * l) / CH, c = (chunk + CHUNK_THREADS * l) % CH;
+        const uint32_t cs = c ^ (keys ? key_swizzle<CH>(key) : value_swizzle<CH>(key));
+        const uint64_t p = (uint64_t)(uintptr_t)from + 16 * (uint64_t)(slot + cs), zeros = (uint64_t)(uintptr_t)&paged_zeros;
+        asm_global_load_lds_b128((const void*)(uintptr_t)(slot != NOWHERE && 8 * (int)cs < D ? p : zeros),
+                                 (uint32_t)wave_lds + to + 16 * CHUNK_THREADS * l);
+    };
+    // K of tile i + NB - 1 and V of tile i + NB - 2 go into the buffers that phases 2i and
+    // 2i + 1 do not read: of the ring, before tile i's and two before it.  A wave asks for
+    // its 2 NL pieces of them between the products of its phase (a load takes the memory
+    // pipeline some 100 cycles to accept), past the last tile too (of zeros or of keys
+    // nobody reads), so that a count of them says which are done.
+    auto before = [](int ring) { return ring ? ring - 1 : NB - 1; };
+    auto piece = [&](int ring, int j, uint32_t slot) {
+        const int k_ring = before(ring), v_ring = before(k_ring);
+        if (j < NL) load_chunks(a.kv.k, slot, j, k_ring * TILE, true);
+        else load_chunks(a.kv.v, slot, j - NL, L::V + v_ring * TILE, false);
+    };
+    auto next_slots = [&](int i) {
+        // half a part ahead: the slots of the next one, in the half whose tiles are done
+        constexpr int PART = SLOT_KEYS / CHUNK_KEYS;
+        const int tv = i + NB - 2;
+        if (tv % PART == PART / 2 && (tv / PART + 1) * PART <= n + NB) find_slots(tv / PART + 1);
+    };
+    // where this lane reads: K chunk 2 st + h2 of key l32, V at key 4 h2 + (lane & 15) / 4
+    // and dims 32 t + 16 ((lane / 16) & 1) + 4 (lane & 3); st and t are one exclusive or
+    // in the row (32 st, 64 t), and the swizzles do not change with the multiples of 32
+    // and 8 keys that the reads add
+    const int vkey = 4 * h2 + ((lane & 15) >> 2), vdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint32_t kat = lds0 + l32 * PB + 16 * (h2 ^ key_swizzle<CH>(l32));
+    const uint32_t vat = lds0 + L::V + vkey * PB + 2 * (vdim & 7) + 16 * ((vdim >> 3) ^ value_swizzle<CH>(vkey));
 
-    float mrun[RW], lrun[RW];                                  // lrun: this lane's keys only
-    f32x16 oacc[RW][DT];
+    float mrun = -INFINITY, lrun = 0.0f;                       // lrun: this lane's keys only
+    f32x16 oacc[DT], s[2];
+    u32x4 pb[PP][4] = {};                                      // P of the tile before, 16 keys each
 #pragma unroll
-    for (int t = 0; t < RW; ++t) {
-        mrun[t] = -INFINITY;
-        lrun[t] = 0.0f;
+    for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) oacc[t][i][r] = 0.0f;
-    }
+        for (int r = 0; r < 16; ++r) oacc[i][r] = 0.0f;
+    bool partial = false;                                      // some of the wave's rows see only part of that tile
 
-    int slot = find_slot(k_begin);
-    if (k_begin < k_end) load_tile(0, slot);
-    int slot_next = find_slot(k_begin + CHUNK_KEYS);
-    int buf = 0;
-    for (int kv0 = k_begin; kv0 < k_end; kv0 += CHUNK_KEYS, buf ^= 1) {
-        const uint64_t gone = __builtin_amdgcn_ballot_w64(slot < 0);
-        asm_wait_vmcnt<0>();
-        __syncthreads();                                       // this tile is in LDS, and the one before is done with
-        slot = slot_next;
-        if (kv0 + CHUNK_KEYS < k_end) load_tile(buf ^ 1, slot);
-        slot_next = find_slot(kv0 + 2 * CHUNK_KEYS);
-        if (kv0 >= wave_end) continue;
-        const uint8_t* kt = lds + 2 * buf * TILE;
-        const uint8_t* vt = kt + TILE;
-
-        f32x16 s[RW][2];
+    // Where tile i's values are read for the second product; the slow path makes it itself.
+    auto values_at = [&](int i, int ring) {
+        uint32_t base = vat + ring * TILE;
+        if (partial) {
+            const uint8_t* vt = lds + L::V + ring * TILE;
+            uint32_t bad = 0;
+            for (int c = lane; c < TILE / 16; c += 64) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(vt + 16 * c);
+                const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+                if (8 * ((c % CH) ^ value_swizzle<CH>(c / CH)) < D)
 #pragma unroll
-        for (int t = 0; t < RW; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[t][u][r] = 0.0f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                const int key = 32 * u + l32;
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + key * PB + 16 * ((2 * st + h2) ^ key_swizzle<CH>(key)));
-#pragma unroll
-                for (int t = 0; t < RW; ++t) s[t][u] = mfma32<BF>(kf, qf[t][st], s[t][u]);
+                    for (int x = 0; x < 4; ++x) bad |= (w[x] & e) == e || ((w[x] >> 16) & e) == e;
             }
-        if (gone || kv0 + CHUNK_KEYS > wave_open) {
-            asm volatile("");                                  // a branch: few tiles need this
+            if (__builtin_amdgcn_ballot_w64(bad)) {
+                float* pw = (float*)(lds + L::P + wave * L::P_WAVE);       // [32 keys][32 rows]
 #pragma unroll
-            for (int t = 0; t < RW; ++t)
+                for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                    for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = 32 * u + 8 * (r >> 2) + 4 * h2 + (r & 3);
-                        if (kv0 + i >= last[t] || ((gone >> i) & 1u)) s[t][u][r] = -INFINITY;
+                        for (int e = 0; e < 8; ++e) {
+                            float p = 0.0f;
+#pragma unroll
+                            for (int w = 0; w < PP; ++w) p += bits_to_f32<std::conditional_t<BF, __hip_bfloat16, __half>>((uint16_t)(pb[w][2 * u + k][e >> 1] >> (16 * (e & 1))));
+                            pw[(16 * k + 8 * (e >> 2) + 4 * h2 + (e & 3)) * 32 + l32] = p;
+                        }
+                    asm_wait_lgkmcnt<0>();
+                    for (int key = 0; key < 32; ++key) {
+                        const float p = pw[key * 32 + l32];
+                        if (k_begin + i * CHUNK_KEYS + 32 * u + key >= last) continue;
+#pragma unroll
+                        for (int t = 0; t < DT; ++t)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int c = (4 * t + q) ^ value_swizzle<CH>(key);
+                                const u32x2 w = *reinterpret_cast<const u32x2*>(vt + (32 * u + key) * PB + 16 * c + 8 * h2);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float v = bits_to_f32<std::conditional_t<BF, __hip_bfloat16, __half>>((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+                                    oacc[t][4 * q + e] = __builtin_fmaf(p, v, oacc[t][4 * q + e]);
+                                }
+                            }
                     }
-        }
-#pragma unroll
-        for (int t = 0; t < RW; ++t) {
-            float tmax = s[t][0][0];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[t][u][r]);
-            tmax *= a.scale_log2;
-            if (__builtin_amdgcn_ballot_w64(tmax > mrun[t] + 8.0f)) {
-                const float mnew = fmaxf(mrun[t], fmaxf(tmax, __shfl_xor(tmax, 32, 64)));
-                const float factor = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun[t] - mnew);
-                lrun[t] *= factor;
-#pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) oacc[t][i][r] *= factor;
-                mrun[t] = mnew;
+                    asm_wait_lgkmcnt<0>();
+                }
+                base = vat - L::V + L::ZEROS;                  // what follows adds zeros
             }
-            const float msafe = mrun[t] == -INFINITY ? 0.0f : mrun[t];
+        }
+        return base;
+    };
+    // The products of a phase: O^T += V^T P^T of tile i - 1 in four steps of 16 keys, then S^T =
+    // K Q^T of tile i in steps of 32 dims.  A step's fragments are read from LDS AHEAD steps
+    // before they are multiplied.
+    // Both are always made, a branch around either would cost copies of the accumulators:
+    // without a tile before, from values of zero (pv false), and behind the last tile into
+    // scores that nobody reads.
+    auto products = [&](int i, int ring, bool pv) {
+        constexpr int PV = 4, STEPS = PV + (KS + 1) / 2;
+        constexpr int AHEAD = DT > 2 ? 1 : 3, SETS = AHEAD + 1;
+        const uint32_t v_at = pv ? values_at(i - 1, before(ring)) : vat - L::V + L::ZEROS, k_at = kat + ring * TILE;
+        const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t slot[2 * NL];
+        u32x4 frag[SETS][4];
+        auto read = [&](auto step) {
+            constexpr int st = decltype(step)::value;
+            if constexpr (st < PV) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int t = 0; t < DT; ++t) {
+                    const uint32_t at = (v_at ^ (64 * t)) + 16 * st * PB;
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + 8 * PB)));
+                    frag[st % SETS][t] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                }
+            } else if constexpr (st < STEPS) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (2 * (st - PV) + e < KS)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            frag[st % SETS][2 * e + u] = *(const lds_u32x4*)(uintptr_t)((k_at ^ (32 * (2 * (st - PV) + e))) + 32 * u * PB);
+            }
+        };
+        static_for<AHEAD>(read);
+#pragma unroll
+        for (int j = 0; j < 2 * NL; ++j) slot[j] = slot_of(i + NB - 1 - j / NL, j % NL);
+        static_for<STEPS>([&](auto step) {
+            constexpr int st = decltype(step)::value;
+            read(std::integral_constant<int, st + AHEAD>{});
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (st < PV) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) oacc[t] = mfma32<BF>(frag[st % SETS][t], pb[0][st], oacc[t]);
+                if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
+#pragma unroll
+                for (int w = 1; w < PP; ++w)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) oacc[t] = mfma32<BF>(frag[st % SETS][t], pb[w][st], oacc[t]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (2 * (st - PV) + e < KS)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int d = 2 * (st - PV) + e;
+                            s[u] = mfma32<BF>(frag[st % SETS][2 * e + u], qf[d], d == 0 ? zero : s[u]);
+                        }
+                if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
+            }
+        });
+    };
+    auto softmax = [&](int i) {
+        const int kv0 = k_begin + i * CHUNK_KEYS;
+        const uint64_t hidden = __builtin_amdgcn_ballot_w64(slots[(uint32_t)(i * CHUNK_KEYS + lane) % (2 * SLOT_KEYS)] == NOWHERE);
+        partial = kv0 + CHUNK_KEYS > wave_open && wave_open < wave_end;
+        if (hidden || kv0 + CHUNK_KEYS > wave_open) {
+            asm volatile("");                                  // a branch: few tiles need this
+            const int seen = last - kv0 - 4 * h2;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t hid = (uint32_t)(hidden >> (32 * u)) >> (4 * h2);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[t][u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][r], a.scale_log2, -msafe));
-                    lrun[t] += s[t][u][r];
+                    const int key = 8 * (r >> 2) + (r & 3);    // and 32 u + 4 h2
+                    if (32 * u + key >= seen || (hid & (1u << key))) s[u][r] = -INFINITY;
                 }
+            }
         }
+        float tmax = s[0][0];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                u32x4 pb[RW][PP];
+            for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[u][r]);
+        tmax *= a.scale_log2;
+        if (__builtin_amdgcn_ballot_w64(tmax > mrun + 8.0f)) {
+            const float mnew = fmaxf(mrun, fmaxf(tmax, __shfl_xor(tmax, 32, 64)));
+            const float factor = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+            lrun *= factor;
 #pragma unroll
-                for (int t = 0; t < RW; ++t) {
-                    float p[8];
+            for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = s[t][u][8 * kk + e];
+                for (int r = 0; r < 16; ++r) oacc[t][r] *= factor;
+            mrun = mnew;
+        }
+        const float msafe = mrun == -INFINITY ? 0.0f : mrun;
 #pragma unroll
-                    for (int w = 0; w < PP; ++w)
+        for (int k = 0; k < 4; ++k) {
+            float p[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) pb[t][w][e] = round2<BF, true>(p[2 * e], p[2 * e + 1]);
-                }
-                // this lane's address: key 4 h2 + (lane & 15) / 4 of the step, dims 16 ((lane / 16) & 1) + 4 (lane & 3)
-                const int key = 32 * u + 16 * kk + 4 * h2 + ((lane & 15) >> 2);
-                const int dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                const uint8_t* vk = vt + key * PB + 2 * (dim & 7);
-#pragma unroll
-                for (int i = 0; i < DT; ++i) {
-                    const int c = (4 * i + (dim >> 3)) ^ value_swizzle<CH>(key);   // the same for key + 8
-                    lds_i16x4* p0 = (lds_i16x4*)(uintptr_t)lds_offset(vk + 16 * c);
-                    lds_i16x4* p1 = (lds_i16x4*)(uintptr_t)lds_offset(vk + 16 * c + 8 * PB);
-                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1));
-#pragma unroll
-                    for (int t = 0; t < RW; ++t)
-#pragma unroll
-                        for (int w = 0; w < PP; ++w) oacc[t][i] = mfma32<BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[t][w], oacc[t][i]);
-                }
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], a.scale_log2, -msafe));
+                lrun += p[e];
             }
-    }
+#pragma unroll
+            for (int w = 0; w < PP; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pb[w][k][e] = round2<BF, true>(p[2 * e], p[2 * e + 1]);
+        }
+    };
 
 #pragma unroll
-    for (int t = 0; t < RW; ++t) {
-        const float sum = lrun[t] + __shfl_xor(lrun[t], 32, 64);
-        const int f = wave_f + 32 * t + l32;
-        if (f >= rows_f) continue;
-        if (it.record >= 0) {
-            float* wo = paged_ws_out<R>(a, it.record + it.split, h) + (int64_t)(f - tile_f) * D;
+    for (int t = 0; t < NB - 1; ++t)
 #pragma unroll
-            for (int i = 0; i < DT; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int d = 32 * i + 8 * q + 4 * h2;
-                    if (d < D)
-                        *reinterpret_cast<f32x4*>(wo + d) = f32x4{oacc[t][i][4 * q], oacc[t][i][4 * q + 1], oacc[t][i][4 * q + 2], oacc[t][i][4 * q + 3]};
-                }
-            if (h2 == 0) paged_ws_ml<R, true>(a, it.record + it.split, h)[f - tile_f] = f32x2{mrun[t], sum};
-            continue;
+        for (int l = 0; l < NL; ++l) {
+            load_chunks(a.kv.k, slot_of(t, l), l, t * TILE, true);
+            if (t < NB - 2) load_chunks(a.kv.v, slot_of(t, l), l, L::V + t * TILE, false);
         }
+    asm_wait_vmcnt<0>();
+    phase_barrier();
+    if (second) phase_barrier();                               // phase 0 of waves 4..7
+    for (int i = 0, ring = 0; i <= n; ++i, ring = ring == NB - 1 ? 0 : ring + 1) {
+        next_slots(i);
+        __builtin_amdgcn_s_setprio(1);
+        products(i, ring, i > 0 && k_begin + (i - 1) * CHUNK_KEYS < wave_end);
+        __builtin_amdgcn_s_setprio(0);
+        // what this wave asked for NB - 2 iterations ago has arrived: K of tile i + 1 and V of tile i
+        if (second) asm_wait_vmcnt<(NB - 2) * 2 * NL>();
+        phase_barrier();
+        if (i < n && k_begin + i * CHUNK_KEYS < wave_end) softmax(i);
+        if (!second) asm_wait_vmcnt<(NB - 2) * 2 * NL>();
+        phase_barrier();
+    }
+    if (!second) phase_barrier();
+    asm_wait_vmcnt<0>();                                       // loads past the last tile write LDS that is about to be reused
+
+    const float sum = lrun + __shfl_xor(lrun, 32, 64);
+    if (f < rows_f) {
+        const PagedParts<R> parts(a, a.many, h);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int d = 32 * i + 8 * q + 4 * h2;
-                if (d < D)
-                    paged_store4<BF>(a, sp, h, f, d, f32x4{oacc[t][i][4 * q] * inv, oacc[t][i][4 * q + 1] * inv,
-                                                           oacc[t][i][4 * q + 2] * inv, oacc[t][i][4 * q + 3] * inv});
+                const int d = 32 * t + 8 * q + 4 * h2;
+                const f32x4 o = {oacc[t][4 * q], oacc[t][4 * q + 1], oacc[t][4 * q + 2], oacc[t][4 * q + 3]};
+                if (d >= D) continue;
+                if (it.record >= 0) parts.store_out(it.record + it.split, f - tile_f, d, o);
+                else paged_store4<BF>(a, sp, h, f, d, o * inv);
             }
+        if (it.record >= 0 && h2 == 0) parts.store_ml(it.record + it.split, f - tile_f, mrun, sum);
+    }
+    if (it.record >= 0) paged_merge<BF, R, CHUNK_THREADS>(a, a.many, it, h, (uint32_t*)lds);
+}
+
+template <int KS, int DT, bool BF, int PP>
+__global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int kv_heads = a.kv.kv_heads, q = (int)blockIdx.x % PAGED_QUEUES, own = (int)blockIdx.x / PAGED_QUEUES;
+    const int blocks = ((int)gridDim.x - q + PAGED_QUEUES - 1) / PAGED_QUEUES;              // of this queue
+    const PagedShare many = paged_share<CHUNK_R, true>(a), few = paged_share<PAGED_R, false>(a);
+    const int many_items = (many.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
+    const int all_items = many_items + (few.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
+    for (int round = 0; round * blocks < all_items; ++round) {
+        const int i = round * blocks + (round & 1 ? blocks - 1 - own : own);
+        if (i < many_items) {
+            const int w = i * PAGED_QUEUES + q, index = w / kv_heads;
+            paged_chunk_item<KS, DT, BF, PP>(a, many.unit, index, w - index * kv_heads, lds);
+        } else if (i < all_items) {
+            const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
+            paged_few_item<DT, BF, PP, 8>(a, few.unit, index, w - index * kv_heads, lds);
+        }
+        __syncthreads();                                       // LDS is free
     }
 }
 
 template <int KS, int DT, bool BF, int PP>
-static void launch_many(PagedLaunch& go) {
-    if (go.a.many.tile == 256) {
-        go(paged_chunk_kernel<KS, DT, BF, PP, 2>, go.a.many.items);
-        go(paged_combine_kernel<BF, 256, true>, go.a.many.tiles);
-    } else {
-        go(paged_chunk_kernel<KS, DT, BF, PP, 1>, go.a.many.items);
-        go(paged_combine_kernel<BF, 128, true>, go.a.many.tiles);
-    }
+static hipError_t launch_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
+    constexpr int few = 8 * PagedLayout<DT>::REGION + 16, bytes = ChunkLayout<DT>::BYTES > few ? ChunkLayout<DT>::BYTES : few;
+    if (const hipError_t e = allow_dynamic_lds<paged_chunk_kernel<KS, DT, BF, PP>>(bytes); e != hipSuccess) return e;
+    const int64_t most = ((int64_t)a.many.items + a.few.items) * a.kv.kv_heads;
+    launch_kernel(paged_chunk_kernel<KS, DT, BF, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),
+                  (uint32_t)bytes, s, a);
+    return hipGetLastError();
 }
 
 template <int KS, int DT>
-static void launch_many_dims(PagedLaunch& go) {
-    const bool wide = go.a.o_dtype == MVLM_F32;
-    if (go.a.kv.dtype == MVLM_F16) {
-        if (wide) launch_many<KS, DT, false, 2>(go);
-        else launch_many<KS, DT, false, 1>(go);
-    } else {
-        if (wide) launch_many<KS, DT, true, 3>(go);
-        else launch_many<KS, DT, true, 1>(go);
-    }
+static hipError_t launch_chunk_dims(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
+    const bool wide = a.o_dtype == MVLM_F32;
+    if (a.kv.dtype == MVLM_F16) return wide ? launch_chunk<KS, DT, false, 2>(s, a, num_cus) : launch_chunk<KS, DT, false, 1>(s, a, num_cus);
+    return wide ? launch_chunk<KS, DT, true, 3>(s, a, num_cus) : launch_chunk<KS, DT, true, 1>(s, a, num_cus);
 }
 
-void launch_attention_paged_chunk(PagedLaunch& go) {
-    const int D = go.a.kv.D;
-    if (D <= 32) launch_many_dims<2, 1>(go);
-    else if (D <= 64) launch_many_dims<4, 2>(go);
-    else if (D <= 80) launch_many_dims<5, 3>(go);
-    else if (D <= 96) launch_many_dims<6, 3>(go);
-    else launch_many_dims<8, 4>(go);
+hipError_t launch_attention_paged_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
+    const int D = a.kv.D;
+    if (D <= 32) return launch_chunk_dims<2, 1>(s, a, num_cus);
+    if (D <= 64) return launch_chunk_dims<4, 2>(s, a, num_cus);
+    if (D <= 80) return launch_chunk_dims<5, 3>(s, a, num_cus);
+    if (D <= 96) return launch_chunk_dims<6, 3>(s, a, num_cus);
+    return launch_chunk_dims<8, 4>(s, a, num_cus);
 }
 
 }  // namespace mvlm

@@ -33,14 +33,17 @@ struct mvlm_device {
     // that allocate nothing; resolved at device creation.
     void* noalloc_scratch = nullptr;
     // Words of self-resetting cross-workgroup protocols (the split token
-    // pick's per-row best key and arrival count): zero between launches, each
-    // launch's last workgroup setting its words back.  Ops of one handle run in
+    // pick's per-row best key and arrival count, the paged attention's counts
+    // of finished splits): zero between launches, each launch's last workgroup
+    // setting its words back.  Ops of one handle run in
     // order on its stream, so they never share a word.  Allocated and zeroed
     // at the first op that needs them.
     void* sync_words = nullptr;
 };
 constexpr int ARGMAX_SYNC_ROWS = 64;                                   // rows of split token picks
-constexpr size_t SYNC_WORDS_BYTES = ARGMAX_SYNC_ROWS * (8 + 4);
+constexpr size_t ARGMAX_SYNC_BYTES = ARGMAX_SYNC_ROWS * (8 + 4);
+constexpr int PAGED_SYNC_WORDS = 8192;                                 // splits' counters of the paged attention
+constexpr size_t SYNC_WORDS_BYTES = ARGMAX_SYNC_BYTES + PAGED_SYNC_WORDS * 4;
 
 struct mvlm_buffer {
     mvlm_device* dev = nullptr;

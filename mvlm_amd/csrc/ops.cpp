@@ -315,10 +315,14 @@ int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, Pag
             in->kv_heads, in->head_dim);
     if (in->head_dim % 8 != 0 || in->head_dim > 128)
         return set_error(MVLM_ERR_UNSUPPORTED, "%s: head_dim=%d must be a multiple of 8 and at most 128", fn, in->head_dim);
+    if (in->kv_heads > PAGED_MAX_KV_HEADS)
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: kv_heads=%d is above %d", fn, in->kv_heads, PAGED_MAX_KV_HEADS);
     const int64_t per_head = (int64_t)in->num_pages * in->page_size;
     if (per_head > INT_MAX / in->kv_heads)
         return set_error(MVLM_ERR_UNSUPPORTED, "%s: %d pages of %d positions of %d heads are 2^31 slots or more", fn,
                          in->num_pages, in->page_size, in->kv_heads);
+    if (per_head * in->kv_heads * (in->head_dim / 8) >= ((int64_t)1 << 32) - 16)
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: K and V of 64 GiB or more", fn);
     const size_t bytes = (size_t)per_head * in->kv_heads * in->head_dim * 2;
     REQUIRE(aligned16(in->k->ptr) && aligned16(in->v->ptr), "%s: K and V must be 16-byte aligned", fn);
     NEED(in->k, bytes, "K");
@@ -450,12 +454,25 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     a.heads = num_heads;
     a.group = num_heads / a.kv.kv_heads;
     a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)a.kv.D) : scale) * 1.4426950408889634f;
-    op->workspace_bytes = plan_attention_paged(&a, dev->prop.multiProcessorCount);
+    plan_attention_paged(&a, dev->prop.multiProcessorCount);
     REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads <= (1 << 30), "%s: shape too large", fn);
+    // the shares run in one launch: partial results and counters of their own
+    const size_t few = (paged_ws_bytes(a, a.few) + 255) & ~(size_t)255, many = paged_ws_bytes(a, a.many);
+    const size_t few_words = paged_words(a, a.few), words = few_words + paged_words(a, a.many);
+    if (words > PAGED_SYNC_WORDS)
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: %zu counters are needed, the device has %d", fn, words, PAGED_SYNC_WORDS);
+    op->workspace_bytes = few + many;
     st = device_scratch(dev, op->workspace_bytes, &op->workspace);
-    a.ws = (float*)op->workspace;
+    void* sync = nullptr;
+    if (st == MVLM_OK) st = device_sync_words(dev, &sync);
+    if (st != MVLM_OK) return st;
+    a.few.ws = (float*)op->workspace;
+    a.many.ws = (float*)((char*)op->workspace + few);
+    a.few.arrived = (uint32_t*)((char*)sync + ARGMAX_SYNC_BYTES);
+    a.many.arrived = a.few.arrived + few_words;
+    op->num_cus = dev->prop.multiProcessorCount;
     op->kind = OP_ATTN_PAGED;
-    return st;
+    return MVLM_OK;
 }
 
 int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
@@ -685,7 +702,7 @@ hipError_t enqueue_op(hipStream_t s, const Op& op, bool with_attn = false) {
         case OP_KV_APPEND:
             return launch_kv_append(s, op.append);
         case OP_ATTN_PAGED:
-            return launch_attention_paged(s, op.paged);
+            return launch_attention_paged(s, op.paged, op.num_cus);
         case OP_LOGITS:
             return launch_logits(s, op.logits, op.num_cus);
     }

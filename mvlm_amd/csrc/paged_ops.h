@@ -25,11 +25,14 @@ struct PagedDivision {
     int tile;                      // f-rows per tile; 0: no sequence is this kernel's
     int64_t blocks_per_head;       // blocks wanted per kv head
     int unit_min, unit_step;       // least keys per block, and what a block's keys are a multiple of
-    int items;                     // grid: upper bound of the items per kv head
-    int tiles;                     // upper bound of the tiles per kv head
-    int records;                   // room in the workspace, in tiles
+    int items;                     // upper bound of the items per kv head
+    int records;                   // room in the workspace, in tiles per kv head
+    float* ws;                     // partial results of split tiles
+    uint32_t* arrived;             // [records][kv_heads] splits that are done, zero between launches
 };
 constexpr int PAGED_FEW = 64;
+constexpr int PAGED_QUEUES = 8;        // one per XCD: their blocks share an L2
+constexpr int PAGED_MAX_KV_HEADS = 1024;
 
 struct PagedAttnArgs {
     PagedSeqs batch;
@@ -38,16 +41,18 @@ struct PagedAttnArgs {
     void* o;                       // [rows][heads][D]
     int o_dtype, heads, group;     // group: heads per kv head
     float scale_log2;              // scale * log2(e)
-    float* ws;                     // partial results of split tiles
     // division of the work (attention_paged.hip) of the sequences with few new
     // rows, f = n group <= PAGED_FEW, and of those with more
     PagedDivision few, many;
 };
 
 hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a);
-// Fills a's division of the work for a device; returns the workspace it needs.
-size_t plan_attention_paged(PagedAttnArgs* a, int num_cus);
-hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a);
+// Fills a's division of the work for a device, all but its memory.
+void plan_attention_paged(PagedAttnArgs* a, int num_cus);
+// Bytes of partial results and words of counters of a share; placing them.
+size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d);
+size_t paged_words(const PagedAttnArgs& a, const PagedDivision& d);
+hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a, int num_cus);
 
 #if defined(__HIPCC__)
 
@@ -116,29 +121,51 @@ __device__ __forceinline__ PagedSpan paged_lane_span(const PagedSeqs& b, int s) 
                        : paged_span(s, s + 1, b.kv_len[s], b.rows, b.positions);
 }
 
-// The index-th item of the batch (TILES: the index-th tile, split 0), the same in
-// all lanes; false past the last one.
-template <int R, bool MANY, bool TILES>
-__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int index, PagedItem* out) {
+// A share's keys per block and its items per kv head, the same in all lanes.
+struct PagedShare {
+    int unit, items;
+};
+__device__ __forceinline__ int paged_splits(int len, int unit) { return len > unit ? (len + unit - 1) / unit : 1; }
+
+template <int R, bool MANY>
+__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     const PagedSeqs& b = a.batch;
     const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
-    PagedSpan sp = paged_lane_span(b, lane);
+    const PagedSpan sp = paged_lane_span(b, lane);
     int64_t total = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
         total += (int64_t)paged_tiles<R, MANY>(p, a.group) * p.len;
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
-    const int unit = paged_unit(div, total);
+    // summed over the lanes as two numbers of 24 and 30 bits; read from one lane, so that
+    // no branch on it is taken as divergent
+    const int64_t lo = __builtin_amdgcn_readlane(wave_scan((int)(total & 0xFFFFFF)), 63);
+    const int64_t hi = __builtin_amdgcn_readlane(wave_scan((int)(total >> 24)), 63);
+    PagedShare sh;
+    sh.unit = paged_unit(div, (hi << 24) + lo);
+    int items = 0;
+    for (int base = 0; base < b.seqs; base += 64) {
+        const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
+        items += paged_tiles<R, MANY>(p, a.group) * paged_splits(p.len, sh.unit);
+    }
+    items = __builtin_amdgcn_readlane(wave_scan(items), 63);
+    // no more than planned for, whatever row_start holds
+    sh.items = items < 0 || items > div.items ? div.items : items;
+    return sh;
+}
+
+// The index-th item of a share, the same in all lanes; false if there is none.
+template <int R, bool MANY>
+__device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, int unit, int index, PagedItem* out) {
+    const PagedSeqs& b = a.batch;
+    const PagedDivision& div = MANY ? a.many : a.few;
+    const int lane = (int)(threadIdx.x & 63);
     int first = 0, record = 0;                             // items and records before this round of sequences
     for (int base = 0; base < b.seqs; base += 64) {
-        if (base) sp = paged_lane_span(b, base + lane);
-        const int tiles = paged_tiles<R, MANY>(sp, a.group);
-        int splits = (sp.len + unit - 1) / unit;
-        if (splits < 1) splits = 1;
-        const int items = TILES ? tiles : tiles * splits, records = splits > 1 ? tiles * splits : 0;
+        const PagedSpan sp = paged_lane_span(b, base + lane);
+        const int tiles = paged_tiles<R, MANY>(sp, a.group), splits = paged_splits(sp.len, unit);
+        const int items = tiles * splits, records = splits > 1 ? tiles * splits : 0;
         const int end = first + wave_scan(items), rec_end = record + wave_scan(records);
         const uint64_t mine = __builtin_amdgcn_ballot_w64(index >= end - items && index < end);
         if (mine) {
@@ -148,11 +175,12 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int index, Pa
             out->span = PagedSpan{at(sp.row0), at(sp.n), at(sp.held), at(sp.len)};
             out->unit = unit;
             const int ns = at(splits), r = index - at(end - items);
-            out->tile = TILES ? r : r / ns;
-            out->split = TILES ? 0 : r - out->tile * ns;
-            out->record = ns > 1 ? at(rec_end - records) + out->tile * ns : -1;
+            const int nth = r / ns;
+            out->tile = at(tiles) - 1 - nth;               // the last tile sees the most keys: it starts first
+            out->split = r - nth * ns;
+            out->record = ns > 1 ? at(rec_end - records) + nth * ns : -1;
             // a batch whose starts decrease can exceed the items and records planned for: refused here
-            return out->tile < at(tiles) && (ns == 1 || (out->record >= 0 && out->record <= div.records - ns));
+            return out->tile >= 0 && (ns == 1 || (out->record >= 0 && out->record <= div.records - ns));
         }
         first = __builtin_amdgcn_readlane(end, 63);
         record = __builtin_amdgcn_readlane(rec_end, 63);

@@ -108,6 +108,8 @@ static void test_paged_refusals() {
     refuses(NOT, "head_dim 60", [](Append& a) { a.kv.head_dim = 60; });
     refuses(NOT, "head_dim 136", [](Append& a) { a.kv.head_dim = 136; });
     refuses(NOT, "2^31 slots", [](Append& a) { a.kv.num_pages = 1 << 25; });
+    refuses(NOT, "64 GiB of keys", [](Append& a) { a.kv.num_pages = 1 << 22, a.kv.head_dim = 128, a.k.bytes = a.v.bytes = SIZE_MAX; });
+    refuses(NOT, "1025 kv heads", [](Append& a) { a.kv.kv_heads = 1025; });
     refuses(SMALL, "cache too small", [](Append& a) { a.k.bytes = 16 * 16 * 4 * 64 * 2 - 1; });
     refuses(SMALL, "v too small", [](Append& a) { a.v.bytes = 16 * 16 * 4 * 64 * 2 - 1; });
     refuses(BAD, "misaligned cache", [](Append& a) { a.k = buffer(1 << 20, 0x10000008); });
