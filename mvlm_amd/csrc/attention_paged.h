@@ -95,7 +95,7 @@ __device__ __forceinline__ void paged_merge(const PagedAttnArgs& a, const PagedD
     const PagedParts<R> parts(a, div, h);
     const int d4 = D / 4;
     // a thread's share, ITEMS quads of outputs at a time, SPLITS splits of them asked for together
-    constexpr int ITEMS = R > 16 ? 4 : 1, SPLITS = R > 16 ? 2 : 8;
+    constexpr int ITEMS = R > 32 ? 4 : R > 16 ? 2 : 1, SPLITS = R > 32 ? 2 : R > 16 ? 4 : 8;
     for (int i0 = (int)threadIdx.x; i0 < rows * d4; i0 += THREADS * ITEMS) {
         int r[ITEMS], d[ITEMS];
         float mx[ITEMS], sum[ITEMS];
@@ -140,7 +140,6 @@ __device__ __forceinline__ void paged_merge(const PagedAttnArgs& a, const PagedD
 }
 
 // ---- few new rows (the method is described in attention_paged.hip) -------------
-constexpr int PAGED_R = 16;        // rows per tile
 constexpr int PAGED_KEYS = 32;     // keys per wave and step
 
 // threadIdx.x, computed anew where it is called: what follows from it is not kept in
@@ -151,53 +150,72 @@ __device__ __forceinline__ int own_thread() {
     return t;
 }
 
-template <bool BF>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (BF)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+template <int R> struct PagedAcc;
+template <> struct PagedAcc<16> { typedef f32x4 type; };
+template <> struct PagedAcc<32> { typedef f32x16 type; };
+
+// v_mfma_f32_16x16x32 (R = 16) or v_mfma_f32_32x32x16 (R = 32): lane l gives row or
+// column l % R and 8 consecutive k from 8 (l / R) on
+template <int R, bool BF>
+__device__ __forceinline__ typename PagedAcc<R>::type mfma_paged(u32x4 a, u32x4 b, typename PagedAcc<R>::type c) {
+    if constexpr (R == 16) {
+        if constexpr (BF)
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+        if constexpr (BF)
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
 }
 
-// LDS of a wave: 32 V rows while it runs, 16 rows of output and their statistics
+// LDS of a wave: 32 V rows while it runs, R rows of output and their statistics
 // when it merges.  V's pitch is 32 mod 64 bytes, so that the 8 rows of 32 bytes
-// that half a transposed read touches lie in different banks.
-template <int KS>
+// that half a transposed read touches lie in different banks (R = 16; of R = 32's 4
+// rows of 64 bytes, two share banks).
+template <int R, int KS32>
 struct PagedLayout {
-    static constexpr int DP = 32 * KS;                         // padded head_dim
+    static constexpr int DP = 32 * KS32;                       // padded head_dim
     static constexpr int VP = DP + 16;                         // halfs
     static constexpr int OP = DP + 4;                          // floats
-    static constexpr int STAGE = PAGED_KEYS * VP * 2;
-    static constexpr int MERGE = PAGED_R * OP * 4 + 2 * PAGED_R * 4;
+    static constexpr int P = PAGED_KEYS * VP * 2, STAGE = P + PAGED_KEYS * R * 4;   // V, then probabilities (by key)
+    static constexpr int MERGE = R * OP * 4 + 2 * R * 4;
     static constexpr int REGION = ((STAGE > MERGE ? STAGE : MERGE) + 15) / 16 * 16;
 };
 
-// KS: head_dim <= 32 KS; BF: bf16 cache; PP: parts of P; NW: waves of the block.
+// The block of R f-rows of a tile and one kv head.  KS: head_dim <= 32 KS; BF: bf16
+// cache; PP: parts of P; NW: waves of the block; lds: NW REGIONs and a word.
 // Makes the index-th item, if there is one.
-template <int KS, bool BF, int PP, int NW>
+template <int R, int KS, bool BF, int PP, int NW>
 __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit, int index, int h, uint8_t* lds) {
-    using L = PagedLayout<KS>;
-    constexpr int DT = 2 * KS, VI = 2 * KS;
+    using L = PagedLayout<R, KS>;
+    using Acc = typename PagedAcc<R>::type;
+    constexpr int NG = 64 / R;                                 // lane groups: l / R
+    constexpr int U = 32 / R, S = KS * 4 / NG;                 // products of 32 keys, steps of 8 NG dims
+    constexpr int NE = R / 2, STEPS = NE / 8;                  // a lane's keys of 32, steps of 8 of them
+    constexpr int DT = L::DP / R, NR = R == 16 ? 4 : 16, VI = 2 * KS;
     const int tid = own_thread(), lane = tid & 63, wave = tid >> 6;
-    const int c16 = lane & 15, g4 = lane >> 4;
+    const int rl = lane % R, g = lane / R;
     const int D = a.kv.D;
     PagedItem it;
-    if (!paged_locate<PAGED_R, false>(a, unit, index, &it)) return;
+    if (!paged_locate<R, false>(a, unit, index, &it)) return;
     const PagedSpan sp = it.span;
 
     // this lane's row of the tile
-    const int f = it.tile * PAGED_R + c16, rows_f = sp.n * a.group;
+    const int f = it.tile * R + rl, rows_f = sp.n * a.group;
     const int j = f / a.group, gh = f - j * a.group;
     const int last = f < rows_f ? sp.visible(j) : 0;           // keys below it are visible
-    const int first_row = it.tile * PAGED_R / a.group, last_row = min(it.tile * PAGED_R + PAGED_R - 1, rows_f - 1) / a.group;
+    const int first_row = it.tile * R / a.group, last_row = min(it.tile * R + R - 1, rows_f - 1) / a.group;
     const int open_end = sp.visible(first_row);                // keys below it are visible to every row
     const int k_begin = it.split * it.unit, k_end = min(k_begin + it.unit, sp.visible(last_row));
     if (it.split > 0 && k_begin >= k_end) return;              // the merge counts on it (paged_merge)
 
-    u32x4 qf[KS];
+    u32x4 qf[S];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        const int d = 32 * s + 8 * g4;
+    for (int s = 0; s < S; ++s) {
+        const int d = 8 * NG * s + 8 * g;
         qf[s] = u32x4{0u, 0u, 0u, 0u};
         if (f < rows_f && d < D)
             qf[s] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(sp.row0 + j) * a.heads + h * a.group + gh) * D + d);
@@ -225,21 +243,23 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit,
     };
 
     float mrun = -INFINITY, lrun = 0.0f;                       // lrun: this lane's keys only
-    f32x4 oacc[DT];
+    Acc oacc[DT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) oacc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) oacc[t][r] = 0.0f;
 
     // K fragments and V chunks of a tile are asked for while the tile before is
     // computed: K's registers are free once its scores are, V's once it is in LDS.
-    u32x4 kf[2][KS], vf[VI];
+    u32x4 kf[U][S], vf[VI];
     auto load_k = [&](int slot) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int sl = max(__shfl(slot, 16 * u + c16, 64), 0);   // a hidden key's score is replaced below
+        for (int u = 0; u < U; ++u) {
+            const int sl = max(__shfl(slot, R * u + rl, 64), 0);     // a hidden key's score is replaced below
             const uint16_t* row = a.kv.k + (int64_t)sl * D;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = 32 * s + 8 * g4;
+            for (int s = 0; s < S; ++s) {
+                const int d = 8 * NG * s + 8 * g;
                 kf[u][s] = *reinterpret_cast<const u32x4*>(row + (d < D ? d : 0));
             }
         }
@@ -257,8 +277,23 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit,
     int slot = slot_of(kv0, ask_page(kv0));
     load_k(slot);
     load_v(slot);
-    for (; kv0 < k_end; kv0 += PAGED_KEYS * NW) {
+    for (; kv0 < k_end; kv0 += STEP) {
         const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(slot < 0);
+        // some rows see only part of this tile: if it holds values that are not finite,
+        // 0 x infinity would reach the rows that do not see them
+        bool by_key = false;
+        if (kv0 + PAGED_KEYS > open_end && open_end < k_end) {
+            asm volatile("");
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < VI; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+                    bad |= vkey[i] < PAGED_KEYS && !((gone >> (vkey[i] & 31)) & 1u) && ((vf[i][x] & e) == e || ((vf[i][x] >> 16) & e) == e);
+                }
+            by_key = __builtin_amdgcn_ballot_w64(bad) != 0;
+        }
 #pragma unroll
         for (int i = 0; i < VI; ++i)
             if (vkey[i] < PAGED_KEYS) {
@@ -272,96 +307,129 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit,
         load_v(slot);
         asm volatile("" ::: "memory");                         // this wave's LDS: its reads follow its stores
 
-        float p[8];
+        float p[NE];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < U; ++u) {
+            Acc s;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
+            for (int r = 0; r < NR; ++r) s[r] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
                 // dims past head_dim: K's registers hold other dims there
-                if (32 * k + 32 > D && 32 * k + 8 * g4 >= D) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
-                s = mfma16<BF>(kf[u][k], qf[k], s);
+                if (8 * NG * k + 8 * NG > D && 8 * NG * k + 8 * g >= D) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
+                s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) p[4 * u + r] = s[r];
+            for (int r = 0; r < NR; ++r) p[NR * u + r] = s[r];
         }
         load_k(slot);
         if (gone || kv0 + PAGED_KEYS > open_end) {
             asm volatile("");                                  // a branch: few tiles need this
-            const int seen = last - kv0 - 4 * g4;
-            const uint32_t hid = gone >> (4 * g4);
+            const int seen = last - kv0 - 4 * g;
+            const uint32_t hid = gone >> (4 * g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = 16 * (e >> 2) + (e & 3);       // and 4 g4
+            for (int e = 0; e < NE; ++e) {
+                const int key = 4 * NG * (e >> 2) + (e & 3);   // and 4 g
                 if (key >= seen || (hid & (1u << key))) p[e] = -INFINITY;
             }
         }
         float tmax = p[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) tmax = fmaxf(tmax, p[e]);
+        for (int e = 1; e < NE; ++e) tmax = fmaxf(tmax, p[e]);
         tmax *= a.scale_log2;
         if (__builtin_amdgcn_ballot_w64(tmax > mrun + 8.0f)) {
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+            if constexpr (R == 16) tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
             tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
             const float mnew = fmaxf(mrun, tmax);
             const float factor = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mnew);
             lrun *= factor;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) oacc[t] *= factor;
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) oacc[t][r] *= factor;
             mrun = mnew;
         }
         const float msafe = mrun == -INFINITY ? 0.0f : mrun;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < NE; ++e) {
             p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.scale_log2, -msafe));
             lrun += p[e];
         }
-        u32x4 pb[PP];
+        if (by_key) {                                          // key by key, over the rows that see the key
+            float* pw = (float*)(lds + wave * L::REGION + L::P);
 #pragma unroll
-        for (int w = 0; w < PP; ++w)
+            for (int e = 0; e < NE; ++e) pw[(4 * NG * (e >> 2) + 4 * g + (e & 3)) * R + rl] = p[e];
+            asm_wait_lgkmcnt<0>();
+            for (int key = 0; key < PAGED_KEYS; ++key) {
+                const float pk = pw[key * R + rl];
+                if (kv0 + key >= last) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pb[w][e] = round2<BF, true>(p[2 * e], p[2 * e + 1]);
-        const uint16_t* vg = vt + (4 * g4 + (c16 >> 2)) * L::VP + 4 * (c16 & 3);
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            lds_i16x4* p0 = (lds_i16x4*)(uintptr_t)lds_offset(vg + 16 * t);
-            lds_i16x4* p1 = (lds_i16x4*)(uintptr_t)lds_offset(vg + 16 * t + 16 * L::VP);
-            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0));
-            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1));
+                    for (int r = 0; r < NR; ++r) {
+                        const uint16_t v = vt[key * L::VP + R * t + 4 * NG * (r >> 2) + 4 * g + (r & 3)];
+                        oacc[t][r] = __builtin_fmaf(pk, BF ? bf16_bits_to_f32(v) : f16_bits_to_f32(v), oacc[t][r]);
+                    }
+            }
+            asm_wait_lgkmcnt<0>();
+            for (int i = lane; i < PAGED_KEYS * L::VP / 8; i += 64)   // what follows adds zeros
+                *reinterpret_cast<u32x4*>(vt + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+            asm_wait_lgkmcnt<0>();
+        }
+        {
+            const uint16_t* vg = vt + (4 * g + ((lane & 15) >> 2)) * L::VP + 16 * ((lane >> 4) & (R / 16 - 1)) + 4 * (lane & 3);
 #pragma unroll
-            for (int w = 0; w < PP; ++w) oacc[t] = mfma16<BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[w], oacc[t]);
+            for (int k = 0; k < STEPS; ++k) {
+                u32x4 pb[PP];
+#pragma unroll
+                for (int w = 0; w < PP; ++w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pb[w][e] = round2<BF, true>(p[8 * k + 2 * e], p[8 * k + 2 * e + 1]);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    lds_i16x4* p0 = (lds_i16x4*)(uintptr_t)lds_offset(vg + 8 * NG * k * L::VP + R * t);
+                    lds_i16x4* p1 = (lds_i16x4*)(uintptr_t)lds_offset(vg + (8 * NG * k + 4 * NG) * L::VP + R * t);
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1));
+#pragma unroll
+                    for (int w = 0; w < PP; ++w) oacc[t] = mfma_paged<R, BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[w], oacc[t]);
+                }
+            }
         }
         asm volatile("" ::: "memory");
     }
-    lrun += __shfl_xor(lrun, 16, 64);
+    if constexpr (R == 16) lrun += __shfl_xor(lrun, 16, 64);
     lrun += __shfl_xor(lrun, 32, 64);
 
     // merge the waves: each parks its rows, then the block combines them
-    float* om = (float*)(lds + wave * L::REGION);              // [16][OP]
-    float* ml = om + PAGED_R * L::OP;                          // max[16], sum[16]
+    float* om = (float*)(lds + wave * L::REGION);              // [R][OP]
+    float* ml = om + R * L::OP;                                // max[R], sum[R]
 #pragma unroll
-    for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(om + c16 * L::OP + 16 * t + 4 * g4) = oacc[t];
-    if (g4 == 0) {
-        ml[c16] = mrun;
-        ml[PAGED_R + c16] = lrun;
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int r = 0; r < NR; r += 4)
+            *reinterpret_cast<f32x4*>(om + rl * L::OP + R * t + NG * r + 4 * g) = f32x4{oacc[t][r], oacc[t][r + 1], oacc[t][r + 2], oacc[t][r + 3]};
+    if (g == 0) {
+        ml[rl] = mrun;
+        ml[R + rl] = lrun;
     }
     __syncthreads();
-    const PagedParts<PAGED_R> parts(a, a.few, h);
+    const PagedParts<R> parts(a, a.few, h);
     const int d4 = D / 4;
-    for (int i = tid; i < PAGED_R * d4; i += 64 * NW) {
+    for (int i = tid; i < R * d4; i += 64 * NW) {
         const int r = i / d4, d = 4 * (i - r * d4);
-        if (it.tile * PAGED_R + r >= rows_f) continue;
+        if (it.tile * R + r >= rows_f) continue;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ((const float*)(lds + w * L::REGION))[PAGED_R * L::OP + r]);
+        for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ((const float*)(lds + w * L::REGION))[R * L::OP + r]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float sum = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float* rw = (const float*)(lds + w * L::REGION);
-            const float e = __builtin_amdgcn_exp2f(rw[PAGED_R * L::OP + r] - ref);
-            sum += e * rw[PAGED_R * L::OP + PAGED_R + r];
+            const float e = __builtin_amdgcn_exp2f(rw[R * L::OP + r] - ref);
+            sum += e * rw[R * L::OP + R + r];
             o += e * *reinterpret_cast<const f32x4*>(rw + r * L::OP + d);
         }
         if (it.record >= 0) {
@@ -369,13 +437,14 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit,
             if (d == 0) parts.store_ml(it.record + it.split, r, mx, sum);
             continue;
         }
-        paged_store4<BF>(a, sp, h, it.tile * PAGED_R + r, d, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / sum));
+        paged_store4<BF>(a, sp, h, it.tile * R + r, d, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / sum));
     }
-    if (it.record >= 0) paged_merge<BF, PAGED_R, 64 * NW>(a, a.few, it, h, (uint32_t*)(lds + NW * L::REGION));
+    if (it.record >= 0) paged_merge<BF, R, 64 * NW>(a, a.few, it, h, (uint32_t*)(lds + NW * L::REGION));
 }
 
 constexpr int CHUNK_KEYS = 64;     // keys per tile of the kernel for many new rows
 constexpr int CHUNK_R = 256;       // its f-rows per tile
+constexpr int CHUNK_UNIT = 1024;   // its least keys per split
 hipError_t launch_attention_paged_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus);
 
 }  // namespace mvlm

@@ -31,17 +31,18 @@
 #include "attention_paged.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace mvlm {
 
 constexpr int PAGED_NW = 4;        // waves per block
 
-template <int KS, bool BF, int PP>
-__global__ __launch_bounds__(64 * PAGED_NW) void paged_attention_kernel(const PagedAttnArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[PAGED_NW * PagedLayout<KS>::REGION + 16];
+template <int R, int KS, bool BF, int PP>
+__global__ __launch_bounds__(64 * PAGED_NW, 2) void paged_attention_kernel(const PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
-    const PagedShare share = paged_share<PAGED_R, false>(a);
-    if (index < share.items) paged_few_item<KS, BF, PP, PAGED_NW>(a, share.unit, index, h, lds);
+    const PagedShare share = paged_share<R, false>(a);
+    if (index < share.items) paged_few_item<R, KS, BF, PP, PAGED_NW>(a, share.unit, index, h, lds);
 }
 
 // Division of the sequences of at most (or of more than) PAGED_FEW f-rows: `blocks`
@@ -63,17 +64,21 @@ static PagedDivision paged_divide(const PagedAttnArgs& a, int tile, int64_t bloc
 void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const PagedSeqs& b = a->batch;
     const int64_t f = (int64_t)b.rows * a->group;
-    const bool single = !b.row_start;                          // every sequence has `group` f-rows
     a->few = a->many = PagedDivision{};
-    if (!single || a->group <= PAGED_FEW) {
-        const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + PAGED_R - 1) / PAGED_R) : f / PAGED_R + b.seqs;
-        a->few = paged_divide(*a, PAGED_R, 4 * (int64_t)num_cus, tiles, PAGED_KEYS * PAGED_NW, PAGED_KEYS * PAGED_NW);
-    }
-    if (single ? a->group > PAGED_FEW : f > PAGED_FEW) {
+    // Tiles of 256 rows pay once they give every CU a block, alone or with the keys that
+    // the tables can hold split; below that tiles of 32 make more of the chip.
+    const int64_t tiles256 = f / CHUNK_R * a->kv.kv_heads;
+    const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
+    a->few_rows = many ? PAGED_FEW : INT_MAX;
+    if (many) {
         // a sequence with more than PAGED_FEW f-rows ends in one tile that is not full
         const int64_t tiles = f / CHUNK_R + std::min<int64_t>(b.seqs, f / PAGED_FEW + 1);
-        a->many = paged_divide(*a, CHUNK_R, num_cus, tiles, 1024, CHUNK_KEYS);
+        a->many = paged_divide(*a, CHUNK_R, num_cus, tiles, CHUNK_UNIT, CHUNK_KEYS);
     }
+    const bool single = !b.row_start;                          // every sequence has `group` f-rows
+    const int R = single && a->group <= 16 && !many ? 16 : 32;
+    const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + R - 1) / R) : f / R + b.seqs;
+    a->few = paged_divide(*a, R, 4 * (int64_t)num_cus, tiles, PAGED_KEYS * PAGED_NW, PAGED_KEYS * PAGED_NW);
 }
 
 size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {
@@ -81,31 +86,34 @@ size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {
 }
 size_t paged_words(const PagedAttnArgs& a, const PagedDivision& d) { return (size_t)d.records * a.kv.kv_heads; }
 
-template <int KS, bool BF, int PP>
-static void launch_few(hipStream_t s, const PagedAttnArgs& a) {
-    launch_kernel(paged_attention_kernel<KS, BF, PP>, dim3((unsigned)(a.kv.kv_heads * a.few.items)), dim3(64 * PAGED_NW),
-                  0, s, a);
+template <int R, int KS, bool BF, int PP>
+static hipError_t launch_few(hipStream_t s, const PagedAttnArgs& a) {
+    constexpr int bytes = PAGED_NW * PagedLayout<R, KS>::REGION + 16;
+    if constexpr (bytes > 65536)
+        if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, BF, PP>>(bytes); e != hipSuccess) return e;
+    launch_kernel(paged_attention_kernel<R, KS, BF, PP>, dim3((unsigned)(a.kv.kv_heads * a.few.items)), dim3(64 * PAGED_NW),
+                  (uint32_t)bytes, s, a);
+    return hipGetLastError();
 }
 
-template <int KS>
-static void launch_few_dims(hipStream_t s, const PagedAttnArgs& a) {
+template <int R, int KS>
+static hipError_t launch_few_dims(hipStream_t s, const PagedAttnArgs& a) {
     const bool wide = a.o_dtype == MVLM_F32;
-    if (a.kv.dtype == MVLM_F16) {
-        if (wide) launch_few<KS, false, 2>(s, a);
-        else launch_few<KS, false, 1>(s, a);
-    } else {
-        if (wide) launch_few<KS, true, 3>(s, a);
-        else launch_few<KS, true, 1>(s, a);
-    }
+    if (a.kv.dtype == MVLM_F16) return wide ? launch_few<R, KS, false, 2>(s, a) : launch_few<R, KS, false, 1>(s, a);
+    return wide ? launch_few<R, KS, true, 3>(s, a) : launch_few<R, KS, true, 1>(s, a);
+}
+
+template <int R>
+static hipError_t launch_few_rows(hipStream_t s, const PagedAttnArgs& a) {
+    if (a.kv.D <= 32) return launch_few_dims<R, 1>(s, a);
+    if (a.kv.D <= 64) return launch_few_dims<R, 2>(s, a);
+    if (a.kv.D <= 96) return launch_few_dims<R, 3>(s, a);
+    return launch_few_dims<R, 4>(s, a);
 }
 
 hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
     if (a.many.tile) return launch_attention_paged_chunk(s, a, num_cus);
-    if (a.kv.D <= 32) launch_few_dims<1>(s, a);
-    else if (a.kv.D <= 64) launch_few_dims<2>(s, a);
-    else if (a.kv.D <= 96) launch_few_dims<3>(s, a);
-    else launch_few_dims<4>(s, a);
-    return hipGetLastError();
+    return a.few.tile == 16 ? launch_few_rows<16>(s, a) : launch_few_rows<32>(s, a);
 }
 
 }  // namespace mvlm

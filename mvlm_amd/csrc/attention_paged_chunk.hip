@@ -388,7 +388,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int kv_heads = a.kv.kv_heads, q = (int)blockIdx.x % PAGED_QUEUES, own = (int)blockIdx.x / PAGED_QUEUES;
     const int blocks = ((int)gridDim.x - q + PAGED_QUEUES - 1) / PAGED_QUEUES;              // of this queue
-    const PagedShare many = paged_share<CHUNK_R, true>(a), few = paged_share<PAGED_R, false>(a);
+    const PagedShare many = paged_share<CHUNK_R, true>(a), few = paged_share<32, false>(a);
     const int many_items = (many.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     const int all_items = many_items + (few.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     for (int round = 0; round * blocks < all_items; ++round) {
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
             paged_chunk_item<KS, DT, BF, PP>(a, many.unit, index, w - index * kv_heads, lds);
         } else if (i < all_items) {
             const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_few_item<DT, BF, PP, 8>(a, few.unit, index, w - index * kv_heads, lds);
+            paged_few_item<32, DT, BF, PP, 8>(a, few.unit, index, w - index * kv_heads, lds);
         }
         __syncthreads();                                       // LDS is free
     }
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
 
 template <int KS, int DT, bool BF, int PP>
 static hipError_t launch_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
-    constexpr int few = 8 * PagedLayout<DT>::REGION + 16, bytes = ChunkLayout<DT>::BYTES > few ? ChunkLayout<DT>::BYTES : few;
+    constexpr int few = 8 * PagedLayout<32, DT>::REGION + 16, bytes = ChunkLayout<DT>::BYTES > few ? ChunkLayout<DT>::BYTES : few;
     if (const hipError_t e = allow_dynamic_lds<paged_chunk_kernel<KS, DT, BF, PP>>(bytes); e != hipSuccess) return e;
     const int64_t most = ((int64_t)a.many.items + a.few.items) * a.kv.kv_heads;
     launch_kernel(paged_chunk_kernel<KS, DT, BF, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),

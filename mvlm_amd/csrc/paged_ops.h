@@ -42,7 +42,8 @@ struct PagedAttnArgs {
     int o_dtype, heads, group;     // group: heads per kv head
     float scale_log2;              // scale * log2(e)
     // division of the work (attention_paged.hip) of the sequences with few new
-    // rows, f = n group <= PAGED_FEW, and of those with more
+    // rows, f = n group <= few_rows, and of those with more
+    int few_rows;
     PagedDivision few, many;
 };
 
@@ -101,9 +102,9 @@ struct PagedItem {
 };
 
 template <int R, bool MANY>
-__device__ __forceinline__ int paged_tiles(const PagedSpan& p, int group) {
+__device__ __forceinline__ int paged_tiles(const PagedSpan& p, int group, int few) {
     const int64_t f = (int64_t)p.n * group;
-    return (f > PAGED_FEW) == MANY ? (int)((f + R - 1) / R) : 0;
+    return (f > few) == MANY ? (int)((f + R - 1) / R) : 0;
 }
 
 // Keys per block: total work (tiles x keys) over the blocks wanted, at least
@@ -136,7 +137,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     int64_t total = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        total += (int64_t)paged_tiles<R, MANY>(p, a.group) * p.len;
+        total += (int64_t)paged_tiles<R, MANY>(p, a.group, a.few_rows) * p.len;
     }
     // summed over the lanes as two numbers of 24 and 30 bits; read from one lane, so that
     // no branch on it is taken as divergent
@@ -147,7 +148,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     int items = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        items += paged_tiles<R, MANY>(p, a.group) * paged_splits(p.len, sh.unit);
+        items += paged_tiles<R, MANY>(p, a.group, a.few_rows) * paged_splits(p.len, sh.unit);
     }
     items = __builtin_amdgcn_readlane(wave_scan(items), 63);
     // no more than planned for, whatever row_start holds
@@ -164,7 +165,7 @@ __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, int unit, i
     int first = 0, record = 0;                             // items and records before this round of sequences
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan sp = paged_lane_span(b, base + lane);
-        const int tiles = paged_tiles<R, MANY>(sp, a.group), splits = paged_splits(sp.len, unit);
+        const int tiles = paged_tiles<R, MANY>(sp, a.group, a.few_rows), splits = paged_splits(sp.len, unit);
         const int items = tiles * splits, records = splits > 1 ? tiles * splits : 0;
         const int end = first + wave_scan(items), rec_end = record + wave_scan(records);
         const uint64_t mine = __builtin_amdgcn_ballot_w64(index >= end - items && index < end);
