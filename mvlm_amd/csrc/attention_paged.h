@@ -189,7 +189,7 @@ struct PagedLayout {
 // cache; PP: parts of P; NW: waves of the block; lds: NW REGIONs and a word.
 // Makes the index-th item, if there is one.
 template <int R, int KS, bool BF, int PP, int NW>
-__device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit, int index, int h, uint8_t* lds) {
+__device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const PagedShare& share, int index, int h, uint8_t* lds) {
     using L = PagedLayout<R, KS>;
     using Acc = typename PagedAcc<R>::type;
     constexpr int NG = 64 / R;                                 // lane groups: l / R
@@ -200,7 +200,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, int unit,
     const int rl = lane % R, g = lane / R;
     const int D = a.kv.D;
     PagedItem it;
-    if (!paged_locate<R, false>(a, unit, index, &it)) return;
+    if (!paged_locate<R, false>(a, share, index, &it)) return;
     const PagedSpan sp = it.span;
 
     // this lane's row of the tile

@@ -38,11 +38,11 @@ namespace mvlm {
 constexpr int PAGED_NW = 4;        // waves per block
 
 template <int R, int KS, bool BF, int PP>
-__global__ __launch_bounds__(64 * PAGED_NW, 2) void paged_attention_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * PAGED_NW, KS <= 2 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
     const PagedShare share = paged_share<R, false>(a);
-    if (index < share.items) paged_few_item<R, KS, BF, PP, PAGED_NW>(a, share.unit, index, h, lds);
+    if (index < share.items) paged_few_item<R, KS, BF, PP, PAGED_NW>(a, share, index, h, lds);
 }
 
 // Division of the sequences of at most (or of more than) PAGED_FEW f-rows: `blocks`
@@ -78,7 +78,10 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int R = single && a->group <= 16 && !many ? 16 : 32;
     const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + R - 1) / R) : f / R + b.seqs;
-    a->few = paged_divide(*a, R, 4 * (int64_t)num_cus, tiles, PAGED_KEYS * PAGED_NW, PAGED_KEYS * PAGED_NW);
+    // blocks wanted per CU, measured at 1.. 6: 16 rows 2 (16 sequences up to 2047: 30.6 us, 33.3 at
+    // 3, 34.0 at 4; 4 of 32768, D = 128: 84.9, 94.7, 88.4), 32 rows 1 (256 rows and 11 single tokens:
+    // 33.4 us, 40.7 at 2, 42.7 at 4)
+    a->few = paged_divide(*a, R, (R == 16 ? 2 : 1) * (int64_t)num_cus, tiles, PAGED_KEYS * PAGED_NW, PAGED_KEYS * PAGED_NW);
 }
 
 size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {

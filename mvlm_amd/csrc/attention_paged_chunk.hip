@@ -82,7 +82,7 @@ struct ChunkLayout {
 
 // KS: head_dim <= 16 KS; DT: head_dim <= 32 DT; PP: parts of P
 template <int KS, int DT, bool BF, int PP>
-__device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, int unit, int index, int h, uint8_t* lds) {
+__device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const PagedShare& share, int index, int h, uint8_t* lds) {
     using L = ChunkLayout<DT>;
     constexpr int CH = L::CH, PB = L::PB, TILE = L::TILE, NB = L::NB, R = CHUNK_R;
     constexpr int NL = CHUNK_KEYS * CH / CHUNK_THREADS;        // chunks of K (and of V) per thread and tile
@@ -91,7 +91,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, int uni
     const bool second = wave >= 4;
     const int D = a.kv.D;
     PagedItem it;
-    if (!paged_locate<R, true>(a, unit, index, &it)) return;
+    if (!paged_locate<R, true>(a, share, index, &it)) return;
     const PagedSpan sp = it.span;
     const int rows_f = sp.n * a.group;
     const int tile_f = it.tile * R, wave_f = tile_f + 32 * wave;
@@ -395,10 +395,10 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
         const int i = round * blocks + (round & 1 ? blocks - 1 - own : own);
         if (i < many_items) {
             const int w = i * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_chunk_item<KS, DT, BF, PP>(a, many.unit, index, w - index * kv_heads, lds);
+            paged_chunk_item<KS, DT, BF, PP>(a, many, index, w - index * kv_heads, lds);
         } else if (i < all_items) {
             const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_few_item<32, DT, BF, PP, 8>(a, few.unit, index, w - index * kv_heads, lds);
+            paged_few_item<32, DT, BF, PP, 8>(a, few, index, w - index * kv_heads, lds);
         }
         __syncthreads();                                       // LDS is free
     }

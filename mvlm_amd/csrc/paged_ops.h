@@ -125,6 +125,7 @@ __device__ __forceinline__ PagedSpan paged_lane_span(const PagedSeqs& b, int s) 
 // A share's keys per block and its items per kv head, the same in all lanes.
 struct PagedShare {
     int unit, items;
+    PagedSpan first;               // of the lane-th sequence
 };
 __device__ __forceinline__ int paged_splits(int len, int unit) { return len > unit ? (len + unit - 1) / unit : 1; }
 
@@ -134,6 +135,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
     const PagedSpan sp = paged_lane_span(b, lane);
+    PagedShare sh;
+    sh.first = sp;
     int64_t total = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
@@ -143,7 +146,6 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     // no branch on it is taken as divergent
     const int64_t lo = __builtin_amdgcn_readlane(wave_scan((int)(total & 0xFFFFFF)), 63);
     const int64_t hi = __builtin_amdgcn_readlane(wave_scan((int)(total >> 24)), 63);
-    PagedShare sh;
     sh.unit = paged_unit(div, (hi << 24) + lo);
     int items = 0;
     for (int base = 0; base < b.seqs; base += 64) {
@@ -158,14 +160,14 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
 
 // The index-th item of a share, the same in all lanes; false if there is none.
 template <int R, bool MANY>
-__device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, int unit, int index, PagedItem* out) {
+__device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, const PagedShare& share, int index, PagedItem* out) {
     const PagedSeqs& b = a.batch;
     const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
     int first = 0, record = 0;                             // items and records before this round of sequences
     for (int base = 0; base < b.seqs; base += 64) {
-        const PagedSpan sp = paged_lane_span(b, base + lane);
-        const int tiles = paged_tiles<R, MANY>(sp, a.group, a.few_rows), splits = paged_splits(sp.len, unit);
+        const PagedSpan sp = base ? paged_lane_span(b, base + lane) : share.first;
+        const int tiles = paged_tiles<R, MANY>(sp, a.group, a.few_rows), splits = paged_splits(sp.len, share.unit);
         const int items = tiles * splits, records = splits > 1 ? tiles * splits : 0;
         const int end = first + wave_scan(items), rec_end = record + wave_scan(records);
         const uint64_t mine = __builtin_amdgcn_ballot_w64(index >= end - items && index < end);
@@ -174,7 +176,7 @@ __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, int unit, i
             auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             out->seq = base + l;
             out->span = PagedSpan{at(sp.row0), at(sp.n), at(sp.held), at(sp.len)};
-            out->unit = unit;
+            out->unit = share.unit;
             const int ns = at(splits), r = index - at(end - items);
             const int nth = r / ns;
             out->tile = at(tiles) - 1 - nth;               // the last tile sees the most keys: it starts first
