@@ -230,16 +230,17 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
         vkey[i] = c / cpr;
         vdim[i] = 8 * (c - vkey[i] * cpr);
     }
-    // page of key kv0 + lane % 32 (asked for a tile before its slot is needed), and
-    // that key's slot, -1 where there is none
+    // page of key kv0 + lane % 32 (asked for a tile before it is needed), and where that
+    // key is, in 16-byte chunks of the cache (below 2^32, checked on the host)
     const int* table = a.batch.table + (int64_t)it.seq * a.batch.width;
     auto ask_page = [&](int kv0) {
         const int key = kv0 + (lane & 31);
         return key < k_end ? table[a.kv.page.quotient(key)] : -1;
     };
-    auto slot_of = [&](int kv0, int page) {
+    auto exists = [&](int page) { return page >= 0 && page < a.kv.num_pages; };
+    auto chunk_of = [&](int kv0, int page) -> uint32_t {       // a hidden key's: the first, so that it may be read
         const int key = kv0 + (lane & 31);
-        return page >= 0 && page < a.kv.num_pages ? a.kv.slot(page, h, key - a.kv.page.quotient(key) * a.kv.page.div) : -1;
+        return exists(page) ? (uint32_t)a.kv.slot(page, h, key - a.kv.page.quotient(key) * a.kv.page.div) * (uint32_t)cpr : 0u;
     };
 
     float mrun = -INFINITY, lrun = 0.0f;                       // lrun: this lane's keys only
@@ -252,33 +253,32 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     // K fragments and V chunks of a tile are asked for while the tile before is
     // computed: K's registers are free once its scores are, V's once it is in LDS.
     u32x4 kf[U][S], vf[VI];
-    auto load_k = [&](int slot) {
+    auto chunk_at = [](const uint16_t* base, uint32_t c) { return reinterpret_cast<const u32x4*>((uintptr_t)base + ((uint64_t)c << 4)); };
+    auto load_k = [&](uint32_t where) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int sl = max(__shfl(slot, R * u + rl, 64), 0);     // a hidden key's score is replaced below
-            const uint16_t* row = a.kv.k + (int64_t)sl * D;
+            const uint32_t c = __shfl(where, R * u + rl, 64);  // a hidden key's score is replaced below
+            const u32x4* row = chunk_at(a.kv.k, c + (uint32_t)g);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const int d = 8 * NG * s + 8 * g;
-                kf[u][s] = *reinterpret_cast<const u32x4*>(row + (d < D ? d : 0));
+                if (NG * (s + 1) * 8 <= 32 * (KS - 1)) kf[u][s] = row[NG * s];
+                else kf[u][s] = *chunk_at(a.kv.k, c + (NG * s + g < cpr ? NG * s + g : 0));   // may be past head_dim
             }
         }
     };
-    auto load_v = [&](int slot) {
+    auto load_v = [&](uint32_t where) {
 #pragma unroll
-        for (int i = 0; i < VI; ++i) {
-            const int sl = max(__shfl(slot, vkey[i] & 31, 64), 0);
-            vf[i] = *reinterpret_cast<const u32x4*>(a.kv.v + (int64_t)sl * D + vdim[i]);
-        }
+        for (int i = 0; i < VI; ++i) vf[i] = *chunk_at(a.kv.v, __shfl(where, vkey[i] & 31, 64) + (uint32_t)(vdim[i] >> 3));
     };
     int kv0 = k_begin + PAGED_KEYS * wave;
     constexpr int STEP = PAGED_KEYS * NW;
     int page_next = ask_page(kv0 + STEP);
-    int slot = slot_of(kv0, ask_page(kv0));
-    load_k(slot);
-    load_v(slot);
+    const int page = ask_page(kv0);
+    uint32_t where = chunk_of(kv0, page), gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page));
+    load_k(where);
+    load_v(where);
     for (; kv0 < k_end; kv0 += STEP) {
-        const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(slot < 0);
+        const uint32_t gone = gone_next;
         // some rows see only part of this tile: if it holds values that are not finite,
         // 0 x infinity would reach the rows that do not see them
         bool by_key = false;
@@ -294,19 +294,31 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
                 }
             by_key = __builtin_amdgcn_ballot_w64(bad) != 0;
         }
+        if (gone) {
+            asm volatile("");                                  // a branch: few tiles need this
+#pragma unroll
+            for (int i = 0; i < VI; ++i)
+                if ((gone >> (vkey[i] & 31)) & 1u) vf[i] = u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (int i = 0; i < VI; ++i)
-            if (vkey[i] < PAGED_KEYS) {
-                if (gone && ((gone >> vkey[i]) & 1u)) vf[i] = u32x4{0u, 0u, 0u, 0u};
-                *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = vf[i];
-            }
+            if (64 * i + 64 <= 128 * (KS - 1) || vkey[i] < PAGED_KEYS) *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = vf[i];
         // the page of the tile after next is asked for before the loads, so that its
         // wait, an iteration later, does not wait for them
-        slot = slot_of(kv0 + STEP, page_next);
+        where = chunk_of(kv0 + STEP, page_next);
+        gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page_next));
         page_next = ask_page(kv0 + 2 * STEP);
-        load_v(slot);
+        load_v(where);
         asm volatile("" ::: "memory");                         // this wave's LDS: its reads follow its stores
 
+        if (D < 32 * KS) {                                     // dims past head_dim: K's registers hold other dims there
+            asm volatile("");
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < S; ++k)
+                    if (NG * (k + 1) * 8 > 32 * (KS - 1) && NG * k + g >= cpr) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
+        }
         float p[NE];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -315,14 +327,12 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             for (int r = 0; r < NR; ++r) s[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < S; ++k) {
-                // dims past head_dim: K's registers hold other dims there
-                if (8 * NG * k + 8 * NG > D && 8 * NG * k + 8 * g >= D) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
                 s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
             }
 #pragma unroll
             for (int r = 0; r < NR; ++r) p[NR * u + r] = s[r];
         }
-        load_k(slot);
+        load_k(where);
         if (gone || kv0 + PAGED_KEYS > open_end) {
             asm volatile("");                                  // a branch: few tiles need this
             const int seen = last - kv0 - 4 * g;

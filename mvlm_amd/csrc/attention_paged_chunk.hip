@@ -348,20 +348,18 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         }
     asm_wait_vmcnt<0>();
     phase_barrier();
-    if (second) phase_barrier();                               // phase 0 of waves 4..7
+    auto in_reach = [&](int i) { return i < n && k_begin + i * CHUNK_KEYS < wave_end; };
     for (int i = 0, ring = 0; i <= n; ++i, ring = ring == NB - 1 ? 0 : ring + 1) {
         next_slots(i);
+        if (second && i > 0 && in_reach(i - 1)) softmax(i - 1);
         __builtin_amdgcn_s_setprio(1);
-        products(i, ring, i > 0 && k_begin + (i - 1) * CHUNK_KEYS < wave_end);
+        products(i, ring, i > 0 && in_reach(i - 1));
         __builtin_amdgcn_s_setprio(0);
+        if (!second && in_reach(i)) softmax(i);
         // what this wave asked for NB - 2 iterations ago has arrived: K of tile i + 1 and V of tile i
-        if (second) asm_wait_vmcnt<(NB - 2) * 2 * NL>();
-        phase_barrier();
-        if (i < n && k_begin + i * CHUNK_KEYS < wave_end) softmax(i);
-        if (!second) asm_wait_vmcnt<(NB - 2) * 2 * NL>();
+        asm_wait_vmcnt<(NB - 2) * 2 * NL>();
         phase_barrier();
     }
-    if (!second) phase_barrier();
     asm_wait_vmcnt<0>();                                       // loads past the last tile write LDS that is about to be reused
 
     const float sum = lrun + __shfl_xor(lrun, 32, 64);
