@@ -35,14 +35,13 @@
 
 namespace mvlm {
 
-constexpr int PAGED_NW = 4;        // waves per block
-
-template <int R, int KS, bool BF, int PP>
-__global__ __launch_bounds__(64 * PAGED_NW, KS <= 2 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
+// NW: waves per block
+template <int R, int KS, bool BF, int PP, int NW>
+__global__ __launch_bounds__(64 * NW, KS <= 2 && NW == 4 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
     const PagedShare share = paged_share<R, false>(a);
-    if (index < share.items) paged_few_item<R, KS, BF, PP, PAGED_NW>(a, share, index, h, lds);
+    if (index < share.items) paged_few_item<R, KS, BF, PP, NW>(a, share, index, h, lds);
 }
 
 // Division of the sequences of at most (or of more than) PAGED_FEW f-rows: `blocks`
@@ -81,7 +80,13 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     // blocks wanted per CU, measured at 1.. 6: 16 rows 2 (16 sequences up to 2047: 30.6 us, 33.3 at
     // 3, 34.0 at 4; 4 of 32768, D = 128: 84.9, 94.7, 88.4), 32 rows 1 (256 rows and 11 single tokens:
     // 33.4 us, 40.7 at 2, 42.7 at 4)
-    a->few = paged_divide(*a, R, (R == 16 ? 2 : 1) * (int64_t)num_cus, tiles, PAGED_KEYS * PAGED_NW, PAGED_KEYS * PAGED_NW);
+    // Tiles that leave most CUs idle, over tables that do not hold more than 512 keys for
+    // each CU, take eight waves instead of four: their splits are few or none (one sequence of
+    // 512: 8.3 -> 7.4 us; 4 of 32768 would take 88.4 us instead of 84.8).
+    const int64_t heads_tiles = tiles * a->kv.kv_heads;
+    const int waves = R == 16 && 2 * heads_tiles <= num_cus && heads_tiles * b.positions <= 512 * (int64_t)num_cus ? 8 : 4;
+    a->few = paged_divide(*a, R, (R == 16 ? 2 : 1) * (int64_t)num_cus, tiles, (waves == 8 ? 2 : 1) * PAGED_KEYS * waves,
+                          PAGED_KEYS * waves);
 }
 
 size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {
@@ -89,14 +94,21 @@ size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {
 }
 size_t paged_words(const PagedAttnArgs& a, const PagedDivision& d) { return (size_t)d.records * a.kv.kv_heads; }
 
-template <int R, int KS, bool BF, int PP>
-static hipError_t launch_few(hipStream_t s, const PagedAttnArgs& a) {
-    constexpr int bytes = PAGED_NW * PagedLayout<R, KS>::REGION + 16;
+template <int R, int KS, bool BF, int PP, int NW>
+static hipError_t launch_waves(hipStream_t s, const PagedAttnArgs& a) {
+    constexpr int bytes = NW * PagedLayout<R, KS>::REGION + 16;
     if constexpr (bytes > 65536)
-        if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, BF, PP>>(bytes); e != hipSuccess) return e;
-    launch_kernel(paged_attention_kernel<R, KS, BF, PP>, dim3((unsigned)(a.kv.kv_heads * a.few.items)), dim3(64 * PAGED_NW),
+        if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, BF, PP, NW>>(bytes); e != hipSuccess) return e;
+    launch_kernel(paged_attention_kernel<R, KS, BF, PP, NW>, dim3((unsigned)(a.kv.kv_heads * a.few.items)), dim3(64 * NW),
                   (uint32_t)bytes, s, a);
     return hipGetLastError();
+}
+
+template <int R, int KS, bool BF, int PP>
+static hipError_t launch_few(hipStream_t s, const PagedAttnArgs& a) {
+    if constexpr (R == 16)
+        if (a.few.unit_step == 8 * PAGED_KEYS) return launch_waves<R, KS, BF, PP, 8>(s, a);
+    return launch_waves<R, KS, BF, PP, 4>(s, a);
 }
 
 template <int R, int KS>

@@ -20,6 +20,12 @@
 namespace mvlm {
 
 constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_AHEAD = 3;
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));   // the rope table's rows may start anywhere
 
 // 8 elements from x[i], fp32
 template <int XD, bool VEC>
@@ -46,11 +52,21 @@ __device__ __forceinline__ void append_load8(const void* x, int64_t i, float (&v
 template <int XD, bool VEC>
 __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppendArgs a) {
     const int row = (int)blockIdx.x;
+    const PagedKv& kv = a.kv;
+    const int D = kv.D, cpr = D / 8, half = a.rot / 2;
+    const int chunks = (a.heads + 2 * kv.kv_heads) * cpr;
+    const int64_t xrow = (int64_t)row * a.ld;
+    // a thread's first chunks are asked for before its sequence is looked up
+    float first[APPEND_AHEAD][8];
+#pragma unroll
+    for (int u = 0; u < APPEND_AHEAD; ++u) {
+        const int c = min((int)threadIdx.x + u * APPEND_THREADS, chunks - 1);
+        append_load8<XD, VEC>(a.qkv, xrow + 8 * (int64_t)c, first[u]);
+    }
     PagedSpan sp;
     const int seq = paged_seq_of_row(a.batch, row, &sp);
     if (seq < 0) return;                                   // behind the last sequence: left as it is
     const int p = sp.position(row - sp.row0);
-    const PagedKv& kv = a.kv;
     // a row without a place: no position, past the table or the rotary table, a page that does not exist
     int slot0 = -1;                                        // slot of kv head 0
     if (p >= 0 && p < a.batch.positions && (a.rot == 0 || p < a.rope_positions)) {
@@ -58,14 +74,10 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
         const int page = a.batch.table[(int64_t)seq * a.batch.width + pi];
         if (page >= 0 && page < kv.num_pages) slot0 = kv.slot(page, 0, p - pi * kv.page.div);
     }
-    const int D = kv.D, cpr = D / 8, half = a.rot / 2;
-    const int chunks = (a.heads + 2 * kv.kv_heads) * cpr;
-    const int64_t xrow = (int64_t)row * a.ld;
     const float* cs = a.rope + (int64_t)p * a.rot;         // [rot / 2][2], read only with a place
-    for (int c = (int)threadIdx.x; c < chunks; c += APPEND_THREADS) {
+    auto make = [&](int c, const float (&v)[8]) {
         const int head = a.chunk.quotient(c), d = 8 * (c - head * cpr);
-        float v[8], o[8];
-        append_load8<XD, VEC>(a.qkv, xrow + (int64_t)head * D + d, v);
+        float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = v[e];
         if (d < a.rot && head < a.heads + kv.kv_heads && slot0 >= 0) {
@@ -83,10 +95,12 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
                 const int i = first ? d : d - half;
                 float w[8];
                 append_load8<XD, VEC>(a.qkv, h0 + (first ? d + half : i), w);
+                const f32x4_any* t = reinterpret_cast<const f32x4_any*>(cs + 2 * i);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float co = cs[2 * (i + e)], si = cs[2 * (i + e) + 1];
-                    o[e] = v[e] * co + (first ? -w[e] : w[e]) * si;
+                for (int e = 0; e < 8; e += 2) {
+                    const f32x4_any q = t[e / 2];
+                    o[e] = v[e] * q[0] + (first ? -w[e] : w[e]) * q[1];
+                    o[e + 1] = v[e + 1] * q[2] + (first ? -w[e + 1] : w[e + 1]) * q[3];
                 }
             } else {
 #pragma unroll
@@ -102,9 +116,11 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
         }
         u32x4 out;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            out[j] = kv.dtype == MVLM_F16 ? (uint32_t)f32_to_f16_bits(o[2 * j]) | (uint32_t)f32_to_f16_bits(o[2 * j + 1]) << 16
-                                          : (uint32_t)f32_to_bf16_bits(o[2 * j]) | (uint32_t)f32_to_bf16_bits(o[2 * j + 1]) << 16;
+        for (int j = 0; j < 4; ++j) {
+            const f32x2 pair = {o[2 * j], o[2 * j + 1]};
+            out[j] = kv.dtype == MVLM_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2_t))
+                                          : __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_t));
+        }
         if (head < a.heads) {
             if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
             *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.heads + head) * D + d) = out;
@@ -114,6 +130,14 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
             const int64_t at = (int64_t)(slot0 + h * kv.page.div) * D + d;
             *reinterpret_cast<u32x4*>((key ? kv.k : kv.v) + at) = out;
         }
+    };
+#pragma unroll
+    for (int u = 0; u < APPEND_AHEAD; ++u)
+        if ((int)threadIdx.x + u * APPEND_THREADS < chunks) make((int)threadIdx.x + u * APPEND_THREADS, first[u]);
+    for (int c = (int)threadIdx.x + APPEND_AHEAD * APPEND_THREADS; c < chunks; c += APPEND_THREADS) {
+        float v[8];
+        append_load8<XD, VEC>(a.qkv, xrow + 8 * (int64_t)c, v);
+        make(c, v);
     }
 }
 
