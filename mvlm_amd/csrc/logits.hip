@@ -116,16 +116,14 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
     const int v0 = ((int)blockIdx.x - row * a.slices) * SLICE, size = min(SLICE, a.n - v0);
     const int tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.ld + v0;
+    __shared__ uint32_t allow[SLICE / 32];
     float v[NV][N];
-    uint32_t mask[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int t = (i * THREADS + tid) * N;
         load_logits<DT, N, VEC>(a.x, base + t, size - t, v[i]);
-        mask[i] = 0xFFFFFFFFu;
-        if (a.allowed && t < size)
-            mask[i] = a.allowed[(int64_t)row * ((a.n + 31) / 32) + ((v0 + t) >> 5)] >> ((v0 + t) & 31);
     }
+    if (a.allowed && 32 * tid < size) allow[tid] = a.allowed[(int64_t)row * ((a.n + 31) / 32) + v0 / 32 + tid];
     ListShare<THREADS, LOGITS_IDS> history(a.penalties ? a.history + (int64_t)row * a.history_width : nullptr,
                                            a.history_width, tid);
     ListShare<THREADS, 1> biases(a.bias_ids ? a.bias_ids + (int64_t)row * a.bias_width : nullptr, a.bias_width, tid);
@@ -182,9 +180,12 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
                     if (w[e]) v[i][q + e] += bias[w[e] - 1];
             }
         }
+        if (a.allowed && t < size) {
+            const uint32_t mask = allow[t >> 5] >> (t & 31);
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (!((mask[i] >> e) & 1u)) v[i][e] = -INFINITY;
+            for (int e = 0; e < N; ++e)
+                if (!((mask >> e) & 1u)) v[i][e] = -INFINITY;
+        }
         store_logits<DT, N, VEC>(a.out, base + t, size - t, v[i]);
     }
 }
