@@ -373,7 +373,7 @@ typedef struct mvlm_rope {
  * row's position (rope NULL: not) in fp32; q goes to q_out [rows][num_heads]
  * [head_dim] and keys and values into the cache, rounded to its type.  A row
  * without a place (no position, no page, or past the rope table) writes zeros to
- * q_out and nothing to the cache. */
+ * q_out and nothing to the cache.  No two rows of a call may have the same place. */
 int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
                          const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
                          mvlm_buffer* q_out, const mvlm_rope* rope, mvlm_event** ev);
@@ -381,7 +381,10 @@ int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, 
  * group = num_heads / kv_heads, over the positions t up to row r's own that exist
  * (what lies in others may be anything).  Q [rows][num_heads][head_dim] in the
  * cache's type, O the same shape in F32 or the cache's type; scale 0:
- * 1/sqrt(head_dim).  A row that sees no position, or only scores of -inf, is 0. */
+ * 1/sqrt(head_dim).  A row that sees no position, or only scores of -inf, is 0.
+ * A value that is not finite makes its element of the rows that see it not
+ * finite (an infinity may become NaN in an F32 O: probabilities are multiplied in
+ * parts) and reaches no other row. */
 int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
                          const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
                          mvlm_event** ev);

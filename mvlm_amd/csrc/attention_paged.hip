@@ -40,7 +40,7 @@ template <int R, int KS, bool BF, int PP, int NW>
 __global__ __launch_bounds__(64 * NW, KS <= 2 && NW == 4 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
-    const PagedShare share = paged_share<R, false>(a);
+    const PagedShare share = paged_share<R, false>(a, paged_lane_span(a.batch, (int)(threadIdx.x & 63)), a.few_rows);
     if (index < share.items) paged_few_item<R, KS, BF, PP, NW>(a, share, index, h, lds);
 }
 
@@ -64,11 +64,13 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const PagedSeqs& b = a->batch;
     const int64_t f = (int64_t)b.rows * a->group;
     a->few = a->many = PagedDivision{};
-    // Tiles of 256 rows pay once they give every CU a block, alone or with the keys that
-    // the tables can hold split; below that tiles of 32 make more of the chip.
+    // Tiles of 256 rows pay once they give every CU a block, alone or with their keys split;
+    // below that tiles of 32 make more of the chip (768 rows of 32 heads: 14 us, 32 in tiles
+    // of 256).  Here by what the tables can hold, in the kernel by what they do hold.
     const int64_t tiles256 = f / CHUNK_R * a->kv.kv_heads;
     const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
     a->few_rows = many ? PAGED_FEW : INT_MAX;
+    a->many_least = (num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
     if (many) {
         // a sequence with more than PAGED_FEW f-rows ends in one tile that is not full
         const int64_t tiles = f / CHUNK_R + std::min<int64_t>(b.seqs, f / PAGED_FEW + 1);

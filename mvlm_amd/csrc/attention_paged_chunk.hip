@@ -36,6 +36,7 @@
 #include "attention_paged.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace mvlm {
 
@@ -381,12 +382,27 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     if (it.record >= 0) paged_merge<BF, R, CHUNK_THREADS>(a, a.many, it, h, (uint32_t*)lds);
 }
 
+// Full tiles of 256 rows per kv head, each times the splits its keys could make: whether
+// they would fill the chip (plan_attention_paged asks the same of what the tables can
+// hold).
+__device__ __forceinline__ int chunk_worth(const PagedAttnArgs& a, const PagedSpan& first) {
+    int worth = 0;
+    for (int base = 0; base < a.batch.seqs; base += 64) {
+        const PagedSpan p = base ? paged_lane_span(a.batch, base + (int)(threadIdx.x & 63)) : first;
+        const int64_t tiles = (int64_t)p.n * a.group / CHUNK_R;
+        worth = min(worth + (int)min(tiles, (int64_t)4096) * min(max(p.len / CHUNK_UNIT, 1), 4096), 1 << 24);
+    }
+    return __builtin_amdgcn_readlane(wave_scan(worth), 63);
+}
+
 template <int KS, int DT, bool BF, int PP>
 __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int kv_heads = a.kv.kv_heads, q = (int)blockIdx.x % PAGED_QUEUES, own = (int)blockIdx.x / PAGED_QUEUES;
     const int blocks = ((int)gridDim.x - q + PAGED_QUEUES - 1) / PAGED_QUEUES;              // of this queue
-    const PagedShare many = paged_share<CHUNK_R, true>(a), few = paged_share<32, false>(a);
+    const PagedSpan span = paged_lane_span(a.batch, (int)(threadIdx.x & 63));
+    const int few_rows = chunk_worth(a, span) >= a.many_least ? a.few_rows : INT_MAX;
+    const PagedShare many = paged_share<CHUNK_R, true>(a, span, few_rows), few = paged_share<32, false>(a, span, few_rows);
     const int many_items = (many.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     const int all_items = many_items + (few.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     for (int round = 0; round * blocks < all_items; ++round) {

@@ -45,6 +45,7 @@ struct PagedAttnArgs {
     // rows, f = n group <= few_rows, and of those with more
     int few_rows;
     PagedDivision few, many;
+    int many_least;                // tiles per kv head, times what their keys can be split, that are worth the second kernel
 };
 
 hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a);
@@ -124,23 +125,24 @@ __device__ __forceinline__ PagedSpan paged_lane_span(const PagedSeqs& b, int s) 
 
 // A share's keys per block and its items per kv head, the same in all lanes.
 struct PagedShare {
-    int unit, items;
+    int unit, items, few_rows;
     PagedSpan first;               // of the lane-th sequence
 };
 __device__ __forceinline__ int paged_splits(int len, int unit) { return len > unit ? (len + unit - 1) / unit : 1; }
 
+// few_rows: the f-rows up to which a sequence belongs to the first share
 template <int R, bool MANY>
-__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
+__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, const PagedSpan& sp, int few_rows) {
     const PagedSeqs& b = a.batch;
     const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
-    const PagedSpan sp = paged_lane_span(b, lane);
     PagedShare sh;
     sh.first = sp;
+    sh.few_rows = few_rows;
     int64_t total = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        total += (int64_t)paged_tiles<R, MANY>(p, a.group, a.few_rows) * p.len;
+        total += (int64_t)paged_tiles<R, MANY>(p, a.group, few_rows) * p.len;
     }
     // summed over the lanes as two numbers of 24 and 30 bits; read from one lane, so that
     // no branch on it is taken as divergent
@@ -150,7 +152,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a) {
     int items = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        items += paged_tiles<R, MANY>(p, a.group, a.few_rows) * paged_splits(p.len, sh.unit);
+        items += paged_tiles<R, MANY>(p, a.group, few_rows) * paged_splits(p.len, sh.unit);
     }
     items = __builtin_amdgcn_readlane(wave_scan(items), 63);
     // no more than planned for, whatever row_start holds
@@ -167,7 +169,7 @@ __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, const Paged
     int first = 0, record = 0;                             // items and records before this round of sequences
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan sp = base ? paged_lane_span(b, base + lane) : share.first;
-        const int tiles = paged_tiles<R, MANY>(sp, a.group, a.few_rows), splits = paged_splits(sp.len, share.unit);
+        const int tiles = paged_tiles<R, MANY>(sp, a.group, share.few_rows), splits = paged_splits(sp.len, share.unit);
         const int items = tiles * splits, records = splits > 1 ? tiles * splits : 0;
         const int end = first + wave_scan(items), rec_end = record + wave_scan(records);
         const uint64_t mine = __builtin_amdgcn_ballot_w64(index >= end - items && index < end);

@@ -84,11 +84,10 @@ def filled_cache(rng, batch, kv_heads, D, dtype, std=1.0):
     """Values at every position the sequences hold, NaN elsewhere."""
     K, V = nan_cache(batch, kv_heads, D, dtype)
     for s, L in enumerate(batch.lens):
-        for t in range(min(L, batch.width * batch.page)):
-            at = batch.place(s, t)
-            if at:
-                K[at[0], :, at[1]] = values(rng, (kv_heads, D), dtype, std)
-                V[at[0], :, at[1]] = values(rng, (kv_heads, D), dtype)
+        at = np.array([a for a in (batch.place(s, t) for t in range(min(L, batch.width * batch.page))) if a])
+        if len(at):
+            K[at[:, 0], :, at[:, 1]] = values(rng, (len(at), kv_heads, D), dtype, std)
+            V[at[:, 0], :, at[:, 1]] = values(rng, (len(at), kv_heads, D), dtype)
     return K, V
 
 
@@ -117,24 +116,31 @@ def attention(batch, q, K, V, dtype, scale, parts):
     O, tol = np.full(q.shape, np.nan), np.zeros(q.shape)
     qd, Kd, Vd = from_bits(q, dtype), from_bits(K, dtype), from_bits(V, dtype)
     uP = HALF_STEP[dtype] if parts == 1 else 2.0 ** -22
-    for r, s, p in batch.each_row():
-        at = [a for a in (batch.place(s, t) for t in range(min(p, batch.width * batch.page - 1) + 1)) if a]
-        if not at:
-            O[r] = 0.0
+    for s, (n, L) in enumerate(zip(batch.news, batch.lens)):
+        if n == 0:
             continue
-        pg, sl = np.array([a[0] for a in at]), np.array([a[1] for a in at])
+        r0 = int(batch.start[s])
+        held = [t for t in range(min(L, batch.width * batch.page)) if batch.place(s, t)]
+        pos = L - n + np.arange(n)
+        O[r0:r0 + n] = 0.0
+        if not held or pos[-1] < held[0]:
+            continue
+        at = np.array([batch.place(s, t) for t in held])
+        seen = np.array(held)[None, :] <= pos[:, None]              # [n][keys]
+        N = seen.sum(1)[:, None]
+        some = N[:, 0] > 0
         for h in range(heads):
-            k, v = Kd[pg, h // group, sl], Vd[pg, h // group, sl]
-            x = scale * (k @ qd[r, h])
-            R = scale * np.max(np.abs(k) @ np.abs(qd[r, h]))
-            w = np.exp(x - x.max())
-            total = w.sum()
-            O[r, h] = w @ v / total
+            k, v = Kd[at[:, 0], h // group, at[:, 1]], Vd[at[:, 0], h // group, at[:, 1]]
+            qh = qd[r0:r0 + n, h]
+            x = np.where(seen, scale * (qh @ k.T), -np.inf)
+            R = np.where(seen, scale * (np.abs(qh) @ np.abs(k).T), 0.0).max(1)[:, None]
+            w = np.exp(x - np.where(some, x.max(1), 0.0)[:, None])
+            total = np.where(some, w.sum(1), 1.0)[:, None]
+            O[r0:r0 + n, h] = w @ v / total
             A = w @ np.abs(v) / total
-            small = w < (2.0 ** -13 if parts == 1 else 2.0 ** -2)
-            F = 2.0 ** -25 * (np.abs(v[small]).sum(0) if dtype == m.F16 else 0.0) / total
-            N = len(at)
-            tol[r, h] = (uP + 4 * D * 2.0 ** -24 * R + 8 * (1 + R) * 2.0 ** -23 + 2 * (N + 64) * 2.0 ** -24) * A + F
+            small = seen & (w < (2.0 ** -13 if parts == 1 else 2.0 ** -2))
+            F = 2.0 ** -25 * (small @ np.abs(v) if dtype == m.F16 else 0.0) / total
+            tol[r0:r0 + n, h] = (uP + 4 * D * 2.0 ** -24 * R + 8 * (1 + R) * 2.0 ** -23 + 2 * (N + 64) * 2.0 ** -24) * A + F
     return O, tol
 
 

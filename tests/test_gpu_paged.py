@@ -241,6 +241,70 @@ def test_attention_not_finite_where_seen(dev):
     assert np.array_equal(np.isnan(got), seen)
 
 
+# Batches that fill the chip with tiles of 256 rows (rows x group / 256 per kv head, times
+# the thousands of keys, at least 256 / kv_heads), so the second kernel makes them.
+LARGE = [
+    ([300], [300], 256, 256, 64, 16, F16, F16, {}),
+    ([293, 1, 3], [500, 700, 3], 256, 128, 128, 48, BF16, BF16, {"lead": 1, "spare": 4}),
+    ([256, 0, 70], [256, 0, 70], 256, 64, 72, 16, F16, F32, {}),
+    ([270, 5], [333, 400], 256, 64, 80, 7, BF16, F32, {"drop": {(0, 1): -1, (0, 40): 1 << 30, (1, 0): -5}}),
+    ([290], [290], 256, 128, 96, 64, F16, F16, {"width": 4}),                # rows past the page table
+    ([260, 16], [200, 16], 256, 256, 8, 16, F16, F16, {}),                   # rows before position 0
+    ([257] * 2 + [1] * 66, [257, 300] + list(range(66)), 256, 256, 32, 32, F16, F16, {}),   # more sequences than lanes
+    ([512, 1], [4200, 9000], 32, 32, 64, 16, F16, F16, {}),                  # splits
+    ([260], [5000], 64, 64, 128, 1, BF16, BF16, {}),                         # splits of more keys than LDS holds slots for
+    ([257], [4097], 64, 64, 48, 100, F16, F32, {}),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_attention_of_many_rows(dev, case):
+    news, lens, heads, kv_heads, D, page, cd, od, opt = LARGE[case]
+    say("many rows", case, news[:4], lens[:4], *LARGE[case][2:])
+    batch = Batch(np.random.default_rng(400 + case), news, lens, page, **opt)
+    check_attention(dev, batch, heads, kv_heads, D, cd, od, 500 + case)
+
+
+def test_attention_short_rows_in_long_tables(dev):
+    """tables that could hold a million positions, of which few are held"""
+    batch = Batch(np.random.default_rng(17), [300, 1, 40], [300, 77, 40], 64, width=16384)
+    check_attention(dev, batch, 4, 2, 64, F16, F16, 18)
+
+
+@pytest.mark.parametrize("news,lens,heads,kv_heads,D,cd,od,key", [
+    ([40], [100], 4, 2, 64, F16, F16, 83), ([40], [40], 2, 2, 128, BF16, F32, 17), ([33], [33], 3, 3, 72, F16, F32, 32),
+    ([300], [300], 256, 256, 64, F16, F16, 200), ([256], [600], 256, 128, 128, BF16, BF16, 500)])
+def test_attention_hidden_values_may_be_anything(dev, news, lens, heads, kv_heads, D, cd, od, key):
+    """infinite and NaN values of a new position reach the rows that see it and no row before"""
+    say("not finite at", key, news, lens, heads, kv_heads, D)
+    rng = np.random.default_rng(19)
+    batch = Batch(rng, news, lens, 16)
+    K, V = filled_cache(rng, batch, kv_heads, D, cd)
+    q = values(rng, (batch.rows, heads, D), cd)
+    inf, nan = (0x7C00, 0x7E00) if cd == F16 else (0x7F80, 0x7FC0)
+    page, slot = batch.place(0, key)
+    V[page, :, slot, 1], V[page, :, slot, D - 1], V[page, 0, slot, 5] = inf, nan, inf | 0x8000
+    got = run_attention(dev, batch, q, K, V, cd, od, heads)
+    clean = V.copy()
+    clean[page, :, slot, 1] = clean[page, :, slot, D - 1] = clean[page, 0, slot, 5] = 0
+    ref, tol = attention(batch, q, K, clean, cd, D ** -0.5, 1 if od != F32 else 2)
+    sees = np.arange(news[0]) >= key - (lens[0] - news[0])
+    group = heads // kv_heads
+    bad = np.zeros(got.shape, bool)
+    bad[np.ix_(sees, np.arange(heads), [1, D - 1])] = True
+    bad[np.ix_(sees, np.arange(group), [5])] = True
+    assert np.all(np.isnan(got[sees][:, :, D - 1]))
+    if od != F32:
+        assert np.all(got[sees][:, :, 1] == np.inf) and np.all(got[sees][:, :group, 5] == -np.inf)
+    else:
+        # p = hi + lo (+ lower) with lo = p - round(p), which is 0 or negative as often as positive: p inf is
+        # hi inf + lo inf, so inf + 0 inf = NaN or inf - inf = NaN, or inf
+        assert not np.any(np.isfinite(got[sees][:, :, 1])) and not np.any(np.isfinite(got[sees][:, :group, 5]))
+        assert not np.any(got[sees][:, :, 1] == -np.inf) and not np.any(got[sees][:, :group, 5] == np.inf)
+    got[bad] = ref[bad] = 0.0
+    assert same_or_close(got, ref, tol, od) <= 1.0
+
+
 # ---- plans ------------------------------------------------------------------------------
 
 def test_plan_replays_as_lengths_grow(dev):
@@ -285,3 +349,117 @@ def test_plan_replays_as_lengths_grow(dev):
         K, V = gK, gV
     ms = plan.profile()
     assert len(ms) == 2 and np.all(ms > 0)
+
+
+def test_graphs_of_one_device_share_workspaces(dev):
+    """two captured graphs, both with split attention, replayed in turn with eager calls between"""
+    rng = np.random.default_rng(31)
+    jobs = []
+    for news, lens, heads, kv_heads, ragged in (([1] * 3, [3000, 20, 1500], 8, 2, False), ([512, 1], [4200, 600], 32, 32, True)):
+        batch = Batch(rng, news, lens, 16, ragged=ragged)
+        K, V = filled_cache(rng, batch, kv_heads, 64, F16)
+        q = dev.upload(values(rng, (batch.rows, heads, 64), F16))
+        cache, b = cache_on(dev, batch, K, V, F16), batch.device(dev)
+        o, eager = (dev.alloc(batch.rows * heads * 64 * 4).zero() for _ in range(2))
+        dev.attention_paged(q, b, cache, eager, F32, heads)
+        plan = m.Plan(dev)
+        plan.add_attention_paged(q, b, cache, o, F32, heads)
+        plan.use_graph(True)
+        jobs.append((plan, o, eager.download(np.uint32), (q, b, cache, eager, heads)))
+    for turn in range(3):
+        for plan, o, _, _ in jobs:
+            o.zero()
+            plan.run(2)
+        for plan, o, first, (q, b, cache, eager, heads) in jobs:
+            dev.attention_paged(q, b, cache, eager, F32, heads)
+            assert np.array_equal(o.download(np.uint32), first)
+            assert np.array_equal(eager.download(np.uint32), first)
+
+
+def test_two_handles_at_once(dev):
+    """two device handles have streams, workspaces and counters of their own"""
+    other = m.Device(0)
+    rng = np.random.default_rng(33)
+    work = []
+    for d in (dev, other):
+        batch = Batch(rng, [1] * 4, [2500, 900, 3100, 40], 16, ragged=False)
+        K, V = filled_cache(rng, batch, 4, 64, F16)
+        q = d.upload(values(rng, (4, 8, 64), F16))
+        work.append((d, q, batch.device(d), cache_on(d, batch, K, V, F16), [d.alloc(4 * 8 * 64 * 4) for _ in range(20)]))
+    for i in range(20):
+        for d, q, b, cache, outs in work:
+            d.attention_paged(q, b, cache, outs[i], F32, 8)
+    for d, q, b, cache, outs in work:
+        first = outs[0].download(np.uint32)
+        assert all(np.array_equal(o.download(np.uint32), first) for o in outs)
+    del work, d, q, b, cache, outs
+    other.close()
+
+
+def test_a_step_of_a_batch(dev, orc):
+    """the operators together, as one graph: quantized QKV products, append, attention, dense product with
+    residual, LM head, logits, pick; the tokens' histories and lengths move on between the replays"""
+    rng = np.random.default_rng(35)
+    S, heads, D, vocab, page, steps = 5, 4, 64, 1000, 16, 4
+    hidden = heads * D
+    W = {n: dev.random_weight(m.Q8_0, rows, hidden, 71 + i, 0.05) for i, (n, rows) in
+         enumerate((("qkv", 3 * hidden), ("dense", hidden), ("head", vocab)))}
+    deq = {n: w.dequant().astype(np.float64) for n, w in W.items()}
+    lens = np.array([0, 3, 15, 40, 100], np.int32)
+    batch = Batch(rng, [1] * S, lens + steps, page, ragged=False)
+    batch.lens = [int(v) for v in lens]
+    K, V = filled_cache(rng, batch, heads, D, F16)
+    cache = cache_on(dev, batch, K, V, F16)
+    b = batch.device(dev)
+    x, qkv, o, y, logits, out = (dev.alloc(S * n * 4) for n in (hidden, 3 * hidden, hidden, hidden, vocab, vocab))
+    q, token = dev.alloc(S * hidden * 2), dev.alloc(S * 4)
+    history, hlen = dev.alloc(S * steps * 4).zero(), dev.alloc(S * 4).zero()
+    pen = np.tile(np.array([[1.3, 0.4, 0.2]], np.float32), (S, 1))
+    controls = m.LogitControls(history=history, history_len=hlen, history_width=steps, penalties=dev.upload(pen))
+    table = rope_table(200, D)
+    plan = m.Plan(dev)
+    plan.add_gemm_quant_grouped(S, [(x, F32, W["qkv"], qkv, F32)])
+    plan.add_kv_append_paged(qkv, F32, 3 * hidden, b, cache, heads, q, m.Rope(dev.upload(table), 200, D))
+    plan.add_attention_paged(q, b, cache, o, F32, heads)
+    plan.add_gemm_quant_grouped(S, [(o, F32, W["dense"], y, F32)], epilogues=[{"residual": x}])
+    plan.add_gemv(y, F32, W["head"], logits, F32, S)
+    plan.add_logits_process(logits, F32, S, vocab, vocab, controls, out)
+    plan.add_argmax(out, F32, S, vocab, vocab, token)
+    plan.use_graph(True)
+    seen = np.zeros((S, steps), np.int32)
+    for step in range(steps):
+        lens = lens + 1
+        batch.lens = [int(v) for v in lens]
+        b.buffers[0].upload(lens)
+        xs = rng.standard_normal((S, hidden)).astype(np.float32)
+        x.upload(xs)
+        history.upload(seen)
+        hlen.upload(np.full(S, step, np.int32))
+        plan.run()
+        # each stage against its definition on the values that the stage before it stored
+        got = {n: buf.download(np.float32).reshape(S, -1).astype(np.float64) for n, buf in
+               (("qkv", qkv), ("o", o), ("y", y), ("logits", logits), ("out", out))}
+        ref, S_ = xs.astype(np.float64) @ deq["qkv"].T, np.abs(xs.astype(np.float64)) @ np.abs(deq["qkv"]).T
+        assert np.all(np.abs(got["qkv"] - ref) <= 1e-5 * S_)
+        gq = q.download(np.uint16).reshape(S, heads, D)
+        gK, gV = (c.download(np.uint16).reshape(K.shape) for c in cache.buffers)
+        ref, qt, rK, rV, Kt = append_reference(batch, got["qkv"], heads, heads, D, F16, table, D, False, K, V)
+        assert same_or_close(from_bits(gq, F16), ref, qt, F16) <= 1.0
+        assert same_or_close(from_bits(gK, F16), rK, Kt, F16) <= 1.0
+        assert same_or_close(from_bits(gV, F16), rV, np.zeros(V.shape), F16) <= 1.0
+        K, V = gK, gV
+        ref, tol = attention(batch, gq, gK, gV, F16, D ** -0.5, 2)
+        assert same_or_close(got["o"].reshape(S, heads, D), ref, tol, F32) <= 1.0
+        ref, S_ = got["o"] @ deq["dense"].T + xs, np.abs(got["o"]) @ np.abs(deq["dense"]).T + np.abs(xs)
+        assert np.all(np.abs(got["y"] - ref) <= 1e-5 * S_)
+        ref, S_ = got["y"] @ deq["head"].T, np.abs(got["y"]) @ np.abs(deq["head"]).T
+        assert np.all(np.abs(got["logits"] - ref) <= 1e-5 * S_)
+        ref = got["logits"].copy()
+        for r in range(S):
+            ids, times = np.unique(seen[r, :step], return_counts=True)
+            z = ref[r, ids]
+            ref[r, ids] = np.where(z > 0, z / np.float64(pen[0, 0]), z * np.float64(pen[0, 0])) - (times * np.float64(pen[0, 1]) + np.float64(pen[0, 2]))
+        assert np.all(np.abs(got["out"] - ref) <= 4 * 2.0 ** -24 * (np.abs(ref) + 3.0))
+        picked = token.download(np.int32)
+        assert np.array_equal(picked, np.argmax(got["out"], 1))
+        seen[:, step] = picked
