@@ -67,7 +67,8 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     // Tiles of 256 rows pay once they give every CU a block, alone or with their keys split;
     // below that tiles of 32 make more of the chip (768 rows of 32 heads: 14 us, 32 in tiles
     // of 256).  Here by what the tables can hold, in the kernel by what they do hold.
-    const int64_t tiles256 = f / CHUNK_R * a->kv.kv_heads;
+    const bool single = !b.row_start;                          // every sequence has `group` f-rows
+    const int64_t tiles256 = (single ? (int64_t)b.seqs * (a->group / CHUNK_R) : f / CHUNK_R) * a->kv.kv_heads;
     const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
     a->few_rows = many ? PAGED_FEW : INT_MAX;
     a->many_least = (num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
@@ -76,7 +77,6 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
         const int64_t tiles = f / CHUNK_R + std::min<int64_t>(b.seqs, f / PAGED_FEW + 1);
         a->many = paged_divide(*a, CHUNK_R, num_cus, tiles, CHUNK_UNIT, CHUNK_KEYS);
     }
-    const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int R = single && a->group <= 16 && !many ? 16 : 32;
     const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + R - 1) / R) : f / R + b.seqs;
     // blocks wanted per CU, measured at 1.. 6: 16 rows 2 (16 sequences up to 2047: 30.6 us, 33.3 at
