@@ -347,8 +347,9 @@ typedef struct mvlm_paged_kv {
  * slot t % page_size of page page_table[s][t / page_size].  A place that the
  * table does not have, or a page outside [0, num_pages), does not exist: it is
  * neither read nor written.  A sequence with kv_len 0 is idle.  Rows of no
- * sequence are left as they were.  At most 65536 sequences, 2^22 rows and 2^30
- * positions in a table. */
+ * sequence are left as they were.  Starts that decrease name no batch: such a call
+ * may do any part of its work, but touches nothing else and harms no later call.
+ * At most 65536 sequences, 2^22 rows and 2^30 positions in a table. */
 typedef struct mvlm_paged_batch {
     int num_seqs;
     int rows;

@@ -455,7 +455,8 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     a.group = num_heads / a.kv.kv_heads;
     a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)a.kv.D) : scale) * 1.4426950408889634f;
     plan_attention_paged(&a, dev->prop.multiProcessorCount);
-    REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads <= (1 << 30), "%s: shape too large", fn);
+    // a launch holds fewer than 2^32 threads, 512 in a block at most
+    REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads < (1 << 23), "%s: shape too large", fn);
     // the shares run in one launch: partial results and counters of their own
     const size_t few = (paged_ws_bytes(a, a.few) + 255) & ~(size_t)255, many = paged_ws_bytes(a, a.many);
     const size_t few_words = paged_words(a, a.few), words = few_words + paged_words(a, a.many);
@@ -481,7 +482,8 @@ int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     REQUIRE(x->dev == dev && out->dev == dev, "%s: buffers belong to another device", fn);
     REQUIRE(is_dense(dtype), "%s: dtype %d is not F32/F16/BF16", fn, dtype);
     REQUIRE(rows > 0 && n > 0 && ld >= n && ld <= ((int64_t)1 << 40), "%s: rows=%d n=%d ld=%lld", fn, rows, n, (long long)ld);
-    REQUIRE(rows <= (1 << 20) && n <= (1 << 30) && (int64_t)rows * ((n + 1023) / 1024) <= INT_MAX, "%s: shape too large", fn);
+    // slices of 4096 tokens, 512 threads each (launch_logits): a launch holds fewer than 2^32
+    REQUIRE(rows <= (1 << 20) && n <= (1 << 30) && (int64_t)rows * ((n + 4095) / 4096) < (1 << 23), "%s: shape too large", fn);
     const size_t es = dtype_size(dtype), bytes = ((size_t)(rows - 1) * (size_t)ld + (size_t)n) * es, R = (size_t)rows;
     NEED(x, bytes, "x");
     NEED(out, bytes, "out");

@@ -149,18 +149,22 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, const 
     const int64_t lo = __builtin_amdgcn_readlane(wave_scan((int)(total & 0xFFFFFF)), 63);
     const int64_t hi = __builtin_amdgcn_readlane(wave_scan((int)(total >> 24)), 63);
     sh.unit = paged_unit(div, (hi << 24) + lo);
+    // A batch whose starts do not decrease makes no more items than were planned for
+    // (paged_divide).  One that makes more is not begun at all, so that no counter of
+    // splits is left in mid-count; the sum stops short of 2^31.
+    constexpr int MOST = 1 << 24;
     int items = 0;
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan p = base ? paged_lane_span(b, base + lane) : sp;
-        items += paged_tiles<R, MANY>(p, a.group, few_rows) * paged_splits(p.len, sh.unit);
+        const int64_t more = (int64_t)paged_tiles<R, MANY>(p, a.group, few_rows) * paged_splits(p.len, sh.unit);
+        items += (int)(more < MOST - items ? more : MOST - items);
     }
-    items = __builtin_amdgcn_readlane(wave_scan(items), 63);
-    // no more than planned for, whatever row_start holds
-    sh.items = items < 0 || items > div.items ? div.items : items;
+    sh.items = __builtin_amdgcn_readlane(wave_scan(items), 63);
+    if (sh.items > div.items) sh.items = 0;
     return sh;
 }
 
-// The index-th item of a share, the same in all lanes; false if there is none.
+// The index-th item of a share, below its items, the same in all lanes; false if there is none.
 template <int R, bool MANY>
 __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, const PagedShare& share, int index, PagedItem* out) {
     const PagedSeqs& b = a.batch;
@@ -184,8 +188,8 @@ __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, const Paged
             out->tile = at(tiles) - 1 - nth;               // the last tile sees the most keys: it starts first
             out->split = r - nth * ns;
             out->record = ns > 1 ? at(rec_end - records) + nth * ns : -1;
-            // a batch whose starts decrease can exceed the items and records planned for: refused here
-            return out->tile >= 0 && (ns == 1 || (out->record >= 0 && out->record <= div.records - ns));
+            // no batch has more records than planned for (paged_divide); a tile's splits agree on it
+            return ns == 1 || out->record <= div.records - ns;
         }
         first = __builtin_amdgcn_readlane(end, 63);
         record = __builtin_amdgcn_readlane(rec_end, 63);

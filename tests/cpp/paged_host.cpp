@@ -157,6 +157,11 @@ static void test_paged_refusals() {
     refuses(BAD, "misaligned O", [](Append& a) { a.o = buffer(1 << 20, 0x90000008); }, false);
     refuses(BAD, "O is Q", [](Append& a) { a.o = a.q; }, false);
     refuses(BAD, "O in the cache", [](Append& a) { a.o = a.v; }, false);
+    refuses(BAD, "more blocks than a launch takes", [](Append& a) {
+        a.batch = mvlm_paged_batch{65536, 65536, nullptr, &a.len, &a.table, 1};
+        a.kv.kv_heads = a.heads = 128;
+        for (mvlm_buffer* b : {&a.k, &a.v, &a.len, &a.table, &a.q, &a.o}) b->ptr = (void*)((uintptr_t)b->ptr << 8), b->bytes = (size_t)1 << 33;
+    }, false);
     refuses(BAD, "O over kv_len", [](Append& a) { a.len = buffer(16, 0x90000000); }, false);
     Append a;
     CHECK(mvlm_kv_append_paged(nullptr, &a.x, 0, a.ld, &a.batch, &a.kv, 8, &a.q, nullptr, nullptr) == BAD, "null device");
@@ -194,6 +199,7 @@ static void test_logits_refusals() {
     refuses_logits(BAD, "no tokens", [](Logits& a) { a.n = 0; });
     refuses_logits(BAD, "short ld", [](Logits& a) { a.ld = 999; });
     refuses_logits(BAD, "too many rows", [](Logits& a) { a.rows = (1 << 20) + 1; });
+    refuses_logits(BAD, "more blocks than a launch takes", [](Logits& a) { a.rows = 1 << 20, a.n = 7 * 4096 + 1, a.ld = a.n; });
     refuses_logits(BAD, "huge ld", [](Logits& a) { a.ld = INT64_MAX; });
     refuses_logits(SMALL, "short x", [](Logits& a) { a.x.bytes -= 1; });
     refuses_logits(SMALL, "short out", [](Logits& a) { a.out.bytes -= 1; });

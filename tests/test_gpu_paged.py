@@ -265,6 +265,20 @@ def test_attention_of_many_rows(dev, case):
     check_attention(dev, batch, heads, kv_heads, D, cd, od, 500 + case)
 
 
+def test_attention_single_rows_of_many_heads(dev):
+    """one row of 256 heads per sequence: a tile of 256 rows each, in tables that could hold a lot"""
+    batch = Batch(np.random.default_rng(23), [1] * 3, [700, 0, 2100], 64, ragged=False, width=2048)
+    check_attention(dev, batch, 512, 2, 64, F16, F16, 24)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_of_more_sequences_than_lanes(dev, ragged):
+    lens = [(37 * i) % 90 for i in range(150)]
+    lens[149] = 2500
+    batch = Batch(np.random.default_rng(25), [1] * 150, lens, 16, ragged=ragged)
+    check_attention(dev, batch, 8, 2, 64, F16, F32, 26)
+
+
 def test_attention_short_rows_in_long_tables(dev):
     """tables that could hold a million positions, of which few are held"""
     batch = Batch(np.random.default_rng(17), [300, 1, 40], [300, 77, 40], 64, width=16384)
@@ -303,6 +317,31 @@ def test_attention_hidden_values_may_be_anything(dev, news, lens, heads, kv_head
         assert not np.any(got[sees][:, :, 1] == -np.inf) and not np.any(got[sees][:, :group, 5] == np.inf)
     got[bad] = ref[bad] = 0.0
     assert same_or_close(got, ref, tol, od) <= 1.0
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows,seqs", [(4, 2, 64, 200), (64, 64, 300, 80)])
+def test_starts_that_decrease_leave_no_trace(dev, heads, kv_heads, rows, seqs):
+    """a row_start that goes back and forth asks for more work than any batch of these rows; whatever it
+    leaves undone, the calls after it, whose split keys are counted in the same words, are right"""
+    say("decreasing starts", heads, kv_heads, rows, seqs)
+    rng = np.random.default_rng(37)
+    good = Batch(rng, [rows], [3000], 16)
+    K, V = filled_cache(rng, good, kv_heads, 64, F16)
+    bits = values(rng, (rows, heads, 64), F16)
+    q, cache, b = dev.upload(bits), cache_on(dev, good, K, V, F16), good.device(dev)
+    start = np.array([0, rows] * (seqs // 2 + 1), np.int32)[:seqs + 1]
+    wild = m.PagedBatch(seqs, rows, dev.upload(np.full(seqs, 3000, np.int32)), dev.upload(np.repeat(good.table, seqs, 0)),
+                        good.width, row_start=dev.upload(start))
+    qkv = dev.upload(np.zeros((rows, (heads + 2 * kv_heads) * 64), np.float32))
+    outs = [dev.alloc(rows * heads * 64 * 2) for _ in range(3)]
+    for o in outs:
+        dev.attention_paged(q, b, cache, o, F16, heads)
+        dev.attention_paged(q, wild, cache, dev.alloc(o.nbytes), F16, heads)
+        dev.kv_append_paged(qkv, F32, (heads + 2 * kv_heads) * 64, wild, cache_on(dev, good, K, V, F16), heads, dev.alloc(o.nbytes), None)
+    ref, tol = attention(good, bits, K, V, F16, 64 ** -0.5, 1)
+    first = outs[0].download(np.uint16)
+    assert same_or_close(from_bits(first.reshape(ref.shape), F16), ref, tol, F16) <= 1.0
+    assert all(np.array_equal(o.download(np.uint16), first) for o in outs)
 
 
 # ---- plans ------------------------------------------------------------------------------
