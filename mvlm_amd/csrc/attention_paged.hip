@@ -4,23 +4,26 @@
 // fp16 or bf16, fp32 scores and softmax, O fp32 or the cache's type; a row
 // that sees no key is 0.
 //
-// Few rows read many keys, so the keys' bytes bound it.  The new rows of a
-// sequence times the heads that share a kv head are one axis, cut into tiles of
-// 16: the group's heads read each key once.  The keys of a tile are cut into
-// splits so that the batch as a whole, whatever its lengths, makes about the
-// wanted number of equal blocks (paged_find); each wave of a block takes every
-// NW-th tile of 32 keys with an online softmax of its own, the block merges
-// its waves through LDS, and a second kernel merges the splits.
+// Few rows read many keys, so the keys' bytes bound it (many rows, whose products
+// do, are attention_paged_chunk.hip's).  The new rows of a sequence times the heads
+// that share a kv head are one axis, cut into tiles of R = 16 (single tokens) or 32:
+// the group's heads read each key once.  The keys of a tile are cut into splits so
+// that the batch as a whole, whatever its lengths, makes about the wanted number of
+// equal blocks (paged_share, found by every block from the lengths in device memory,
+// so that one captured launch serves every step); each wave of a block takes every
+// NW-th tile of 32 keys with an online softmax of its own, the block merges its waves
+// through LDS, and the block of a tile that ends last merges the splits (paged_merge),
+// always in their order.
 //
-//  * S^T = K Q^T, v_mfma_f32_16x16x32: A = 16 keys straight from memory in the
-//    operand's layout (lane l: key l % 16, dims 8 (l / 16) .. +7), B = Q.  Lane
-//    l's results are row l % 16 and keys 4 (l / 16) .. +3, so a row's
-//    statistics are per lane.
-//  * O^T = V^T P^T: the two S^T results of a tile are its B operand as they
-//    stand when V^T is read in the same key order, keys 4g .. 4g+3 and
-//    16+4g .. +3 for g = l / 16, which ds_read_b64_tr_b16 gives from V rows in
-//    LDS (lane 4k + i of 16 reads dims 4i .. of key k and receives dim
-//    lane % 16 of 4 keys).
+//  * S^T = K Q^T, v_mfma_f32_16x16x32 or 32x32x16: A = R keys straight from memory in
+//    the operand's layout (lane l: key l % R, 8 dims from 8 (l / R) on), B = Q.  Lane
+//    l's results are row l % R and every (64 / R)-th four keys from 4 (l / R) on, so a
+//    row's statistics are per lane.
+//  * O^T = V^T P^T: the S^T results of a tile are its B operand as they stand when V^T
+//    is read in the same key order, which ds_read_b64_tr_b16 gives from V rows in LDS
+//    (lane 4k + i of 16 reads dims 4i .. of key k and receives dim lane % 16 of 4 keys).
+//  * K and V of the next tile are asked for while this one is computed, the page of the
+//    one behind it before them: a wave has about 12 KB (head_dim 64) in flight.
 //  * P is rounded to the cache's type for a 16-bit O, as the rounding of O
 //    itself is of that size; for an fp32 O it is kept to 22 bits and more, as
 //    the sum of two fp16 or three bf16 parts, one product each.
@@ -28,6 +31,13 @@
 //    the exp2 domain), so P stays below 2^8 and most tiles rescale nothing.
 //  * hidden keys may hold anything: their scores are replaced, not added to,
 //    and their V rows are staged as zeros.
+//
+// Measured (fp16 unless said): 16 sequences of 30 .. 2047 positions, 32 heads of 64,
+// 132 MB: 31.5 us, 4.2 TB/s (a large copy reaches 5.1); 64 sequences of 1000 .. 1500:
+// 121 us, 5.4 TB/s; 4 of 20000 .. 32768, bf16, 32 heads of 128 over 8, 448 MB: 84 us,
+// 5.3 TB/s; one of 512: 7.35 us, the launch and a chain of loads (lengths, table, keys).
+// Each block walks the lengths of all sequences three times: beyond some 500 that is
+// felt (1024 sequences of 200 .. 400, 32 heads of 128 over 8: 373 us, 3.4 TB/s).
 #include "attention_paged.h"
 
 #include <algorithm>
@@ -44,8 +54,8 @@ __global__ __launch_bounds__(64 * NW, KS <= 2 && NW == 4 ? 3 : 2) void paged_att
     if (index < share.items) paged_few_item<R, KS, BF, PP, NW>(a, share, index, h, lds);
 }
 
-// Division of the sequences of at most (or of more than) PAGED_FEW f-rows: `blocks`
-// blocks are wanted.  The sum of ceil(len / unit) over tiles is at most total / unit
+// Division of one kernel's share of the sequences (those of at most few_rows f-rows, or
+// those of more) for `blocks` blocks.  The sum of ceil(len / unit) over tiles is at most total / unit
 // + tiles, and a tile is split when len > unit, so split tiles make at most
 // 2 total / unit records.
 static PagedDivision paged_divide(const PagedAttnArgs& a, int tile, int64_t blocks, int64_t tiles, int unit_min,
@@ -77,6 +87,8 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
         const int64_t tiles = f / CHUNK_R + std::min<int64_t>(b.seqs, f / PAGED_FEW + 1);
         a->many = paged_divide(*a, CHUNK_R, num_cus, tiles, CHUNK_UNIT, CHUNK_KEYS);
     }
+    // Tiles of 16 rows where no sequence has more; half of a tile of 32 would be empty (4 of 32768,
+    // D = 128: 84 us and 128; 16 of 2047 34.3 and 34.8; one of 512 7.2 and 8.9)
     const int R = single && a->group <= 16 && !many ? 16 : 32;
     const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + R - 1) / R) : f / R + b.seqs;
     // blocks wanted per CU, measured at 1.. 6: 16 rows 2 (16 sequences up to 2047: 30.6 us, 33.3 at

@@ -4,18 +4,24 @@
 // A block of eight waves owns 256 f-rows of one kv head, wave w rows 32 w .. of
 // them, and walks the keys in tiles of 64 that all its waves share.  The matrix
 // cores and the vector ALUs bound it about equally: a tile costs a wave 32
-// matrix instructions of 32 cycles and, for its 2048 scores, about as many cycles of
-// exponentials, maxima, sums and conversions.  So the two waves of a SIMD (w and
-// w + 4) alternate: while one runs the products of its tile, O^T += V^T P^T of
-// the tile before and S^T = K Q^T, the other runs its softmax, and a barrier
-// swaps them.  Phases 2i and 2i + 1 hold the products of tile i of waves 0..3 and
-// of waves 4..7, so both use K of tile i and V of tile i - 1 there, while the tiles
-// after them are on their way into the other buffers of a ring: the blocks of one kv
-// head walk its keys in step, so each tile comes from memory once for all of them
-// and its loads have to cover that latency.
+// matrix instructions of 32 cycles (head_dim 128) and, for its 2048 scores, about as
+// many cycles of exponentials, maxima, sums and conversions.  So the two waves of a
+// SIMD (w and w + 4) are half a tile apart.  Iteration i, between two barriers, holds
+// the products O^T += V^T P^T of tile i - 1 and S^T = K Q^T of tile i of all waves;
+// waves 0..3 run them first and then the softmax of tile i, waves 4..7 run the softmax
+// of tile i - 1 first and then the products, so that one wave of a SIMD has matrix
+// instructions while the other has vector ones.  The products have the higher
+// priority.  One barrier per tile is enough, as both groups read K of tile i and V of
+// tile i - 1 there, while the tiles after them are on their way into the other buffers
+// of a ring: the blocks of one kv head walk its keys in step, so each tile comes from
+// memory once for all of them and its loads have to cover that latency.
+// 2048 bf16 rows on 8192 positions, 32 heads of 128 over 8 kv heads (309 GFLOP): 298 ..
+// 316 us on different boxes, 977 .. 1037 TFLOP/s, of the 1229 .. 1275 that a large
+// library product of that type reaches here; with both groups in step 384 us, with two
+// barriers per tile 349.
 //  * K and V tiles go straight from memory to LDS in 16-byte chunks; a hidden
-//    key's chunks and those past head_dim come from zeros.  Their rows are found through the page table for
-//    SLOT_KEYS keys at a time, kept in LDS, so that no load that a wave waits for
+//    key's chunks and those past head_dim come from zeros.  Their rows are found through
+//    the page table for SLOT_KEYS keys at a time, kept in LDS, so that no load that a wave waits for
 //    comes between them.
 //  * LDS rows are CH chunks; chunk c of key k lies at c ^ key_swizzle(k), so that
 //    16 lanes reading one chunk of 16 keys touch all 64 banks, and c ^
@@ -54,7 +60,7 @@ __device__ __forceinline__ int key_swizzle(int key) { return CH == 16 ? key & 15
 template <int CH>
 __device__ __forceinline__ int value_swizzle(int key) { return CH == 16 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
 
-// Barrier between phases: this wave's LDS reads are complete, its direct loads
+// Barrier between iterations: this wave's LDS reads are complete, its direct loads
 // stay in flight, and no instruction moves to the other side.
 __device__ __forceinline__ void phase_barrier() {
     asm_wait_lgkmcnt<0>();
@@ -147,10 +153,10 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         asm_global_load_lds_b128((const void*)(uintptr_t)(slot != NOWHERE && 8 * (int)cs < D ? p : zeros),
                                  (uint32_t)wave_lds + to + 16 * CHUNK_THREADS * l);
     };
-    // K of tile i + NB - 1 and V of tile i + NB - 2 go into the buffers that phases 2i and
-    // 2i + 1 do not read: of the ring, before tile i's and two before it.  A wave asks for
-    // its 2 NL pieces of them between the products of its phase (a load takes the memory
-    // pipeline some 100 cycles to accept), past the last tile too (of zeros or of keys
+    // K of tile i + NB - 1 and V of tile i + NB - 2 go into the buffers that iteration i
+    // does not read: of the ring, before tile i's and two before it.  A wave asks for
+    // its 2 NL pieces of them between its products (a load takes the memory pipeline some
+    // 100 cycles to accept), past the last tile too (of zeros or of keys
     // nobody reads), so that a count of them says which are done.
     auto before = [](int ring) { return ring ? ring - 1 : NB - 1; };
     auto piece = [&](int ring, int j, uint32_t slot) {
@@ -231,7 +237,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         }
         return base;
     };
-    // The products of a phase: O^T += V^T P^T of tile i - 1 in four steps of 16 keys, then S^T =
+    // The products of an iteration: O^T += V^T P^T of tile i - 1 in four steps of 16 keys, then S^T =
     // K Q^T of tile i in steps of 32 dims.  A step's fragments are read from LDS AHEAD steps
     // before they are multiplied.
     // Both are always made, a branch around either would cost copies of the accumulators:

@@ -12,7 +12,11 @@
 // elements of one head: a 16-byte store whatever the types are, and its partner
 // elements (a chunk further on in the same head, or its own) come from the lines
 // that its neighbours read.  One block per row, so sequence, position, page
-// and table row are found once per wave.
+// and table row are found once per wave; the elements are asked for before that chain of
+// loads (95 -> 80 us below).
+// Measured: 4 x 4096 bf16 rows, 32 + 2 x 8 heads of 128, 405 MB: 80 us, 5.1 TB/s, what a
+// large copy reaches; 768 fp16 rows, 3 x 32 heads of 64, 19 MB: 6.1 us; one row 3.8 us, a
+// launch.
 #include "common.h"
 #include "device_math.h"
 #include "paged_ops.h"

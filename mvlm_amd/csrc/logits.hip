@@ -14,6 +14,10 @@
 // memory.  A thread asks for its logits, its mask bits and its share of the
 // history before it waits for any of them.  Every block of a row reads the row's
 // history, from L2 after the first: history / slice of the logits' own traffic.
+// Measured: 128 rows of 128000 fp32 logits with mask, 64 biases and 4096 tokens of
+// history, 135 MB: 29 .. 31 us, 4.4 .. 4.6 TB/s (116 us where each load was waited for
+// before the next, 32.7 with the mask words read by every thread itself); one row of
+// 51200: 3.8 us, a launch.
 // Integer counts and the maximum of entry numbers do not depend on the order in
 // which the threads arrive.
 #include "common.h"
@@ -201,8 +205,9 @@ static void launch_slices(hipStream_t s, LogitsArgs a) {
 hipError_t launch_logits(hipStream_t s, const LogitsArgs& a, int num_cus) {
     const int es = a.dtype == MVLM_F32 ? 4 : 2;
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.out) & 15u) == 0 && (a.ld * es) % 16 == 0;
-    // slices of 4096 read the history a quarter as often as slices of 1024, which
-    // share few rows among more CUs
+    // slices of 4096 tokens read the history a quarter as often as slices of 1024, which
+    // share few rows among more CUs (16 rows of 128000 5.7 us against 6.5, 128 rows 25
+    // against 32; one row of 51200 4.3 us against 3.5, from 8 rows of 128000 on no difference)
     const bool large = (int64_t)a.rows * ((a.n + 4095) / 4096) >= 2 * (int64_t)num_cus;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;

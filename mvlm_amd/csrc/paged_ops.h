@@ -30,7 +30,10 @@ struct PagedDivision {
     float* ws;                     // partial results of split tiles
     uint32_t* arrived;             // [records][kv_heads] splits that are done, zero between launches
 };
-constexpr int PAGED_FEW = 64;
+// f-rows up to which a sequence next to ones of many stays with tiles of 32 (2048 rows and 8 times
+// n on 500 .. 3000 positions, 32 heads of 64: n = 48 179 us and 201 in tiles of 256, 100 198 and
+// 203, 200 240 and 217)
+constexpr int PAGED_FEW = 128;
 constexpr int PAGED_QUEUES = 8;        // one per XCD: their blocks share an L2
 constexpr int PAGED_MAX_KV_HEADS = 1024;
 
