@@ -16,7 +16,7 @@
 // of a ring: the blocks of one kv head walk its keys in step, so each tile comes from
 // memory once for all of them and its loads have to cover that latency.
 // 2048 bf16 rows on 8192 positions, 32 heads of 128 over 8 kv heads (309 GFLOP): 298 ..
-// 316 us on different boxes, 977 .. 1037 TFLOP/s, of the 1229 .. 1275 that a large
+// 316 us as the clock allows, 977 .. 1037 TFLOP/s, of the 1229 .. 1275 that a large
 // library product of that type reaches here; with both groups in step 384 us, with two
 // barriers per tile 349.
 //  * K and V tiles go straight from memory to LDS in 16-byte chunks; a hidden
