@@ -250,15 +250,36 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
 #pragma unroll
         for (int r = 0; r < NR; ++r) oacc[t][r] = 0.0f;
 
-    // K fragments and V chunks of a tile are asked for while the tile before is
-    // computed: K's registers are free once its scores are, V's once it is in LDS.
-    u32x4 kf[U][S], vf[VI];
-    auto chunk_at = [](const uint16_t* base, uint32_t c) { return reinterpret_cast<const u32x4*>((uintptr_t)base + ((uint64_t)c << 4)); };
+    // K and V of a tile are asked for while the tile before is computed.  For R = 16 K
+    // comes as fragments, 64 bytes of each key per load, whose registers are free once its
+    // scores are.  For R = 32 those would be 32 bytes, and the L1's accesses per load what
+    // bounds it (the texture addresser was busy 65% of the time), so K comes in whole rows,
+    // like V, and goes through V's place in LDS before V does: 256 rows and 11 single tokens,
+    // 32 heads of 64, 35.7 -> 28.7 us, 8 heads of 128 64 -> 53, 768 rows 14.0 -> 12.1.  Not
+    // for head_dims of 72 .. 96, whose rows are no multiple of a line or leave loads half empty
+    // (768 rows of 32 heads of 80 22.4 us, staged 23.4; 256 and 11 of 96 41.4 and 40.7), and not
+    // for 128 inside the kernel for many rows, whose registers it would spill (306 -> 330 us).
+    constexpr bool STAGED = R == 32 && KS != 3 && (KS < 4 || NW == 4);
+    u32x4 kf[U][S], kr[STAGED ? VI : 1], vf[VI];
+    uint32_t at[VI];                                           // where this lane's chunks are
+    // in the global address space: a generic load counts as one of LDS too, and every wait for LDS
+    // would be one for it
+    typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
+    auto chunk_at = [](const uint16_t* base, uint32_t c) { return (global_u32x4*)((uintptr_t)base + ((uint64_t)c << 4)); };
+    auto locate = [&](uint32_t where) {
+#pragma unroll
+        for (int i = 0; i < VI; ++i) at[i] = __shfl(where, vkey[i] & 31, 64) + (uint32_t)(vdim[i] >> 3);
+    };
     auto load_k = [&](uint32_t where) {
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int i = 0; i < VI; ++i) kr[i] = *chunk_at(a.kv.k, at[i]);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t c = __shfl(where, R * u + rl, 64);  // a hidden key's score is replaced below
-            const u32x4* row = chunk_at(a.kv.k, c + (uint32_t)g);
+            global_u32x4* row = chunk_at(a.kv.k, c + (uint32_t)g);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 if (NG * (s + 1) * 8 <= 32 * (KS - 1)) kf[u][s] = row[NG * s];
@@ -266,19 +287,69 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             }
         }
     };
-    auto load_v = [&](uint32_t where) {
+    auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < VI; ++i) vf[i] = *chunk_at(a.kv.v, __shfl(where, vkey[i] & 31, 64) + (uint32_t)(vdim[i] >> 3));
+        for (int i = 0; i < VI; ++i) vf[i] = *chunk_at(a.kv.v, at[i]);
+    };
+    auto store = [&](const u32x4* from) {                      // a tile's chunks into LDS
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+            if (64 * i + 64 <= 128 * (KS - 1) || vkey[i] < PAGED_KEYS) *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = from[i];
     };
     int kv0 = k_begin + PAGED_KEYS * wave;
     constexpr int STEP = PAGED_KEYS * NW;
     int page_next = ask_page(kv0 + STEP);
     const int page = ask_page(kv0);
     uint32_t where = chunk_of(kv0, page), gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page));
+    locate(where);
     load_k(where);
-    load_v(where);
+    load_v();
     for (; kv0 < k_end; kv0 += STEP) {
         const uint32_t gone = gone_next;
+        // the page of the tile after next is asked for before the loads, so that its
+        // wait, an iteration later, does not wait for them
+        auto next = [&] {
+            where = chunk_of(kv0 + STEP, page_next);
+            gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page_next));
+            page_next = ask_page(kv0 + 2 * STEP);
+            locate(where);
+        };
+        // dims past head_dim: K's registers hold other dims there
+        auto clear_dims = [&] {
+            if (D < 32 * KS) {
+                asm volatile("");
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < S; ++k)
+                        if (NG * (k + 1) * 8 > 32 * (KS - 1) && NG * k + g >= cpr) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
+            }
+        };
+        float p[NE];
+        auto scores = [&] {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Acc s;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) s[r] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < S; ++k) s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) p[NR * u + r] = s[r];
+            }
+        };
+        if constexpr (STAGED) {
+            store(kr);
+            asm volatile("" ::: "memory");                     // this wave's LDS: its reads follow its stores
+#pragma unroll
+            for (int k = 0; k < S; ++k) kf[0][k] = *reinterpret_cast<const u32x4*>(vt + rl * L::VP + 8 * NG * k + 8 * g);
+            asm volatile("" ::: "memory");
+            next();
+            if constexpr (KS < 4) load_k(where);
+            clear_dims();
+            scores();
+            if constexpr (KS == 4) load_k(where);              // the registers do not hold both
+        }
         // some rows see only part of this tile: if it holds values that are not finite,
         // 0 x infinity would reach the rows that do not see them
         bool by_key = false;
@@ -300,39 +371,15 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             for (int i = 0; i < VI; ++i)
                 if ((gone >> (vkey[i] & 31)) & 1u) vf[i] = u32x4{0u, 0u, 0u, 0u};
         }
-#pragma unroll
-        for (int i = 0; i < VI; ++i)
-            if (64 * i + 64 <= 128 * (KS - 1) || vkey[i] < PAGED_KEYS) *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = vf[i];
-        // the page of the tile after next is asked for before the loads, so that its
-        // wait, an iteration later, does not wait for them
-        where = chunk_of(kv0 + STEP, page_next);
-        gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page_next));
-        page_next = ask_page(kv0 + 2 * STEP);
-        load_v(where);
+        store(vf);
+        if constexpr (!STAGED) next();
+        load_v();
         asm volatile("" ::: "memory");                         // this wave's LDS: its reads follow its stores
-
-        if (D < 32 * KS) {                                     // dims past head_dim: K's registers hold other dims there
-            asm volatile("");
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int k = 0; k < S; ++k)
-                    if (NG * (k + 1) * 8 > 32 * (KS - 1) && NG * k + g >= cpr) kf[u][k] = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (!STAGED) {
+            clear_dims();
+            scores();
+            load_k(where);
         }
-        float p[NE];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Acc s;
-#pragma unroll
-            for (int r = 0; r < NR; ++r) s[r] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < S; ++k) {
-                s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
-            }
-#pragma unroll
-            for (int r = 0; r < NR; ++r) p[NR * u + r] = s[r];
-        }
-        load_k(where);
         if (gone || kv0 + PAGED_KEYS > open_end) {
             asm volatile("");                                  // a branch: few tiles need this
             const int seen = last - kv0 - 4 * g;

@@ -75,7 +75,7 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const int64_t f = (int64_t)b.rows * a->group;
     a->few = a->many = PagedDivision{};
     // Tiles of 256 rows pay once they give every CU a block, alone or with their keys split;
-    // below that tiles of 32 make more of the chip (768 rows of 32 heads: 14 us, 32 in tiles
+    // below that tiles of 32 make more of the chip (768 rows of 32 heads: 12 us, 32 in tiles
     // of 256).  Here by what the tables can hold, in the kernel by what they do hold.
     const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int64_t tiles256 = (single ? (int64_t)b.seqs * (a->group / CHUNK_R) : f / CHUNK_R) * a->kv.kv_heads;
@@ -93,7 +93,7 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     const int64_t tiles = single ? (int64_t)b.seqs * ((a->group + R - 1) / R) : f / R + b.seqs;
     // blocks wanted per CU, measured at 1.. 6: 16 rows 2 (16 sequences up to 2047: 30.6 us, 33.3 at
     // 3, 34.0 at 4; 4 of 32768, D = 128: 84.9, 94.7, 88.4), 32 rows 1 (256 rows and 11 single tokens:
-    // 33.4 us, 40.7 at 2, 42.7 at 4)
+    // 28.5 us, 29.7 at 2; 256 and 7 of 8 heads of 128 52.9 and 62.1)
     // Tiles that leave most CUs idle, over tables that do not hold more than 512 keys for
     // each CU, take eight waves instead of four: their splits are few or none (one sequence of
     // 512: 8.3 -> 7.4 us; 4 of 32768 would take 88.4 us instead of 84.8).
