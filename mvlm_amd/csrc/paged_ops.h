@@ -173,7 +173,7 @@ __device__ __forceinline__ bool paged_locate(const PagedAttnArgs& a, const Paged
     const PagedSeqs& b = a.batch;
     const PagedDivision& div = MANY ? a.many : a.few;
     const int lane = (int)(threadIdx.x & 63);
-    int first = 0, record = 0;                             // items and records before this round of sequences
+    int first = 0, record = 0;                             // items and records before these 64 sequences
     for (int base = 0; base < b.seqs; base += 64) {
         const PagedSpan sp = base ? paged_lane_span(b, base + lane) : share.first;
         const int tiles = paged_tiles<R, MANY>(sp, a.group, share.few_rows), splits = paged_splits(sp.len, share.unit);
