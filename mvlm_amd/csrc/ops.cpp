@@ -968,7 +968,8 @@ static bool attach_sync(mvlm_plan* plan, Op& op, StreamAttnDesc d) {
         (void)hipGetLastError();
         return false;
     }
-    bool ok = hipMemset(d.sync, 0, SYNC_BYTES) == hipSuccess &&
+    // on the handle's own stream, which the null stream does not order
+    bool ok = hipMemsetAsync(d.sync, 0, SYNC_BYTES, dev->stream) == hipSuccess &&
               stream_attn_check(op.gcount, op.gx, op.a_dtype, op.gw, op.gy, op.gyd, d, op.num_cus) == hipSuccess;
     if (ok) {
         try {
@@ -1281,7 +1282,7 @@ extern "C" int mvlm_plan_check(mvlm_plan* plan) {
         HIP_TRY(hipMemcpy(&err, (const char*)op.attn.sync + SYNC_ERR_OFFSET, 4, hipMemcpyDeviceToHost));
         if (!err) continue;
         ++failed;
-        HIP_TRY(hipMemset(op.attn.sync, 0, SYNC_BYTES));   // counters the failed launch left part-way
+        HIP_TRY(hipMemsetAsync(op.attn.sync, 0, SYNC_BYTES, dev->stream));   // counters the failed launch left part-way
     }
     if (!failed) return MVLM_OK;
     return set_error(MVLM_ERR_HIP, "mvlm_plan_check: %d fused launch site(s) gave up waiting for their attention "

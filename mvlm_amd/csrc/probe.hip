@@ -213,7 +213,8 @@ extern "C" int mvlm_probe_grid_barrier(mvlm_device* dev, int variant, int rounds
     const size_t total = off_bg + bg_bytes;
     char* mem = nullptr;
     HIP_TRY(hipMalloc(&mem, total));
-    int st = check_hip(hipMemset(mem, 0, total), "probe memset");
+    // on the launch's own stream: a flag cleared after its owner has raised it would never be seen
+    int st = check_hip(hipMemsetAsync(mem, 0, total, dev->stream), "probe memset");
     ProbeArgs a{};
     a.cnt = (uint32_t*)mem;
     a.flags = (uint32_t*)(mem + off_flags);
