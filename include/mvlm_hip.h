@@ -394,8 +394,8 @@ int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
  * generated; penalties[r] = repetition (> 0), frequency, presence.  Biases:
  * bias_values[r][i] for token bias_ids[r][i], i < bias_len[r]; the last entry of a
  * token counts.  allowed: one bit per token, bit t % 32 of word t / 32, 0 = masked.
- * Lengths are taken within [0, width], ids outside [0, n) name nothing.  Each
- * group may be absent (all its pointers NULL). */
+ * Lengths are taken within [0, width], ids outside [0, n) name nothing; widths
+ * are at most 2^30.  Each group may be absent (all its pointers NULL). */
 typedef struct mvlm_logit_controls {
     const mvlm_buffer* history;          /* int32 [rows][history_width] */
     const mvlm_buffer* history_len;      /* int32 [rows] */

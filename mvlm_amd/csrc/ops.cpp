@@ -501,7 +501,9 @@ int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     REQUIRE(!c->penalties == !c->history && !c->history == !c->history_len && (c->history || !c->generated_from),
             "%s: penalties, history and history_len go together, generated_from with them", fn);
     if (c->penalties) {
-        REQUIRE(c->history_width > 0, "%s: history_width=%d must be positive", fn, c->history_width);
+        // an entry's index and the 512 x 8 entries that are asked for ahead of it stay below 2^31
+        REQUIRE(c->history_width > 0 && c->history_width <= (1 << 30), "%s: history_width=%d must be positive and at most 2^30", fn,
+                c->history_width);
         st = ints(c->penalties, 3 * R, "penalties", (const void**)&a.penalties);
         if (st == MVLM_OK) st = ints(c->history, R * c->history_width, "history", (const void**)&a.history);
         if (st == MVLM_OK) st = ints(c->history_len, R, "history_len", (const void**)&a.history_len);
@@ -511,7 +513,7 @@ int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     if (st != MVLM_OK) return st;
     REQUIRE(!c->bias_ids == !c->bias_values && !c->bias_ids == !c->bias_len, "%s: bias_ids, bias_values and bias_len go together", fn);
     if (c->bias_ids) {
-        REQUIRE(c->bias_width > 0, "%s: bias_width=%d must be positive", fn, c->bias_width);
+        REQUIRE(c->bias_width > 0 && c->bias_width <= (1 << 30), "%s: bias_width=%d must be positive and at most 2^30", fn, c->bias_width);
         st = ints(c->bias_ids, R * c->bias_width, "bias_ids", (const void**)&a.bias_ids);
         if (st == MVLM_OK) st = ints(c->bias_values, R * c->bias_width, "bias_values", (const void**)&a.bias_values);
         if (st == MVLM_OK) st = ints(c->bias_len, R, "bias_len", (const void**)&a.bias_len);
