@@ -382,7 +382,7 @@ int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, 
  * group = num_heads / kv_heads, over the positions t up to row r's own that exist
  * (what lies in others may be anything).  Q [rows][num_heads][head_dim] in the
  * cache's type, O the same shape in F32 or the cache's type; scale 0:
- * 1/sqrt(head_dim).  A row that sees no position, or only scores of -inf, is 0.
+ * 1/sqrt(head_dim); scale log2(e) must be finite in fp32.  A row that sees no position, or only scores of -inf, is 0.
  * A value that is not finite makes its element of the rows that see it not
  * finite (an infinity may become NaN in an F32 O: probabilities are multiplied in
  * parts) and reaches no other row. */

@@ -454,6 +454,7 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     a.heads = num_heads;
     a.group = num_heads / a.kv.kv_heads;
     a.scale_log2 = (scale == 0.0f ? 1.0f / sqrtf((float)a.kv.D) : scale) * 1.4426950408889634f;
+    REQUIRE(a.scale_log2 < INFINITY, "%s: scale %g is too large", fn, (double)scale);   // 0 x inf would be NaN
     plan_attention_paged(&a, dev->prop.multiProcessorCount);
     // a launch holds fewer than 2^32 threads, 512 in a block at most
     REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads < (1 << 23), "%s: shape too large", fn);

@@ -40,9 +40,20 @@ static void logits_lists(const char* kind) {
     }
 }
 
+// Scores are scaled by scale log2(e) in fp32; were that infinite, a score of 0 would become NaN.
+static void attention_scales() {
+    mvlm_buffer k = buffer(1 << 20, 0x10000000), v = buffer(1 << 20, 0x20000000), len = buffer(16, 0x30000000),
+                table = buffer(64, 0x40000000), q = buffer(1 << 20, 0x50000000), o = buffer(1 << 20, 0x60000000);
+    const mvlm_paged_kv kv{&k, &v, MVLM_F16, 16, 16, 4, 64};
+    const mvlm_paged_batch batch{4, 4, nullptr, &len, &table, 4};
+    for (float scale : {FLT_MAX, FLT_MAX / 1.4426f})
+        refused("a scale that log2(e) makes infinite", mvlm_attention_paged(&dev, &q, &batch, &kv, &o, MVLM_F32, 4, scale, nullptr));
+}
+
 int main() {
     setenv("MVLM_QUIET", "1", 1);
     logits_lists("a list of more than 2^30 entries");
+    attention_scales();
     std::printf("%d failures\n", failures);
     return failures != 0;
 }
