@@ -29,8 +29,8 @@
 //  * v_mfma_f32_32x32x16: lane l's results are row l % 32 and keys
 //    8 (r / 4) + 4 (l / 32) + r % 4, which are the B operand of the second product
 //    as they stand when V^T is read in the same key order.
-//  * a tile that only some of a wave's rows see in part is checked for values that are
-//    not finite (0 x infinity would reach rows that do not see it); if it holds any,
+//  * a tile with keys that some of a wave's rows do not see is checked for values that are
+//    not finite (0 x infinity would reach rows that do not see them); if it holds any,
 //    its second product is made key by key over the rows that see the key.
 // The sequences with few new rows are items of paged_few_item in the same launch,
 // behind those with many.  A block fills a CU (its LDS), so there is one per CU, and
@@ -185,7 +185,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) oacc[i][r] = 0.0f;
-    bool partial = false;                                      // some of the wave's rows see only part of that tile
+    bool partial = false;                                      // the tile holds keys that some of the wave's rows do not see
 
     // Where tile i's values are read for the second product; the slow path makes it itself.
     auto values_at = [&](int i, int ring) {
@@ -300,7 +300,9 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     auto softmax = [&](int i) {
         const int kv0 = k_begin + i * CHUNK_KEYS;
         const uint64_t hidden = __builtin_amdgcn_ballot_w64(slots[(uint32_t)(i * CHUNK_KEYS + lane) % (2 * SLOT_KEYS)] == NOWHERE);
-        partial = kv0 + CHUNK_KEYS > wave_open && wave_open < wave_end;
+        // keys up to k_end are in LDS with their values: the last of a tile may be hidden from all the wave's rows
+        // (group >= 32: one token's) and visible to later waves' only
+        partial = kv0 + CHUNK_KEYS > wave_open && wave_open < k_end;
         if (hidden || kv0 + CHUNK_KEYS > wave_open) {
             asm volatile("");                                  // a branch: few tiles need this
             const int seen = last - kv0 - 4 * h2;
