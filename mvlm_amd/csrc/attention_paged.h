@@ -28,6 +28,24 @@ __device__ __forceinline__ uint32_t round2(float& lo, float& hi) {
     }
 }
 
+// Probabilities are kept relative to a reference that follows a row's maximum: it moves
+// when a score exceeds the maximum it was taken from by more than SLACK (in the exp2
+// domain), and lies BIAS below that, so they stay up to 2^(SLACK + BIAS).  Numerators
+// and sums carry the same factor.  bf16 has fp32's range and rescales seldom.  An fp16 part
+// is a multiple of 2^-24, so with the row's largest at 2^12 or above it is off by 2^-37 of
+// that at most, and has its 11 bits down to 2^-26 of it (with the largest at 1: to 2^-14, and thousands
+// of keys ten nats and more below one lost the same bits).  A second part is rounded 2^11
+// times as large and summed apart: both together hold 22 bits down to 2^-26 of the largest
+// and are off by 2^-48 of it at most below.
+// SLACK 3 costs 1% and less (2048 fp16 rows on 8192, 32 heads of 128 over 8: 326 -> 328 us, 32 heads of 64
+// 209 -> 212; SLACK 1 334 and 220), the second sum 3 .. 10% where the matrix cores bound
+// (fp32 O: 433 -> 470 us, 312 -> 331; 768 rows 14.0 -> 14.4) and nothing for single tokens.
+template <bool BF>
+struct PagedP {
+    static constexpr float SLACK = BF ? 8.0f : 3.0f, BIAS = BF ? 0.0f : 12.0f;
+    static constexpr float REST = BF ? 1.0f : 2048.0f;
+};
+
 // Partial results of a split tile: per record (one split of one tile of one kv
 // head) its R rows of D floats of unnormalized output, then, behind all records, R
 // (max, sum) pairs each.  They cross workgroups, so they move with device-scope
@@ -243,7 +261,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
         return exists(page) ? (uint32_t)a.kv.slot(page, h, key - a.kv.page.quotient(key) * a.kv.page.div) * (uint32_t)cpr : 0u;
     };
 
-    float mrun = -INFINITY, lrun = 0.0f;                       // lrun: this lane's keys only
+    float mrun = -INFINITY, lrun = 0.0f;                       // the reference (PagedP), and this lane's keys' sum
     Acc oacc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -394,10 +412,10 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
 #pragma unroll
         for (int e = 1; e < NE; ++e) tmax = fmaxf(tmax, p[e]);
         tmax *= a.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(tmax > mrun + 8.0f)) {
+        if (__builtin_amdgcn_ballot_w64(tmax > mrun + (PagedP<BF>::BIAS + PagedP<BF>::SLACK))) {
             if constexpr (R == 16) tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
             tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-            const float mnew = fmaxf(mrun, tmax);
+            const float mnew = fmaxf(mrun, tmax - PagedP<BF>::BIAS);
             const float factor = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mnew);
             lrun *= factor;
 #pragma unroll
@@ -435,21 +453,51 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
         }
         {
             const uint16_t* vg = vt + (4 * g + ((lane & 15) >> 2)) * L::VP + 16 * ((lane >> 4) & (R / 16 - 1)) + 4 * (lane & 3);
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                u32x4 pb[PP];
+            auto values = [&](int k, int t) {
+                lds_i16x4* p0 = (lds_i16x4*)(uintptr_t)lds_offset(vg + 8 * NG * k * L::VP + R * t);
+                lds_i16x4* p1 = (lds_i16x4*)(uintptr_t)lds_offset(vg + (8 * NG * k + 4 * NG) * L::VP + R * t);
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1));
+                return u32x4{lo[0], lo[1], hi[0], hi[1]};
+            };
+            u32x4 pb[STEPS][PP];
+            auto parts = [&](int k) {
 #pragma unroll
                 for (int w = 0; w < PP; ++w)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) pb[w][e] = round2<BF, true>(p[8 * k + 2 * e], p[8 * k + 2 * e + 1]);
+                    for (int e = 0; e < 4; ++e) {
+                        float &lo = p[8 * k + 2 * e], &hi = p[8 * k + 2 * e + 1];
+                        if (w == 1) lo *= PagedP<BF>::REST, hi *= PagedP<BF>::REST;
+                        pb[k][w][e] = round2<BF, true>(lo, hi);
+                    }
+            };
+            if constexpr (PP > 1 && PagedP<BF>::REST != 1.0f) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) parts(k);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    lds_i16x4* p0 = (lds_i16x4*)(uintptr_t)lds_offset(vg + 8 * NG * k * L::VP + R * t);
-                    lds_i16x4* p1 = (lds_i16x4*)(uintptr_t)lds_offset(vg + (8 * NG * k + 4 * NG) * L::VP + R * t);
-                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1));
+                    Acc rest;
 #pragma unroll
-                    for (int w = 0; w < PP; ++w) oacc[t] = mfma_paged<R, BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[w], oacc[t]);
+                    for (int r = 0; r < NR; ++r) rest[r] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const u32x4 v = values(k, t);
+                        rest = mfma_paged<R, BF>(v, pb[k][1], rest);
+                        oacc[t] = mfma_paged<R, BF>(v, pb[k][0], oacc[t]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) oacc[t][r] = __builtin_fmaf(rest[r], 1.0f / PagedP<BF>::REST, oacc[t][r]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    parts(k);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const u32x4 v = values(k, t);
+#pragma unroll
+                        for (int w = 0; w < PP; ++w) oacc[t] = mfma_paged<R, BF>(v, pb[k][w], oacc[t]);
+                    }
                 }
             }
         }

@@ -26,9 +26,9 @@
 //    one behind it before them: a wave has about 12 KB (head_dim 64) in flight.
 //  * P is rounded to the cache's type for a 16-bit O, as the rounding of O
 //    itself is of that size; for an fp32 O it is kept to 22 bits and more, as
-//    the sum of two fp16 or three bf16 parts, one product each.
-//  * the running maximum moves only when a score exceeds it by more than 8 (in
-//    the exp2 domain), so P stays below 2^8 and most tiles rescale nothing.
+//    the sum of two fp16 or three bf16 parts, one product each (PagedP).
+//  * the running maximum moves only when a score exceeds it by more than SLACK
+//    (PagedP), so most tiles rescale nothing.
 //  * hidden keys may hold anything: their scores are replaced, not added to,
 //    and their V rows are staged as zeros.
 //

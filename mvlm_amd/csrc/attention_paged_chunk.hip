@@ -178,7 +178,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     const uint32_t kat = lds0 + l32 * PB + 16 * (h2 ^ key_swizzle<CH>(l32));
     const uint32_t vat = lds0 + L::V + vkey * PB + 2 * (vdim & 7) + 16 * ((vdim >> 3) ^ value_swizzle<CH>(vkey));
 
-    float mrun = -INFINITY, lrun = 0.0f;                       // lrun: this lane's keys only
+    float mrun = -INFINITY, lrun = 0.0f;                       // the reference (PagedP), and this lane's keys' sum
     f32x16 oacc[DT], s[2];
     u32x4 pb[PP][4] = {};                                      // P of the tile before, 16 keys each
 #pragma unroll
@@ -210,7 +210,9 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
                         for (int e = 0; e < 8; ++e) {
                             float p = 0.0f;
 #pragma unroll
-                            for (int w = 0; w < PP; ++w) p += bits_to_f32<std::conditional_t<BF, __hip_bfloat16, __half>>((uint16_t)(pb[w][2 * u + k][e >> 1] >> (16 * (e & 1))));
+                            for (int w = 0; w < PP; ++w)
+                                p += (w == 1 ? 1.0f / PagedP<BF>::REST : 1.0f) *
+                                     bits_to_f32<std::conditional_t<BF, __hip_bfloat16, __half>>((uint16_t)(pb[w][2 * u + k][e >> 1] >> (16 * (e & 1))));
                             pw[(16 * k + 8 * (e >> 2) + 4 * h2 + (e & 3)) * 32 + l32] = p;
                         }
                     asm_wait_lgkmcnt<0>();
@@ -237,14 +239,16 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         }
         return base;
     };
-    // The products of an iteration: O^T += V^T P^T of tile i - 1 in four steps of 16 keys, then S^T =
-    // K Q^T of tile i in steps of 32 dims.  A step's fragments are read from LDS AHEAD steps
-    // before they are multiplied.
+    // The products of an iteration: O^T += V^T P^T of tile i - 1 in four steps of 16 keys (or, where
+    // the second parts are summed apart (PagedP), in steps of 32 dims), then S^T = K Q^T of tile i in steps
+    // of 32 dims.  A step's fragments are read from LDS AHEAD steps before they are multiplied.
     // Both are always made, a branch around either would cost copies of the accumulators:
     // without a tile before, from values of zero (pv false), and behind the last tile into
     // scores that nobody reads.
     auto products = [&](int i, int ring, bool pv) {
-        constexpr int PV = 4, STEPS = PV + (KS + 1) / 2;
+        constexpr bool APART = PP > 1 && PagedP<BF>::REST != 1.0f;
+        constexpr int PV = APART ? DT : 4, STEPS = PV + (KS + 1) / 2;
+        static_assert(2 * NL <= STEPS, "a step asks for one piece at most");
         constexpr int AHEAD = DT > 2 ? 1 : 3, SETS = AHEAD + 1;
         const uint32_t v_at = pv ? values_at(i - 1, before(ring)) : vat - L::V + L::ZEROS, k_at = kat + ring * TILE;
         const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -254,11 +258,12 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             constexpr int st = decltype(step)::value;
             if constexpr (st < PV) {
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    const uint32_t at = (v_at ^ (64 * t)) + 16 * st * PB;
+                for (int x = 0; x < (APART ? 4 : DT); ++x) {   // the step's keys of one t, or its t of 16 keys
+                    const int t = APART ? st : x, k16 = APART ? x : st;
+                    const uint32_t at = (v_at ^ (64 * t)) + 16 * k16 * PB;
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at));
                     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + 8 * PB)));
-                    frag[st % SETS][t] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    frag[st % SETS][x] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
             } else if constexpr (st < STEPS) {
 #pragma unroll
@@ -276,7 +281,18 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             constexpr int st = decltype(step)::value;
             read(std::integral_constant<int, st + AHEAD>{});
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (st < PV) {
+            if constexpr (st < PV && APART) {
+                f32x16 rest = zero;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    rest = mfma32<BF>(frag[st % SETS][x], pb[PP - 1][x], rest);
+                    oacc[st] = mfma32<BF>(frag[st % SETS][x], pb[0][x], oacc[st]);
+                    if constexpr (st < 2 * NL)
+                        if (x == 0) piece(ring, st, slot[st]);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) oacc[st][r] = __builtin_fmaf(rest[r], 1.0f / PagedP<BF>::REST, oacc[st][r]);
+            } else if constexpr (st < PV) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) oacc[t] = mfma32<BF>(frag[st % SETS][t], pb[0][st], oacc[t]);
                 if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
@@ -322,8 +338,8 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
 #pragma unroll
             for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[u][r]);
         tmax *= a.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(tmax > mrun + 8.0f)) {
-            const float mnew = fmaxf(mrun, fmaxf(tmax, __shfl_xor(tmax, 32, 64)));
+        if (__builtin_amdgcn_ballot_w64(tmax > mrun + (PagedP<BF>::BIAS + PagedP<BF>::SLACK))) {
+            const float mnew = fmaxf(mrun, fmaxf(tmax, __shfl_xor(tmax, 32, 64)) - PagedP<BF>::BIAS);
             const float factor = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mnew);
             lrun *= factor;
 #pragma unroll
@@ -344,7 +360,10 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
 #pragma unroll
             for (int w = 0; w < PP; ++w)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pb[w][k][e] = round2<BF, true>(p[2 * e], p[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) {
+                    if (w == 1) p[2 * e] *= PagedP<BF>::REST, p[2 * e + 1] *= PagedP<BF>::REST;
+                    pb[w][k][e] = round2<BF, true>(p[2 * e], p[2 * e + 1]);
+                }
         }
     };
 

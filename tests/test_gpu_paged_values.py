@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import mvlm_amd as m
-from paged_ref import Batch, attention, filled_cache, values
+from paged_ref import HALF_STEP, Batch, attention, close, filled_cache, to_bits, values
 from test_gpu_paged import run_attention, same_or_close, say
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,56 @@ def test_not_finite_values_of_later_tokens_reach_no_row_before(dev, news, lens, 
     ref, tol = attention(batch, q, K, clean, cd, D ** -0.5, 1 if od != F32 else 2)
     got[bad] = ref[bad] = 0.0
     assert same_or_close(got, ref, tol, od) <= 1.0
+
+
+@pytest.mark.parametrize("gap", [14, 18, 21])
+@pytest.mark.parametrize("news,lens,heads,kv_heads,D,cd,od,opt", [
+    ([1], [1000], 4, 2, 64, F16, F32, {"ragged": False}),
+    ([1, 1], [5000, 700], 4, 2, 128, F16, F32, {"ragged": False}),                  # splits
+    ([1], [1000], 32, 32, 64, F16, F16, {"ragged": False}),
+    ([1] * 3, [600, 1, 900], 8, 2, 96, BF16, F32, {"ragged": False}),
+    ([1] * 3, [600, 1, 900], 8, 2, 32, BF16, BF16, {"ragged": False}),
+    ([40], [900], 4, 2, 64, F16, F32, {}),
+    ([40, 1], [700, 950], 4, 4, 128, F16, F32, {}),
+    ([33], [900], 6, 2, 80, F16, F16, {}),
+    ([256], [600], 256, 256, 64, F16, F32, {}),
+    ([256, 3], [500, 400], 256, 256, 64, F16, F16, {}),
+    ([300], [500], 256, 128, 128, F16, F32, {}),
+    ([300], [1100], 128, 64, 96, F16, F32, {}),
+    ([256], [400], 256, 256, 32, F16, F32, {})])
+def test_keys_far_below_the_largest(dev, news, lens, heads, kv_heads, D, cd, od, opt, gap):
+    """Every 32nd key scores `gap` nats above the others and has values of zero, so that all of O comes from
+    probabilities of exp(-gap).  Scores are exact (one product each), so with A as in paged_ref.attention what is
+    rounded moves O by at most
+      u_P A                   P in the cache's type, where O has it; in parts 2^-22
+      F                       fp16: a part is a multiple of 2^-24 of a scale on which the row's largest is at least
+                              2^12: 2^-37 a key, with the second part rounded 2^11 times as large 2^-48
+      8 (1 + gap) 2^-23 A     the exponent's argument and the exponential, in numerator and denominator
+      2 (N + 64) 2^-24 A      sums over N keys and the merge of their parts
+    and the store by half a step."""
+    say("far below", gap, news, lens, heads, kv_heads, D, cd, od)
+    rng = np.random.default_rng(43)
+    batch = Batch(rng, news, lens, 16, **opt)
+    K, V = (np.zeros((batch.pages, kv_heads, 16, D), np.uint16) for _ in range(2))
+    q = np.zeros((batch.rows, heads, D), np.float32)
+    q[..., 0] = 8.0
+    ref, tol = np.zeros(q.shape), np.zeros(q.shape)
+    u_p = 2.0 ** -22 if od == F32 else HALF_STEP[cd]
+    f = 0.0 if cd == BF16 else 2.0 ** -48 if od == F32 else 2.0 ** -37
+    for s, (n, L) in enumerate(zip(news, lens)):
+        at = np.array([batch.place(s, t) for t in range(L)])
+        sink = np.arange(L) % 32 == 0
+        v = rng.integers(1, 4, (L, kv_heads, D)) * 8192.0 * ~sink[:, None, None]
+        K[at[:, 0], :, at[:, 1], 0] = to_bits(sink * float(gap), cd)[:, None]
+        V[at[:, 0], :, at[:, 1]] = to_bits(v, cd)
+        seen = np.arange(L - n, L)
+        total = (np.cumsum(sink) + np.exp(-float(gap)) * np.cumsum(~sink))[seen]
+        values_sum = np.repeat(np.cumsum(v, 0)[seen], heads // kv_heads, 1)
+        A = np.exp(-float(gap)) * values_sum / total[:, None, None]
+        r = slice(int(batch.start[s]), int(batch.start[s]) + n)
+        ref[r] = A
+        tol[r] = (u_p + 8 * (1 + gap) * 2.0 ** -23 + 2 * (L + 64) * 2.0 ** -24) * A + f * values_sum / total[:, None, None]
+    got = run_attention(dev, batch, to_bits(q, cd), K, V, cd, od, heads, 0.125)
+    worst = close(got, ref, tol, od)
+    say("worst", worst)
+    assert worst <= 1.0
