@@ -550,6 +550,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
 constexpr int CHUNK_KEYS = 64;     // keys per tile of the kernel for many new rows
 constexpr int CHUNK_R = 256;       // its f-rows per tile
 constexpr int CHUNK_UNIT = 1024;   // its least keys per split
+// The launch that comes first where a batch may be worth tiles of 256 rows (a.many.tile).
 hipError_t launch_attention_paged_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus);
 
 }  // namespace mvlm

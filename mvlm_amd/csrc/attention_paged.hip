@@ -50,11 +50,13 @@ template <int R, int KS, bool BF, int PP, int NW>
 __global__ __launch_bounds__(64 * NW, KS <= 2 && NW == 4 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
-    const PagedShare share = paged_share<R, false>(a, paged_lane_span(a.batch, (int)(threadIdx.x & 63)), a.few_rows);
+    if constexpr (R == 32 && NW == 4)
+        if (a.many.tile && *a.made) return;                    // by the kernel for many rows, which ran before
+    const PagedShare share = paged_share<R, false>(a, paged_lane_span(a.batch, (int)(threadIdx.x & 63)), INT_MAX);
     if (index < share.items) paged_few_item<R, KS, BF, PP, NW>(a, share, index, h, lds);
 }
 
-// Division of one kernel's share of the sequences (those of at most few_rows f-rows, or
+// Division of a share of the sequences (those of at most PAGED_FEW f-rows or all, or
 // those of more) for `blocks` blocks.  The sum of ceil(len / unit) over tiles is at most total / unit
 // + tiles, and a tile is split when len > unit, so split tiles make at most
 // 2 total / unit records.
@@ -76,11 +78,12 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     a->few = a->many = PagedDivision{};
     // Tiles of 256 rows pay once they give every CU a block, alone or with their keys split;
     // below that tiles of 32 make more of the chip (768 rows of 32 heads: 12 us, 32 in tiles
-    // of 256).  Here by what the tables can hold, in the kernel by what they do hold.
+    // of 256).  Where what the tables can hold would be enough, both kernels are launched, and
+    // the first decides by what is held; the one that has nothing to do costs about 2.5 us (768 rows in a
+    // table of 768 positions 13.5 us, of 32768 16.1; 2048 bf16 rows on 8192 303 us without the second launch, 306).
     const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int64_t tiles256 = (single ? (int64_t)b.seqs * (a->group / CHUNK_R) : f / CHUNK_R) * a->kv.kv_heads;
     const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
-    a->few_rows = many ? PAGED_FEW : INT_MAX;
     a->many_least = (num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
     if (many) {
         // a sequence with more than PAGED_FEW f-rows ends in one tile that is not full
@@ -113,8 +116,9 @@ static hipError_t launch_waves(hipStream_t s, const PagedAttnArgs& a) {
     constexpr int bytes = NW * PagedLayout<R, KS>::REGION + 16;
     if constexpr (bytes > 65536)
         if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, BF, PP, NW>>(bytes); e != hipSuccess) return e;
-    launch_kernel(paged_attention_kernel<R, KS, BF, PP, NW>, dim3((unsigned)(a.kv.kv_heads * a.few.items)), dim3(64 * NW),
-                  (uint32_t)bytes, s, a);
+    const dim3 grid((unsigned)(a.kv.kv_heads * a.few.items));
+    if (a.many.tile) launch_kernel_part(LaunchPart::Last, paged_attention_kernel<R, KS, BF, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
+    else launch_kernel(paged_attention_kernel<R, KS, BF, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
     return hipGetLastError();
 }
 
@@ -141,7 +145,8 @@ static hipError_t launch_few_rows(hipStream_t s, const PagedAttnArgs& a) {
 }
 
 hipError_t launch_attention_paged(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
-    if (a.many.tile) return launch_attention_paged_chunk(s, a, num_cus);
+    if (a.many.tile)
+        if (const hipError_t e = launch_attention_paged_chunk(s, a, num_cus); e != hipSuccess) return e;
     return a.few.tile == 16 ? launch_few_rows<16>(s, a) : launch_few_rows<32>(s, a);
 }
 

@@ -32,8 +32,9 @@
 //  * a tile with keys that some of a wave's rows do not see is checked for values that are
 //    not finite (0 x infinity would reach rows that do not see them); if it holds any,
 //    its second product is made key by key over the rows that see the key.
-// The sequences with few new rows are items of paged_few_item in the same launch,
-// behind those with many.  A block fills a CU (its LDS), so there is one per CU, and
+// Whether tiles of 256 rows pay depends on the lengths, which only the device knows (chunk_worth): this
+// kernel is launched before the one for few rows, and either makes the whole batch, the sequences with few new
+// rows as items of paged_few_item behind those with many, or ends at once and leaves it to that one (made).  A block fills a CU (its LDS), so there is one per CU, and
 // they take items from queues, one per XCD: item w belongs to queue w % 8, so with a
 // multiple of 8 kv heads the tiles of a head run on one XCD and share its L2.  A
 // sequence's tiles come in order of their keys, the most first, and the blocks take
@@ -42,7 +43,6 @@
 #include "attention_paged.h"
 
 #include <algorithm>
-#include <climits>
 
 namespace mvlm {
 
@@ -379,8 +379,11 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     auto in_reach = [&](int i) { return i < n && k_begin + i * CHUNK_KEYS < wave_end; };
     for (int i = 0, ring = 0; i <= n; ++i, ring = ring == NB - 1 ? 0 : ring + 1) {
         next_slots(i);
-        if (second && i > 0 && in_reach(i - 1)) softmax(i - 1);
+        // a softmax of the second group goes before one of the first, or its products, which come after it,
+        // find no vector instructions to run beside (2048 fp16 rows on 8192, 32 heads of 64: 234 -> 224 us, with fp32 O
+        // 341 -> 316; head_dim 128 the same)
         __builtin_amdgcn_s_setprio(1);
+        if (second && i > 0 && in_reach(i - 1)) softmax(i - 1);
         products(i, ring, i > 0 && in_reach(i - 1));
         __builtin_amdgcn_s_setprio(0);
         if (!second && in_reach(i)) softmax(i);
@@ -411,7 +414,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
 
 // Full tiles of 256 rows per kv head, each times the splits its keys could make: whether
 // they would fill the chip (plan_attention_paged asks the same of what the tables can
-// hold).
+// hold).  The same in all lanes; first: the lane-th sequence's span.
 __device__ __forceinline__ int chunk_worth(const PagedAttnArgs& a, const PagedSpan& first) {
     int worth = 0;
     for (int base = 0; base < a.batch.seqs; base += 64) {
@@ -422,24 +425,38 @@ __device__ __forceinline__ int chunk_worth(const PagedAttnArgs& a, const PagedSp
     return __builtin_amdgcn_readlane(wave_scan(worth), 63);
 }
 
+// The kernel's arguments, loaded anew for an item.  Kept from item to item, what both kinds of item
+// use is more than the scalar registers hold, and 128 of them are kept in lanes of vector registers and read back inside
+// the loops: 51 when they are loaded anew (2048 rows on 8192, 32 heads of 64: 221 -> 211 us, with fp32 O
+// 309 -> 292).  With more than two accumulators that cost more than it gave (heads of 80 155 -> 157 us, of 128 307 -> 324).
+template <int DT>
+__device__ __forceinline__ const PagedAttnArgs& item_args(const PagedAttnArgs& a) {
+    if constexpr (DT > 2) return a;
+    uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();     // where a, the only argument, is
+    asm volatile("" : "+s"(p));
+    return *(const PagedAttnArgs*)(const __attribute__((address_space(4))) PagedAttnArgs*)p;
+}
+
 template <int KS, int DT, bool BF, int PP>
 __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int kv_heads = a.kv.kv_heads, q = (int)blockIdx.x % PAGED_QUEUES, own = (int)blockIdx.x / PAGED_QUEUES;
     const int blocks = ((int)gridDim.x - q + PAGED_QUEUES - 1) / PAGED_QUEUES;              // of this queue
     const PagedSpan span = paged_lane_span(a.batch, (int)(threadIdx.x & 63));
-    const int few_rows = chunk_worth(a, span) >= a.many_least ? a.few_rows : INT_MAX;
-    const PagedShare many = paged_share<CHUNK_R, true>(a, span, few_rows), few = paged_share<32, false>(a, span, few_rows);
+    const bool worth = chunk_worth(a, span) >= a.many_least;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.made = worth;
+    if (!worth) return;                                        // the kernel for few rows makes everything
+    const PagedShare many = paged_share<CHUNK_R, true>(a, span, PAGED_FEW), few = paged_share<32, false>(a, span, PAGED_FEW);
     const int many_items = (many.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     const int all_items = many_items + (few.items * kv_heads - q + PAGED_QUEUES - 1) / PAGED_QUEUES;
     for (int round = 0; round * blocks < all_items; ++round) {
         const int i = round * blocks + (round & 1 ? blocks - 1 - own : own);
         if (i < many_items) {
             const int w = i * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_chunk_item<KS, DT, BF, PP>(a, many, index, w - index * kv_heads, lds);
+            paged_chunk_item<KS, DT, BF, PP>(item_args<DT>(a), many, index, w - index * kv_heads, lds);
         } else if (i < all_items) {
             const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_few_item<32, DT, BF, PP, 8>(a, few, index, w - index * kv_heads, lds);
+            paged_few_item<32, DT, BF, PP, 8>(item_args<DT>(a), few, index, w - index * kv_heads, lds);
         }
         __syncthreads();                                       // LDS is free
     }
@@ -450,7 +467,7 @@ static hipError_t launch_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cu
     constexpr int few = 8 * PagedLayout<32, DT>::REGION + 16, bytes = ChunkLayout<DT>::BYTES > few ? ChunkLayout<DT>::BYTES : few;
     if (const hipError_t e = allow_dynamic_lds<paged_chunk_kernel<KS, DT, BF, PP>>(bytes); e != hipSuccess) return e;
     const int64_t most = ((int64_t)a.many.items + a.few.items) * a.kv.kv_heads;
-    launch_kernel(paged_chunk_kernel<KS, DT, BF, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),
+    launch_kernel_part(LaunchPart::First, paged_chunk_kernel<KS, DT, BF, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),
                   (uint32_t)bytes, s, a);
     return hipGetLastError();
 }

@@ -459,17 +459,18 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     // a launch holds fewer than 2^32 threads, 512 in a block at most
     REQUIRE(((int64_t)a.few.items + a.many.items) * a.kv.kv_heads < (1 << 23), "%s: shape too large", fn);
     // the shares run in one launch: partial results and counters of their own
-    const size_t few = (paged_ws_bytes(a, a.few) + 255) & ~(size_t)255, many = paged_ws_bytes(a, a.many);
+    const size_t few = (paged_ws_bytes(a, a.few) + 255) & ~(size_t)255, many = (paged_ws_bytes(a, a.many) + 255) & ~(size_t)255;
     const size_t few_words = paged_words(a, a.few), words = few_words + paged_words(a, a.many);
     if (words > PAGED_SYNC_WORDS)
         return set_error(MVLM_ERR_UNSUPPORTED, "%s: %zu counters are needed, the device has %d", fn, words, PAGED_SYNC_WORDS);
-    op->workspace_bytes = few + many;
+    op->workspace_bytes = few + many + sizeof(*a.made);
     st = device_scratch(dev, op->workspace_bytes, &op->workspace);
     void* sync = nullptr;
     if (st == MVLM_OK) st = device_sync_words(dev, &sync);
     if (st != MVLM_OK) return st;
     a.few.ws = (float*)op->workspace;
     a.many.ws = (float*)((char*)op->workspace + few);
+    a.made = (uint32_t*)((char*)op->workspace + few + many);
     a.few.arrived = (uint32_t*)((char*)sync + ARGMAX_SYNC_BYTES);
     a.many.arrived = a.few.arrived + few_words;
     op->num_cus = dev->prop.multiProcessorCount;

@@ -22,7 +22,7 @@ struct KvAppendArgs {
 
 // How one kernel's share of a batch is cut into blocks.
 struct PagedDivision {
-    int tile;                      // f-rows per tile; 0: no sequence is this kernel's
+    int tile;                      // f-rows per tile; 0: there is no such share
     int64_t blocks_per_head;       // blocks wanted per kv head
     int unit_min, unit_step;       // least keys per block, and what a block's keys are a multiple of
     int items;                     // upper bound of the items per kv head
@@ -44,10 +44,11 @@ struct PagedAttnArgs {
     void* o;                       // [rows][heads][D]
     int o_dtype, heads, group;     // group: heads per kv head
     float scale_log2;              // scale * log2(e)
-    // division of the work (attention_paged.hip) of the sequences with few new
-    // rows, f = n group <= few_rows, and of those with more
-    int few_rows;
+    // division of the work (attention_paged.hip): of all sequences, or, where tiles of 256
+    // rows are made (many.tile != 0 and the lengths are worth it), of those with
+    // few new rows, f = n group <= PAGED_FEW, and of those with more
     PagedDivision few, many;
+    uint32_t* made;                // written by the kernel for many rows: whether it made the batch
     int many_least;                // tiles per kv head, times what their keys can be split, that are worth the second kernel
 };
 
@@ -133,7 +134,7 @@ struct PagedShare {
 };
 __device__ __forceinline__ int paged_splits(int len, int unit) { return len > unit ? (len + unit - 1) / unit : 1; }
 
-// few_rows: the f-rows up to which a sequence belongs to the first share
+// few_rows: the f-rows up to which a sequence belongs to the share of few
 template <int R, bool MANY>
 __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, const PagedSpan& sp, int few_rows) {
     const PagedSeqs& b = a.batch;

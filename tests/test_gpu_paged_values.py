@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import mvlm_amd as m
-from paged_ref import HALF_STEP, Batch, attention, close, filled_cache, to_bits, values
+from paged_ref import HALF_STEP, Batch, attention, cache_on, close, filled_cache, to_bits, values
 from test_gpu_paged import run_attention, same_or_close, say
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +96,34 @@ def test_keys_far_below_the_largest(dev, news, lens, heads, kv_heads, D, cd, od,
     worst = close(got, ref, tol, od)
     say("worst", worst)
     assert worst <= 1.0
+
+
+@pytest.mark.parametrize("news,lens,heads,kv_heads,D", [([768], [768], 32, 32, 64), ([256] + [1] * 11, [900] + [700] * 11, 32, 32, 64),
+                                                        ([768], [768], 32, 8, 128)])
+def test_tables_with_room_choose_by_what_is_held(dev, news, lens, heads, kv_heads, D):
+    """A table for 32768 positions of which few are held gives the values and, but for a launch that has
+    nothing to do, the time of a table for just those: 20 calls in a graph, the two taken in turn, the best of 10.
+    (Eight-wave blocks for what such tables hold took 1.4 to 1.9 times as long.)"""
+    plans = []
+    for width in (-(-max(lens) // 64), 512):
+        rng = np.random.default_rng(45)
+        batch = Batch(rng, news, lens, 64, width=width)
+        K, V = filled_cache(rng, batch, kv_heads, D, F16)
+        q, o = dev.upload(values(rng, (batch.rows, heads, D), F16)), dev.alloc(batch.rows * heads * D * 2)
+        b, cache = batch.device(dev), cache_on(dev, batch, K, V, F16)
+        plan = m.Plan(dev)
+        for _ in range(20):
+            plan.add_attention_paged(q, b, cache, o, F16, heads)
+        plan.use_graph(True)
+        plans.append((plan, o))
+    best = [np.inf, np.inf]
+    for _ in range(10):
+        for i, (plan, _) in enumerate(plans):
+            ev = plan.run(event=True)
+            ev.wait()
+            best[i] = min(best[i], ev.elapsed_ms() * 1000 / 20)
+            ev.release()
+    say("just wide enough, 32768 positions:", best, "us")
+    outs = [o.download(np.uint16) for _, o in plans]
+    assert np.array_equal(outs[0], outs[1])
+    assert best[1] <= 1.25 * best[0] + 2.0
