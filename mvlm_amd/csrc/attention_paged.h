@@ -198,7 +198,7 @@ struct PagedLayout {
     static constexpr int DP = 32 * KS32;                       // padded head_dim
     static constexpr int VP = DP + 16;                         // halfs
     static constexpr int OP = DP + 4;                          // floats
-    static constexpr int P = PAGED_KEYS * VP * 2, STAGE = P + PAGED_KEYS * R * 4;   // V, then probabilities (by key)
+    static constexpr int P = PAGED_KEYS * VP * 2, STAGE = P + (R > 16 ? PAGED_KEYS * R * 4 : 0);   // V, then probabilities (by key)
     static constexpr int MERGE = R * OP * 4 + 2 * R * 4;
     static constexpr int REGION = ((STAGE > MERGE ? STAGE : MERGE) + 15) / 16 * 16;
 };
@@ -369,9 +369,10 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             if constexpr (KS == 4) load_k(where);              // the registers do not hold both
         }
         // some rows see only part of this tile: if it holds values that are not finite,
-        // 0 x infinity would reach the rows that do not see them
+        // 0 x infinity would reach the rows that do not see them (R = 16: the rows are one
+        // token's, whose hidden keys are behind k_end)
         bool by_key = false;
-        if (kv0 + PAGED_KEYS > open_end && open_end < k_end) {
+        if (R > 16 && kv0 + PAGED_KEYS > open_end && open_end < k_end) {
             asm volatile("");
             uint32_t bad = 0;
 #pragma unroll
@@ -430,7 +431,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.scale_log2, -msafe));
             lrun += p[e];
         }
-        if (by_key) {                                          // key by key, over the rows that see the key
+        if (R > 16 && by_key) {                                // key by key, over the rows that see the key
             float* pw = (float*)(lds + wave * L::REGION + L::P);
 #pragma unroll
             for (int e = 0; e < NE; ++e) pw[(4 * NG * (e >> 2) + 4 * g + (e & 3)) * R + rl] = p[e];
