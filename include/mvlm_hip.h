@@ -382,14 +382,14 @@ int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, 
  * group = num_heads / kv_heads, over the positions t up to row r's own that exist
  * (what lies in others may be anything).  Q [rows][num_heads][head_dim] in the
  * cache's type, O the same shape in F32 or the cache's type; scale 0:
- * 1/sqrt(head_dim); scale log2(e) must be finite in fp32.  A row that sees no position, or only scores of -inf, is 0.
+ * 1/sqrt(head_dim); scale log2(e) must be finite in fp32.  A row that sees no
+ * position, or only scores of -inf, is 0.
  * Scores, maxima, sums and O before its store are fp32.  Probabilities are rounded
- * for the second product: to the cache's type where O has it (half a step, as large
- * as the rounding of O; fp16: plus 2^-37 of the row's largest), and for an F32 O to 22
- * bits or more (fp16: plus 2^-48 of the row's largest).
+ * for the second product: to the cache's type or finer where O has it (half a step,
+ * as large as the rounding of O; fp16: plus 2^-37 of the row's largest), and for an
+ * F32 O to 22 bits or more (fp16: plus 2^-48 of the row's largest).
  * A value that is not finite makes its element of the rows that see it not
- * finite (an infinity may become NaN in an F32 O: probabilities are multiplied in
- * parts) and reaches no other row. */
+ * finite (an infinity may become NaN: probabilities may be multiplied in parts) and reaches no other row. */
 int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
                          const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
                          mvlm_event** ev);

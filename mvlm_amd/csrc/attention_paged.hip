@@ -25,7 +25,7 @@
 //  * K and V of the next tile are asked for while this one is computed, the page of the
 //    one behind it before them: a wave has about 12 KB (head_dim 64) in flight.
 //  * P is rounded to the cache's type for a 16-bit O, as the rounding of O
-//    itself is of that size; for an fp32 O it is kept to 22 bits and more, as
+//    itself is of that size (bf16 single tokens: kept to 16 bits); for an fp32 O it is kept to 22 bits and more, as
 //    the sum of two fp16 or three bf16 parts, one product each (PagedP).
 //  * the running maximum moves only when a score exceeds it by more than SLACK
 //    (PagedP), so most tiles rescale nothing.
@@ -132,8 +132,11 @@ static hipError_t launch_few(hipStream_t s, const PagedAttnArgs& a) {
 template <int R, int KS>
 static hipError_t launch_few_dims(hipStream_t s, const PagedAttnArgs& a) {
     const bool wide = a.o_dtype == MVLM_F32;
+    // bf16 single tokens have two parts for a bf16 O as well, as their products cost next to nothing (4 of
+    // 32768 85.4 us with one and with two, 64 of 500 .. 1500 18.5 and 18.8, one of 512 7.1 and 7.3; fp16, whose
+    // one part is 8 times as fine and whose second is summed apart, 18.5 and 19.1, 7.2 and 7.5)
     if (a.kv.dtype == MVLM_F16) return wide ? launch_few<R, KS, false, 2>(s, a) : launch_few<R, KS, false, 1>(s, a);
-    return wide ? launch_few<R, KS, true, 3>(s, a) : launch_few<R, KS, true, 1>(s, a);
+    return wide ? launch_few<R, KS, true, 3>(s, a) : launch_few<R, KS, true, R == 16 ? 2 : 1>(s, a);
 }
 
 template <int R>

@@ -127,3 +127,20 @@ def test_tables_with_room_choose_by_what_is_held(dev, news, lens, heads, kv_head
     outs = [o.download(np.uint16) for _, o in plans]
     assert np.array_equal(outs[0], outs[1])
     assert best[1] <= 1.25 * best[0] + 2.0
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,D", [([2, 3, 5, 9, 40, 0, 1], 8, 8, 64), ([4, 6, 30, 700], 32, 4, 128),
+                                                   ([1500, 7], 6, 2, 72)])
+def test_bf16_single_tokens_round_once(dev, lens, heads, kv_heads, D):
+    """A bf16 O of single tokens is its value in 64 bits rounded once, but for what fp32 arithmetic (the bound of
+    paged_ref.attention) and probabilities of 16 bits (2^-17 each; values are positive, so 2^-17 O) move it by."""
+    say("round once", lens, heads, kv_heads, D)
+    rng = np.random.default_rng(47)
+    batch = Batch(rng, [1] * len(lens), lens, 16, ragged=False)
+    K, V = filled_cache(rng, batch, kv_heads, D, BF16)
+    V &= np.uint16(0x7FFF)
+    q = values(rng, (batch.rows, heads, D), BF16)
+    got = run_attention(dev, batch, q, K, V, BF16, BF16, heads)
+    ref, tol = attention(batch, q, K, V, BF16, D ** -0.5, 2)
+    half_step = 2.0 ** (np.floor(np.log2(np.maximum(ref + tol, 1e-30))) - 8)
+    assert np.all(np.abs(got - ref) <= half_step + tol + 2.0 ** -17 * ref)
