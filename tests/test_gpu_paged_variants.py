@@ -6,9 +6,9 @@ import numpy as np
 import pytest
 
 import mvlm_amd as m
-from paged_ref import Batch, from_bits, values
+from paged_ref import Batch, attention, cache_on, filled_cache, from_bits, values
 from test_gpu_logits import NP, Controls, check
-from test_gpu_paged import check_attention, say
+from test_gpu_paged import check_attention, same_or_close, say
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,38 @@ def test_logits_of_many_rows_off_the_grid(dev, rows, n, dt, history, bias, mask,
     check(from_bits(got[offset:].reshape(rows, ld)[:, :n], dt), ref, tol, dt)
     assert np.all(got[offset:].reshape(rows, ld)[:, n:] == 7) and np.all(got[:offset] == 7)
     assert np.array_equal(x.download(NP[dt]), flat)
+
+
+def test_one_graph_crosses_from_few_keys_to_many_and_back(dev):
+    """a graph captured for a table with room: as the lengths change, tiles of 32 rows, of 256, and of 256 with split
+    keys make the batch; every replay against the definition and an eager call, with two graphs in turn"""
+    rng = np.random.default_rng(55)
+    heads, D, steps = 64, 64, ([300, 20], [5000, 33], [256, 1], [4200, 900], [6000, 7])
+    jobs = []
+    for od in (F16, F32):
+        batch = Batch(rng, [256, 1], [6000, 900], 16, width=500)
+        K, V = filled_cache(rng, batch, heads, D, F16)
+        bits = values(rng, (batch.rows, heads, D), F16)
+        q, cache, b = dev.upload(bits), cache_on(dev, batch, K, V, F16), batch.device(dev)
+        o, eager = (dev.alloc(batch.rows * heads * D * 4) for _ in range(2))
+        plan = m.Plan(dev)
+        plan.add_attention_paged(q, b, cache, o, od, heads)
+        plan.use_graph(True)
+        jobs.append((plan, batch, bits, K, V, q, cache, b, o, eager, od))
+    for lens in steps:
+        for plan, batch, *_, b, o, _, _ in jobs:
+            batch.lens = lens
+            b.buffers[0].upload(np.asarray(lens, np.int32))
+            o.zero()
+        for plan, *_ in jobs:
+            plan.run(2)
+        for plan, batch, bits, K, V, q, cache, b, o, eager, od in jobs:
+            dev.attention_paged(q, b, cache, eager, od, heads)
+            got = o.download(NP[od])[:bits.size]
+            assert np.array_equal(got.view(np.uint8), eager.download(NP[od])[:bits.size].view(np.uint8))
+            ref, tol = attention(batch, bits, K, V, F16, D ** -0.5, 1 if od != F32 else 2)
+            worst = same_or_close(from_bits(got, od).reshape(ref.shape), ref, tol, od)
+            say("lengths", lens, "worst", worst)
+            assert worst <= 1.0
+    ms = jobs[0][0].profile()
+    assert len(ms) == 1 and ms[0] > 0
