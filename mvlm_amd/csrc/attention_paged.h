@@ -276,7 +276,8 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     // 32 heads of 64, 35.7 -> 28.7 us, 8 heads of 128 64 -> 53, 768 rows 14.0 -> 12.1.  Not
     // for head_dims of 72 .. 96, whose rows are no multiple of a line or leave loads half empty
     // (768 rows of 32 heads of 80 22.4 us, staged 23.4; 256 and 11 of 96 41.4 and 40.7), and not
-    // for 128 inside the kernel for many rows, whose registers it would spill (306 -> 330 us).
+    // for 128 inside the kernel for many rows, more of whose registers it would spill (306 -> 330 us;
+    // here 3 spill, outside the key loop).
     constexpr bool STAGED = R == 32 && KS != 3 && (KS < 4 || NW == 4);
     u32x4 kf[U][S], kr[STAGED ? VI : 1], vf[VI];
     uint32_t at[VI];                                           // where this lane's chunks are

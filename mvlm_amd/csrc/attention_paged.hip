@@ -99,7 +99,8 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     // 28.5 us, 29.7 at 2; 256 and 7 of 8 heads of 128 52.9 and 62.1)
     // Tiles that leave most CUs idle, over tables that do not hold more than 512 keys for
     // each CU, take eight waves instead of four: their splits are few or none (one sequence of
-    // 512: 8.3 -> 7.4 us; 4 of 32768 would take 88.4 us instead of 84.8).
+    // 512: 8.4 -> 7.4 us, also where its table has room for more than this rule takes; 4 of 32768 would take
+    // 88.4 us instead of 84.8, one of 8192 22.7 instead of 18.8).
     const int64_t heads_tiles = tiles * a->kv.kv_heads;
     const int waves = R == 16 && 2 * heads_tiles <= num_cus && heads_tiles * b.positions <= 512 * (int64_t)num_cus ? 8 : 4;
     a->few = paged_divide(*a, R, (R == 16 ? 2 : 1) * (int64_t)num_cus, tiles, (waves == 8 ? 2 : 1) * PAGED_KEYS * waves,

@@ -10,15 +10,17 @@
 // the products O^T += V^T P^T of tile i - 1 and S^T = K Q^T of tile i of all waves;
 // waves 0..3 run them first and then the softmax of tile i, waves 4..7 run the softmax
 // of tile i - 1 first and then the products, so that one wave of a SIMD has matrix
-// instructions while the other has vector ones.  The products have the higher
-// priority.  One barrier per tile is enough, as both groups read K of tile i and V of
+// instructions while the other has vector ones.  The products, and the softmax of waves 4..7, have
+// the higher priority.  One barrier per tile is enough, as both groups read K of tile i and V of
 // tile i - 1 there, while the tiles after them are on their way into the other buffers
 // of a ring: the blocks of one kv head walk its keys in step, so each tile comes from
 // memory once for all of them and its loads have to cover that latency.
-// 2048 bf16 rows on 8192 positions, 32 heads of 128 over 8 kv heads (309 GFLOP): 298 ..
-// 316 us as the clock allows, 977 .. 1037 TFLOP/s, of the 1229 .. 1275 that a large
+// 2048 bf16 rows on 8192 positions, 32 heads of 128 over 8 kv heads (309 GFLOP): 302 ..
+// 322 us as the clock allows, 960 .. 1023 TFLOP/s, of the 1229 .. 1275 that a large
 // library product of that type reaches here; with both groups in step 384 us, with two
-// barriers per tile 349.
+// barriers per tile 349.  For an fp32 O, whose probabilities have two (fp16) or three (bf16) parts, 470
+// and 510.  At head_dim 128 all 256 registers are in use and 13 to 18 values spill, outside
+// the key loop of the tiles of 256 rows.
 //  * K and V tiles go straight from memory to LDS in 16-byte chunks; a hidden
 //    key's chunks and those past head_dim come from zeros.  Their rows are found through
 //    the page table for SLOT_KEYS keys at a time, kept in LDS, so that no load that a wave waits for
