@@ -389,7 +389,8 @@ int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, 
  * as large as the rounding of O; fp16: plus 2^-37 of the row's largest), and for an
  * F32 O to 22 bits or more (fp16: plus 2^-48 of the row's largest).
  * A value that is not finite makes its element of the rows that see it not
- * finite (an infinity may become NaN: probabilities may be multiplied in parts) and reaches no other row. */
+ * finite (an infinity may become NaN: probabilities may be multiplied in parts)
+ * and reaches no other row. */
 int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
                          const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
                          mvlm_event** ev);

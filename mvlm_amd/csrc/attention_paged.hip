@@ -25,8 +25,9 @@
 //  * K and V of the next tile are asked for while this one is computed, the page of the
 //    one behind it before them: a wave has about 12 KB (head_dim 64) in flight.
 //  * P is rounded to the cache's type for a 16-bit O, as the rounding of O
-//    itself is of that size (bf16 single tokens: kept to 16 bits); for an fp32 O it is kept to 22 bits and more, as
-//    the sum of two fp16 or three bf16 parts, one product each (PagedP).
+//    itself is of that size (bf16 single tokens: kept to 16 bits); for an fp32 O
+//    it is kept to 22 bits and more, as the sum of two fp16 or three bf16 parts,
+//    one product each (PagedP).
 //  * the running maximum moves only when a score exceeds it by more than SLACK
 //    (PagedP), so most tiles rescale nothing.
 //  * hidden keys may hold anything: their scores are replaced, not added to,

@@ -34,14 +34,15 @@
 //  * a tile with keys that some of a wave's rows do not see is checked for values that are
 //    not finite (0 x infinity would reach rows that do not see them); if it holds any,
 //    its second product is made key by key over the rows that see the key.
-// Whether tiles of 256 rows pay depends on the lengths, which only the device knows (chunk_worth): this
-// kernel is launched before the one for few rows, and either makes the whole batch, the sequences with few new
-// rows as items of paged_few_item behind those with many, or ends at once and leaves it to that one (made).  A block fills a CU (its LDS), so there is one per CU, and
-// they take items from queues, one per XCD: item w belongs to queue w % 8, so with a
-// multiple of 8 kv heads the tiles of a head run on one XCD and share its L2.  A
-// sequence's tiles come in order of their keys, the most first, and the blocks take
-// them in turn, from the last block to the first in every other round, so that who
-// had the longest takes the shortest next.
+// Whether tiles of 256 rows pay depends on the lengths, which only the device knows
+// (chunk_worth): this kernel is launched before the one for few rows, and either makes
+// the whole batch, the sequences with few new rows as items of paged_few_item behind
+// those with many, or ends at once and leaves it to that one (made).  A block fills a
+// CU (its LDS), so there is one per CU, and they take items from queues, one per XCD:
+// item w belongs to queue w % 8, so with a multiple of 8 kv heads the tiles of a head
+// run on one XCD and share its L2.  A sequence's tiles come in order of their keys, the
+// most first, and the blocks take them in turn, from the last block to the first in
+// every other round, so that who had the longest takes the shortest next.
 #include "attention_paged.h"
 
 #include <algorithm>
