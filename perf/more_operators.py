@@ -371,9 +371,9 @@ def _plain_sample(case, t):
     w = torch.where((w >= min_p) & (rank < limit), w, 0.0)
     before = torch.cumsum(w, 1) - w
     w = torch.where((rank == 0) | (top_p >= 1.0) | (before < top_p * w.sum(1, keepdim=True)), w, 0.0)
-    sums = torch.cumsum(torch.zeros_like(w).scatter_(1, token, w), 1)
-    picked = (sums <= u * sums[:, -1:]).sum(1)
-    return [torch.where(t["temperature"] > 0, picked, token[:, 0]).int()]
+    sums = torch.cumsum(w, 1)
+    picked = torch.where(t["temperature"][:, None] > 0, (sums <= u * sums[:, -1:]).sum(1, keepdim=True), 0)
+    return [token.gather(1, picked)[:, 0].int()]
 
 
 # ---- the framework's calls -------------------------------------------------------------
@@ -573,6 +573,5 @@ def _exact_token(case, t, r):
     kept = [i for i in order[:int(t["top_k"][r]) or len(x)] if w[i] >= min_p]
     if top_p < 1.0:
         kept = kept[:int(np.searchsorted(np.cumsum(w[kept]), top_p * math.fsum(w[kept]))) + 1]
-    kept = sorted(kept)
     sums = np.cumsum(w[kept])
     return int(kept[int(np.searchsorted(sums, u * sums[-1], side="right"))])
