@@ -51,7 +51,10 @@ enum mvlm_dtype {
     MVLM_F16 = 1,
     MVLM_Q4_0 = 2,
     MVLM_Q8_0 = 8,
-    MVLM_BF16 = 30
+    MVLM_BF16 = 30,
+    /* Paged caches only, not a ggml type: e4m3 codes in blocks of 32 dims of a
+     * head that share a power of two (OCP microscaling; mvlm_paged_kv). */
+    MVLM_MXFP8 = 100
 };
 
 enum mvlm_layout { MVLM_LAYOUT_NK = 0, MVLM_LAYOUT_KN = 1 };
@@ -328,9 +331,21 @@ int mvlm_argmax(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
  * every step of a batch of the same shape.
  *
  * A cache: K and V hold num_pages pages of [kv_heads][page_size][head_dim]
- * elements (F16 or BF16), 16-byte aligned, not overlapping; head_dim a multiple
- * of 8, at most 128; at most 1024 kv_heads; fewer than 2^31 slots num_pages
- * kv_heads page_size, and K less than 64 GiB. */
+ * elements (F16, BF16 or MXFP8), 16-byte aligned, not overlapping; head_dim a
+ * multiple of 8, at most 128; at most 1024 kv_heads; fewer than 2^31 slots
+ * num_pages kv_heads page_size, and K less than 64 GiB (MXFP8: 32 GiB of codes).
+ *
+ * MXFP8: K and V each hold a byte per element, in the order above, and from the
+ * next multiple of 16 bytes on, in the order of the slots, four bytes per slot:
+ * byte b belongs to dims 32 b .. 32 b + 31.  The value of an e4m3 code c under byte
+ * E is c 2^(E - 127).  mvlm_kv_append_paged takes the least E of 27 .. 247 under
+ * which the block's largest magnitude a is at most 448 2^(E - 127), rounds
+ * x 2^(127 - E) to the nearest code (even), infinities and NaN to the code of NaN, and
+ * magnitudes from 31 2^123 up (which would round to 2^128) to 15 2^124.  A value is
+ * off by half a step at most: 2^-4 of itself, or 2^-10 2^(E - 127) <= 2^-17 a where that is more (a below
+ * 2^-91: 2^-110).  Every value is a bf16 number, and q is BF16 with such a cache.
+ * Bytes for dims past head_dim are not used; other bytes than 27 .. 247 may
+ * only lie where no position is held. */
 typedef struct mvlm_paged_kv {
     mvlm_buffer* k;
     mvlm_buffer* v;
@@ -340,6 +355,9 @@ typedef struct mvlm_paged_kv {
     int kv_heads;
     int head_dim;
 } mvlm_paged_kv;
+/* Bytes that K needs, and V as much, from the cache's dtype and sizes (its
+ * buffers are not looked at and may be NULL). */
+int mvlm_paged_kv_bytes(const mvlm_paged_kv* cache, size_t* bytes);
 /* A batch: sequence s owns rows [row_start[s], row_start[s + 1]) of the step's
  * tensors (row_start: int32 [num_seqs + 1], not decreasing; NULL: row s alone,
  * rows == num_seqs) and holds kv_len[s] positions, its new rows' among them: its
@@ -372,16 +390,40 @@ typedef struct mvlm_rope {
 /* Row r of qkv (F32, F16 or BF16, ld elements apart) is num_heads q heads, then
  * kv_heads key heads, then kv_heads value heads.  q and keys are rotated to the
  * row's position (rope NULL: not) in fp32; q goes to q_out [rows][num_heads]
- * [head_dim] and keys and values into the cache, rounded to its type.  A row
+ * [head_dim] and keys and values into the cache, rounded to its type (MXFP8: q
+ * to BF16).  A row
  * without a place (no position, no page, or past the rope table) writes zeros to
  * q_out and nothing to the cache.  No two rows of a call may have the same place. */
 int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
                          const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
                          mvlm_buffer* q_out, const mvlm_rope* rope, mvlm_event** ev);
+/* Norms of q and k heads, before the rotation: each head x becomes
+ * x w / sqrt(mean(x^2) + eps), w fp32 [head_dim], in fp32 (a head whose sum of squares
+ * overflows becomes 0).  A NULL weight leaves its kind as it is (not both);
+ * eps is finite and not negative. */
+typedef struct mvlm_head_norm {
+    const mvlm_buffer* q_weight;
+    const mvlm_buffer* k_weight;
+    float eps;
+} mvlm_head_norm;
+/* mvlm_kv_append_paged with norms (NULL = none) in the same pass. */
+int mvlm_kv_append_paged_ex(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                            const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                            mvlm_buffer* q_out, const mvlm_rope* rope, const mvlm_head_norm* norm, mvlm_event** ev);
+/* Reads a cache back: row r of the batch, at the position that it has there, to
+ * rows of K_out and V_out, [rows][kv_heads][head_dim] in out_dtype (F32, F16 or
+ * BF16), ld elements apart (one of the two may be NULL).  With row_start counting
+ * all of a sequence's positions that is the sequence, contiguous, as
+ * mvlm_attention takes it.  Values are rounded once where out_dtype has fewer
+ * bits.  A row without a place is zeros; rows of no sequence and elements between the
+ * rows are left as they were. */
+int mvlm_kv_read_paged(mvlm_device* dev, const mvlm_paged_batch* batch, const mvlm_paged_kv* cache,
+                       mvlm_buffer* K_out, mvlm_buffer* V_out, int out_dtype, int64_t ld, mvlm_event** ev);
 /* O[r][h] = sum over t of softmax(scale Q[r][h] . K[t][h / group]) V[t][h / group],
  * group = num_heads / kv_heads, over the positions t up to row r's own that exist
  * (what lies in others may be anything).  Q [rows][num_heads][head_dim] in the
- * cache's type, O the same shape in F32 or the cache's type; scale 0:
+ * cache's type, O the same shape in F32 or the cache's type (MXFP8: both have
+ * BF16 in its place); scale 0:
  * 1/sqrt(head_dim); scale log2(e) must be finite in fp32.  A row that sees no
  * position, or only scores of -inf, is 0.
  * Scores, maxima, sums and O before its store are fp32.  Probabilities are rounded
@@ -422,6 +464,33 @@ typedef struct mvlm_logit_controls {
  * out may be x. */
 int mvlm_logits_process(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
                         const mvlm_logit_controls* controls, mvlm_buffer* out, mvlm_event** ev);
+/* How a token of each row is drawn.  With v the row's logits (NaN counts as an
+ * infinity of its sign), m their largest and T the row's temperature,
+ *   w_i = exp((v_i - m) / T)          (v_i = -inf: 0; v_i = m: 1)
+ * and the tokens in order of falling v, the lower index first among equals:
+ *   kept: the tokens with w_i >= min_p, of them the first top_k, of those the
+ *         shortest start whose sum is at least top_p of theirs (one at least);
+ *   picked: the first of the kept whose running sum exceeds uniform times theirs.
+ * uniform: fp32 [rows], 0 <= u < 1, the caller's random numbers (below 0 or NaN
+ * counts as 0, 1 and above as the last kept).  The others may be NULL, or have no effect by
+ * value: temperature fp32 (NULL: 1; 0, below or NaN: the first token of the
+ * largest v), top_k int32 (0 or below: all), top_p fp32 (1, above or NaN: all; 0 or below: one token),
+ * min_p fp32 (0, below or NaN: all; above 1 counts as 1).  A row that holds only -inf picks token 0, as mvlm_argmax
+ * does.
+ * w is computed in 64 bits and rounded to a multiple of 2^-s, s = 62 - ceil(log2 n), at most 51
+ * (what rounds to 0 is never picked unless it is the only one); sums of these are exact, so a
+ * call's result does not depend on the order of its work. */
+typedef struct mvlm_sampling {
+    const mvlm_buffer* uniform;          /* fp32 [rows] */
+    const mvlm_buffer* temperature;      /* fp32 [rows] or NULL */
+    const mvlm_buffer* top_k;            /* int32 [rows] or NULL */
+    const mvlm_buffer* top_p;            /* fp32 [rows] or NULL */
+    const mvlm_buffer* min_p;            /* fp32 [rows] or NULL */
+} mvlm_sampling;
+/* out_index[r] (int32, device) = the token drawn from row r of x (rows x n, ld
+ * elements apart, F32/F16/BF16, n at most 2^24).  x is left as it is. */
+int mvlm_sample(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                const mvlm_sampling* sampling, mvlm_buffer* out_index, mvlm_event** ev);
 
 /* ---- synthetic inputs on the device ------------------------------------- */
 /* SplitMix64 -> Box-Muller fills (same generator as the CPU oracle, computed
@@ -483,10 +552,17 @@ int mvlm_plan_add_argmax(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int r
 int mvlm_plan_add_kv_append_paged(mvlm_plan* plan, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
                                   const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
                                   mvlm_buffer* q_out, const mvlm_rope* rope);
+int mvlm_plan_add_kv_append_paged_ex(mvlm_plan* plan, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                     const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                     mvlm_buffer* q_out, const mvlm_rope* rope, const mvlm_head_norm* norm);
+int mvlm_plan_add_kv_read_paged(mvlm_plan* plan, const mvlm_paged_batch* batch, const mvlm_paged_kv* cache,
+                                mvlm_buffer* K_out, mvlm_buffer* V_out, int out_dtype, int64_t ld);
 int mvlm_plan_add_attention_paged(mvlm_plan* plan, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
                                   const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale);
 int mvlm_plan_add_logits_process(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
                                  const mvlm_logit_controls* controls, mvlm_buffer* out);
+int mvlm_plan_add_sample(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                         const mvlm_sampling* sampling, mvlm_buffer* out_index);
 /* enable != 0: capture the plan into a HIP graph (now) and replay it on run. */
 int mvlm_plan_use_graph(mvlm_plan* plan, int enable);
 /* Enqueue the plan `repeats` times; `ev` (optional) spans everything enqueued. */

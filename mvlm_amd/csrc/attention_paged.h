@@ -203,17 +203,31 @@ struct PagedLayout {
     static constexpr int REGION = ((STAGE > MERGE ? STAGE : MERGE) + 15) / 16 * 16;
 };
 
-// The block of R f-rows of a tile and one kv head.  KS: head_dim <= 32 KS; BF: bf16
-// cache; PP: parts of P; NW: waves of the block; lds: NW REGIONs and a word.
+// Eight codes of an 8-bit cache as bf16, which holds every one of them exactly; up: their block's power of two
+__device__ __forceinline__ u32x4 mx_values(uint32_t lo, uint32_t hi, float up) {
+    auto two = [&](uint32_t w, auto high) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, up, decltype(high)::value));
+    };
+    return u32x4{two(lo, std::false_type{}), two(lo, std::true_type{}), two(hi, std::false_type{}), two(hi, std::true_type{})};
+}
+// the power of two in byte b of a slot's word
+__device__ __forceinline__ float mx_power(uint32_t word, int b) { return __uint_as_float((word >> (8 * b) & 0xFFu) << 23); }
+
+// The block of R f-rows of a tile and one kv head.  KS: head_dim <= 32 KS; CT: the
+// cache's type; PP: parts of P; NW: waves of the block; lds: NW REGIONs and a word.
 // Makes the index-th item, if there is one.
-template <int R, int KS, bool BF, int PP, int NW>
+template <int R, int KS, int CT, int PP, int NW>
 __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const PagedShare& share, int index, int h, uint8_t* lds) {
     using L = PagedLayout<R, KS>;
     using Acc = typename PagedAcc<R>::type;
+    constexpr bool MX = CT == MVLM_MXFP8, BF = CT != MVLM_F16;
     constexpr int NG = 64 / R;                                 // lane groups: l / R
-    constexpr int U = 32 / R, S = KS * 4 / NG;                 // products of 32 keys, steps of 8 NG dims
+    // products of 32 keys, steps of 8 NG dims (of 8-bit fragments in pairs, as 16 bytes hold two steps)
+    constexpr bool PAIRS = MX && R == 16;
+    constexpr int U = 32 / R, S = PAIRS ? (KS + 1) / 2 * 2 : KS * 4 / NG;
     constexpr int NE = R / 2, STEPS = NE / 8;                  // a lane's keys of 32, steps of 8 of them
-    constexpr int DT = L::DP / R, NR = R == 16 ? 4 : 16, VI = 2 * KS;
+    constexpr int CE = MX ? 16 : 8;                            // elements of a 16-byte chunk
+    constexpr int DT = L::DP / R, NR = R == 16 ? 4 : 16, VI = 16 * KS / CE;
     const int tid = own_thread(), lane = tid & 63, wave = tid >> 6;
     const int rl = lane % R, g = lane / R;
     const int D = a.kv.D;
@@ -233,23 +247,24 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     u32x4 qf[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int d = 8 * NG * s + 8 * g;
+        const int d = PAIRS ? 16 * NG * (s / 2) + 16 * g + 8 * (s & 1) : 8 * NG * s + 8 * g;
         qf[s] = u32x4{0u, 0u, 0u, 0u};
         if (f < rows_f && d < D)
             qf[s] = *reinterpret_cast<const u32x4*>(a.q + ((int64_t)(sp.row0 + j) * a.heads + h * a.group + gh) * D + d);
     }
 
     uint16_t* vt = (uint16_t*)(lds + wave * L::REGION);        // [32 keys][VP]
-    const int cpr = D / 8;
-    int vkey[VI], vdim[VI];                                    // V chunk c = lane + 64 i: key c / cpr, dims 8 (c % cpr)
+    const int cpr = (D + CE - 1) / CE;                         // the last chunk of a row of 8 bits may reach 8 bytes past it,
+                                                               // which are the next slot's or the scales' behind the last
+    int vkey[VI], vdim[VI];                                    // V chunk c = lane + 64 i: key c / cpr, dims CE (c % cpr)
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
         const int c = lane + 64 * i;
         vkey[i] = c / cpr;
-        vdim[i] = 8 * (c - vkey[i] * cpr);
+        vdim[i] = CE * (c - vkey[i] * cpr);
     }
     // page of key kv0 + lane % 32 (asked for a tile before it is needed), and where that
-    // key is, in 16-byte chunks of the cache (below 2^32, checked on the host)
+    // key is, in 16-byte chunks of the cache (below 2^32, checked on the host; of 8 bits: its slot)
     const int* table = a.batch.table + (int64_t)it.seq * a.batch.width;
     auto ask_page = [&](int kv0) {
         const int key = kv0 + (lane & 31);
@@ -258,7 +273,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     auto exists = [&](int page) { return page >= 0 && page < a.kv.num_pages; };
     auto chunk_of = [&](int kv0, int page) -> uint32_t {       // a hidden key's: the first, so that it may be read
         const int key = kv0 + (lane & 31);
-        return exists(page) ? (uint32_t)a.kv.slot(page, h, key - a.kv.page.quotient(key) * a.kv.page.div) * (uint32_t)cpr : 0u;
+        return exists(page) ? (uint32_t)a.kv.slot(page, h, key - a.kv.page.quotient(key) * a.kv.page.div) * (uint32_t)(MX ? 1 : cpr) : 0u;
     };
 
     float mrun = -INFINITY, lrun = 0.0f;                       // the reference (PagedP), and this lane's keys' sum
@@ -278,26 +293,43 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     // (768 rows of 32 heads of 80 22.4 us, staged 23.4; 256 and 11 of 96 41.4 and 40.7), and not
     // for 128 inside the kernel for many rows, more of whose registers it would spill (306 -> 330 us;
     // here 3 spill, outside the key loop).
-    constexpr bool STAGED = R == 32 && KS != 3 && (KS < 4 || NW == 4);
-    u32x4 kf[U][S], kr[STAGED ? VI : 1], vf[VI];
+    // Of 8 bits a tile in LDS is made of the registers' values as it is stored, K's and V's alike.
+    constexpr bool STAGED = R == 32 && (MX || (KS != 3 && (KS < 4 || NW == 4)));
+    u32x4 kf[U][PAIRS ? S / 2 : S], kr[STAGED ? VI : 1], vf[VI];
+    uint32_t scale = 0, scale_next = 0;                        // of key kv0 + lane % 32: K's, in lanes 32.. V's
     uint32_t at[VI];                                           // where this lane's chunks are
     // in the global address space: a generic load counts as one of LDS too, and every wait for LDS
     // would be one for it
     typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
+    typedef const __attribute__((address_space(1))) uint32_t global_u32;
     auto chunk_at = [](const uint16_t* base, uint32_t c) { return (global_u32x4*)((uintptr_t)base + ((uint64_t)c << 4)); };
+    // 16 codes of a slot; rows lie at multiples of 8 bytes
+    typedef u32x4 u32x4_any __attribute__((aligned(8)));
+    typedef const __attribute__((address_space(1))) u32x4_any global_codes;
+    auto codes_at = [&](const uint16_t* base, uint32_t slot, int d) {
+        return *(global_codes*)((uintptr_t)base + (uint64_t)slot * (uint32_t)D + (uint32_t)d);
+    };
     auto locate = [&](uint32_t where) {
 #pragma unroll
-        for (int i = 0; i < VI; ++i) at[i] = __shfl(where, vkey[i] & 31, 64) + (uint32_t)(vdim[i] >> 3);
+        for (int i = 0; i < VI; ++i) at[i] = __shfl(where, vkey[i] & 31, 64) + (MX ? 0u : (uint32_t)(vdim[i] >> 3));
+    };
+    auto load_scale = [&](uint32_t where) {
+        if constexpr (MX) scale_next = *(global_u32*)((uintptr_t)(lane < 32 ? a.kv.k_scale : a.kv.v_scale) + ((uint64_t)where << 2));
     };
     auto load_k = [&](uint32_t where) {
         if constexpr (STAGED) {
 #pragma unroll
-            for (int i = 0; i < VI; ++i) kr[i] = *chunk_at(a.kv.k, at[i]);
+            for (int i = 0; i < VI; ++i) kr[i] = MX ? codes_at(a.kv.k, at[i], vdim[i]) : *chunk_at(a.kv.k, at[i]);
             return;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t c = __shfl(where, R * u + rl, 64);  // a hidden key's score is replaced below
+            if constexpr (PAIRS) {
+#pragma unroll
+                for (int s = 0; s < S / 2; ++s) kf[u][s] = codes_at(a.kv.k, c, NG * s + g < cpr ? CE * (NG * s + g) : 0);
+                continue;
+            }
             global_u32x4* row = chunk_at(a.kv.k, c + (uint32_t)g);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
@@ -308,12 +340,31 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     };
     auto load_v = [&] {
 #pragma unroll
-        for (int i = 0; i < VI; ++i) vf[i] = *chunk_at(a.kv.v, at[i]);
+        for (int i = 0; i < VI; ++i) vf[i] = MX ? codes_at(a.kv.v, at[i], vdim[i]) : *chunk_at(a.kv.v, at[i]);
     };
     auto store = [&](const u32x4* from) {                      // a tile's chunks into LDS
 #pragma unroll
         for (int i = 0; i < VI; ++i)
             if (64 * i + 64 <= 128 * (KS - 1) || vkey[i] < PAGED_KEYS) *reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]) = from[i];
+    };
+    // a tile's 8-bit chunks as bf16; first: the lane whose scale is that of the tile's first key
+    auto widen = [&](const u32x4* from, int first, u32x4 (*to)[2]) {
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+            const uint32_t word = __shfl(scale, first + (vkey[i] & 31), 64);
+            const float up = mx_power(word, vdim[i] >> 5);
+            to[i][0] = mx_values(from[i][0], from[i][1], up);
+            to[i][1] = mx_values(from[i][2], from[i][3], up);
+        }
+    };
+    auto store_wide = [&](const u32x4 (*from)[2]) {
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+            if (vkey[i] < PAGED_KEYS) {
+                u32x4* to = reinterpret_cast<u32x4*>(vt + vkey[i] * L::VP + vdim[i]);
+                to[0] = from[i][0];
+                to[1] = from[i][1];
+            }
     };
     int kv0 = k_begin + PAGED_KEYS * wave;
     constexpr int STEP = PAGED_KEYS * NW;
@@ -321,10 +372,12 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     const int page = ask_page(kv0);
     uint32_t where = chunk_of(kv0, page), gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page));
     locate(where);
+    load_scale(where);
     load_k(where);
     load_v();
     for (; kv0 < k_end; kv0 += STEP) {
         const uint32_t gone = gone_next;
+        scale = scale_next;
         // the page of the tile after next is asked for before the loads, so that its
         // wait, an iteration later, does not wait for them
         auto next = [&] {
@@ -332,10 +385,30 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             gone_next = (uint32_t)__builtin_amdgcn_ballot_w64(!exists(page_next));
             page_next = ask_page(kv0 + 2 * STEP);
             locate(where);
+            load_scale(where);
         };
         // dims past head_dim: K's registers hold other dims there
         auto clear_dims = [&] {
-            if (D < 32 * KS) {
+            if constexpr (MX) {
+                if constexpr (PAIRS) {
+                    if (D < 16 * NG * (S / 2)) {
+                        asm volatile("");
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int k = 0; k < S / 2; ++k) {
+                                const int d = CE * (NG * k + g);
+                                if (d >= D) kf[u][k][0] = kf[u][k][1] = 0u;
+                                if (d + 8 >= D) kf[u][k][2] = kf[u][k][3] = 0u;
+                            }
+                    }
+                } else if (D < 32 * KS) {                      // fragments of the tile in LDS, in 16 bits
+                    asm volatile("");
+#pragma unroll
+                    for (int k = 0; k < S; ++k)
+                        if (8 * (NG * k + g) >= D) kf[0][k] = u32x4{0u, 0u, 0u, 0u};
+                }
+            } else if (D < 32 * KS) {
                 asm volatile("");
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -352,13 +425,24 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
 #pragma unroll
                 for (int r = 0; r < NR; ++r) s[r] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < S; ++k) s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
+                for (int k = 0; k < S; ++k) {
+                    if constexpr (PAIRS) {
+                        const float up = mx_power(__shfl(scale, R * u + rl, 64), min((NG * (k / 2) + g) >> 1, (D - 1) >> 5));
+                        s = mfma_paged<R, BF>(mx_values(kf[u][k / 2][2 * (k & 1)], kf[u][k / 2][2 * (k & 1) + 1], up), qf[k], s);
+                    } else
+                        s = mfma_paged<R, BF>(kf[u][k], qf[k], s);
+                }
 #pragma unroll
                 for (int r = 0; r < NR; ++r) p[NR * u + r] = s[r];
             }
         };
+        u32x4 wide[MX ? VI : 1][2];
         if constexpr (STAGED) {
-            store(kr);
+            if constexpr (MX) {
+                widen(kr, 0, wide);
+                store_wide(wide);
+            } else
+                store(kr);
             asm volatile("" ::: "memory");                     // this wave's LDS: its reads follow its stores
 #pragma unroll
             for (int k = 0; k < S; ++k) kf[0][k] = *reinterpret_cast<const u32x4*>(vt + rl * L::VP + 8 * NG * k + 8 * g);
@@ -373,15 +457,17 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
         // 0 x infinity would reach the rows that do not see them (R = 16: the rows are one
         // token's, whose hidden keys are behind k_end)
         bool by_key = false;
+        if constexpr (MX) widen(vf, 32, wide);
         if (R > 16 && kv0 + PAGED_KEYS > open_end && open_end < k_end) {
             asm volatile("");
             uint32_t bad = 0;
 #pragma unroll
             for (int i = 0; i < VI; ++i)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
-                    bad |= vkey[i] < PAGED_KEYS && !((gone >> (vkey[i] & 31)) & 1u) && ((vf[i][x] & e) == e || ((vf[i][x] >> 16) & e) == e);
+                for (int x = 0; x < (MX ? 8 : 4); ++x) {
+                    const uint32_t e = BF ? 0x7F80u : 0x7C00u, w = MX ? wide[i][x >> 2][x & 3] : vf[i][x & 3];
+                    bad |= vkey[i] < PAGED_KEYS && !((gone >> (vkey[i] & 31)) & 1u) && (!MX || vdim[i] + (x >> 2) * 8 < D) &&
+                           ((w & e) == e || ((w >> 16) & e) == e);
                 }
             by_key = __builtin_amdgcn_ballot_w64(bad) != 0;
         }
@@ -389,9 +475,13 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
             asm volatile("");                                  // a branch: few tiles need this
 #pragma unroll
             for (int i = 0; i < VI; ++i)
-                if ((gone >> (vkey[i] & 31)) & 1u) vf[i] = u32x4{0u, 0u, 0u, 0u};
+                if ((gone >> (vkey[i] & 31)) & 1u) {
+                    if constexpr (MX) wide[i][0] = wide[i][1] = u32x4{0u, 0u, 0u, 0u};
+                    else vf[i] = u32x4{0u, 0u, 0u, 0u};
+                }
         }
-        store(vf);
+        if constexpr (MX) store_wide(wide);
+        else store(vf);
         if constexpr (!STAGED) next();
         load_v();
         asm volatile("" ::: "memory");                         // this wave's LDS: its reads follow its stores

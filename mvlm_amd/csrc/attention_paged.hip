@@ -47,14 +47,14 @@
 namespace mvlm {
 
 // NW: waves per block
-template <int R, int KS, bool BF, int PP, int NW>
+template <int R, int KS, int CT, int PP, int NW>
 __global__ __launch_bounds__(64 * NW, KS <= 2 && NW == 4 ? 3 : 2) void paged_attention_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int index = (int)(blockIdx.x / (uint32_t)a.kv.kv_heads), h = (int)blockIdx.x - index * a.kv.kv_heads;
     if constexpr (R == 32 && NW == 4)
         if (a.many.tile && *a.made) return;                    // by the kernel for many rows, which ran before
     const PagedShare share = paged_share<R, false>(a, paged_lane_span(a.batch, (int)(threadIdx.x & 63)), INT_MAX);
-    if (index < share.items) paged_few_item<R, KS, BF, PP, NW>(a, share, index, h, lds);
+    if (index < share.items) paged_few_item<R, KS, CT, PP, NW>(a, share, index, h, lds);
 }
 
 // Division of a share of the sequences (those of at most PAGED_FEW f-rows or all, or
@@ -84,7 +84,7 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     // table of 768 positions 13.5 us, of 32768 16.1; 2048 bf16 rows on 8192 303 us without the second launch, 306).
     const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int64_t tiles256 = (single ? (int64_t)b.seqs * (a->group / CHUNK_R) : f / CHUNK_R) * a->kv.kv_heads;
-    const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
+    const bool many = a->kv.dtype != MVLM_MXFP8 && tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
     a->many_least = (num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
     if (many) {
         // a sequence with more than PAGED_FEW f-rows ends in one tile that is not full
@@ -113,22 +113,22 @@ size_t paged_ws_bytes(const PagedAttnArgs& a, const PagedDivision& d) {
 }
 size_t paged_words(const PagedAttnArgs& a, const PagedDivision& d) { return (size_t)d.records * a.kv.kv_heads; }
 
-template <int R, int KS, bool BF, int PP, int NW>
+template <int R, int KS, int CT, int PP, int NW>
 static hipError_t launch_waves(hipStream_t s, const PagedAttnArgs& a) {
     constexpr int bytes = NW * PagedLayout<R, KS>::REGION + 16;
     if constexpr (bytes > 65536)
-        if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, BF, PP, NW>>(bytes); e != hipSuccess) return e;
+        if (const hipError_t e = allow_dynamic_lds<paged_attention_kernel<R, KS, CT, PP, NW>>(bytes); e != hipSuccess) return e;
     const dim3 grid((unsigned)(a.kv.kv_heads * a.few.items));
-    if (a.many.tile) launch_kernel_part(LaunchPart::Last, paged_attention_kernel<R, KS, BF, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
-    else launch_kernel(paged_attention_kernel<R, KS, BF, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
+    if (a.many.tile) launch_kernel_part(LaunchPart::Last, paged_attention_kernel<R, KS, CT, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
+    else launch_kernel(paged_attention_kernel<R, KS, CT, PP, NW>, grid, dim3(64 * NW), (uint32_t)bytes, s, a);
     return hipGetLastError();
 }
 
-template <int R, int KS, bool BF, int PP>
+template <int R, int KS, int CT, int PP>
 static hipError_t launch_few(hipStream_t s, const PagedAttnArgs& a) {
     if constexpr (R == 16)
-        if (a.few.unit_step == 8 * PAGED_KEYS) return launch_waves<R, KS, BF, PP, 8>(s, a);
-    return launch_waves<R, KS, BF, PP, 4>(s, a);
+        if (a.few.unit_step == 8 * PAGED_KEYS) return launch_waves<R, KS, CT, PP, 8>(s, a);
+    return launch_waves<R, KS, CT, PP, 4>(s, a);
 }
 
 template <int R, int KS>
@@ -137,8 +137,10 @@ static hipError_t launch_few_dims(hipStream_t s, const PagedAttnArgs& a) {
     // bf16 single tokens have two parts for a bf16 O as well, as their products cost next to nothing (4 of
     // 32768 85.4 us with one and with two, 64 of 500 .. 1500 18.5 and 18.8, one of 512 7.1 and 7.3; fp16, whose
     // one part is 8 times as fine and whose second is summed apart, 18.5 and 19.1, 7.2 and 7.5)
-    if (a.kv.dtype == MVLM_F16) return wide ? launch_few<R, KS, false, 2>(s, a) : launch_few<R, KS, false, 1>(s, a);
-    return wide ? launch_few<R, KS, true, 3>(s, a) : launch_few<R, KS, true, R == 16 ? 2 : 1>(s, a);
+    constexpr int ONE = R == 16 ? 2 : 1;
+    if (a.kv.dtype == MVLM_F16) return wide ? launch_few<R, KS, MVLM_F16, 2>(s, a) : launch_few<R, KS, MVLM_F16, 1>(s, a);
+    if (a.kv.dtype == MVLM_MXFP8) return wide ? launch_few<R, KS, MVLM_MXFP8, 3>(s, a) : launch_few<R, KS, MVLM_MXFP8, ONE>(s, a);
+    return wide ? launch_few<R, KS, MVLM_BF16, 3>(s, a) : launch_few<R, KS, MVLM_BF16, ONE>(s, a);
 }
 
 template <int R>

@@ -459,7 +459,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
             paged_chunk_item<KS, DT, BF, PP>(item_args<DT>(a), many, index, w - index * kv_heads, lds);
         } else if (i < all_items) {
             const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_few_item<32, DT, BF, PP, 8>(item_args<DT>(a), few, index, w - index * kv_heads, lds);
+            paged_few_item<32, DT, BF ? MVLM_BF16 : MVLM_F16, PP, 8>(item_args<DT>(a), few, index, w - index * kv_heads, lds);
         }
         __syncthreads();                                       // LDS is free
     }

@@ -145,12 +145,175 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
     }
 }
 
+// The same where a head's elements need each other: norms (a sum of squares over the head) and 8-bit caches (the
+// largest magnitude of 32 dims).
+//   x' = x w / sqrt(sum x^2 / D + eps), then the rotation; e = mx_exponent(max |x|), code = e4m3(x 2^-e)
+// Bytes bound it as well.  L = 1 .. 16 lanes make a head, 8 dims each, and sum over one another; a lane has the
+// same dims of every head that it makes, so the weights and the row's cos and sin are in its registers once.  Codes
+// leave in 8-byte stores (a head of 64 dims is half a line, its neighbours in the page come from the next rows), a
+// head's scales in one word.
+template <int XD, bool VEC>
+__global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const KvAppendArgs a) {
+    const int row = (int)blockIdx.x;
+    const PagedKv& kv = a.kv;
+    const int D = kv.D, half = a.rot / 2, qk = a.heads + kv.kv_heads, all = qk + kv.kv_heads;
+    const int shift = D > 64 ? 4 : D > 32 ? 3 : D > 16 ? 2 : D > 8 ? 1 : 0, lanes = 1 << shift;
+    const int sub = (int)threadIdx.x & (lanes - 1), d = 8 * sub, step = APPEND_THREADS >> shift;
+    const int own = (int)threadIdx.x >> shift;
+    const int dl = min(d, D - 8);                          // a lane past the head's end reads its last dims
+    const int64_t xrow = (int64_t)row * a.ld;
+    float ahead[APPEND_AHEAD][8];
+#pragma unroll
+    for (int u = 0; u < APPEND_AHEAD; ++u) append_load8<XD, VEC>(a.qkv, xrow + (int64_t)min(own + u * step, all - 1) * D + dl, ahead[u]);
+    float qw[8], kw[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        qw[e] = a.q_weight ? a.q_weight[dl + e] : 1.0f;
+        kw[e] = a.k_weight ? a.k_weight[dl + e] : 1.0f;
+    }
+    PagedSpan sp;
+    const int seq = paged_seq_of_row(a.batch, row, &sp);
+    if (seq < 0) return;                                   // behind the last sequence: left as it is
+    const int p = sp.position(row - sp.row0);
+    int slot0 = -1;                                        // slot of kv head 0; no place: as in kv_append_kernel
+    if (p >= 0 && p < a.batch.positions && (a.rot == 0 || p < a.rope_positions)) {
+        const int pi = kv.page.quotient(p);
+        const int page = a.batch.table[(int64_t)seq * a.batch.width + pi];
+        if (page >= 0 && page < kv.num_pages) slot0 = kv.slot(page, 0, p - pi * kv.page.div);
+    }
+    // cos and sin of this lane's dims: of pairs d / 2 .. (interleaved), or of each of them
+    float co[8], si[8];
+    const bool turns = d < a.rot && slot0 >= 0, by_chunk = half % 8 == 0;
+    const float* cs = a.rope + (int64_t)p * a.rot;         // [rot / 2][2]
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        co[e] = 1.0f, si[e] = 0.0f;
+        if (turns && d + e < a.rot) {
+            const int i = a.interleaved ? (d + e) / 2 : d + e < half ? d + e : d + e - half;
+            co[e] = cs[2 * i];
+            si[e] = cs[2 * i + 1];
+        }
+    }
+    auto make = [&](int head, const float (&x)[8]) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = d < D ? x[e] : 0.0f;
+        const bool is_q = head < a.heads, is_k = !is_q && head < qk;
+        const float* weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
+        float r = 1.0f;
+        if (a.q_weight || a.k_weight) {                    // all lanes of a wave sum
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
+            for (int off = 1; off < lanes; off <<= 1) ss += __shfl_xor(ss, off, 64);
+            if (weight) {
+                r = 1.0f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (is_q ? qw[e] : kw[e]);
+            }
+        }
+        if (a.rot) {
+            float w[8];                                    // the pairs' other elements
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = v[e ^ 1];
+            } else if (by_chunk) {                         // a chunk lies in one half, its partner chunk in the other
+                const int other = ((int)threadIdx.x & 63) + (d < half ? half / 8 : -(half / 8));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = __shfl(v[e], other & 63, 64);
+            } else if (turns && (is_q || is_k)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = min(d + e, a.rot - 1), j = i < half ? i + half : i - half;
+                    w[e] = load_as_f32(a.qkv, xrow + (int64_t)head * D + j, XD);
+                    if (weight) w[e] = w[e] * r * weight[j];
+                }
+            }
+            if (turns && (is_q || is_k)) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool first = a.interleaved ? (e & 1) == 0 : d + e < half;
+                    o[e] = d + e < a.rot ? v[e] * co[e] + (first ? -w[e] : w[e]) * si[e] : v[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = o[e];
+            }
+        }
+        const bool mx = kv.dtype == MVLM_MXFP8;
+        if (mx && !is_q) {
+            uint32_t most = 0;
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t m = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+                most = m < 0x7F800000u ? max(most, m) : most;
+                odd |= m >= 0x7F800000u;
+            }
+            for (int off = 1; off < min(lanes, MX_BLOCK / 8); off <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
+            const int ex = mx_exponent(most);
+            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), limit = ex == MX_MOST ? 240.0f : 448.0f;
+            uint32_t code[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = fminf(fmaxf(v[4 * j + e] * down, -limit), limit);
+                int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+                code[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+            }
+            if (odd) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((__float_as_uint(v[e]) & 0x7FFFFFFFu) >= 0x7F800000u) code[e >> 2] |= 0x7Fu << (8 * (e & 3));
+            }
+            uint32_t word = (uint32_t)(ex + MX_BIAS) << (d / MX_BLOCK * 8);
+            for (int off = MX_BLOCK / 8; off < lanes; off <<= 1) word |= (uint32_t)__shfl_xor((int)word, off, 64);
+            if (slot0 < 0) return;
+            const int64_t slot = slot0 + (int64_t)(head - (is_k ? a.heads : qk)) * kv.page.div;
+            if (d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + slot * D + d) = u32x2{code[0], code[1]};
+            if (sub == 0) (is_k ? kv.k_scale : kv.v_scale)[slot] = word;
+            return;
+        }
+        u32x4 out;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x2 pair = {v[2 * j], v[2 * j + 1]};
+            out[j] = kv.dtype == MVLM_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2_t))
+                                          : __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_t));
+        }
+        if (d >= D) return;
+        if (is_q) {
+            if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.heads + head) * D + d) = out;
+        } else if (slot0 >= 0) {
+            const int64_t slot = slot0 + (int64_t)(head - (is_k ? a.heads : qk)) * kv.page.div;
+            *reinterpret_cast<u32x4*>((is_k ? kv.k : kv.v) + slot * D + d) = out;
+        }
+    };
+    // A wave's lanes go round together, so that each finds the others of its head; one past the last head ends there.
+#pragma unroll
+    for (int u = 0; u < APPEND_AHEAD; ++u)
+        if (own + u * step < all) make(own + u * step, ahead[u]);
+    for (int head = own + APPEND_AHEAD * step; head < all; head += step) {
+        float x[8];
+        append_load8<XD, VEC>(a.qkv, xrow + (int64_t)head * D + dl, x);
+        make(head, x);
+    }
+}
+
 hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a) {
     const size_t es = dtype_size(a.x_dtype);
     const bool vec = ((uintptr_t)a.qkv & 15u) == 0 && (a.ld * (int64_t)es) % 16 == 0;
     const dim3 grid((unsigned)a.batch.rows), block(APPEND_THREADS);
+    const bool by_head = a.kv.dtype == MVLM_MXFP8 || a.q_weight || a.k_weight;
     auto go = [&](auto dt) {
         constexpr int XD = decltype(dt)::value;
+        if (by_head) {
+            if (vec) launch_kernel(kv_append_heads_kernel<XD, true>, grid, block, 0, s, a);
+            else launch_kernel(kv_append_heads_kernel<XD, false>, grid, block, 0, s, a);
+            return;
+        }
         if (vec) launch_kernel(kv_append_kernel<XD, true>, grid, block, 0, s, a);
         else launch_kernel(kv_append_kernel<XD, false>, grid, block, 0, s, a);
     };

@@ -9,6 +9,7 @@
 #include "common.h"
 #include "logits.h"
 #include "paged_ops.h"
+#include "sample.h"
 
 #include <climits>
 #include <cmath>
@@ -21,7 +22,7 @@ using namespace mvlm;
 namespace {
 
 enum OpKind { OP_GEMM_ORDER, OP_GEMV_EXACT, OP_GEMM_MFMA, OP_GEMV_DENSE, OP_GEMV_QUANT, OP_GEMV_GROUP, OP_ATTENTION,
-              OP_ATTN_STEP, OP_ARGMAX, OP_KV_APPEND, OP_ATTN_PAGED, OP_LOGITS };
+              OP_ATTN_STEP, OP_ARGMAX, OP_KV_APPEND, OP_KV_READ, OP_ATTN_PAGED, OP_LOGITS, OP_SAMPLE };
 
 struct Op {
     OpKind kind;
@@ -52,6 +53,8 @@ struct Op {
     KvAppendArgs append{};
     PagedAttnArgs paged{};
     LogitsArgs logits{};
+    KvReadArgs read{};
+    SampleArgs sample{};
     // plan fusion: a grouped GEMV whose launch can also compute a decode
     // attention entry next to it; 1: the entry before it (some entries read
     // its output as x), 2: the entry after it (a decode step whose q, k, v
@@ -306,10 +309,11 @@ int need_ints(mvlm_device* dev, const mvlm_buffer* b, size_t count, const char* 
     return need(b, count * 4, fn, name);
 }
 
-int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, PagedKv* out) {
-    REQUIRE(in && in->k && in->v, "%s: null cache", fn);
-    REQUIRE(in->k->dev == dev && in->v->dev == dev, "%s: the cache belongs to another device", fn);
-    REQUIRE(in->dtype == MVLM_F16 || in->dtype == MVLM_BF16, "%s: cache dtype %d is not F16/BF16", fn, in->dtype);
+// The sizes of a cache, and the bytes that K needs and V as much.
+int check_paged_kv(const mvlm_paged_kv* in, const char* fn, size_t* bytes) {
+    REQUIRE(in, "%s: null cache", fn);
+    REQUIRE(in->dtype == MVLM_F16 || in->dtype == MVLM_BF16 || in->dtype == MVLM_MXFP8,
+            "%s: cache dtype %d is not F16/BF16/MXFP8", fn, in->dtype);
     REQUIRE(in->num_pages > 0 && in->page_size > 0 && in->kv_heads > 0 && in->head_dim > 0,
             "%s: num_pages=%d page_size=%d kv_heads=%d head_dim=%d must be positive", fn, in->num_pages, in->page_size,
             in->kv_heads, in->head_dim);
@@ -322,14 +326,29 @@ int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, Pag
         return set_error(MVLM_ERR_UNSUPPORTED, "%s: %d pages of %d positions of %d heads are 2^31 slots or more", fn,
                          in->num_pages, in->page_size, in->kv_heads);
     if (per_head * in->kv_heads * (in->head_dim / 8) >= ((int64_t)1 << 32) - 16)
-        return set_error(MVLM_ERR_UNSUPPORTED, "%s: K and V of 64 GiB or more", fn);
-    const size_t bytes = (size_t)per_head * in->kv_heads * in->head_dim * 2;
+        return set_error(MVLM_ERR_UNSUPPORTED, "%s: K and V of 2^35 elements or more", fn);
+    const size_t slots = (size_t)per_head * in->kv_heads;
+    *bytes = in->dtype == MVLM_MXFP8 ? (size_t)round_up((int64_t)slots * in->head_dim, 16) + 4 * slots : slots * in->head_dim * 2;
+    return MVLM_OK;
+}
+
+int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, PagedKv* out) {
+    REQUIRE(in && in->k && in->v, "%s: null cache", fn);
+    REQUIRE(in->k->dev == dev && in->v->dev == dev, "%s: the cache belongs to another device", fn);
+    size_t bytes = 0;
+    const int st = check_paged_kv(in, fn, &bytes);
+    if (st != MVLM_OK) return st;
     REQUIRE(aligned16(in->k->ptr) && aligned16(in->v->ptr), "%s: K and V must be 16-byte aligned", fn);
     NEED(in->k, bytes, "K");
     NEED(in->v, bytes, "V");
     REQUIRE(!overlaps(in->k->ptr, bytes, in->v->ptr, bytes), "%s: K and V overlap", fn);
+    const size_t slots = (size_t)in->num_pages * in->page_size * in->kv_heads;
+    const bool mx = in->dtype == MVLM_MXFP8;
     out->k = (uint16_t*)in->k->ptr;
     out->v = (uint16_t*)in->v->ptr;
+    out->k_scale = mx ? (uint32_t*)((char*)in->k->ptr + (bytes - 4 * slots)) : nullptr;
+    out->v_scale = mx ? (uint32_t*)((char*)in->v->ptr + (bytes - 4 * slots)) : nullptr;
+    out->bytes = bytes;
     out->dtype = in->dtype;
     out->num_pages = in->num_pages;
     out->kv_heads = in->kv_heads;
@@ -337,7 +356,6 @@ int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, Pag
     out->page = fast_div(in->page_size);
     return MVLM_OK;
 }
-size_t kv_bytes(const PagedKv& kv) { return (size_t)kv.num_pages * kv.page.div * kv.kv_heads * kv.D * 2; }
 
 int make_paged_batch(mvlm_device* dev, const mvlm_paged_batch* in, int page_size, const char* fn, PagedSeqs* out) {
     REQUIRE(in && in->kv_len && in->page_table, "%s: null batch", fn);
@@ -376,8 +394,8 @@ int check_heads(int num_heads, const PagedKv& kv, const char* fn) {
 }
 
 int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld, const mvlm_paged_batch* batch,
-                   const mvlm_paged_kv* cache, int num_heads, mvlm_buffer* q_out, const mvlm_rope* rope, const char* fn,
-                   Op* op) {
+                   const mvlm_paged_kv* cache, int num_heads, mvlm_buffer* q_out, const mvlm_rope* rope,
+                   const mvlm_head_norm* norm, const char* fn, Op* op) {
     REQUIRE(dev && qkv && q_out, "%s: null argument", fn);
     REQUIRE(qkv->dev == dev && q_out->dev == dev, "%s: buffers belong to another device", fn);
     REQUIRE(is_dense(x_dtype), "%s: qkv dtype %d is not F32/F16/BF16", fn, x_dtype);
@@ -409,10 +427,22 @@ int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_
         a.rot = rope->rot_dim;
         a.interleaved = rope->interleaved != 0;
     }
-    const size_t kvb = kv_bytes(a.kv);
+    size_t q_norm = 0, k_norm = 0;
+    if (norm) {
+        REQUIRE(norm->q_weight || norm->k_weight, "%s: a norm of neither q nor k", fn);
+        REQUIRE(norm->eps >= 0.0f && norm->eps < INFINITY, "%s: eps %g must be finite and not negative", fn, (double)norm->eps);
+        if (norm->q_weight) st = need_ints(dev, norm->q_weight, q_norm = (size_t)a.kv.D, fn, "q_weight");
+        if (st == MVLM_OK && norm->k_weight) st = need_ints(dev, norm->k_weight, k_norm = (size_t)a.kv.D, fn, "k_weight");
+        if (st != MVLM_OK) return st;
+        a.q_weight = q_norm ? (const float*)norm->q_weight->ptr : nullptr;
+        a.k_weight = k_norm ? (const float*)norm->k_weight->ptr : nullptr;
+        a.eps = norm->eps;
+    }
+    const size_t kvb = a.kv.bytes;
     const struct { const void* p; size_t bytes; } written[3] = {{a.kv.k, kvb}, {a.kv.v, kvb}, {q_out->ptr, q_bytes}};
     for (const auto& w : written)
         REQUIRE(!overlaps(w.p, w.bytes, qkv->ptr, x_bytes) && !overlaps(w.p, w.bytes, a.rope, rope_bytes) &&
+                    !overlaps(w.p, w.bytes, a.q_weight, 4 * q_norm) && !overlaps(w.p, w.bytes, a.k_weight, 4 * k_norm) &&
                     !holds_batch(w.p, w.bytes, a.batch),
                 "%s: the cache and q_out must not overlap what is read", fn);
     REQUIRE(!overlaps(q_out->ptr, q_bytes, a.kv.k, kvb) && !overlaps(q_out->ptr, q_bytes, a.kv.v, kvb),
@@ -427,6 +457,41 @@ int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_
     return MVLM_OK;
 }
 
+int make_kv_read(mvlm_device* dev, const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, mvlm_buffer* K_out,
+                 mvlm_buffer* V_out, int out_dtype, int64_t ld, const char* fn, Op* op) {
+    REQUIRE(dev && (K_out || V_out), "%s: null argument", fn);
+    REQUIRE((!K_out || K_out->dev == dev) && (!V_out || V_out->dev == dev), "%s: buffers belong to another device", fn);
+    REQUIRE(is_dense(out_dtype), "%s: output dtype %d is not F32/F16/BF16", fn, out_dtype);
+    KvReadArgs& a = op->read;
+    int st = make_paged_kv(dev, cache, fn, &a.kv);
+    if (st == MVLM_OK) st = make_paged_batch(dev, batch, a.kv.page.div, fn, &a.batch);
+    if (st != MVLM_OK) return st;
+    const int64_t width = (int64_t)a.kv.kv_heads * a.kv.D;
+    REQUIRE(ld >= width && ld <= ((int64_t)1 << 40), "%s: ld=%lld of rows of %lld elements", fn, (long long)ld, (long long)width);
+    const size_t es = dtype_size(out_dtype), bytes = ((size_t)(a.batch.rows - 1) * (size_t)ld + (size_t)width) * es;
+    for (const mvlm_buffer* out : {K_out, V_out}) {
+        if (!out) continue;
+        NEED(out, bytes, out == K_out ? "K_out" : "V_out");
+        REQUIRE((uintptr_t)out->ptr % es == 0, "%s: an output does not start at a multiple of %zu bytes", fn, es);
+        REQUIRE(!overlaps(out->ptr, bytes, a.kv.k, a.kv.bytes) && !overlaps(out->ptr, bytes, a.kv.v, a.kv.bytes) &&
+                    !holds_batch(out->ptr, bytes, a.batch),
+                "%s: outputs must not overlap what is read", fn);
+    }
+    // rows of the one may lie between the rows of the other
+    if (K_out && V_out) {
+        const char *k = (const char*)K_out->ptr, *v = (const char*)V_out->ptr;
+        const size_t apart = (size_t)(k < v ? v - k : k - v), step = (size_t)ld * es, row = (size_t)width * es;
+        REQUIRE(apart >= bytes || (apart % step >= row && step - apart % step >= row), "%s: K_out and V_out overlap", fn);
+    }
+    a.chunk = fast_div(a.kv.D / 8);
+    a.k_out = K_out ? K_out->ptr : nullptr;
+    a.v_out = V_out ? V_out->ptr : nullptr;
+    a.dtype = out_dtype;
+    a.ld = ld;
+    op->kind = OP_KV_READ;
+    return MVLM_OK;
+}
+
 int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
                          const mvlm_paged_kv* cache, mvlm_buffer* O, int o_dtype, int num_heads, float scale,
                          const char* fn, Op* op) {
@@ -437,7 +502,8 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     if (st == MVLM_OK) st = make_paged_batch(dev, batch, a.kv.page.div, fn, &a.batch);
     if (st == MVLM_OK) st = check_heads(num_heads, a.kv, fn);
     if (st != MVLM_OK) return st;
-    REQUIRE(o_dtype == MVLM_F32 || o_dtype == a.kv.dtype, "%s: output dtype %d is neither F32 nor the cache's", fn, o_dtype);
+    REQUIRE(o_dtype == MVLM_F32 || o_dtype == (a.kv.dtype == MVLM_MXFP8 ? (int)MVLM_BF16 : a.kv.dtype),
+            "%s: output dtype %d is neither F32 nor the cache's", fn, o_dtype);
     REQUIRE(scale >= 0.0f && scale < INFINITY, "%s: scale %g must be finite and non-negative", fn, (double)scale);
     REQUIRE((int64_t)a.batch.rows * num_heads <= (1 << 28), "%s: shape too large", fn);
     REQUIRE(aligned16(Q->ptr) && aligned16(O->ptr), "%s: Q and O must be 16-byte aligned", fn);
@@ -445,8 +511,8 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     const size_t o_bytes = elems * dtype_size(o_dtype);
     NEED(Q, elems * 2, "Q");
     NEED(O, o_bytes, "O");
-    REQUIRE(!overlaps(O->ptr, o_bytes, Q->ptr, elems * 2) && !overlaps(O->ptr, o_bytes, a.kv.k, kv_bytes(a.kv)) &&
-                !overlaps(O->ptr, o_bytes, a.kv.v, kv_bytes(a.kv)) && !holds_batch(O->ptr, o_bytes, a.batch),
+    REQUIRE(!overlaps(O->ptr, o_bytes, Q->ptr, elems * 2) && !overlaps(O->ptr, o_bytes, a.kv.k, a.kv.bytes) &&
+                !overlaps(O->ptr, o_bytes, a.kv.v, a.kv.bytes) && !holds_batch(O->ptr, o_bytes, a.batch),
             "%s: O must not overlap what is read", fn);
     a.q = (const uint16_t*)Q->ptr;
     a.o = O->ptr;
@@ -531,6 +597,45 @@ int make_logits(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     a.ld = ld;
     op->num_cus = dev->prop.multiProcessorCount;
     op->kind = OP_LOGITS;
+    return MVLM_OK;
+}
+
+int make_sample(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld, const mvlm_sampling* c,
+                mvlm_buffer* out, const char* fn, Op* op) {
+    REQUIRE(dev && x && c && c->uniform && out, "%s: null argument", fn);
+    REQUIRE(x->dev == dev, "%s: buffers belong to another device", fn);
+    REQUIRE(is_dense(dtype), "%s: dtype %d is not F32/F16/BF16", fn, dtype);
+    REQUIRE(rows > 0 && n > 0 && ld >= n && ld <= ((int64_t)1 << 40), "%s: rows=%d n=%d ld=%lld", fn, rows, n, (long long)ld);
+    REQUIRE(rows <= (1 << 20) && n <= SAMPLE_MAX_TOKENS, "%s: shape too large", fn);
+    const size_t es = dtype_size(dtype), bytes = ((size_t)(rows - 1) * (size_t)ld + (size_t)n) * es, R = (size_t)rows;
+    NEED(x, bytes, "x");
+    REQUIRE((uintptr_t)x->ptr % es == 0, "%s: x does not start at a multiple of %zu bytes", fn, es);
+    SampleArgs& a = op->sample;
+    int st = need_ints(dev, out, R, fn, "out_index");
+    if (st != MVLM_OK) return st;
+    REQUIRE(!overlaps(out->ptr, 4 * R, x->ptr, bytes), "%s: out_index overlaps x", fn);
+    const struct { const mvlm_buffer* b; const char* name; const void** to; } settings[] = {
+        {c->uniform, "uniform", (const void**)&a.uniform}, {c->temperature, "temperature", (const void**)&a.temperature},
+        {c->top_k, "top_k", (const void**)&a.top_k}, {c->top_p, "top_p", (const void**)&a.top_p},
+        {c->min_p, "min_p", (const void**)&a.min_p}};
+    for (const auto& g : settings) {
+        if (!g.b) continue;
+        st = need_ints(dev, g.b, R, fn, g.name);
+        if (st != MVLM_OK) return st;
+        REQUIRE(!overlaps(out->ptr, 4 * R, g.b->ptr, 4 * R), "%s: out_index overlaps %s", fn, g.name);
+        *g.to = g.b->ptr;
+    }
+    a.x = x->ptr;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.n = n;
+    a.ld = ld;
+    a.out = (int*)out->ptr;
+    a.bits = 62;
+    while (((int64_t)1 << (62 - a.bits)) < n) --a.bits;
+    if (a.bits > 51) a.bits = 51;
+    op->num_cus = dev->prop.multiProcessorCount;
+    op->kind = OP_SAMPLE;
     return MVLM_OK;
 }
 
@@ -707,6 +812,10 @@ hipError_t enqueue_op(hipStream_t s, const Op& op, bool with_attn = false) {
             return launch_attn_decode(s, attn_step_desc(op), op.num_cus);
         case OP_KV_APPEND:
             return launch_kv_append(s, op.append);
+        case OP_KV_READ:
+            return launch_kv_read(s, op.read);
+        case OP_SAMPLE:
+            return launch_sample(s, op.sample, op.num_cus);
         case OP_ATTN_PAGED:
             return launch_attention_paged(s, op.paged, op.num_cus);
         case OP_LOGITS:
@@ -904,7 +1013,27 @@ extern "C" int mvlm_kv_append_paged(mvlm_device* dev, const mvlm_buffer* qkv, in
                                     const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
                                     mvlm_buffer* q_out, const mvlm_rope* rope, mvlm_event** ev) {
     const char* fn = __func__;
-    RUN(make_kv_append(dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, fn, &op));
+    RUN(make_kv_append(dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, nullptr, fn, &op));
+}
+
+extern "C" int mvlm_kv_append_paged_ex(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                       const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                       mvlm_buffer* q_out, const mvlm_rope* rope, const mvlm_head_norm* norm,
+                                       mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_kv_append(dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, norm, fn, &op));
+}
+
+extern "C" int mvlm_paged_kv_bytes(const mvlm_paged_kv* cache, size_t* bytes) {
+    const char* fn = __func__;
+    REQUIRE(bytes, "%s: null argument", fn);
+    return check_paged_kv(cache, fn, bytes);
+}
+
+extern "C" int mvlm_kv_read_paged(mvlm_device* dev, const mvlm_paged_batch* batch, const mvlm_paged_kv* cache,
+                                  mvlm_buffer* K_out, mvlm_buffer* V_out, int out_dtype, int64_t ld, mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_kv_read(dev, batch, cache, K_out, V_out, out_dtype, ld, fn, &op));
 }
 
 extern "C" int mvlm_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_paged_batch* batch,
@@ -918,6 +1047,12 @@ extern "C" int mvlm_logits_process(mvlm_device* dev, const mvlm_buffer* x, int d
                                    const mvlm_logit_controls* controls, mvlm_buffer* out, mvlm_event** ev) {
     const char* fn = __func__;
     RUN(make_logits(dev, x, dtype, rows, n, ld, controls, out, fn, &op));
+}
+
+extern "C" int mvlm_sample(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                           const mvlm_sampling* sampling, mvlm_buffer* out_index, mvlm_event** ev) {
+    const char* fn = __func__;
+    RUN(make_sample(dev, x, dtype, rows, n, ld, sampling, out_index, fn, &op));
 }
 
 // ---------------------------------------------------------------------------
@@ -1217,7 +1352,35 @@ extern "C" int mvlm_plan_add_kv_append_paged(mvlm_plan* plan, const mvlm_buffer*
     const char* fn = __func__;
     REQUIRE(plan, "%s: null argument", fn);
     Op op{};
-    const int st = make_kv_append(plan->dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, fn, &op);
+    const int st = make_kv_append(plan->dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, nullptr, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_kv_append_paged_ex(mvlm_plan* plan, const mvlm_buffer* qkv, int x_dtype, int64_t ld,
+                                                const mvlm_paged_batch* batch, const mvlm_paged_kv* cache, int num_heads,
+                                                mvlm_buffer* q_out, const mvlm_rope* rope, const mvlm_head_norm* norm) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_kv_append(plan->dev, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope, norm, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_kv_read_paged(mvlm_plan* plan, const mvlm_paged_batch* batch, const mvlm_paged_kv* cache,
+                                           mvlm_buffer* K_out, mvlm_buffer* V_out, int out_dtype, int64_t ld) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_kv_read(plan->dev, batch, cache, K_out, V_out, out_dtype, ld, fn, &op);
+    return st != MVLM_OK ? st : plan_push(plan, op);
+}
+
+extern "C" int mvlm_plan_add_sample(mvlm_plan* plan, const mvlm_buffer* x, int dtype, int rows, int n, int64_t ld,
+                                    const mvlm_sampling* sampling, mvlm_buffer* out_index) {
+    const char* fn = __func__;
+    REQUIRE(plan, "%s: null argument", fn);
+    Op op{};
+    const int st = make_sample(plan->dev, x, dtype, rows, n, ld, sampling, out_index, fn, &op);
     return st != MVLM_OK ? st : plan_push(plan, op);
 }
 

@@ -9,6 +9,7 @@
 // Everything read from device memory is clamped before it is used as an index.
 #pragma once
 
+#include <cstddef>
 #include <cstdint>
 
 #if defined(__HIPCC__)
@@ -37,8 +38,11 @@ inline FastDiv fast_div(int d) {
 }
 
 struct PagedKv {
-    uint16_t* k;
+    uint16_t* k;               // elements of 16 bits, or codes of 8 (MVLM_MXFP8)
     uint16_t* v;
+    uint32_t* k_scale;         // MVLM_MXFP8: a word per slot, else null
+    uint32_t* v_scale;
+    size_t bytes;              // of K, and of V
     int dtype;
     int num_pages, kv_heads, D;
     FastDiv page;              // by page_size
@@ -48,6 +52,15 @@ struct PagedKv {
         return (page_id * kv_heads + head) * page.div + offset;
     }
 };
+
+// An 8-bit cache (MVLM_MXFP8): blocks of 32 dims of a head share a power of two, 2^e, kept as e + 127.
+constexpr int MX_BLOCK = 32, MX_BIAS = 127;
+constexpr int MX_LEAST = -100, MX_MOST = 120;      // of e
+// e of a block whose largest finite magnitude has these bits: the least with a <= 448 2^e = 1.75 2^(e + 8)
+MVLM_HD int mx_exponent(uint32_t magnitude) {
+    const int e = (int)(magnitude >> 23) - 127 - 8 + ((magnitude & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < MX_LEAST ? MX_LEAST : e;
+}
 
 struct PagedSeqs {
     int seqs, rows;

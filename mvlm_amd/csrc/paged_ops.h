@@ -17,7 +17,20 @@ struct KvAppendArgs {
     FastDiv chunk;                 // by head_dim / 8
     const float* rope;             // [rope_positions][rot / 2][2] cos, sin
     int rope_positions, rot, interleaved;
-    uint16_t* q_out;               // [rows][heads][D], the cache's type
+    uint16_t* q_out;               // [rows][heads][D], the cache's type (bf16 for an 8-bit cache)
+    const float* q_weight;         // [D] norms of q and k heads; null: none
+    const float* k_weight;
+    float eps;
+};
+
+struct KvReadArgs {
+    PagedSeqs batch;
+    PagedKv kv;
+    FastDiv chunk;                 // by head_dim / 8
+    void* k_out;                   // [rows][kv_heads][D], rows ld elements apart; null: not wanted
+    void* v_out;
+    int dtype;
+    int64_t ld;
 };
 
 // How one kernel's share of a batch is cut into blocks.
@@ -40,7 +53,7 @@ constexpr int PAGED_MAX_KV_HEADS = 1024;
 struct PagedAttnArgs {
     PagedSeqs batch;
     PagedKv kv;
-    const uint16_t* q;             // [rows][heads][D], the cache's type
+    const uint16_t* q;             // [rows][heads][D], the cache's type (bf16 for an 8-bit cache)
     void* o;                       // [rows][heads][D]
     int o_dtype, heads, group;     // group: heads per kv head
     float scale_log2;              // scale * log2(e)
@@ -53,6 +66,7 @@ struct PagedAttnArgs {
 };
 
 hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a);
+hipError_t launch_kv_read(hipStream_t s, const KvReadArgs& a);
 // Fills a's division of the work for a device, all but its memory.
 void plan_attention_paged(PagedAttnArgs* a, int num_cus);
 // Bytes of partial results and words of counters of a share; placing them.

@@ -16,9 +16,10 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MVLM_LIB_PATH") or os.path.join(PKG, "lib", "libmvlm_hip.so")
 
 F32, F16, Q4_0, Q8_0, BF16 = 0, 1, 2, 8, 30
+MXFP8 = 100                     # paged caches only
 LAYOUT_NK, LAYOUT_KN = 0, 1
 DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2}
-DTYPE_NAMES = {F32: "f32", F16: "f16", BF16: "bf16", Q8_0: "q8_0", Q4_0: "q4_0"}
+DTYPE_NAMES = {F32: "f32", F16: "f16", BF16: "bf16", Q8_0: "q8_0", Q4_0: "q4_0", MXFP8: "mxfp8"}
 
 OK = 0
 ERR_INVALID_ARG, ERR_NO_DEVICE, ERR_OUT_OF_MEMORY, ERR_HIP, ERR_UNSUPPORTED, ERR_BUFFER_TOO_SMALL = -1, -2, -3, -4, -5, -6
@@ -80,6 +81,15 @@ class _Rope(ctypes.Structure):
     _fields_ = [("table", c_void_p), ("positions", c_int), ("rot_dim", c_int), ("interleaved", c_int)]
 
 
+class _HeadNorm(ctypes.Structure):
+    _fields_ = [("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float)]
+
+
+class _Sampling(ctypes.Structure):
+    _fields_ = [("uniform", c_void_p), ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p),
+                ("min_p", c_void_p)]
+
+
 class _LogitControls(ctypes.Structure):
     _fields_ = [("history", c_void_p), ("history_len", c_void_p), ("generated_from", c_void_p),
                 ("history_width", c_int), ("penalties", c_void_p), ("bias_ids", c_void_p), ("bias_values", c_void_p),
@@ -91,7 +101,8 @@ def _handle(buf):
 
 
 class PagedKV:
-    """A paged key/value cache: k and v hold num_pages pages of [kv_heads][page_size][head_dim]."""
+    """A paged key/value cache: k and v hold num_pages pages of [kv_heads][page_size][head_dim] (MXFP8: of codes,
+    then their scales; paged_kv_bytes says how large they are)."""
 
     def __init__(self, k, v, dtype, num_pages, page_size, kv_heads, head_dim):
         self.buffers = [k, v]
@@ -113,6 +124,23 @@ class Rope:
     def __init__(self, table, positions, rot_dim, interleaved=False):
         self.buffers = [table]
         self.struct = _Rope(_handle(table), positions, rot_dim, 1 if interleaved else 0)
+
+
+class HeadNorm:
+    """Norms of q and k heads before the rotation: fp32 weights [head_dim], either may be None."""
+
+    def __init__(self, q_weight, k_weight, eps):
+        self.buffers = [b for b in (q_weight, k_weight) if b is not None]
+        self.struct = _HeadNorm(_handle(q_weight), _handle(k_weight), eps)
+
+
+class Sampling:
+    """How tokens are drawn: fp32 uniform numbers [rows] and, where not None, temperature, top_k (int32), top_p and
+    min_p of each row."""
+
+    def __init__(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        self.buffers = [b for b in (uniform, temperature, top_k, top_p, min_p) if b is not None]
+        self.struct = _Sampling(_handle(uniform), _handle(temperature), _handle(top_k), _handle(top_p), _handle(min_p))
 
 
 class LogitControls:
@@ -192,6 +220,15 @@ _SIGNATURES = {
     "mvlm_plan_add_argmax": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, _P]),
     "mvlm_kv_append_paged": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV), c_int, _P,
                                      POINTER(_Rope), _PP]),
+    "mvlm_paged_kv_bytes": (c_int, [POINTER(_PagedKV), POINTER(c_size_t)]),
+    "mvlm_kv_append_paged_ex": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV), c_int, _P,
+                                        POINTER(_Rope), POINTER(_HeadNorm), _PP]),
+    "mvlm_kv_read_paged": (c_int, [_P, POINTER(_PagedBatch), POINTER(_PagedKV), _P, _P, c_int, c_int64, _PP]),
+    "mvlm_sample": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, POINTER(_Sampling), _P, _PP]),
+    "mvlm_plan_add_kv_append_paged_ex": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV),
+                                                 c_int, _P, POINTER(_Rope), POINTER(_HeadNorm)]),
+    "mvlm_plan_add_kv_read_paged": (c_int, [_P, POINTER(_PagedBatch), POINTER(_PagedKV), _P, _P, c_int, c_int64]),
+    "mvlm_plan_add_sample": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, POINTER(_Sampling), _P]),
     "mvlm_attention_paged": (c_int, [_P, _P, POINTER(_PagedBatch), POINTER(_PagedKV), _P, c_int, c_int, c_float, _PP]),
     "mvlm_logits_process": (c_int, [_P, _P, c_int, c_int, c_int, c_int64, POINTER(_LogitControls), _P, _PP]),
     "mvlm_plan_add_kv_append_paged": (c_int, [_P, _P, c_int, c_int64, POINTER(_PagedBatch), POINTER(_PagedKV), c_int,
@@ -265,6 +302,13 @@ def check(status: int, fn: str) -> None:
 
 def _call(name, *args):
     check(getattr(lib(), name)(*args), name)
+
+
+def paged_kv_bytes(dtype, num_pages, page_size, kv_heads, head_dim) -> int:
+    """Bytes that the K buffer of a paged cache needs, and its V buffer as much."""
+    n = c_size_t()
+    _call("mvlm_paged_kv_bytes", byref(_PagedKV(None, None, dtype, num_pages, page_size, kv_heads, head_dim)), byref(n))
+    return n.value
 
 
 def device_count() -> int:
@@ -575,6 +619,20 @@ class Plan:
         self._keep += [qkv, q_out, *batch.buffers, *cache.buffers, *(rope.buffers if rope else [])]
         return self
 
+    def add_kv_append_paged_ex(self, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope=None, norm=None):
+        _call("mvlm_plan_add_kv_append_paged_ex", self.handle, qkv.handle, x_dtype, ld, byref(batch.struct),
+              byref(cache.struct), num_heads, q_out.handle, byref(rope.struct) if rope else None,
+              byref(norm.struct) if norm else None)
+        self._keep += [qkv, q_out, *batch.buffers, *cache.buffers, *(rope.buffers if rope else []),
+                       *(norm.buffers if norm else [])]
+        return self
+
+    def add_kv_read_paged(self, batch, cache, K_out, V_out, out_dtype, ld):
+        _call("mvlm_plan_add_kv_read_paged", self.handle, byref(batch.struct), byref(cache.struct), _handle(K_out),
+              _handle(V_out), out_dtype, ld)
+        self._keep += [*batch.buffers, *cache.buffers, *[b for b in (K_out, V_out) if b is not None]]
+        return self
+
     def add_attention_paged(self, Q, batch, cache, O, o_dtype, num_heads, scale=0.0):
         _call("mvlm_plan_add_attention_paged", self.handle, Q.handle, byref(batch.struct), byref(cache.struct),
               O.handle, o_dtype, num_heads, scale)
@@ -585,6 +643,12 @@ class Plan:
         _call("mvlm_plan_add_logits_process", self.handle, x.handle, dtype, rows, n, ld, byref(controls.struct),
               out.handle)
         self._keep += [x, out, *controls.buffers]
+        return self
+
+    def add_sample(self, x, dtype, rows, n, ld, sampling, out_index):
+        _call("mvlm_plan_add_sample", self.handle, x.handle, dtype, rows, n, ld, byref(sampling.struct),
+              out_index.handle)
+        self._keep += [x, out_index, *sampling.buffers]
         return self
 
     def use_graph(self, enable=True):
@@ -807,6 +871,18 @@ class Device:
                                                      byref(cache.struct), num_heads, q_out.handle,
                                                      byref(rope.struct) if rope else None), event)
 
+    def kv_append_paged_ex(self, qkv, x_dtype, ld, batch, cache, num_heads, q_out, rope=None, norm=None, event=False):
+        """kv_append_paged with norms of the q and k heads before the rotation, in the same pass."""
+        return self._launch("mvlm_kv_append_paged_ex", (qkv.handle, x_dtype, ld, byref(batch.struct),
+                                                        byref(cache.struct), num_heads, q_out.handle,
+                                                        byref(rope.struct) if rope else None,
+                                                        byref(norm.struct) if norm else None), event)
+
+    def kv_read_paged(self, batch, cache, K_out, V_out, out_dtype, ld, event=False):
+        """Keys and values of the rows' positions out of the paged cache, rows ld elements apart; either may be None."""
+        return self._launch("mvlm_kv_read_paged", (byref(batch.struct), byref(cache.struct), _handle(K_out),
+                                                   _handle(V_out), out_dtype, ld), event)
+
     def attention_paged(self, Q, batch, cache, O, o_dtype, num_heads, scale=0.0, event=False):
         """Attention of each sequence's new rows over its pages, up to their own positions."""
         return self._launch("mvlm_attention_paged", (Q.handle, byref(batch.struct), byref(cache.struct), O.handle,
@@ -815,6 +891,11 @@ class Device:
     def logits_process(self, x, dtype, rows, n, ld, controls, out, event=False):
         """Penalties, biases and masks on rows of logits; out may be x."""
         return self._launch("mvlm_logits_process", (x.handle, dtype, rows, n, ld, byref(controls.struct), out.handle),
+                            event)
+
+    def sample(self, x, dtype, rows, n, ld, sampling, out_index, event=False):
+        """out_index[r] (int32 on the device) = the token drawn from row r of the logits."""
+        return self._launch("mvlm_sample", (x.handle, dtype, rows, n, ld, byref(sampling.struct), out_index.handle),
                             event)
 
     def gemm_quant(self, X, W, Y, M, N, K, event=False):
