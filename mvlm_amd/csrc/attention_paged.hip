@@ -84,7 +84,7 @@ void plan_attention_paged(PagedAttnArgs* a, int num_cus) {
     // table of 768 positions 13.5 us, of 32768 16.1; 2048 bf16 rows on 8192 303 us without the second launch, 306).
     const bool single = !b.row_start;                          // every sequence has `group` f-rows
     const int64_t tiles256 = (single ? (int64_t)b.seqs * (a->group / CHUNK_R) : f / CHUNK_R) * a->kv.kv_heads;
-    const bool many = a->kv.dtype != MVLM_MXFP8 && tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
+    const bool many = tiles256 * std::max(1, b.positions / CHUNK_UNIT) >= num_cus;
     a->many_least = (num_cus + a->kv.kv_heads - 1) / a->kv.kv_heads;
     if (many) {
         // a sequence with more than PAGED_FEW f-rows ends in one tile that is not full

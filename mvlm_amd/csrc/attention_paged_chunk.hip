@@ -78,23 +78,27 @@ typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 constexpr int CHUNK_THREADS = 512;
 
 constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
-constexpr int SLOT_KEYS = 2048;                                // keys whose slots LDS holds, twice
 
-template <int DT>
+template <int DT, bool MX>
 struct ChunkLayout {
     static constexpr int CH = DT > 2 ? 16 : 8;                 // chunks per LDS row
     static constexpr int PB = 16 * CH, TILE = CHUNK_KEYS * PB;
-    static constexpr int NB = DT > 2 ? 3 : 4;                  // tiles of the K ring, and of the V ring behind it
-    static constexpr int V = NB * TILE, SLOTS = 2 * NB * TILE, P = SLOTS + 2 * SLOT_KEYS * 4;
+    static constexpr int NB = MX ? 2 : DT > 2 ? 3 : 4;         // tiles of the K ring, and of the V ring behind it
+    static constexpr int SLOT_KEYS = MX ? 1024 : 2048;         // keys whose slots LDS holds, twice
+    // 8 bits: a thread's pieces of a tile of K and one of V, of 16 codes each, and the scales' words, for two iterations
+    static constexpr int PIECES = CHUNK_KEYS * CH / CHUNK_THREADS;
+    static constexpr int V = NB * TILE, RAW = 2 * NB * TILE, WORDS = RAW + (MX ? 2 * PIECES * CHUNK_THREADS * 16 : 0);
+    static constexpr int SLOTS = WORDS + (MX ? 2 * PIECES * CHUNK_THREADS * 4 : 0), P = SLOTS + 2 * SLOT_KEYS * 4;
     static constexpr int P_WAVE = 32 * 32 * 4;                 // 32 keys x 32 rows of probabilities (slow path)
     static constexpr int ZEROS = P + 8 * P_WAVE, BYTES = ZEROS + TILE;   // a V tile of zeros
 };
 
-// KS: head_dim <= 16 KS; DT: head_dim <= 32 DT; PP: parts of P
-template <int KS, int DT, bool BF, int PP>
+// KS: head_dim <= 16 KS; DT: head_dim <= 32 DT; CT: the cache's type; PP: parts of P
+template <int KS, int DT, int CT, int PP>
 __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const PagedShare& share, int index, int h, uint8_t* lds) {
-    using L = ChunkLayout<DT>;
-    constexpr int CH = L::CH, PB = L::PB, TILE = L::TILE, NB = L::NB, R = CHUNK_R;
+    constexpr bool MX = CT == MVLM_MXFP8, BF = CT != MVLM_F16;
+    using L = ChunkLayout<DT, MX>;
+    constexpr int CH = L::CH, PB = L::PB, TILE = L::TILE, NB = L::NB, R = CHUNK_R, SLOT_KEYS = L::SLOT_KEYS;
     constexpr int NL = CHUNK_KEYS * CH / CHUNK_THREADS;        // chunks of K (and of V) per thread and tile
     const int tid = own_thread(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
@@ -124,7 +128,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     for (int i = tid; i < TILE / 16; i += CHUNK_THREADS) *reinterpret_cast<u32x4*>(lds + L::ZEROS + 16 * i) = u32x4{0u, 0u, 0u, 0u};
     const int n = (max(k_end - k_begin, 0) + CHUNK_KEYS - 1) / CHUNK_KEYS;
     // where the part-th SLOT_KEYS keys are, in 16-byte chunks of the cache (below 2^32, checked
-    // on the host) or NOWHERE, into their half of the buffer
+    // on the host; of 8 bits: their slots) or NOWHERE, into their half of the buffer
     const int* table = a.batch.table + (int64_t)it.seq * a.batch.width;
     uint32_t* slots = (uint32_t*)(lds + L::SLOTS);
     auto find_slots = [&](int part) {
@@ -135,7 +139,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             if (key < k_end) {
                 const int pi = a.kv.page.quotient(key), page = table[pi];
                 if (page >= 0 && page < a.kv.num_pages)
-                    at = (uint32_t)a.kv.slot(page, h, key - pi * a.kv.page.div) * (uint32_t)(D / 8);
+                    at = (uint32_t)a.kv.slot(page, h, key - pi * a.kv.page.div) * (uint32_t)(MX ? 1 : D / 8);
             }
             slots[(part & 1) * SLOT_KEYS + i] = at;
         }
@@ -169,9 +173,55 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     };
     auto next_slots = [&](int i) {
         // half a part ahead: the slots of the next one, in the half whose tiles are done
-        constexpr int PART = SLOT_KEYS / CHUNK_KEYS;
-        const int tv = i + NB - 2;
-        if (tv % PART == PART / 2 && (tv / PART + 1) * PART <= n + NB) find_slots(tv / PART + 1);
+        constexpr int PART = SLOT_KEYS / CHUNK_KEYS, AHEAD = MX ? 4 : NB;
+        const int tv = i + AHEAD - 2;
+        if (tv % PART == PART / 2 && (tv / PART + 1) * PART <= n + AHEAD) find_slots(tv / PART + 1);
+    };
+    // 8 bits.  Each thread owns PIECES of the 16-code pieces that make tile j + 1 of K and tile j of V: it asks for
+    // them two iterations ahead, into 16 bytes of LDS of its own (and 4 for the word of scales), so it needs no barrier
+    // before it reads them, and makes bf16 of them in iteration j, which reads neither tile's buffer.  With two pieces
+    // one is K's and one V's; with one, waves 0..3 have K's and 4..7 V's.
+    constexpr int PIECES = L::PIECES, CH8 = CH / 2;
+    auto is_key = [&](int w) { return PIECES == 2 ? w == 0 : !second; };
+    const int piece_at = PIECES == 2 ? tid : tid & 255, pkey = piece_at / CH8, pdim = 16 * (piece_at % CH8);
+    auto code_address = [&](uint32_t slot, bool keys) {
+        const uint64_t p = (uint64_t)(uintptr_t)(keys ? a.kv.k : a.kv.v) + (uint64_t)slot * (uint32_t)D + (uint32_t)pdim;
+        return (const void*)(uintptr_t)(slot != NOWHERE && pdim < D ? p : (uint64_t)(uintptr_t)&paged_zeros);
+    };
+    auto word_address = [&](uint32_t slot, bool keys) {
+        const uint64_t p = (uint64_t)(uintptr_t)(keys ? a.kv.k_scale : a.kv.v_scale) + 4 * (uint64_t)slot;
+        return (const void*)(uintptr_t)(slot != NOWHERE ? p : (uint64_t)(uintptr_t)&paged_zeros);
+    };
+    auto ask = [&](int j, int w) {
+        const bool keys = is_key(w);
+        const uint32_t slot = slots[(uint32_t)((keys ? j + 1 : j) * CHUNK_KEYS + pkey) % (2 * SLOT_KEYS)];
+        const uint32_t to = (uint32_t)((j & 1) * PIECES + w) * CHUNK_THREADS + 64 * wave;
+        asm_global_load_lds_b128(code_address(slot, keys), lds0 + L::RAW + 16 * to);
+        asm_global_load_lds_b32(word_address(slot, keys), lds0 + L::WORDS + 4 * to);
+    };
+    // 16 codes and their power of two as bf16 into tile buffer `ring` of K or V
+    auto widen = [&](u32x4 codes, uint32_t word, bool keys, int ring) {
+        const float up = mx_power(word, min(pdim, D - 1) >> 5);
+        u32x4 lo = mx_values(codes[0], codes[1], up), hi = mx_values(codes[2], codes[3], up);
+        if (pdim + 8 >= D) hi = u32x4{0u, 0u, 0u, 0u};         // the row's last piece may reach past it
+        const int c = pdim / 8, x = keys ? key_swizzle<CH>(pkey) : value_swizzle<CH>(pkey);
+        const uint32_t row = lds0 + (keys ? 0 : L::V) + ring * TILE + pkey * PB;
+        *(lds_u32x4*)(uintptr_t)(row + 16 * (c ^ x)) = lo;
+        *(lds_u32x4*)(uintptr_t)(row + 16 * ((c + 1) ^ x)) = hi;
+    };
+    u32x4 raw;
+    uint32_t raw_word;
+    // the three parts of a piece's work in iteration i, at steps apart
+    auto mx_work = [&](int i, int ring, auto step) {
+        constexpr int st = decltype(step)::value, w = st / 2;
+        if constexpr (st <= 2 * PIECES && st % 2 == 0 && st > 0) ask(i + 2, w - 1);
+        if constexpr (st < 2 * PIECES && st % 2 == 0) {
+            asm_wait_vmcnt<2 * (2 * PIECES - 1)>();            // all later than this piece's may be on their way
+            const uint32_t from = (uint32_t)((i & 1) * PIECES + w) * CHUNK_THREADS + tid;
+            raw = *(const lds_u32x4*)(uintptr_t)(lds0 + L::RAW + 16 * from);
+            raw_word = *(const __attribute__((address_space(3))) uint32_t*)(uintptr_t)(lds0 + L::WORDS + 4 * from);
+        }
+        if constexpr (st < 2 * PIECES && st % 2 == 1) widen(raw, raw_word, is_key(w), is_key(w) ? 1 - ring : ring);
     };
     // where this lane reads: K chunk 2 st + h2 of key l32, V at key 4 h2 + (lane & 15) / 4
     // and dims 32 t + 16 ((lane / 16) & 1) + 4 (lane & 3); st and t are one exclusive or
@@ -251,7 +301,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
     auto products = [&](int i, int ring, bool pv) {
         constexpr bool APART = PP > 1 && PagedP<BF>::REST != 1.0f;
         constexpr int PV = APART ? DT : 4, STEPS = PV + (KS + 1) / 2;
-        static_assert(2 * NL <= STEPS, "a step asks for one piece at most");
+        static_assert(MX ? 2 * PIECES + 1 <= STEPS : 2 * NL <= STEPS, "a step asks for one piece at most");
         constexpr int AHEAD = DT > 2 ? 1 : 3, SETS = AHEAD + 1;
         const uint32_t v_at = pv ? values_at(i - 1, before(ring)) : vat - L::V + L::ZEROS, k_at = kat + ring * TILE;
         const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -278,8 +328,10 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             }
         };
         static_for<AHEAD>(read);
+        if constexpr (!MX) {
 #pragma unroll
-        for (int j = 0; j < 2 * NL; ++j) slot[j] = slot_of(i + NB - 1 - j / NL, j % NL);
+            for (int j = 0; j < 2 * NL; ++j) slot[j] = slot_of(i + NB - 1 - j / NL, j % NL);
+        }
         static_for<STEPS>([&](auto step) {
             constexpr int st = decltype(step)::value;
             read(std::integral_constant<int, st + AHEAD>{});
@@ -290,7 +342,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
                 for (int x = 0; x < 4; ++x) {
                     rest = mfma32<BF>(frag[st % SETS][x], pb[PP - 1][x], rest);
                     oacc[st] = mfma32<BF>(frag[st % SETS][x], pb[0][x], oacc[st]);
-                    if constexpr (st < 2 * NL)
+                    if constexpr (!MX && st < 2 * NL)
                         if (x == 0) piece(ring, st, slot[st]);
                 }
 #pragma unroll
@@ -298,7 +350,8 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             } else if constexpr (st < PV) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) oacc[t] = mfma32<BF>(frag[st % SETS][t], pb[0][st], oacc[t]);
-                if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
+                if constexpr (MX) mx_work(i, ring, step);
+                else if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
 #pragma unroll
                 for (int w = 1; w < PP; ++w)
 #pragma unroll
@@ -312,7 +365,8 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
                             const int d = 2 * (st - PV) + e;
                             s[u] = mfma32<BF>(frag[st % SETS][2 * e + u], qf[d], d == 0 ? zero : s[u]);
                         }
-                if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
+                if constexpr (MX) mx_work(i, ring, step);
+                else if constexpr (st < 2 * NL) piece(ring, st, slot[st]);
             }
         });
     };
@@ -370,6 +424,18 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         }
     };
 
+    if constexpr (MX) {
+        if (is_key(0)) {
+            const uint32_t slot = slots[pkey];
+            typedef u32x4 u32x4_any __attribute__((aligned(8)));
+            const u32x4 codes = *(const u32x4_any*)code_address(slot, true);
+            widen(codes, *(const uint32_t*)word_address(slot, true), true, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int w = 0; w < PIECES; ++w) ask(j, w);
+    } else
 #pragma unroll
     for (int t = 0; t < NB - 1; ++t)
 #pragma unroll
@@ -377,7 +443,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
             load_chunks(a.kv.k, slot_of(t, l), l, t * TILE, true);
             if (t < NB - 2) load_chunks(a.kv.v, slot_of(t, l), l, L::V + t * TILE, false);
         }
-    asm_wait_vmcnt<0>();
+    if constexpr (!MX) asm_wait_vmcnt<0>();
     phase_barrier();
     auto in_reach = [&](int i) { return i < n && k_begin + i * CHUNK_KEYS < wave_end; };
     for (int i = 0, ring = 0; i <= n; ++i, ring = ring == NB - 1 ? 0 : ring + 1) {
@@ -391,7 +457,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedAttnArgs& a, const P
         __builtin_amdgcn_s_setprio(0);
         if (!second && in_reach(i)) softmax(i);
         // what this wave asked for NB - 2 iterations ago has arrived: K of tile i + 1 and V of tile i
-        asm_wait_vmcnt<(NB - 2) * 2 * NL>();
+        if constexpr (!MX) asm_wait_vmcnt<(NB - 2) * 2 * NL>();
         phase_barrier();
     }
     asm_wait_vmcnt<0>();                                       // loads past the last tile write LDS that is about to be reused
@@ -440,7 +506,7 @@ __device__ __forceinline__ const PagedAttnArgs& item_args(const PagedAttnArgs& a
     return *(const PagedAttnArgs*)(const __attribute__((address_space(4))) PagedAttnArgs*)p;
 }
 
-template <int KS, int DT, bool BF, int PP>
+template <int KS, int DT, int CT, int PP>
 __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int kv_heads = a.kv.kv_heads, q = (int)blockIdx.x % PAGED_QUEUES, own = (int)blockIdx.x / PAGED_QUEUES;
@@ -456,21 +522,21 @@ __global__ __launch_bounds__(CHUNK_THREADS, 2) void paged_chunk_kernel(const Pag
         const int i = round * blocks + (round & 1 ? blocks - 1 - own : own);
         if (i < many_items) {
             const int w = i * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_chunk_item<KS, DT, BF, PP>(item_args<DT>(a), many, index, w - index * kv_heads, lds);
+            paged_chunk_item<KS, DT, CT, PP>(item_args<DT>(a), many, index, w - index * kv_heads, lds);
         } else if (i < all_items) {
             const int w = (i - many_items) * PAGED_QUEUES + q, index = w / kv_heads;
-            paged_few_item<32, DT, BF ? MVLM_BF16 : MVLM_F16, PP, 8>(item_args<DT>(a), few, index, w - index * kv_heads, lds);
+            paged_few_item<32, DT, CT, PP, 8>(item_args<DT>(a), few, index, w - index * kv_heads, lds);
         }
         __syncthreads();                                       // LDS is free
     }
 }
 
-template <int KS, int DT, bool BF, int PP>
+template <int KS, int DT, int CT, int PP>
 static hipError_t launch_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
-    constexpr int few = 8 * PagedLayout<32, DT>::REGION + 16, bytes = ChunkLayout<DT>::BYTES > few ? ChunkLayout<DT>::BYTES : few;
-    if (const hipError_t e = allow_dynamic_lds<paged_chunk_kernel<KS, DT, BF, PP>>(bytes); e != hipSuccess) return e;
+    constexpr int few = 8 * PagedLayout<32, DT>::REGION + 16, chunk = ChunkLayout<DT, CT == MVLM_MXFP8>::BYTES, bytes = chunk > few ? chunk : few;
+    if (const hipError_t e = allow_dynamic_lds<paged_chunk_kernel<KS, DT, CT, PP>>(bytes); e != hipSuccess) return e;
     const int64_t most = ((int64_t)a.many.items + a.few.items) * a.kv.kv_heads;
-    launch_kernel_part(LaunchPart::First, paged_chunk_kernel<KS, DT, BF, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),
+    launch_kernel_part(LaunchPart::First, paged_chunk_kernel<KS, DT, CT, PP>, dim3((unsigned)std::min<int64_t>(num_cus, most)), dim3(CHUNK_THREADS),
                   (uint32_t)bytes, s, a);
     return hipGetLastError();
 }
@@ -478,8 +544,9 @@ static hipError_t launch_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cu
 template <int KS, int DT>
 static hipError_t launch_chunk_dims(hipStream_t s, const PagedAttnArgs& a, int num_cus) {
     const bool wide = a.o_dtype == MVLM_F32;
-    if (a.kv.dtype == MVLM_F16) return wide ? launch_chunk<KS, DT, false, 2>(s, a, num_cus) : launch_chunk<KS, DT, false, 1>(s, a, num_cus);
-    return wide ? launch_chunk<KS, DT, true, 3>(s, a, num_cus) : launch_chunk<KS, DT, true, 1>(s, a, num_cus);
+    if (a.kv.dtype == MVLM_F16) return wide ? launch_chunk<KS, DT, MVLM_F16, 2>(s, a, num_cus) : launch_chunk<KS, DT, MVLM_F16, 1>(s, a, num_cus);
+    if (a.kv.dtype == MVLM_MXFP8) return wide ? launch_chunk<KS, DT, MVLM_MXFP8, 3>(s, a, num_cus) : launch_chunk<KS, DT, MVLM_MXFP8, 1>(s, a, num_cus);
+    return wide ? launch_chunk<KS, DT, MVLM_BF16, 3>(s, a, num_cus) : launch_chunk<KS, DT, MVLM_BF16, 1>(s, a, num_cus);
 }
 
 hipError_t launch_attention_paged_chunk(hipStream_t s, const PagedAttnArgs& a, int num_cus) {

@@ -150,27 +150,73 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
 //   x' = x w / sqrt(sum x^2 / D + eps), then the rotation; e = mx_exponent(max |x|), code = e4m3(x 2^-e)
 // Bytes bound it as well.  L = 1 .. 16 lanes make a head, 8 dims each, and sum over one another; a lane has the
 // same dims of every head that it makes, so the weights and the row's cos and sin are in its registers once.  Codes
-// leave in 8-byte stores (a head of 64 dims is half a line, its neighbours in the page come from the next rows), a
-// head's scales in one word.
+// leave in 8-byte stores, a head's scales in one word.
+constexpr int HEADS_AHEAD = 3;
+
+// 8 elements as they lie in memory
 template <int XD, bool VEC>
+struct AppendRaw {
+    u32x4 w[VEC && XD != MVLM_F32 ? 1 : 2];
+    __device__ __forceinline__ void load(const void* x, int64_t i) {
+        if constexpr (!VEC) {
+            float v[8];
+            append_load8<XD, false>(x, i, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = __float_as_uint(v[e]);
+        } else if constexpr (XD == MVLM_F32) {
+            const u32x4* p = reinterpret_cast<const u32x4*>((const float*)x + i);
+            w[0] = p[0], w[1] = p[1];
+        } else
+            w[0] = *reinterpret_cast<const u32x4*>((const uint16_t*)x + i);
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (!VEC || XD == MVLM_F32) return __uint_as_float(w[e >> 2][e & 3]);
+        else if constexpr (XD == MVLM_BF16) return __uint_as_float(e & 1 ? w[0][e >> 1] & 0xFFFF0000u : w[0][e >> 1] << 16);
+        else return f16_bits_to_f32((uint16_t)(w[0][e >> 1] >> (16 * (e & 1))));
+    }
+};
+
+// f(v, the value of the lane that is off away by exclusive or), over groups of `lanes` lanes; off = 1, 2, 4, 8
+// in turn, after which a group's lanes agree where f is a sum or a maximum (the mirrors reach the lane 4 or 8 away because
+// its neighbours agree by then)
+template <class T, class F>
+__device__ __forceinline__ T over_lanes(T v, int from, int lanes, F&& f) {
+    auto move = [](T x, auto ctrl) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    if (from <= 1 && lanes > 1) v = f(v, move(v, std::integral_constant<int, 0xB1>{}));      // quad_perm [1, 0, 3, 2]
+    if (from <= 2 && lanes > 2) v = f(v, move(v, std::integral_constant<int, 0x4E>{}));      // quad_perm [2, 3, 0, 1]
+    if (from <= 4 && lanes > 4) v = f(v, move(v, std::integral_constant<int, 0x141>{}));     // row_half_mirror
+    if (lanes > 8) v = f(v, move(v, std::integral_constant<int, 0x140>{}));                  // row_mirror
+    return v;
+}
+
+// XD: type of qkv; VEC: its rows are 16-byte aligned; MX: 8-bit cache; NORM: of q or k heads
+template <int XD, bool VEC, bool MX, bool NORM>
 __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const KvAppendArgs a) {
     const int row = (int)blockIdx.x;
     const PagedKv& kv = a.kv;
     const int D = kv.D, half = a.rot / 2, qk = a.heads + kv.kv_heads, all = qk + kv.kv_heads;
     const int shift = D > 64 ? 4 : D > 32 ? 3 : D > 16 ? 2 : D > 8 ? 1 : 0, lanes = 1 << shift;
-    const int sub = (int)threadIdx.x & (lanes - 1), d = 8 * sub, step = APPEND_THREADS >> shift;
+    const int sub = (int)threadIdx.x & (lanes - 1), d = 8 * sub, step = (int)blockDim.x >> shift;
     const int own = (int)threadIdx.x >> shift;
     const int dl = min(d, D - 8);                          // a lane past the head's end reads its last dims
     const int64_t xrow = (int64_t)row * a.ld;
-    float ahead[APPEND_AHEAD][8];
+    AppendRaw<XD, VEC> ahead[HEADS_AHEAD];
 #pragma unroll
-    for (int u = 0; u < APPEND_AHEAD; ++u) append_load8<XD, VEC>(a.qkv, xrow + (int64_t)min(own + u * step, all - 1) * D + dl, ahead[u]);
-    float qw[8], kw[8];
+    for (int u = 0; u < HEADS_AHEAD; ++u) ahead[u].load(a.qkv, xrow + (int64_t)min(own + u * step, all - 1) * D + dl);
+    // the weights of the kind of head that the lane is at, of which each follows the other
+    float wt[8];
+    const float* weight = nullptr;
+    auto weigh = [&](const float* w) {
+        weight = w;
+        if (!w) return;
+        const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(w + dl), hi = *reinterpret_cast<const f32x4_any*>(w + dl + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        qw[e] = a.q_weight ? a.q_weight[dl + e] : 1.0f;
-        kw[e] = a.k_weight ? a.k_weight[dl + e] : 1.0f;
-    }
+        for (int e = 0; e < 4; ++e) wt[e] = lo[e], wt[4 + e] = hi[e];
+    };
+    int kind_end = a.heads;                                // heads below it are of that kind
+    if constexpr (NORM) weigh(a.q_weight);
     PagedSpan sp;
     const int seq = paged_seq_of_row(a.batch, row, &sp);
     if (seq < 0) return;                                   // behind the last sequence: left as it is
@@ -181,35 +227,68 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
         const int page = a.batch.table[(int64_t)seq * a.batch.width + pi];
         if (page >= 0 && page < kv.num_pages) slot0 = kv.slot(page, 0, p - pi * kv.page.div);
     }
-    // cos and sin of this lane's dims: of pairs d / 2 .. (interleaved), or of each of them
+    // cos and signed sin of this lane's dims: x' = x co + (its pair's other element) si
     float co[8], si[8];
-    const bool turns = d < a.rot && slot0 >= 0, by_chunk = half % 8 == 0;
+    const bool turns = d < a.rot && slot0 >= 0;
+    const bool whole = (a.interleaved ? a.rot : half) % 8 == 0;   // a chunk turns as a whole
     const float* cs = a.rope + (int64_t)p * a.rot;         // [rot / 2][2]
+    if (turns) {
+        if (whole && a.interleaved) {
+            const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(cs + d), hi = *reinterpret_cast<const f32x4_any*>(cs + d + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        co[e] = 1.0f, si[e] = 0.0f;
-        if (turns && d + e < a.rot) {
-            const int i = a.interleaved ? (d + e) / 2 : d + e < half ? d + e : d + e - half;
-            co[e] = cs[2 * i];
-            si[e] = cs[2 * i + 1];
+            for (int e = 0; e < 8; e += 2) {
+                const f32x4_any& q = e < 4 ? lo : hi;
+                co[e] = co[e + 1] = q[e & 2];
+                si[e] = -q[(e & 2) + 1];
+                si[e + 1] = q[(e & 2) + 1];
+            }
+        } else if (whole) {
+            const f32x4_any* t = reinterpret_cast<const f32x4_any*>(cs + 2 * (d < half ? d : d - half));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const f32x4_any q = t[e / 2];
+                co[e] = q[0], co[e + 1] = q[2];
+                si[e] = d < half ? -q[1] : q[1], si[e + 1] = d < half ? -q[3] : q[3];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool first = a.interleaved ? (e & 1) == 0 : d + e < half;
+                const int i = min(a.interleaved ? (d + e) / 2 : first ? d + e : d + e - half, half - 1);
+                co[e] = cs[2 * i];
+                si[e] = first ? -cs[2 * i + 1] : cs[2 * i + 1];
+            }
         }
     }
-    auto make = [&](int head, const float (&x)[8]) {
+    // where the lane's dims of q head 0 and of kv head 0 go; a kv head further on is a page's slots further on
+    uint16_t* const q_to = a.q_out + (int64_t)row * a.heads * D + d;
+    const int64_t kv_to = (int64_t)max(slot0, 0) * D + d;
+    const int kv_step = kv.page.div * D;                   // below 2^31 2^7 / kv_heads: 64 bits where multiplied
+    const int partner = ((int)threadIdx.x & 63) + (d < half ? half / 8 : -(half / 8));
+    auto make = [&](int head, const AppendRaw<XD, VEC>& x) {
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = d < D ? x[e] : 0.0f;
+        for (int e = 0; e < 8; ++e) v[e] = x.get(e);
+        if (8 * lanes > D) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = d < D ? v[e] : 0.0f;
+        }
         const bool is_q = head < a.heads, is_k = !is_q && head < qk;
-        const float* weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
         float r = 1.0f;
-        if (a.q_weight || a.k_weight) {                    // all lanes of a wave sum
+        if constexpr (NORM) {
+            if (head >= kind_end) {
+                weigh(is_k ? a.k_weight : nullptr);
+                kind_end = is_k ? qk : all;
+            }
             float ss = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
-            for (int off = 1; off < lanes; off <<= 1) ss += __shfl_xor(ss, off, 64);
+            ss = over_lanes(ss, 1, lanes, [](float u, float w) { return u + w; });
             if (weight) {
-                r = 1.0f / sqrtf(ss / (float)D + a.eps);
+                const float mean = __builtin_fmaf(ss, a.per_dim, a.eps);
+                r = mean >= 0x1p-120f ? __builtin_amdgcn_rsqf(mean) : 1.0f / sqrtf(mean);   // the first takes no subnormals
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (is_q ? qw[e] : kw[e]);
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * wt[e];
             }
         }
         if (a.rot) {
@@ -217,10 +296,9 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
             if (a.interleaved) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = v[e ^ 1];
-            } else if (by_chunk) {                         // a chunk lies in one half, its partner chunk in the other
-                const int other = ((int)threadIdx.x & 63) + (d < half ? half / 8 : -(half / 8));
+            } else if (whole) {                            // a chunk lies in one half, its partner chunk in the other
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = __shfl(v[e], other & 63, 64);
+                for (int e = 0; e < 8; ++e) w[e] = __shfl(v[e], partner & 63, 64);
             } else if (turns && (is_q || is_k)) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -230,74 +308,76 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
                 }
             }
             if (turns && (is_q || is_k)) {
-                float o[8];
+                if (whole) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool first = a.interleaved ? (e & 1) == 0 : d + e < half;
-                    o[e] = d + e < a.rot ? v[e] * co[e] + (first ? -w[e] : w[e]) * si[e] : v[e];
+                    for (int e = 0; e < 8; ++e) w[e] = v[e] * co[e] + w[e] * si[e];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = w[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = d + e < a.rot ? v[e] * co[e] + w[e] * si[e] : v[e];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = w[e];
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = o[e];
             }
         }
-        const bool mx = kv.dtype == MVLM_MXFP8;
-        if (mx && !is_q) {
-            uint32_t most = 0;
-            bool odd = false;
+        if (is_q || !MX) {
+            u32x4 out;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t m = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-                most = m < 0x7F800000u ? max(most, m) : most;
-                odd |= m >= 0x7F800000u;
+            for (int j = 0; j < 4; ++j) {
+                const f32x2 pair = {v[2 * j], v[2 * j + 1]};
+                out[j] = !MX && kv.dtype == MVLM_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2_t))
+                                                     : __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_t));
             }
-            for (int off = 1; off < min(lanes, MX_BLOCK / 8); off <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
-            const int ex = mx_exponent(most);
-            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), limit = ex == MX_MOST ? 240.0f : 448.0f;
-            uint32_t code[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = fminf(fmaxf(v[4 * j + e] * down, -limit), limit);
-                int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-                code[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
-            }
-            if (odd) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if ((__float_as_uint(v[e]) & 0x7FFFFFFFu) >= 0x7F800000u) code[e >> 2] |= 0x7Fu << (8 * (e & 3));
-            }
-            uint32_t word = (uint32_t)(ex + MX_BIAS) << (d / MX_BLOCK * 8);
-            for (int off = MX_BLOCK / 8; off < lanes; off <<= 1) word |= (uint32_t)__shfl_xor((int)word, off, 64);
-            if (slot0 < 0) return;
-            const int64_t slot = slot0 + (int64_t)(head - (is_k ? a.heads : qk)) * kv.page.div;
-            if (d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + slot * D + d) = u32x2{code[0], code[1]};
-            if (sub == 0) (is_k ? kv.k_scale : kv.v_scale)[slot] = word;
+            if (d >= D) return;
+            if (is_q) {
+                if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4*>(q_to + head * D) = out;
+            } else if (slot0 >= 0)
+                *reinterpret_cast<u32x4*>((is_k ? kv.k : kv.v) + (kv_to + (int64_t)(head - (is_k ? a.heads : qk)) * kv_step)) = out;
             return;
         }
-        u32x4 out;
+        if constexpr (MX) {
+            const auto larger = [](float u, float w) { return fmaxf(u, w); };
+            float most = 0.0f;                             // of |v|; a NaN is not taken
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const f32x2 pair = {v[2 * j], v[2 * j + 1]};
-            out[j] = kv.dtype == MVLM_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2_t))
-                                          : __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_t));
-        }
-        if (d >= D) return;
-        if (is_q) {
-            if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
-            *reinterpret_cast<u32x4*>(a.q_out + ((int64_t)row * a.heads + head) * D + d) = out;
-        } else if (slot0 >= 0) {
-            const int64_t slot = slot0 + (int64_t)(head - (is_k ? a.heads : qk)) * kv.page.div;
-            *reinterpret_cast<u32x4*>((is_k ? kv.k : kv.v) + slot * D + d) = out;
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+            if (most == INFINITY) {                        // few have any: the largest of the others
+                most = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fabsf(v[e]) < INFINITY ? fmaxf(most, fabsf(v[e])) : most;
+            }
+            most = over_lanes(most, 1, min(lanes, MX_BLOCK / 8), larger);
+            const int ex = mx_exponent(__float_as_uint(most));
+            const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = v[e] * down;
+            if (ex == MX_MOST) {                           // 248 and above would round to 2^8, a value of 2^128
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (fabsf(v[e]) < INFINITY) y[e] = fminf(fmaxf(y[e], -240.0f), 240.0f);
+            }
+            u32x2 code;                                    // the conversion makes NaN of infinities as well
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j], y[4 * j + 1], 0, false);
+                code[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j + 2], y[4 * j + 3], c, true);
+            }
+            uint32_t word = (uint32_t)(ex + MX_BIAS) << (d / MX_BLOCK * 8);
+            word = over_lanes(word, MX_BLOCK / 8, lanes, [](uint32_t u, uint32_t w) { return u | w; });
+            if (slot0 < 0) return;
+            const int h = head - (is_k ? a.heads : qk);
+            if (d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + (kv_to + (int64_t)h * kv_step)) = code;
+            if (sub == 0) (is_k ? kv.k_scale : kv.v_scale)[slot0 + h * kv.page.div] = word;
         }
     };
-    // A wave's lanes go round together, so that each finds the others of its head; one past the last head ends there.
+    // The lanes of a head go round together, so that each finds the others.
+    for (int head = own; head < all; head += step) {
+        const AppendRaw<XD, VEC> x = ahead[0];
 #pragma unroll
-    for (int u = 0; u < APPEND_AHEAD; ++u)
-        if (own + u * step < all) make(own + u * step, ahead[u]);
-    for (int head = own + APPEND_AHEAD * step; head < all; head += step) {
-        float x[8];
-        append_load8<XD, VEC>(a.qkv, xrow + (int64_t)head * D + dl, x);
+        for (int u = 0; u + 1 < HEADS_AHEAD; ++u) ahead[u] = ahead[u + 1];
+        ahead[HEADS_AHEAD - 1].load(a.qkv, xrow + (int64_t)min(head + HEADS_AHEAD * step, all - 1) * D + dl);
         make(head, x);
     }
 }
@@ -306,12 +386,21 @@ hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a) {
     const size_t es = dtype_size(a.x_dtype);
     const bool vec = ((uintptr_t)a.qkv & 15u) == 0 && (a.ld * (int64_t)es) % 16 == 0;
     const dim3 grid((unsigned)a.batch.rows), block(APPEND_THREADS);
+    // a row's prologue is paid by each of its waves: two of them where the rows fill the chip (16162 rows of 32 + 2 x 8
+    // heads of 128: 93 us, with four 102, with one 93), four where they do not (768 of 3 x 32 heads of 64: 7.3 us, with two 9.0)
+    const dim3 hblock(a.batch.rows >= 2048 ? APPEND_THREADS / 2 : APPEND_THREADS);
     const bool by_head = a.kv.dtype == MVLM_MXFP8 || a.q_weight || a.k_weight;
     auto go = [&](auto dt) {
         constexpr int XD = decltype(dt)::value;
         if (by_head) {
-            if (vec) launch_kernel(kv_append_heads_kernel<XD, true>, grid, block, 0, s, a);
-            else launch_kernel(kv_append_heads_kernel<XD, false>, grid, block, 0, s, a);
+            auto heads = [&](auto mx, auto norm) {
+                if (vec) launch_kernel(kv_append_heads_kernel<XD, true, decltype(mx)::value, decltype(norm)::value>, grid, hblock, 0, s, a);
+                else launch_kernel(kv_append_heads_kernel<XD, false, decltype(mx)::value, decltype(norm)::value>, grid, hblock, 0, s, a);
+            };
+            const bool norm = a.q_weight || a.k_weight;
+            if (a.kv.dtype != MVLM_MXFP8) heads(std::false_type{}, std::true_type{});
+            else if (norm) heads(std::true_type{}, std::true_type{});
+            else heads(std::true_type{}, std::false_type{});
             return;
         }
         if (vec) launch_kernel(kv_append_kernel<XD, true>, grid, block, 0, s, a);

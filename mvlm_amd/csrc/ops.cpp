@@ -437,6 +437,7 @@ int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_
         a.q_weight = q_norm ? (const float*)norm->q_weight->ptr : nullptr;
         a.k_weight = k_norm ? (const float*)norm->k_weight->ptr : nullptr;
         a.eps = norm->eps;
+        a.per_dim = 1.0f / (float)a.kv.D;
     }
     const size_t kvb = a.kv.bytes;
     const struct { const void* p; size_t bytes; } written[3] = {{a.kv.k, kvb}, {a.kv.v, kvb}, {q_out->ptr, q_bytes}};

@@ -20,7 +20,7 @@ struct KvAppendArgs {
     uint16_t* q_out;               // [rows][heads][D], the cache's type (bf16 for an 8-bit cache)
     const float* q_weight;         // [D] norms of q and k heads; null: none
     const float* k_weight;
-    float eps;
+    float eps, per_dim;            // per_dim: 1 / head_dim
 };
 
 struct KvReadArgs {
