@@ -10,10 +10,18 @@
 //   picked   the first at which it reaches floor(u x the sum kept) + 1
 // so one search serves all three.  Values are compared as integers that order like them (sample_key).
 //
-// One block per row.  It reads the row for m, then counts the live tokens by t in steps of 1/32 (at most 1664 of
-// them), with their weights where more than LIST tokens may be kept.  If those that matter fit a list in LDS, a
-// pass collects them, they are sorted, and running sums give all answers.  Otherwise each search goes on inside its
-// step: by list if that fits, else by counting in ranges of keys, and among equal values by index.
+// One block per row.
+//  * Few tokens can be kept, or picked: the candidates, the tokens above a bound, go into LDS.  With the k-th
+//    largest of the threads' largest values as bound, k tokens at least lie above it (some THREADS ln(THREADS /
+//    (THREADS - k)) of them where values do not depend on their places).  So top_k of up to RANKS has all that it
+//    may keep among the candidates, min_p has with the bound that it sets itself, and top_p most likely has with
+//    the RANKS-th, of which it knows once the sum of all weights is made.
+//  * Up to LIST candidates that are all that can be kept are sorted, and running sums give the answers.  More of them
+//    (or, where the candidates do not hold what is looked for, all live tokens of the row) are counted by t in steps of
+//    1/STEPS, with their weights.  A search finds its step in the running sums, sorts the step's tokens, and finds
+//    its place among them; a step of more tokens than the list holds is counted again in ranges of keys, down to
+//    equal values, of which the index decides.
+// Running sums are over THREADS bins or entries, one of each thread's, which then knows whether a place is its own.
 #include "common.h"
 #include "device_math.h"
 #include "sample.h"
@@ -21,10 +29,17 @@
 namespace mvlm {
 
 constexpr int SAMPLE_THREADS = 1024;
-constexpr int SAMPLE_BATCH = 4;        // 16-byte chunks in flight per thread
-constexpr int BINS = 2048;
-constexpr int LIST = 4096;             // entries of the list in LDS
-constexpr int STEPS = 32;              // bins per factor of two of the weight; (51 + 1) 32 < BINS
+constexpr int SAMPLE_BATCH = 8;        // 16-byte chunks in flight per thread behind the held ones
+constexpr int HOLD = 52;               // words of tokens that a thread keeps: 53248 fp32 tokens of a row, twice as many of 16 bits
+constexpr int CANDIDATES = 8192;       // room for them in LDS
+constexpr int LIST = SAMPLE_THREADS;   // entries that are sorted at once
+constexpr int RANKED = 256;            // of which so many by counting
+constexpr int RANKS = 1000;            // of the threads' largest values
+constexpr int RANK_BINS = 256, RANK_STEPS = 8;   // in which they are counted, per factor of two of the weight
+constexpr int BINS = SAMPLE_THREADS;
+constexpr int STEPS = 16;              // bins per factor of two of the weight
+constexpr int MOST_BITS = 51;
+static_assert((MOST_BITS + 2) * STEPS <= BINS, "all live tokens have a bin");
 
 typedef unsigned long long u64;
 
@@ -38,39 +53,42 @@ __device__ __forceinline__ uint32_t sample_key(float f) {
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu, KEY_INF = 0xFF800000u;
 
-// 2^x for x <= 0: 2^round(x) times the exponential series of (x - round(x)) ln 2, |..| <= 0.347, whose 14th term is
-// below 2^-57 of the sum
+// 2^x for -1 <= x <= 51: 2^n times the exponential series of f ln 2, n the integer next to x, f = x - n; its 14th
+// term is below 2^-57 of the sum.  Adding 1.5 2^52 leaves n in the low bits: additions go at four times the
+// rate of conversions and roundings in 64 bits.
 __device__ __forceinline__ double exp2_series(double x) {
-    const double n = __builtin_rint(x), f = (x - n) * 0.69314718055994530942;
-    double p = 1.0 / 6227020800.0;
-    p = __builtin_fma(p, f, 1.0 / 479001600.0);
-    p = __builtin_fma(p, f, 1.0 / 39916800.0);
-    p = __builtin_fma(p, f, 1.0 / 3628800.0);
-    p = __builtin_fma(p, f, 1.0 / 362880.0);
-    p = __builtin_fma(p, f, 1.0 / 40320.0);
-    p = __builtin_fma(p, f, 1.0 / 5040.0);
-    p = __builtin_fma(p, f, 1.0 / 720.0);
-    p = __builtin_fma(p, f, 1.0 / 120.0);
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+    constexpr double L1 = 0.69314718055994530942, L2 = L1 * L1, L4 = L2 * L2, L8 = L4 * L4;
+    constexpr double HALVES = 6755399441055744.0;
+    const double r = x + HALVES, f = x - (r - HALVES);
+    double p = L8 * L4 * L1 / 6227020800.0;
+    p = __builtin_fma(p, f, L8 * L4 / 479001600.0);
+    p = __builtin_fma(p, f, L8 * L2 * L1 / 39916800.0);
+    p = __builtin_fma(p, f, L8 * L2 / 3628800.0);
+    p = __builtin_fma(p, f, L8 * L1 / 362880.0);
+    p = __builtin_fma(p, f, L8 / 40320.0);
+    p = __builtin_fma(p, f, L4 * L2 * L1 / 5040.0);
+    p = __builtin_fma(p, f, L4 * L2 / 720.0);
+    p = __builtin_fma(p, f, L4 * L1 / 120.0);
+    p = __builtin_fma(p, f, L4 / 24.0);
+    p = __builtin_fma(p, f, L2 * L1 / 6.0);
+    p = __builtin_fma(p, f, L2 / 2.0);
+    p = __builtin_fma(p, f, L1);
     p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n);
+    const u64 b = (u64)__double_as_longlong(p);
+    return __longlong_as_double((long long)(b + ((u64)(uint32_t)__double_as_longlong(r) << 52)));
 }
 
 // What a row's block knows of it.
 struct SampleRow {
     uint32_t top;                      // key of the largest value
-    double m, c;                       // that value, log2(e) / T
-    int bits;
-    // t of a key that is not above top
-    __device__ __forceinline__ double t(uint32_t key) const { return key == top ? 0.0 : ((double)key_value(key) - m) * c; }
-    __device__ __forceinline__ u64 weight(uint32_t key) const {
-        const double w = exp2_series(t(key) + bits);               // at most 2^51
-        return (u64)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;   // + 2^52: rounded to an integer
+    double m, c;                       // that value, log2(e) / T; where it is infinite, 0 and 0: its like have t = 0
+    double bits;
+    __device__ __forceinline__ double t(float v) const { return ((double)fminf(v, 3.402823466e38f) - m) * c; }
+    __device__ __forceinline__ u64 weight(double t) const {
+        const double w = exp2_series(t + bits);                        // at most 2^51
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to an integer
     }
-    __device__ __forceinline__ int bin(uint32_t key) const { return min((int)(t(key) * -STEPS), BINS - 1); }
+    __device__ __forceinline__ int bin(double t) const { return min((int)(t * -STEPS), BINS - 1); }
 };
 
 // ceil(p z) (p in (0, 1), UP) or floor(p z) of a float p in [0, 1) and an integer z, exactly
@@ -95,92 +113,192 @@ __device__ __forceinline__ u64 part_of(float p, u64 z) {
     return q + (UP && rest ? 1 : 0);
 }
 
-// f(key, index) for every token of a row
-template <int DT, bool VEC, class F>
-__device__ __forceinline__ void each_token(const void* x, int64_t row, int n, F&& f) {
-    constexpr int EPC = DT == MVLM_F32 ? 4 : 8;
-    const int tid = (int)threadIdx.x;
-    int from = 0;
-    if constexpr (VEC) {
-        const int chunks = n / EPC;
-        const u32x4* p = reinterpret_cast<const u32x4*>((const char*)x + row * (DT == MVLM_F32 ? 4 : 2));
-        for (int base = tid; base < chunks; base += SAMPLE_THREADS * SAMPLE_BATCH) {
+// A row's tokens as a thread sees them: chunks of 16 bytes (EPC tokens), THREADS apart, -inf behind the row's end.
+template <int DT, bool VEC>
+struct RowTokens {
+    static constexpr int EPC = DT == MVLM_F32 ? 4 : 8, CHUNKS = HOLD / 4;
+    const void* x;
+    int64_t row;
+    int n, chunks;                     // tokens, chunks (the last may be short)
+    u32x4 held[CHUNKS];
+
+    __device__ __forceinline__ u32x4 load(int c) const {
+        if (VEC && (c + 1) * EPC <= n)
+            return *reinterpret_cast<const u32x4*>((const char*)x + (row + (int64_t)c * EPC) * (DT == MVLM_F32 ? 4 : 2));
+        constexpr uint32_t NONE = DT == MVLM_F32 ? 0xFF800000u : DT == MVLM_F16 ? 0xFC00u : 0xFF80u;
+        uint32_t t[EPC];
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) {
+            const int64_t i = row + (int64_t)c * EPC + e;
+            t[e] = c * EPC + e >= n ? NONE : DT == MVLM_F32 ? ((const uint32_t*)x)[i] : ((const uint16_t*)x)[i];
+        }
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = EPC == 4 ? t[e] : t[(2 * e) % EPC] | t[(2 * e + 1) % EPC] << 16;
+        return w;
+    }
+    __device__ __forceinline__ static float value(uint32_t w, int e) {
+        if constexpr (DT == MVLM_F32) return __uint_as_float(w);
+        else if constexpr (DT == MVLM_BF16) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+        else return f16_bits_to_f32((uint16_t)(e & 1 ? w >> 16 : w));
+    }
+    __device__ __forceinline__ float at(int i) const { return load_as_f32(x, row + i, DT); }
+    // f(value) for the held tokens
+    template <class F>
+    __device__ __forceinline__ void each_held(F&& f) const {
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            if (u * SAMPLE_THREADS >= chunks) break;
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) f(value(held[u][e * 4 / EPC], e));
+        }
+    }
+    // index of the nth of them
+    __device__ __forceinline__ int held_index(int nth) const {
+        return ((int)threadIdx.x + nth / EPC * SAMPLE_THREADS) * EPC + nth % EPC;
+    }
+    // f(value, index) for the tokens of chunks [first, chunks)
+    template <class F>
+    __device__ __forceinline__ void each_from(int first, F&& f) const {
+        for (int base = (int)threadIdx.x + first; base < chunks; base += SAMPLE_THREADS * SAMPLE_BATCH) {
             u32x4 w[SAMPLE_BATCH];
 #pragma unroll
-            for (int u = 0; u < SAMPLE_BATCH; ++u) w[u] = p[min(base + u * SAMPLE_THREADS, chunks - 1)];
+            for (int u = 0; u < SAMPLE_BATCH; ++u) w[u] = load(min(base + u * SAMPLE_THREADS, chunks - 1));
 #pragma unroll
-            for (int u = 0; u < SAMPLE_BATCH; ++u) {
-                const int c = base + u * SAMPLE_THREADS;
-                if (c >= chunks) break;
+            for (int u = 0; u < SAMPLE_BATCH; ++u)
+                if (base + u * SAMPLE_THREADS < chunks)
 #pragma unroll
-                for (int e = 0; e < EPC; ++e) {
-                    float v;
-                    if constexpr (DT == MVLM_F32) v = __uint_as_float(w[u][e]);
-                    else {
-                        const uint16_t h = (uint16_t)(w[u][e >> 1] >> (16 * (e & 1)));
-                        v = DT == MVLM_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
-                    }
-                    f(sample_key(v), c * EPC + e);
-                }
-            }
+                    for (int e = 0; e < EPC; ++e) f(value(w[u][e * 4 / EPC], e), (base + u * SAMPLE_THREADS) * EPC + e);
         }
-        from = chunks * EPC;
     }
-    for (int i = from + tid; i < n; i += SAMPLE_THREADS) f(sample_key(load_as_f32(x, row + i, DT)), i);
-}
-
-struct SampleLds {
-    u64 sums[BINS];                    // weights of the bins, then running sums
-    uint32_t counts[BINS];             // tokens of the bins, then running counts
-    union {
-        struct {
-            u64 list[LIST];            // ~key, index
-            u64 weights[LIST];         // running sums of their weights
-        };
-        struct {
-            u64 part_sums[BINS];       // of a range of keys
-            uint32_t part_counts[BINS];
-        };
-    };
-    u64 wave_sums[SAMPLE_THREADS / 64];
-    uint32_t wave_counts[SAMPLE_THREADS / 64];
-    uint32_t listed, word;
-    u64 found[4];
+    template <class F>
+    __device__ __forceinline__ void each_other(F&& f) const { each_from(CHUNKS * SAMPLE_THREADS, f); }
+    template <class F>
+    __device__ __forceinline__ void each(F&& f) const { each_from(0, f); }
+    __device__ __forceinline__ void hold() {
+        const uint32_t none = DT == MVLM_F32 ? 0xFF800000u : DT == MVLM_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            const int c = (int)threadIdx.x + u * SAMPLE_THREADS;
+            held[u] = c < chunks ? load(c) : u32x4{none, none, none, none};
+        }
+    }
 };
 
-// Running sums of sums[] and counts[], size of them a multiple of SAMPLE_THREADS or below it, by all threads.
-template <bool COUNTS>
-__device__ __forceinline__ void running(u64* sums, uint32_t* counts, int size, SampleLds& s) {
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int each = (size + SAMPLE_THREADS - 1) / SAMPLE_THREADS, from = min(tid * each, size), to = min(from + each, size);
-    u64 w = 0;
-    uint32_t c = 0;
-    for (int i = from; i < to; ++i) {
-        w += sums[i];
-        if (COUNTS) c += counts[i];
+// The least key of [lo, hi] for which f holds; f holds for hi and from some key on.  By a wave.
+template <class F>
+__device__ __forceinline__ uint32_t least_where(uint32_t lo, uint32_t hi, F&& f) {
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
+        const uint32_t key = hi - lo >= lane * step ? lo + lane * step : hi;
+        const uint64_t holds = __builtin_amdgcn_ballot_w64(f(key));
+        // lane l's key is lo + l step or hi; the first that holds bounds the least from above, the one before from below
+        const uint32_t l = holds ? (uint32_t)__builtin_ctzll(holds) : 64u;
+        const uint32_t above = l < 64 && hi - lo >= l * step ? lo + l * step : hi;
+        if (l) lo += (l - 1) * step + 1;
+        hi = above;
     }
-    u64 iw = w;
-    uint32_t ic = c;
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 a = __shfl_up(iw, off, 64);
-        const uint32_t b = __shfl_up(ic, off, 64);
-        if (lane >= off) iw += a, ic += b;
-    }
+    return hi;
+}
+
+// A bin or a list entry of each thread: what lies before it, and its own.
+struct Share {
+    u64 before, own;
+    uint32_t above, count;
+};
+struct SamplePlace {
+    u64 before, own;
+    uint32_t above, count;
+    int index;
+};
+
+struct SampleLds {
+    u64 candidates[CANDIDATES];        // ~key, index
+    u64 list[LIST];                    // the same
+    u64 sums[BINS], part_sums[BINS];   // weights of the bins, and of those of a range of keys
+    uint32_t counts[BINS], part_counts[BINS];
+    u64 wave_sums[SAMPLE_THREADS / 64];
+    uint32_t wave_counts[SAMPLE_THREADS / 64];
+    float wave_values[SAMPLE_THREADS / 64];
+    SamplePlace place[2];
+    uint32_t listed, word;
+};
+
+// v plus the values of the lanes before
+__device__ __forceinline__ u64 scan_wave(u64 v) {
+    auto step = [&](auto ctrl, auto rows, auto bound) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, decltype(bound)::value);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xF, decltype(bound)::value);
+        v += (u64)hi << 32 | lo;
+    };
+    using all = std::integral_constant<int, 0xF>;
+    step(std::integral_constant<int, 0x111>{}, all{}, std::true_type{});   // row_shr:1
+    step(std::integral_constant<int, 0x112>{}, all{}, std::true_type{});   // row_shr:2
+    step(std::integral_constant<int, 0x114>{}, all{}, std::true_type{});   // row_shr:4
+    step(std::integral_constant<int, 0x118>{}, all{}, std::true_type{});   // row_shr:8
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{}, std::false_type{});   // row_bcast:15 into rows 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{}, std::false_type{});   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// The shares of threads that own w and c, and the sums of all; by all threads, which have synchronised since they
+// read what an earlier call left.
+__device__ __forceinline__ Share share_out(u64 w, uint32_t c, SampleLds& s, u64* sum, uint32_t* count) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const u64 iw = scan_wave(w);
+    const uint32_t ic = (uint32_t)scan_wave((u64)c);
     if (lane == 63) s.wave_sums[wave] = iw, s.wave_counts[wave] = ic;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) iw += s.wave_sums[i], ic += s.wave_counts[i];
-    iw -= w;
-    ic -= c;
-    for (int i = from; i < to; ++i) {
-        iw += sums[i];
-        sums[i] = iw;
-        if (COUNTS) ic += counts[i], counts[i] = ic;
+    Share m{iw - w, w, ic - c, c};
+    u64 sw = 0;
+    uint32_t sc = 0;
+#pragma unroll
+    for (int i = 0; i < SAMPLE_THREADS / 64; ++i) {
+        const u64 a = s.wave_sums[i];
+        const uint32_t b = s.wave_counts[i];
+        m.before += i < wave ? a : 0;
+        m.above += i < wave ? b : 0;
+        sw += a;
+        sc += b;
     }
+    *sum = sw;
+    *count = sc;
+    return m;
+}
+
+// v over the lanes of a wave with f, in all lanes
+template <class F>
+__device__ __forceinline__ float over_wave(float v, F&& f) {
+    auto move = [](float x, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    v = f(v, move(v, std::integral_constant<int, 0xB1>{}));        // quad_perm [1, 0, 3, 2]
+    v = f(v, move(v, std::integral_constant<int, 0x4E>{}));        // quad_perm [2, 3, 0, 1]
+    v = f(v, move(v, std::integral_constant<int, 0x141>{}));       // row_half_mirror
+    v = f(v, move(v, std::integral_constant<int, 0x140>{}));       // row_mirror: 16 lanes agree
+    v = f(v, __shfl_xor(v, 16, 64));
+    return f(v, __shfl_xor(v, 32, 64));
+}
+
+// list[0 .. size) in ascending order (entries differ), by all threads; size <= RANKED.  Each entry's place is the
+// number of entries below it; THREADS / RANKED threads count for one.
+__device__ __forceinline__ void rank_list(u64* list, int size) {
+    constexpr int PARTS = SAMPLE_THREADS / RANKED;
+    const int i = (int)threadIdx.x / PARTS, part = (int)threadIdx.x % PARTS;
+    const u64 own = list[max(min(i, size - 1), 0)];
+    int below = 0;
+    for (int j = part; j < size; j += PARTS) below += list[j] < own;
+    below += __shfl_xor(below, 1, 64);
+    below += __shfl_xor(below, 2, 64);
+    static_assert(PARTS == 4, "two exchanges");
+    __syncthreads();
+    if (part == 0 && i < size) list[below] = own;
     __syncthreads();
 }
 
-// list[0 .. size) in ascending order, by all threads; size <= LIST
+// the same for size <= LIST, by exchanges
 __device__ __forceinline__ void sort_list(u64* list, int size) {
+    if (size <= RANKED) return rank_list(list, size);
     int padded = 2;
     while (padded < size) padded *= 2;
     for (int i = size + (int)threadIdx.x; i < padded; i += SAMPLE_THREADS) list[i] = ~0ull;
@@ -196,234 +314,332 @@ __device__ __forceinline__ void sort_list(u64* list, int size) {
         }
 }
 
-// Where a search ends: the place's token and the sum of weights up to and with it.
-struct SamplePlace {
-    uint32_t key;
-    int token;                         // -1: not looked for
-    u64 sum;
-};
-
 template <int DT, bool VEC>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs a) {
     __shared__ SampleLds s;
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x, n = a.n;
-    const int64_t base = (int64_t)row * a.ld;
-
-    // the largest value, and its first token
-    uint32_t best = 0;
-    int at = n;
-    each_token<DT, VEC>(a.x, base, n, [&](uint32_t key, int i) {
-        if (key > best) best = key, at = i;
-    });
-    for (int off = 32; off; off >>= 1) {
-        const uint32_t k = (uint32_t)__shfl_xor((int)best, off, 64);
-        const int i = __shfl_xor(at, off, 64);
-        if (k > best || (k == best && i < at)) best = k, at = i;
-    }
-    if ((tid & 63) == 0) s.wave_sums[tid >> 6] = (u64)best << 32 | (uint32_t)~at;
-    __syncthreads();
-    u64 first = 0;
-    for (int w = 0; w < SAMPLE_THREADS / 64; ++w) first = max(first, s.wave_sums[w]);
-    __syncthreads();
-    if (tid == 0) s.word = 0;
-    SampleRow r;
-    r.top = (uint32_t)(first >> 32);
+    RowTokens<DT, VEC> tokens;
+    tokens.x = a.x;
+    tokens.row = (int64_t)row * a.ld;
+    tokens.n = n;
+    tokens.chunks = (n + tokens.EPC - 1) / tokens.EPC;
+    tokens.hold();
     const float T = a.temperature ? a.temperature[row] : 1.0f;
-    if (r.top == KEY_NEG_INF || !(T > 0.0f)) {
-        if (tid == 0) a.out[row] = r.top == KEY_NEG_INF ? 0 : ~(int)(uint32_t)first;
-        return;
-    }
-    r.m = (double)key_value(r.top);
-    r.c = 1.4426950408889634074 / (double)T;
-    r.bits = a.bits;
     float min_p = a.min_p ? a.min_p[row] : 0.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
     const int top_k = a.top_k ? a.top_k[row] : 0;
     if (!(u > 0.0f)) u = 0.0f;
+    if (tid == 0) s.word = (uint32_t)n, s.listed = 0, s.place[0] = s.place[1] = SamplePlace{};
 
-    // the least key with t >= t_least; t does not fall as keys rise
-    auto least_key = [&](double t_least) {
-        uint32_t lo = KEY_NEG_INF + 1, hi = r.top;             // hi has it
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (r.t(mid) >= t_least) hi = mid;
-            else lo = mid + 1;
-        }
-        return hi;
+    // the largest value over all threads
+    auto largest = [&](float v) {
+        v = over_wave(v, [](float x, float y) { return fmaxf(x, y); });
+        __syncthreads();
+        if ((tid & 63) == 0) s.wave_values[tid >> 6] = v;
+        __syncthreads();
+        v = s.wave_values[0];
+#pragma unroll
+        for (int w = 1; w < SAMPLE_THREADS / 64; ++w) v = fmaxf(v, s.wave_values[w]);
+        return v;
     };
-    double t_least = -(double)(a.bits + 1);
+    const auto as_number = [](float v) { return v == v ? v : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x7F800000u); };
+    float own = -INFINITY;                                     // the largest of those that this thread holds
+    bool odd = false;
+    tokens.each_held([&](float v) {
+        own = fmaxf(own, v);                                   // a NaN is not taken
+        odd |= v != v;
+    });
+    if (odd) tokens.each_held([&](float v) { own = fmaxf(own, as_number(v)); });
+    float top = largest(own);
+    const bool more = tokens.chunks > tokens.CHUNKS * SAMPLE_THREADS;
+
+    if (!(T > 0.0f)) {                                         // the first token of the largest value
+        if (more) {
+            float v = own;
+            tokens.each_other([&](float x, int) { v = fmaxf(v, as_number(x)); });
+            top = largest(v);
+        }
+        int at = n;
+        tokens.each([&](float x, int i) {
+            if (as_number(x) == top) at = min(at, i);
+        });
+        for (int off = 32; off; off >>= 1) at = min(at, __shfl_xor(at, off, 64));
+        if ((tid & 63) == 0) atomicMin(&s.word, (uint32_t)at);
+        __syncthreads();
+        if (tid == 0) a.out[row] = top == -INFINITY ? 0 : (int)s.word;
+        return;
+    }
+
+    SampleRow r;
+    const double c = 1.4426950408889634074 / (double)T;
+    r.bits = (double)a.bits;
+    auto with_top = [&] {
+        r.top = sample_key(top);
+        r.m = top < INFINITY ? (double)top : 0.0;
+        r.c = top < INFINITY ? c : 0.0;
+    };
+    with_top();
+    double t_least = -(r.bits + 1.0);
     if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
-    const uint32_t live = r.top == KEY_INF ? KEY_INF : least_key(t_least);
-
-    // tokens by t; their weights too unless few may be kept
-    const bool few = top_k > 0 || min_p > 0.0f;
-    auto count_bins = [&](bool weights) __attribute__((always_inline)) {
-        for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.counts[i] = 0, s.sums[i] = 0;
-        __syncthreads();
-        each_token<DT, VEC>(a.x, base, n, [&](uint32_t key, int) {
-            if (key < live) return;
-            const int b = r.bin(key);
-            atomicAdd(&s.counts[b], 1u);
-            if (weights) atomicAdd(&s.sums[b], r.weight(key));
-        });
-        __syncthreads();
-        running<true>(s.sums, s.counts, BINS, s);
+    // a finite value that is below those of all tokens with t >= t_to, by a little
+    auto value_below = [&](double t_to) {
+        const uint32_t k = sample_key((float)(r.m + t_to / c));
+        return key_value(max(k, KEY_NEG_INF + 9) - 8);
     };
-    count_bins(!few);
-    const uint32_t all = s.counts[BINS - 1];
-    const uint32_t k = top_k > 0 && (uint32_t)top_k < all ? (uint32_t)top_k : all;   // tokens kept by count
-
-    // tokens with keys in [lo, hi] into the list, sorted, with running sums of their weights
-    auto make_list = [&](uint32_t lo, uint32_t hi) __attribute__((always_inline)) {
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-        each_token<DT, VEC>(a.x, base, n, [&](uint32_t key, int i) {
-            if (key < lo || key > hi) return;
-            const uint32_t to = atomicAdd(&s.listed, 1u);
-            if (to < LIST) s.list[to] = (u64)~key << 32 | (uint32_t)i;
+    // The candidates: from `least` on.  `closed`: no other token can be kept.
+    const bool by_rank = top_k > 0 && top_k <= RANKS;
+    const bool closed = by_rank || min_p > 0.0f;
+    float least = -3.402823466e38f;
+    if (top > -INFINITY && top < INFINITY) {
+        if (by_rank || !closed) {                              // the step of the k-th of the threads' largest
+            if (tid < RANK_BINS) s.counts[tid] = 0;
+            __syncthreads();
+            if (own > -INFINITY) atomicAdd(&s.counts[(int)fmin(r.t(own) * -RANK_STEPS, RANK_BINS - 1.0)], 1u);
+            __syncthreads();
+            const uint32_t kth = by_rank ? top_k : RANKS;
+            uint32_t n4[RANK_BINS / 64], run = 0;
+#pragma unroll
+            for (int i = 0; i < RANK_BINS / 64; ++i) run += n4[i] = s.counts[(tid & 63) * (RANK_BINS / 64) + i];
+            const uint32_t upto = (uint32_t)scan_wave((u64)run);
+            const uint64_t reached = __builtin_amdgcn_ballot_w64(upto >= kth);
+            if (reached) {
+                const int l = __builtin_ctzll(reached);
+                uint32_t sum = (uint32_t)__builtin_amdgcn_readlane((int)(upto - run), l);
+                int bin = l * (RANK_BINS / 64) - 1;
+#pragma unroll
+                for (int i = 0; i < RANK_BINS / 64; ++i) {
+                    const uint32_t v = (uint32_t)__builtin_amdgcn_readlane((int)n4[i], l);
+                    if (sum < kth) sum += v, ++bin;
+                }
+                if (bin < RANK_BINS - 1) least = value_below(-(bin + 1.0) / RANK_STEPS);
+            }
+        }
+        if (min_p > 0.0f) least = fmaxf(least, value_below(t_least));
+    }
+    // into a list in LDS with room for `room`
+    auto to_list = [&](u64* list, uint32_t room, uint32_t key, int i) {
+        if (*(volatile uint32_t*)&s.listed > room) return;     // nobody will look at it
+        const uint32_t to = atomicAdd(&s.listed, 1u);
+        if (to < room) list[to] = (u64)~key << 32 | (uint32_t)i;
+    };
+    if (more) {
+        float v = own;
+        tokens.each_other([&](float x, int i) {
+            v = fmaxf(v, as_number(x));
+            if (x >= least) to_list(s.candidates, CANDIDATES, sample_key(x), i);
         });
+        top = largest(v);
+        with_top();
+        if (min_p > 0.0f && top < INFINITY) least = fmaxf(least, value_below(t_least));
+    }
+    if (top == -INFINITY) {
+        if (tid == 0) a.out[row] = 0;
+        return;
+    }
+    int candidates;
+    bool compact;                                              // all of them are in LDS
+    {
+        // few of the held ones are candidates: they are marked, then read again, four at a time
+        u64 marks[2] = {0, 0};
+        int nth = 0;
+        tokens.each_held([&](float v) {
+            if (v >= least) marks[nth / 52] |= 1ull << nth % 52;
+            ++nth;
+        });
+        const uint32_t marked = (uint32_t)(__popcll(marks[0]) + __popcll(marks[1]));
+        u64 sum;
+        uint32_t all;
         __syncthreads();
-        const int size = min((int)s.listed, LIST);
+        const uint32_t others = s.listed;
+        const Share mine = share_out(0, marked, s, &sum, &all);
+        compact = others + all <= CANDIDATES && top < INFINITY;
+        candidates = (int)(others + all);
+        if (compact) {
+            uint32_t to = others + mine.above;
+            while (marks[0] | marks[1]) {
+                int i[4];
+                float v[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int half = marks[0] ? 0 : 1;
+                    const u64 left = marks[half];
+                    i[q] = left ? tokens.held_index(52 * half + __builtin_ctzll(left)) : -1;
+                    if (half) marks[1] = left & (left - 1);
+                    else marks[0] = left & (left - 1);
+                    v[q] = tokens.at(max(i[q], 0));
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i[q] >= 0) s.candidates[to++] = (u64)~sample_key(v[q]) << 32 | (uint32_t)i[q];
+            }
+        }
+        __syncthreads();
+    }
+
+    int turn = 0;
+    // what the thread with `mine` knows, to all threads
+    auto announce = [&](bool mine, const Share& m) {
+        if (mine) s.place[turn] = SamplePlace{m.before, m.own, m.above, m.count, tid};
+        __syncthreads();
+        const SamplePlace p = s.place[turn];
+        turn ^= 1;                                             // the next one is written while this is still read
+        return p;
+    };
+    // where the running count or sum reaches need
+    auto reaches = [&](const Share& m, bool by_count, u64 need) {
+        const u64 before = by_count ? (u64)m.above : m.before;
+        return announce(before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
+    };
+    // the list sorted, an entry to each thread
+    auto share_list = [&](int size) __attribute__((always_inline)) {
         sort_list(s.list, size);
-        for (int i = tid; i < size; i += SAMPLE_THREADS) s.weights[i] = r.weight(~(uint32_t)(s.list[i] >> 32));
-        __syncthreads();
-        running<false>(s.weights, nullptr, size, s);
-        return size;
+        u64 sum;
+        uint32_t count;
+        const double t = tid < size ? r.t(key_value(~(uint32_t)(s.list[tid] >> 32))) : -INFINITY;
+        return share_out(t >= t_least ? r.weight(t) : 0, tid < size ? 1u : 0u, s, &sum, &count);
     };
-    // the first entry of the list with entry + 1 >= need (by count) or running sum >= need
-    auto in_list = [&](int size, bool by_count, u64 need) {
-        if (by_count) return (int)need - 1;
-        for (int i = tid; i < size; i += SAMPLE_THREADS)
-            if (s.weights[i] >= need && (i == 0 || s.weights[i - 1] < need)) s.word = (uint32_t)i;
+    const auto top_p_need = [&](u64 kept) { return top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : (u64)1; };
+    const auto token_need = [&](u64 kept) { return u < 1.0f ? part_of<false>(u, kept) + 1 : kept; };
+    if (compact && closed && candidates <= LIST) {
+        const int size = candidates;
+        if (tid < size) s.list[tid] = s.candidates[tid];
         __syncthreads();
-        const int i = max(min((int)s.word, size - 1), 0);
-        __syncthreads();
-        return i;
+        const Share m = share_list(size);
+        const int live = __syncthreads_count(tid < size && r.t(key_value(~(uint32_t)(s.list[tid] >> 32))) >= t_least);
+        SamplePlace p = announce(tid == (top_k > 0 ? min(top_k, live) : live) - 1, m);
+        if (top_p < 1.0f) p = reaches(m, false, top_p_need(p.before + p.own));
+        p = reaches(m, false, token_need(p.before + p.own));
+        if (tid == 0) a.out[row] = (int)(uint32_t)s.list[p.index];
+        return;
+    }
+
+    const uint32_t live = r.top == KEY_INF ? KEY_INF : least_where(KEY_NEG_INF + 1, r.top, [&](uint32_t key) { return r.t(key_value(key)) >= t_least; });
+    const float live_value = key_value(live);
+    // f(t, key, index) for the live tokens of the row (a NaN passes the first test)
+    auto each_live = [&](auto&& f) __attribute__((always_inline)) {
+        tokens.each([&](float v, int i) {
+            if (v < live_value) return;
+            const uint32_t key = sample_key(v);
+            if (key >= live) f(r.t(v), key, i);
+        });
     };
-    // the bin (of running sums and counts) in which the place lies
-    auto in_bins = [&](const u64* sums, const uint32_t* counts, bool by_count, u64 need) {
-        for (int i = tid; i < BINS; i += SAMPLE_THREADS) {
-            const u64 end = by_count ? counts[i] : sums[i], begin = i == 0 ? 0 : by_count ? counts[i - 1] : sums[i - 1];
-            if (end >= need && begin < need) s.word = (uint32_t)i;
-        }
+    // of all live tokens, where the candidates may not be all that is kept
+    u64 sum_all = 0;
+    uint32_t count_all = 0;
+    if (compact && !closed) {
+        u64 w = 0;
+        uint32_t k = 0;
+        tokens.each([&](float v, int) {                        // the largest is finite: there is no NaN but below it
+            if (v >= live_value) w += r.weight(r.t(v)), ++k;
+        });
+        share_out(w, k, s, &sum_all, &count_all);
         __syncthreads();
-        const int i = min((int)s.word, BINS - 1);
-        __syncthreads();
-        return i;
-    };
-    // the keys of a bin of t
-    auto keys_of = [&](int bin, uint32_t* lo, uint32_t* hi) {
-        uint32_t l = live, h = r.top;                          // the least key with a bin <= this one
-        while (l < h) {
-            const uint32_t mid = l + (h - l) / 2;
-            if (r.bin(mid) <= bin) h = mid;
-            else l = mid + 1;
+    }
+    // the same for the candidates, or the row
+    auto each = [&](bool of_row, auto&& f) __attribute__((always_inline)) {
+        if (of_row) return each_live(f);
+        for (int i = tid; i < candidates; i += SAMPLE_THREADS) {
+            const uint32_t key = ~(uint32_t)(s.candidates[i] >> 32);
+            if (key >= live) f(r.t(key_value(key)), key, (int)(uint32_t)s.candidates[i]);
         }
-        *lo = h;
-        l = h, h = r.top;                                      // the largest with a bin >= this one
-        while (l < h) {
-            const uint32_t mid = l + (h - l + 1) / 2;
-            if (r.bin(mid) >= bin) l = mid;
-            else h = mid - 1;
-        }
-        *hi = l;
     };
 
-    if (few) {
-        // all that the count lets through, if the list has room for it
-        const int last = in_bins(s.sums, s.counts, true, k);
-        if (s.counts[last] <= LIST) {
-            uint32_t lo, hi;
-            keys_of(last, &lo, &hi);
-            const int size = make_list(lo, r.top);
-            u64 kept = s.weights[k - 1];
-            if (top_p < 1.0f) kept = s.weights[in_list(size, false, top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : 1)];
-            const u64 need = u < 1.0f ? part_of<false>(u, kept) + 1 : kept;
-            const int i = in_list(size, false, need);
-            if (tid == 0) a.out[row] = (int)(uint32_t)s.list[i];
+    // Twice at most: among the candidates, then, where they do not hold a place that is looked for, in the row.
+    for (int of_row = compact ? 0 : 1; of_row < 2; ++of_row) {
+        s.counts[tid] = 0, s.sums[tid] = 0;
+        __syncthreads();
+        each(of_row, [&](double t, uint32_t, int) {
+            const int b = r.bin(t);
+            atomicAdd(&s.counts[b], 1u);
+            atomicAdd(&s.sums[b], r.weight(t));
+        });
+        __syncthreads();
+        u64 sum_here;
+        uint32_t here;
+        const Share bins = share_out(s.sums[tid], s.counts[tid], s, &sum_here, &here);
+        const uint32_t all = of_row || closed ? here : count_all;
+        const uint32_t k = top_k > 0 && (uint32_t)top_k < all ? (uint32_t)top_k : all;   // tokens kept by count
+        u64 kept = of_row || closed ? sum_here : sum_all;
+        int token = 0;
+        bool found = false;
+        for (int step = 0; step < 3; ++step) {                 // top-k, top-p, the token
+            if ((step == 0 && k == all) || (step == 1 && !(top_p < 1.0f))) continue;
+            const bool by_count = step == 0;
+            const u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
+            if (need > (by_count ? here : sum_here)) break;    // not among the candidates
+            found = step == 2;
+            SamplePlace p = reaches(bins, by_count, need);
+            u64 before = p.before;                             // of the tokens above the range
+            uint32_t above = p.above, inside = p.count;
+            // the range's keys: from the least with a bin <= this one to the one before the least with a bin below it
+            uint32_t lo = least_where(live, r.top, [&](uint32_t key) { return r.bin(r.t(key_value(key))) <= p.index; });
+            uint32_t hi = p.index == 0 ? r.top : least_where(lo, r.top, [&](uint32_t key) { return r.bin(r.t(key_value(key))) < p.index; }) - 1;
+            while (inside > LIST && lo < hi) {
+                const uint32_t span = hi - lo;                 // keys less one
+                int shift = 0;
+                while ((span >> shift) >= (uint32_t)BINS) ++shift;
+                s.part_counts[tid] = 0, s.part_sums[tid] = 0;
+                __syncthreads();
+                each(of_row, [&](double t, uint32_t key, int) {
+                    if (key < lo || key > hi) return;
+                    const uint32_t b = (hi - key) >> shift;
+                    atomicAdd(&s.part_counts[b], 1u);
+                    atomicAdd(&s.part_sums[b], r.weight(t));
+                });
+                __syncthreads();
+                u64 sum;
+                uint32_t count;
+                const Share parts = share_out(s.part_sums[tid], s.part_counts[tid], s, &sum, &count);
+                p = reaches(parts, by_count, need - (by_count ? (u64)above : before));
+                inside = p.count;
+                before += p.before;
+                above += p.above;
+                hi -= (uint32_t)p.index << shift;
+                lo = max(lo, hi - ((1u << shift) - 1u));
+            }
+            if (inside <= LIST) {
+                if (tid == 0) s.listed = 0;
+                __syncthreads();
+                each(of_row, [&](double, uint32_t key, int i) {
+                    if (key >= lo && key <= hi) to_list(s.list, LIST, key, i);
+                });
+                __syncthreads();
+                const Share m = share_list(min((int)s.listed, LIST));
+                p = reaches(m, by_count, need - (by_count ? (u64)above : before));
+                token = (int)(uint32_t)s.list[p.index];
+                kept = before + p.before + p.own;
+                __syncthreads();
+                continue;
+            }
+            // equal values: the rank among them, and its index where the token is asked for
+            const u64 w = r.weight(r.t(key_value(lo)));
+            const u64 rank = by_count ? need - above : (need - before + w - 1) / w;
+            kept = before + rank * w;
+            if (step < 2) continue;
+            // THREADS tokens at a time, in their order
+            uint32_t seen = 0;
+            for (int from = 0; from < n; from += SAMPLE_THREADS) {
+                const int i = from + tid;
+                const bool same = i < n && sample_key(tokens.at(i)) == lo;
+                const uint64_t mask = __builtin_amdgcn_ballot_w64(same);
+                if ((tid & 63) == 0) s.wave_counts[tid >> 6] = (uint32_t)__popcll(mask);
+                __syncthreads();
+                uint32_t mine = seen + (uint32_t)__popcll(mask & ((1ull << (tid & 63)) - 1)), total = 0;
+                for (int w2 = 0; w2 < SAMPLE_THREADS / 64; ++w2) {
+                    if (w2 < (tid >> 6)) mine += s.wave_counts[w2];
+                    total += s.wave_counts[w2];
+                }
+                if (same && mine + 1 == rank) s.word = (uint32_t)i;
+                __syncthreads();
+                if (seen + total >= rank) break;
+                seen += total;
+            }
+            token = (int)s.word;
+        }
+        if (found) {
+            if (tid == 0) a.out[row] = token;
             return;
         }
-        count_bins(true);
     }
-
-    // the place that a search ends in; `token`: whether its index is asked for
-    auto search = [&](bool by_count, u64 need, bool token) __attribute__((always_inline)) {
-        SamplePlace place{0, -1, 0};
-        int bin = in_bins(s.sums, s.counts, by_count, need);
-        u64 before = bin ? s.sums[bin - 1] : 0;                // of the tokens above the range
-        uint32_t above = bin ? s.counts[bin - 1] : 0, inside = s.counts[bin] - above;
-        uint32_t lo, hi;
-        keys_of(bin, &lo, &hi);
-        while (inside > LIST && lo < hi) {
-            const uint32_t span = hi - lo;                     // keys less one
-            int shift = 0;
-            while ((span >> shift) >= (uint32_t)BINS) ++shift;
-            for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.part_counts[i] = 0, s.part_sums[i] = 0;
-            __syncthreads();
-            each_token<DT, VEC>(a.x, base, n, [&](uint32_t key, int) {
-                if (key < lo || key > hi) return;
-                const uint32_t b = (hi - key) >> shift;
-                atomicAdd(&s.part_counts[b], 1u);
-                atomicAdd(&s.part_sums[b], r.weight(key));
-            });
-            __syncthreads();
-            running<true>(s.part_sums, s.part_counts, BINS, s);
-            bin = in_bins(s.part_sums, s.part_counts, by_count, need - (by_count ? (u64)above : before));
-            const u64 less = bin ? s.part_sums[bin - 1] : 0;
-            const uint32_t fewer = bin ? s.part_counts[bin - 1] : 0;
-            inside = s.part_counts[bin] - fewer;
-            before += less;
-            above += fewer;
-            hi -= (uint32_t)bin << shift;
-            lo = max(lo, hi - ((1u << shift) - 1u));
-            __syncthreads();
-        }
-        if (inside <= LIST) {
-            const int size = make_list(lo, hi);
-            const int i = in_list(size, by_count, need - (by_count ? (u64)above : before));
-            place.key = ~(uint32_t)(s.list[i] >> 32);
-            place.token = (int)(uint32_t)s.list[i];
-            place.sum = before + s.weights[i];
-            __syncthreads();
-            return place;
-        }
-        // equal values: the rank among them, and its index where asked for
-        const u64 w = r.weight(lo);
-        const u64 rank = by_count ? need - above : (need - before + w - 1) / w;
-        place.key = lo;
-        place.sum = before + rank * w;
-        if (!token) return place;
-        // THREADS tokens at a time, in their order
-        uint32_t seen = 0;
-        for (int from = 0; from < n; from += SAMPLE_THREADS) {
-            const int i = from + tid;
-            const bool same = i < n && sample_key(load_as_f32(a.x, base + i, DT)) == lo;
-            const uint64_t mask = __builtin_amdgcn_ballot_w64(same);
-            if ((tid & 63) == 0) s.wave_counts[tid >> 6] = (uint32_t)__popcll(mask);
-            __syncthreads();
-            uint32_t mine = seen + (uint32_t)__popcll(mask & ((1ull << (tid & 63)) - 1)), total = 0;
-            for (int w2 = 0; w2 < SAMPLE_THREADS / 64; ++w2) {
-                if (w2 < (tid >> 6)) mine += s.wave_counts[w2];
-                total += s.wave_counts[w2];
-            }
-            if (same && mine + 1 == rank) s.word = (uint32_t)i;
-            __syncthreads();
-            if (seen + total >= rank) break;
-            seen += total;
-        }
-        place.token = (int)s.word;
-        return place;
-    };
-    u64 kept = s.sums[BINS - 1];
-    SamplePlace place{0, 0, 0};
-    for (int step = 0; step < 3; ++step) {                     // top-k, top-p, the token
-        if ((step == 0 && k == all) || (step == 1 && !(top_p < 1.0f))) continue;
-        u64 need = k;
-        if (step == 1) need = top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : 1;
-        if (step == 2) need = u < 1.0f ? part_of<false>(u, kept) + 1 : kept;
-        place = search(step == 0, need, step == 2);
-        kept = place.sum;
-    }
-    if (tid == 0) a.out[row] = place.token;
 }
 
 hipError_t launch_sample(hipStream_t s, const SampleArgs& a, int) {
