@@ -34,7 +34,7 @@ struct mvlm_device {
     void* noalloc_scratch = nullptr;
     // Words of self-resetting cross-workgroup protocols (the split token
     // pick's per-row best key and arrival count, the paged attention's counts
-    // of finished splits): zero between launches, each launch's last workgroup
+    // of finished splits, the token draw's of finished slices): zero between launches, each launch's last workgroup
     // setting its words back.  Ops of one handle run in
     // order on its stream, so they never share a word.  Allocated and zeroed
     // at the first op that needs them.
@@ -43,7 +43,8 @@ struct mvlm_device {
 constexpr int ARGMAX_SYNC_ROWS = 64;                                   // rows of split token picks
 constexpr size_t ARGMAX_SYNC_BYTES = ARGMAX_SYNC_ROWS * (8 + 4);
 constexpr int PAGED_SYNC_WORDS = 8192;                                 // splits' counters of the paged attention
-constexpr size_t SYNC_WORDS_BYTES = ARGMAX_SYNC_BYTES + PAGED_SYNC_WORDS * 4;
+constexpr int SAMPLE_SYNC_WORDS = 1024;                                // rows of token draws that are made in slices
+constexpr size_t SYNC_WORDS_BYTES = ARGMAX_SYNC_BYTES + (PAGED_SYNC_WORDS + SAMPLE_SYNC_WORDS) * 4;
 
 struct mvlm_buffer {
     mvlm_device* dev = nullptr;

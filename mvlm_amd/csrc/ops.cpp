@@ -11,6 +11,7 @@
 #include "paged_ops.h"
 #include "sample.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdlib>
@@ -635,7 +636,16 @@ int make_sample(mvlm_device* dev, const mvlm_buffer* x, int dtype, int rows, int
     a.bits = 62;
     while (((int64_t)1 << (62 - a.bits)) < n) --a.bits;
     if (a.bits > 51) a.bits = 51;
-    op->num_cus = dev->prop.multiProcessorCount;
+    a.slices = sample_slices(dtype, rows, n, std::min(dev->prop.multiProcessorCount, SAMPLE_SYNC_WORDS));
+    if (a.slices > 1) {
+        op->workspace_bytes = sample_workspace_bytes(a);
+        st = device_scratch(dev, op->workspace_bytes, &op->workspace);
+        void* sync = nullptr;
+        if (st == MVLM_OK) st = device_sync_words(dev, &sync);
+        if (st != MVLM_OK) return st;
+        sample_place(&a, op->workspace);
+        a.arrived = (uint32_t*)((char*)sync + ARGMAX_SYNC_BYTES) + PAGED_SYNC_WORDS;   // rows of them: at most a CU each
+    }
     op->kind = OP_SAMPLE;
     return MVLM_OK;
 }
@@ -816,7 +826,7 @@ hipError_t enqueue_op(hipStream_t s, const Op& op, bool with_attn = false) {
         case OP_KV_READ:
             return launch_kv_read(s, op.read);
         case OP_SAMPLE:
-            return launch_sample(s, op.sample, op.num_cus);
+            return launch_sample(s, op.sample);
         case OP_ATTN_PAGED:
             return launch_attention_paged(s, op.paged, op.num_cus);
         case OP_LOGITS:

@@ -18,7 +18,16 @@ struct SampleArgs {
     const float* min_p;
     int* out;
     int bits;                      // weights are multiples of 2^-bits
+    int slices;                    // blocks per row
+    // where slices > 1: the slices' parts, and the row's finished slices, zero between launches
+    unsigned long long* slice_sums;
+    uint32_t* slice_counts;
+    float* slice_tops;
+    uint32_t* arrived;
 };
-hipError_t launch_sample(hipStream_t s, const SampleArgs& a, int num_cus);
+int sample_slices(int dtype, int rows, int n, int num_cus);
+size_t sample_workspace_bytes(const SampleArgs& a);
+void sample_place(SampleArgs* a, void* workspace);
+hipError_t launch_sample(hipStream_t s, const SampleArgs& a);
 
 }  // namespace mvlm

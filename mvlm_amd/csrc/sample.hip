@@ -10,21 +10,23 @@
 //   picked   the first at which it reaches floor(u x the sum kept) + 1
 // so one search serves all three.  Values are compared as integers that order like them (sample_key).
 //
-// One block per row.
-//  * Few tokens can be kept, or picked: the candidates, the tokens above a bound, go into LDS.  With the k-th
-//    largest of the threads' largest values as bound, k tokens at least lie above it (some THREADS ln(THREADS /
-//    (THREADS - k)) of them where values do not depend on their places).  So top_k of up to RANKS has all that it
-//    may keep among the candidates, min_p has with the bound that it sets itself, and top_p most likely has with
-//    the RANKS-th, of which it knows once the sum of all weights is made.
-//  * Up to LIST candidates that are all that can be kept are sorted, and running sums give the answers.  More of them
-//    (or, where the candidates do not hold what is looked for, all live tokens of the row) are counted by t in steps of
-//    1/STEPS, with their weights.  A search finds its step in the running sums, sorts the step's tokens, and finds
-//    its place among them; a step of more tokens than the list holds is counted again in ranges of keys, down to
-//    equal values, of which the index decides.
+//  * Few tokens can be kept: the candidates, the tokens above a bound, go into LDS.  With the k-th largest of the
+//    threads' largest values as bound, k tokens at least lie above it (some THREADS ln(THREADS / (THREADS - k)) of
+//    them where values do not depend on their places).  So top_k of up to RANKS has all that it may keep among the
+//    candidates, and min_p has with the bound that it sets itself.
+//  * Up to LIST candidates are sorted, and running sums give the answers.  More of them (or all live tokens of the
+//    row) are counted in steps of t of 1 / STEPS, with their weights.  A search finds its step in the running sums,
+//    sorts the step's tokens, and finds its place among them; a step of more tokens than the list holds is counted
+//    again in ranges of keys, down to equal values, of which the index decides.
+// A row whose candidates are enough is made by one block.  Of the others, whose weights all count, each of `slices` blocks
+// counts a slice, in steps of v log2(e) / T, which need no m, with weights relative to the step's octave, and the
+// block that ends last adds the slices up and searches.  No block waits for another.
 // Running sums are over THREADS bins or entries, one of each thread's, which then knows whether a place is its own.
 #include "common.h"
 #include "device_math.h"
 #include "sample.h"
+
+#include <algorithm>
 
 namespace mvlm {
 
@@ -88,7 +90,10 @@ struct SampleRow {
         const double w = exp2_series(t + bits);                        // at most 2^51
         return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to an integer
     }
-    __device__ __forceinline__ int bin(double t) const { return min((int)(t * -STEPS), BINS - 1); }
+    // The bin of a value: how many steps of v log2(e) / T lie between its own and the largest's.
+    double steps = STEPS, step0;
+    __device__ __forceinline__ double step(float v, double c) const { return __builtin_floor((double)fminf(v, 3.402823466e38f) * c * steps); }
+    __device__ __forceinline__ int bin(float v) const { return (int)fmin(step0 - step(v, c), BINS - 1.0); }
 };
 
 // ceil(p z) (p in (0, 1), UP) or floor(p z) of a float p in [0, 1) and an integer z, exactly
@@ -122,9 +127,11 @@ struct RowTokens {
     int n, chunks;                     // tokens, chunks (the last may be short)
     u32x4 held[CHUNKS];
 
+    __device__ __forceinline__ u32x4 whole_chunk(int c) const {
+        return *reinterpret_cast<const u32x4*>((const char*)x + (row + (int64_t)c * EPC) * (DT == MVLM_F32 ? 4 : 2));
+    }
     __device__ __forceinline__ u32x4 load(int c) const {
-        if (VEC && (c + 1) * EPC <= n)
-            return *reinterpret_cast<const u32x4*>((const char*)x + (row + (int64_t)c * EPC) * (DT == MVLM_F32 ? 4 : 2));
+        if (VEC && (c + 1) * EPC <= n) return whole_chunk(c);
         constexpr uint32_t NONE = DT == MVLM_F32 ? 0xFF800000u : DT == MVLM_F16 ? 0xFC00u : 0xFF80u;
         uint32_t t[EPC];
 #pragma unroll
@@ -157,24 +164,55 @@ struct RowTokens {
     __device__ __forceinline__ int held_index(int nth) const {
         return ((int)threadIdx.x + nth / EPC * SAMPLE_THREADS) * EPC + nth % EPC;
     }
-    // f(value, index) for the tokens of chunks [first, chunks)
-    template <class F>
-    __device__ __forceinline__ void each_from(int first, F&& f) const {
-        for (int base = (int)threadIdx.x + first; base < chunks; base += SAMPLE_THREADS * SAMPLE_BATCH) {
+    // f(value, nth of the batch) for the tokens of chunks [first, last), end(first index of the batch, THREADS apart by
+    // chunks) after each batch, then rest(value, index) for those of a chunk that the row cuts short
+    template <class F, class E, class R>
+    __device__ __forceinline__ void each_batch(int first, int last, F&& f, E&& end, R&& rest) const {
+        const int whole = VEC ? min(last, n / EPC) : last;     // chunks read in one load, but where rows are not aligned
+        for (int base = first; base < whole; base += SAMPLE_THREADS * SAMPLE_BATCH) {
             u32x4 w[SAMPLE_BATCH];
 #pragma unroll
-            for (int u = 0; u < SAMPLE_BATCH; ++u) w[u] = load(min(base + u * SAMPLE_THREADS, chunks - 1));
+            for (int u = 0; u < SAMPLE_BATCH; ++u) {
+                const int c = min(base + (int)threadIdx.x + u * SAMPLE_THREADS, whole - 1);
+                if constexpr (VEC) w[u] = whole_chunk(c);
+                else w[u] = load(c);
+            }
 #pragma unroll
             for (int u = 0; u < SAMPLE_BATCH; ++u)
-                if (base + u * SAMPLE_THREADS < chunks)
+                if (base + (int)threadIdx.x + u * SAMPLE_THREADS < whole)
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e) f(value(w[u][e * 4 / EPC], e), u * EPC + e);
+            end((base + (int)threadIdx.x) * EPC);
+        }
+        if constexpr (VEC)
+            for (int i = max(whole, first) * EPC + (int)threadIdx.x; i < min(last * EPC, n); i += SAMPLE_THREADS) rest(at(i), i);
+    }
+    __device__ __forceinline__ static int batch_index(int from, int nth) { return from + nth / EPC * SAMPLE_THREADS * EPC + nth % EPC; }
+    // f(value, index) for the tokens of chunks [first, last)
+    template <class F>
+    __device__ __forceinline__ void each_between(int first, int last, F&& f) const {
+        const int whole = VEC ? min(last, n / EPC) : last;
+        for (int base = (int)threadIdx.x + first; base < whole; base += SAMPLE_THREADS * SAMPLE_BATCH) {
+            u32x4 w[SAMPLE_BATCH];
+#pragma unroll
+            for (int u = 0; u < SAMPLE_BATCH; ++u) {
+                const int c = min(base + u * SAMPLE_THREADS, whole - 1);
+                if constexpr (VEC) w[u] = whole_chunk(c);
+                else w[u] = load(c);
+            }
+#pragma unroll
+            for (int u = 0; u < SAMPLE_BATCH; ++u)
+                if (base + u * SAMPLE_THREADS < whole)
 #pragma unroll
                     for (int e = 0; e < EPC; ++e) f(value(w[u][e * 4 / EPC], e), (base + u * SAMPLE_THREADS) * EPC + e);
         }
+        if constexpr (VEC)
+            for (int i = max(whole, first) * EPC + (int)threadIdx.x; i < min(last * EPC, n); i += SAMPLE_THREADS) f(at(i), i);
     }
     template <class F>
-    __device__ __forceinline__ void each_other(F&& f) const { each_from(CHUNKS * SAMPLE_THREADS, f); }
+    __device__ __forceinline__ void each_other(F&& f) const { each_between(CHUNKS * SAMPLE_THREADS, chunks, f); }
     template <class F>
-    __device__ __forceinline__ void each(F&& f) const { each_from(0, f); }
+    __device__ __forceinline__ void each(F&& f) const { each_between(0, chunks, f); }
     __device__ __forceinline__ void hold() {
         const uint32_t none = DT == MVLM_F32 ? 0xFF800000u : DT == MVLM_F16 ? 0xFC00FC00u : 0xFF80FF80u;
 #pragma unroll
@@ -221,6 +259,7 @@ struct SampleLds {
     uint32_t wave_counts[SAMPLE_THREADS / 64];
     float wave_values[SAMPLE_THREADS / 64];
     SamplePlace place[2];
+    float tops[SAMPLE_SYNC_WORDS];     // of a row's slices
     uint32_t listed, word;
 };
 
@@ -296,34 +335,41 @@ __device__ __forceinline__ void rank_list(u64* list, int size) {
     __syncthreads();
 }
 
-// the same for size <= LIST, by exchanges
+// the same for size <= LIST, by exchanges: each thread has an entry, and its partner's comes from the wave's lanes or
+// through LDS
 __device__ __forceinline__ void sort_list(u64* list, int size) {
     if (size <= RANKED) return rank_list(list, size);
-    int padded = 2;
-    while (padded < size) padded *= 2;
-    for (int i = size + (int)threadIdx.x; i < padded; i += SAMPLE_THREADS) list[i] = ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= padded; k *= 2)
+    const int tid = (int)threadIdx.x;
+    u64 own = tid < size ? list[tid] : ~0ull;
+    for (int k = 2; k < 2 * size; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int i = (int)threadIdx.x; i < padded / 2; i += SAMPLE_THREADS) {
-                const int lo = (i & ~(j - 1)) * 2 + (i & (j - 1)), hi = lo + j;
-                const u64 a = list[lo], b = list[hi];
-                if ((a > b) == ((lo & k) == 0)) list[lo] = b, list[hi] = a;
-            }
-            __syncthreads();
+            u64 other;
+            if (j >= 64) {
+                __syncthreads();
+                list[tid] = own;
+                __syncthreads();
+                other = list[tid ^ j];
+            } else
+                other = __shfl_xor(own, j, 64);
+            own = ((tid & j) == 0) == ((tid & k) == 0) ? min(own, other) : max(own, other);
         }
+    __syncthreads();
+    list[tid] = own;
+    __syncthreads();
 }
 
-template <int DT, bool VEC>
+// SPLIT: a row may be made by several blocks
+template <int DT, bool VEC, bool SPLIT>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs a) {
     __shared__ SampleLds s;
-    const int row = (int)blockIdx.x, tid = (int)threadIdx.x, n = a.n;
+    const int row = SPLIT ? (int)(blockIdx.x / (uint32_t)a.slices) : (int)blockIdx.x, slice = SPLIT ? (int)blockIdx.x - row * a.slices : 0;
+    const int tid = (int)threadIdx.x, n = a.n;
     RowTokens<DT, VEC> tokens;
     tokens.x = a.x;
     tokens.row = (int64_t)row * a.ld;
     tokens.n = n;
     tokens.chunks = (n + tokens.EPC - 1) / tokens.EPC;
-    tokens.hold();
+    if constexpr (!SPLIT) tokens.hold();
     const float T = a.temperature ? a.temperature[row] : 1.0f;
     float min_p = a.min_p ? a.min_p[row] : 0.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
     const int top_k = a.top_k ? a.top_k[row] : 0;
@@ -341,27 +387,121 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         for (int w = 1; w < SAMPLE_THREADS / 64; ++w) v = fmaxf(v, s.wave_values[w]);
         return v;
     };
+    // The candidates are enough where `closed`: no other token can be kept.
+    const bool by_rank = top_k > 0 && top_k <= RANKS, closed = by_rank || min_p > 0.0f;
+    const double c = 1.4426950408889634074 / (double)T;
+    const bool split = SPLIT && T > 0.0f && !closed;
+    if (slice > 0 && !split) return;
     const auto as_number = [](float v) { return v == v ? v : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x7F800000u); };
-    float own = -INFINITY;                                     // the largest of those that this thread holds
-    bool odd = false;
-    tokens.each_held([&](float v) {
-        own = fmaxf(own, v);                                   // a NaN is not taken
-        odd |= v != v;
-    });
-    if (odd) tokens.each_held([&](float v) { own = fmaxf(own, as_number(v)); });
-    float top = largest(own);
-    const bool more = tokens.chunks > tokens.CHUNKS * SAMPLE_THREADS;
+    float own = -INFINITY, top;                                // the largest of those that this thread holds, of all
+    u64 slice_sum = 0;                                         // of this thread's bin, where the slices are added up
+    uint32_t slice_count = 0;
+    bool summed = false;
+    SampleRow r;
+    r.bits = (double)a.bits;
+    auto with_top = [&] {
+        r.top = sample_key(top);
+        r.m = top < INFINITY ? (double)top : 0.0;
+        r.c = top < INFINITY ? c : 0.0;
+        r.step0 = r.step(top, r.c);
+    };
+    if (split) {
+        const int per = (tokens.chunks + a.slices - 1) / a.slices, from = min(slice * per, tokens.chunks), to = min(from + per, tokens.chunks);
+        tokens.each_between(from, to, [&](float v, int) { own = fmaxf(own, as_number(v)); });
+        top = largest(own);
+        const double step0 = r.step(top, c);
+        s.counts[tid] = 0, s.sums[tid] = 0;
+        __syncthreads();
+        if (top > -INFINITY && top < INFINITY)
+            tokens.each_between(from, to, [&](float v, int) {
+                if (!(v > -INFINITY)) return;                  // a NaN lies below all others here
+                const double steps = r.step(v, c), down = step0 - steps;
+                if (down >= BINS) return;
+                const double octave = __builtin_floor(steps * (1.0 / STEPS));
+                SampleRow one;
+                one.bits = (double)(a.bits - 1);
+                atomicAdd(&s.counts[(int)down], 1u);
+                atomicAdd(&s.sums[(int)down], one.weight((double)v * c - octave));
+            });
+        __syncthreads();
+        // The slices' parts cross workgroups: device-scope stores and loads, complete before a block counts itself in.
+        const int64_t part = (int64_t)row * a.slices + slice;
+        __hip_atomic_store(a.slice_sums + part * BINS + tid, s.sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.slice_counts + part * BINS + tid, s.counts[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) __hip_atomic_store(a.slice_tops + part, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            const uint32_t before = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (before == (uint32_t)a.slices - 1) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.word = before;
+        }
+        __syncthreads();
+        if (s.word != (uint32_t)a.slices - 1) return;
+        const int64_t first = (int64_t)row * a.slices;
+        for (int i = tid; i < a.slices; i += SAMPLE_THREADS)   // at most a CU each
+            s.tops[i] = __hip_atomic_load(a.slice_tops + first + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        top = -INFINITY;
+        for (int i = 0; i < a.slices; ++i) top = fmaxf(top, s.tops[i]);
+        with_top();
+        // beyond that the 64 bits of v log2(e) / T leave too few for its fraction
+        summed = top > -INFINITY && top < INFINITY && fabs(r.m * c) < 1024.0;
+        if (summed) {
+            // 2^(octave - m c), from the slices' unit to the row's
+            const double unit = exp2(__builtin_floor((r.step0 - tid) * (1.0 / STEPS)) - r.m * c + 1.0);
+            constexpr int AHEAD = 8;
+            for (int i = 0; i < a.slices; i += AHEAD) {
+                u64 w[AHEAD];
+                uint32_t k[AHEAD];
+                bool has[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q) {
+                    const int slice = min(i + q, a.slices - 1);
+                    const double down = r.step0 - r.step(s.tops[slice], c);
+                    has[q] = i + q < a.slices && down <= tid;  // not where the slice holds nothing
+                    const int64_t at = (first + slice) * BINS + (has[q] ? tid - (int)down : 0);
+                    w[q] = __hip_atomic_load(a.slice_sums + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    k[q] = __hip_atomic_load(a.slice_counts + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+                    if (has[q]) slice_sum += (u64)__builtin_rint((double)w[q] * unit), slice_count += k[q];
+            }
+        }
+        if (tid == 0) s.word = 0;
+        __syncthreads();
+    } else {
+        if constexpr (SPLIT) tokens.hold();
+        bool odd = false;
+        tokens.each_held([&](float v) {
+            own = fmaxf(own, v);                               // a NaN is not taken
+            odd |= v != v;
+        });
+        if (odd) tokens.each_held([&](float v) { own = fmaxf(own, as_number(v)); });
+        top = largest(own);
+        with_top();
+    }
+    const bool more = !split && tokens.chunks > tokens.CHUNKS * SAMPLE_THREADS;
 
     if (!(T > 0.0f)) {                                         // the first token of the largest value
-        if (more) {
-            float v = own;
-            tokens.each_other([&](float x, int) { v = fmaxf(v, as_number(x)); });
-            top = largest(v);
-        }
+        const float held = own;
         int at = n;
-        tokens.each([&](float x, int i) {
-            if (as_number(x) == top) at = min(at, i);
-        });
+        if (more) {
+            tokens.each_other([&](float x, int i) {
+                if (as_number(x) > own) own = as_number(x), at = i;
+            });
+            top = largest(own);
+            if (own < top) at = n;
+        }
+        if (held == top) {
+            int nth = 0;
+            at = n;
+            tokens.each_held([&](float v) {
+                if (as_number(v) == top) at = min(at, tokens.held_index(nth));
+                ++nth;
+            });
+        }
         for (int off = 32; off; off >>= 1) at = min(at, __shfl_xor(at, off, 64));
         if ((tid & 63) == 0) atomicMin(&s.word, (uint32_t)at);
         __syncthreads();
@@ -369,15 +509,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         return;
     }
 
-    SampleRow r;
-    const double c = 1.4426950408889634074 / (double)T;
-    r.bits = (double)a.bits;
-    auto with_top = [&] {
-        r.top = sample_key(top);
-        r.m = top < INFINITY ? (double)top : 0.0;
-        r.c = top < INFINITY ? c : 0.0;
-    };
-    with_top();
     double t_least = -(r.bits + 1.0);
     if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
     // a finite value that is below those of all tokens with t >= t_to, by a little
@@ -385,17 +516,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         const uint32_t k = sample_key((float)(r.m + t_to / c));
         return key_value(max(k, KEY_NEG_INF + 9) - 8);
     };
-    // The candidates: from `least` on.  `closed`: no other token can be kept.
-    const bool by_rank = top_k > 0 && top_k <= RANKS;
-    const bool closed = by_rank || min_p > 0.0f;
+    // the candidates: from `least` on
     float least = -3.402823466e38f;
-    if (top > -INFINITY && top < INFINITY) {
-        if (by_rank || !closed) {                              // the step of the k-th of the threads' largest
+    if (closed && top > -INFINITY && top < INFINITY) {
+        if (by_rank) {                                         // the step of the k-th of the threads' largest
             if (tid < RANK_BINS) s.counts[tid] = 0;
             __syncthreads();
             if (own > -INFINITY) atomicAdd(&s.counts[(int)fmin(r.t(own) * -RANK_STEPS, RANK_BINS - 1.0)], 1u);
             __syncthreads();
-            const uint32_t kth = by_rank ? top_k : RANKS;
+            const uint32_t kth = (uint32_t)top_k;
             uint32_t n4[RANK_BINS / 64], run = 0;
 #pragma unroll
             for (int i = 0; i < RANK_BINS / 64; ++i) run += n4[i] = s.counts[(tid & 63) * (RANK_BINS / 64) + i];
@@ -415,17 +544,37 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         }
         if (min_p > 0.0f) least = fmaxf(least, value_below(t_least));
     }
-    // into a list in LDS with room for `room`
-    auto to_list = [&](u64* list, uint32_t room, uint32_t key, int i) {
-        if (*(volatile uint32_t*)&s.listed > room) return;     // nobody will look at it
+    auto to_list = [&](uint32_t key, int i) {
         const uint32_t to = atomicAdd(&s.listed, 1u);
-        if (to < room) list[to] = (u64)~key << 32 | (uint32_t)i;
+        if (to < LIST) s.list[to] = (u64)~key << 32 | (uint32_t)i;
+    };
+    int candidates = 0;
+    bool compact = false;                                      // all of them are in LDS
+    // the indices of marked tokens to the candidates, from place `to` on
+    auto put = [&](u64 marks, uint32_t to, auto&& index) {
+        for (; marks; marks &= marks - 1, ++to)
+            if (to < CANDIDATES) s.candidates[to] = (u64)(uint32_t)index(__builtin_ctzll(marks));
+    };
+    // room for `own` of them from each lane of a wave
+    auto places = [&](uint32_t own) {
+        const uint32_t upto = (uint32_t)scan_wave((u64)own);
+        uint32_t to = 0;
+        if ((tid & 63) == 63) to = atomicAdd(&s.listed, upto);
+        return (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
     };
     if (more) {
         float v = own;
-        tokens.each_other([&](float x, int i) {
+        u64 marks = 0;
+        tokens.each_batch(tokens.CHUNKS * SAMPLE_THREADS, tokens.chunks, [&](float x, int nth) {
             v = fmaxf(v, as_number(x));
-            if (x >= least) to_list(s.candidates, CANDIDATES, sample_key(x), i);
+            if (closed && x >= least) marks |= 1ull << nth;
+        }, [&](int from) {
+            if (!__builtin_amdgcn_ballot_w64(marks != 0)) return;
+            put(marks, places((uint32_t)__popcll(marks)), [&](int nth) { return tokens.batch_index(from, nth); });
+            marks = 0;
+        }, [&](float x, int i) {
+            v = fmaxf(v, as_number(x));
+            if (closed && x >= least) put(1, atomicAdd(&s.listed, 1u), [&](int) { return i; });
         });
         top = largest(v);
         with_top();
@@ -435,44 +584,89 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         if (tid == 0) a.out[row] = 0;
         return;
     }
-    int candidates;
-    bool compact;                                              // all of them are in LDS
-    {
-        // few of the held ones are candidates: they are marked, then read again, four at a time
+    if (closed) {
         u64 marks[2] = {0, 0};
         int nth = 0;
         tokens.each_held([&](float v) {
             if (v >= least) marks[nth / 52] |= 1ull << nth % 52;
             ++nth;
         });
-        const uint32_t marked = (uint32_t)(__popcll(marks[0]) + __popcll(marks[1]));
-        u64 sum;
-        uint32_t all;
+        const uint32_t first = (uint32_t)__popcll(marks[0]), to = places(first + (uint32_t)__popcll(marks[1]));
+        put(marks[0], to, [&](int nth) { return tokens.held_index(nth); });
+        put(marks[1], to + first, [&](int nth) { return tokens.held_index(52 + nth); });
         __syncthreads();
-        const uint32_t others = s.listed;
-        const Share mine = share_out(0, marked, s, &sum, &all);
-        compact = others + all <= CANDIDATES && top < INFINITY;
-        candidates = (int)(others + all);
+        candidates = (int)min(s.listed, CANDIDATES + 1u);
+        compact = candidates <= CANDIDATES && top < INFINITY;
         if (compact) {
-            uint32_t to = others + mine.above;
-            while (marks[0] | marks[1]) {
-                int i[4];
-                float v[4];
+            // their values, again from memory
+            constexpr int EACH = CANDIDATES / SAMPLE_THREADS;
+            float v[EACH];
+            int at[EACH];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int half = marks[0] ? 0 : 1;
-                    const u64 left = marks[half];
-                    i[q] = left ? tokens.held_index(52 * half + __builtin_ctzll(left)) : -1;
-                    if (half) marks[1] = left & (left - 1);
-                    else marks[0] = left & (left - 1);
-                    v[q] = tokens.at(max(i[q], 0));
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (i[q] >= 0) s.candidates[to++] = (u64)~sample_key(v[q]) << 32 | (uint32_t)i[q];
+            for (int q = 0; q < EACH; ++q) {
+                at[q] = tid + q * SAMPLE_THREADS < candidates ? (int)(uint32_t)s.candidates[tid + q * SAMPLE_THREADS] : 0;
+                v[q] = q * SAMPLE_THREADS < candidates ? tokens.at(at[q]) : 0.0f;
             }
+#pragma unroll
+            for (int q = 0; q < EACH; ++q)
+                if (tid + q * SAMPLE_THREADS < candidates) s.candidates[tid + q * SAMPLE_THREADS] = (u64)~sample_key(v[q]) << 32 | (uint32_t)at[q];
         }
         __syncthreads();
+        // their steps as fine as the bins allow
+        if (compact) {
+            const double span = 2.0 - fmax(t_least, r.t(least));
+            while (r.steps * 2.0 * span < BINS && r.steps < 65536.0) r.steps *= 2.0;
+            with_top();
+        }
+    }
+
+    const auto top_p_need = [&](u64 kept) { return top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : (u64)1; };
+    const auto token_need = [&](u64 kept) { return u < 1.0f ? part_of<false>(u, kept) + 1 : kept; };
+    if (compact && candidates <= 128) {                        // a wave's work: two entries to a lane, and no barriers
+        if (tid >= 64) return;
+        const int size = candidates;
+        u64 e[2];
+        int place[2] = {0, 0};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) e[q] = tid + 64 * q < size ? s.candidates[tid + 64 * q] : ~0ull;
+        for (int j = 0; j < size; ++j) {
+            const u64 other = s.candidates[j];
+            place[0] += other < e[0];
+            place[1] += other < e[1];
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            if (tid + 64 * q < size) *(volatile u64*)&s.list[place[q]] = e[q];
+        asm_wait_lgkmcnt<0>();
+        u64 w[2];
+        bool lives[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            e[q] = 2 * tid + q < size ? *(volatile u64*)&s.list[2 * tid + q] : 0ull;
+            const double t = 2 * tid + q < size ? r.t(key_value(~(uint32_t)(e[q] >> 32))) : -INFINITY;
+            lives[q] = t >= t_least;
+            w[q] = lives[q] ? r.weight(t) : 0;
+        }
+        const u64 upto1 = scan_wave(w[0] + w[1]), upto0 = upto1 - w[1];
+        const auto lane_of = [](u64 v, int l) {
+            return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+        };
+        const int live = __popcll(__builtin_amdgcn_ballot_w64(lives[0])) + __popcll(__builtin_amdgcn_ballot_w64(lives[1]));
+        const int last = max(top_k > 0 ? min(top_k, live) : live, 1) - 1;
+        u64 kept = lane_of(last & 1 ? upto1 : upto0, last >> 1);
+        // the first entry up to which the sum is need
+        const auto entry = [&](u64 need) {
+            const uint64_t reached = __builtin_amdgcn_ballot_w64(upto1 >= min(need, kept));
+            const int l = reached ? __builtin_ctzll(reached) : 0;
+            return 2 * l + (lane_of(upto0, l) >= min(need, kept) ? 0 : 1);
+        };
+        if (top_p < 1.0f) {
+            const int i = entry(top_p_need(kept));
+            kept = lane_of(i & 1 ? upto1 : upto0, i >> 1);
+        }
+        const int i = entry(token_need(kept));
+        if (tid == 0) a.out[row] = (int)(uint32_t)s.list[i];
+        return;
     }
 
     int turn = 0;
@@ -484,30 +678,29 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         turn ^= 1;                                             // the next one is written while this is still read
         return p;
     };
-    // where the running count or sum reaches need
-    auto reaches = [&](const Share& m, bool by_count, u64 need) {
+    // where the running count or sum reaches need, or, where slices' sums were rounded and it just does not, ends
+    auto reaches = [&](const Share& m, bool by_count, u64 need, u64 sum) {
+        need = max(min(need, sum), (u64)1);
         const u64 before = by_count ? (u64)m.above : m.before;
         return announce(before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
     };
     // the list sorted, an entry to each thread
-    auto share_list = [&](int size) __attribute__((always_inline)) {
+    auto share_list = [&](int size, u64* sum) __attribute__((always_inline)) {
         sort_list(s.list, size);
-        u64 sum;
         uint32_t count;
         const double t = tid < size ? r.t(key_value(~(uint32_t)(s.list[tid] >> 32))) : -INFINITY;
-        return share_out(t >= t_least ? r.weight(t) : 0, tid < size ? 1u : 0u, s, &sum, &count);
+        return share_out(t >= t_least ? r.weight(t) : 0, tid < size ? 1u : 0u, s, sum, &count);
     };
-    const auto top_p_need = [&](u64 kept) { return top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : (u64)1; };
-    const auto token_need = [&](u64 kept) { return u < 1.0f ? part_of<false>(u, kept) + 1 : kept; };
-    if (compact && closed && candidates <= LIST) {
+    if (compact && candidates <= LIST) {
         const int size = candidates;
         if (tid < size) s.list[tid] = s.candidates[tid];
         __syncthreads();
-        const Share m = share_list(size);
+        u64 sum;
+        const Share m = share_list(size, &sum);
         const int live = __syncthreads_count(tid < size && r.t(key_value(~(uint32_t)(s.list[tid] >> 32))) >= t_least);
         SamplePlace p = announce(tid == (top_k > 0 ? min(top_k, live) : live) - 1, m);
-        if (top_p < 1.0f) p = reaches(m, false, top_p_need(p.before + p.own));
-        p = reaches(m, false, token_need(p.before + p.own));
+        if (top_p < 1.0f) p = reaches(m, false, top_p_need(p.before + p.own), sum);
+        p = reaches(m, false, token_need(p.before + p.own), sum);
         if (tid == 0) a.out[row] = (int)(uint32_t)s.list[p.index];
         return;
     }
@@ -522,18 +715,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             if (key >= live) f(r.t(v), key, i);
         });
     };
-    // of all live tokens, where the candidates may not be all that is kept
-    u64 sum_all = 0;
-    uint32_t count_all = 0;
-    if (compact && !closed) {
-        u64 w = 0;
-        uint32_t k = 0;
-        tokens.each([&](float v, int) {                        // the largest is finite: there is no NaN but below it
-            if (v >= live_value) w += r.weight(r.t(v)), ++k;
-        });
-        share_out(w, k, s, &sum_all, &count_all);
-        __syncthreads();
-    }
     // the same for the candidates, or the row
     auto each = [&](bool of_row, auto&& f) __attribute__((always_inline)) {
         if (of_row) return each_live(f);
@@ -543,36 +724,40 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         }
     };
 
-    // Twice at most: among the candidates, then, where they do not hold a place that is looked for, in the row.
-    for (int of_row = compact ? 0 : 1; of_row < 2; ++of_row) {
+    const bool of_row = !compact;
+    u64 bin_sum = 0;
+    uint32_t bin_count = 0;
+    if (!summed) {
         s.counts[tid] = 0, s.sums[tid] = 0;
         __syncthreads();
-        each(of_row, [&](double t, uint32_t, int) {
-            const int b = r.bin(t);
+        each(of_row, [&](double t, uint32_t key, int) {
+            const int b = r.bin(key_value(key));
             atomicAdd(&s.counts[b], 1u);
             atomicAdd(&s.sums[b], r.weight(t));
         });
         __syncthreads();
+        bin_sum = s.sums[tid], bin_count = s.counts[tid];
+    } else {
+        bin_sum = slice_sum, bin_count = slice_count;
+    }
+    {
         u64 sum_here;
-        uint32_t here;
-        const Share bins = share_out(s.sums[tid], s.counts[tid], s, &sum_here, &here);
-        const uint32_t all = of_row || closed ? here : count_all;
+        uint32_t all;
+        const Share bins = share_out(bin_sum, bin_count, s, &sum_here, &all);
         const uint32_t k = top_k > 0 && (uint32_t)top_k < all ? (uint32_t)top_k : all;   // tokens kept by count
-        u64 kept = of_row || closed ? sum_here : sum_all;
+        u64 kept = sum_here;
         int token = 0;
-        bool found = false;
         for (int step = 0; step < 3; ++step) {                 // top-k, top-p, the token
             if ((step == 0 && k == all) || (step == 1 && !(top_p < 1.0f))) continue;
             const bool by_count = step == 0;
             const u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
-            if (need > (by_count ? here : sum_here)) break;    // not among the candidates
-            found = step == 2;
-            SamplePlace p = reaches(bins, by_count, need);
+            u64 sum = by_count ? all : sum_here;
+            SamplePlace p = reaches(bins, by_count, need, sum);
             u64 before = p.before;                             // of the tokens above the range
             uint32_t above = p.above, inside = p.count;
             // the range's keys: from the least with a bin <= this one to the one before the least with a bin below it
-            uint32_t lo = least_where(live, r.top, [&](uint32_t key) { return r.bin(r.t(key_value(key))) <= p.index; });
-            uint32_t hi = p.index == 0 ? r.top : least_where(lo, r.top, [&](uint32_t key) { return r.bin(r.t(key_value(key))) < p.index; }) - 1;
+            uint32_t lo = least_where(live, r.top, [&](uint32_t key) { return r.bin(key_value(key)) <= p.index; });
+            uint32_t hi = p.index == 0 ? r.top : least_where(lo, r.top, [&](uint32_t key) { return r.bin(key_value(key)) < p.index; }) - 1;
             while (inside > LIST && lo < hi) {
                 const uint32_t span = hi - lo;                 // keys less one
                 int shift = 0;
@@ -586,10 +771,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     atomicAdd(&s.part_sums[b], r.weight(t));
                 });
                 __syncthreads();
-                u64 sum;
                 uint32_t count;
                 const Share parts = share_out(s.part_sums[tid], s.part_counts[tid], s, &sum, &count);
-                p = reaches(parts, by_count, need - (by_count ? (u64)above : before));
+                p = reaches(parts, by_count, need - (by_count ? (u64)above : before), by_count ? (u64)count : sum);
                 inside = p.count;
                 before += p.before;
                 above += p.above;
@@ -599,12 +783,19 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             if (inside <= LIST) {
                 if (tid == 0) s.listed = 0;
                 __syncthreads();
-                each(of_row, [&](double, uint32_t key, int i) {
-                    if (key >= lo && key <= hi) to_list(s.list, LIST, key, i);
-                });
+                if (of_row && top < INFINITY) {                // there is no NaN but below
+                    const float low = key_value(lo), high = key_value(hi);
+                    tokens.each([&](float v, int i) {
+                        if (v >= low && v <= high) to_list(sample_key(v), i);
+                    });
+                } else
+                    each(of_row, [&](double, uint32_t key, int i) {
+                        if (key >= lo && key <= hi) to_list(key, i);
+                    });
                 __syncthreads();
-                const Share m = share_list(min((int)s.listed, LIST));
-                p = reaches(m, by_count, need - (by_count ? (u64)above : before));
+                const int size = min((int)s.listed, LIST);
+                const Share m = share_list(size, &sum);
+                p = reaches(m, by_count, need - (by_count ? (u64)above : before), by_count ? (u64)size : sum);
                 token = (int)(uint32_t)s.list[p.index];
                 kept = before + p.before + p.own;
                 __syncthreads();
@@ -612,7 +803,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             }
             // equal values: the rank among them, and its index where the token is asked for
             const u64 w = r.weight(r.t(key_value(lo)));
-            const u64 rank = by_count ? need - above : (need - before + w - 1) / w;
+            const u64 rank = min(by_count ? need - above : (need - before + w - 1) / max(w, (u64)1), (u64)inside);
             kept = before + rank * w;
             if (step < 2) continue;
             // THREADS tokens at a time, in their order
@@ -635,20 +826,41 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             }
             token = (int)s.word;
         }
-        if (found) {
-            if (tid == 0) a.out[row] = token;
-            return;
-        }
+        if (tid == 0) a.out[row] = token;
     }
 }
 
-hipError_t launch_sample(hipStream_t s, const SampleArgs& a, int) {
+// Blocks per row: so many that they fill the chip once (a block's LDS leaves room for no other on its CU), each with
+// SAMPLE_THREADS chunks of 16 bytes at least.
+int sample_slices(int dtype, int rows, int n, int num_cus) {
+    const int chunks = (n + (dtype == MVLM_F32 ? 3 : 7)) / (dtype == MVLM_F32 ? 4 : 8);
+    return std::max(1, std::min(num_cus / rows, chunks / SAMPLE_THREADS));
+}
+
+// Bytes of the slices' parts; placing them.
+size_t sample_workspace_bytes(const SampleArgs& a) {
+    return a.slices == 1 ? 0 : (size_t)a.rows * a.slices * (BINS * (sizeof(u64) + sizeof(uint32_t)) + sizeof(float));
+}
+void sample_place(SampleArgs* a, void* workspace) {
+    const size_t parts = (size_t)a->rows * a->slices;
+    a->slice_sums = (unsigned long long*)workspace;
+    a->slice_counts = (uint32_t*)(a->slice_sums + parts * BINS);
+    a->slice_tops = (float*)(a->slice_counts + parts * BINS);
+}
+
+hipError_t launch_sample(hipStream_t s, const SampleArgs& a) {
     const int es = a.dtype == MVLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)a.x & 15u) == 0 && (a.ld * es) % 16 == 0;
+    const dim3 grid((unsigned)(a.rows * a.slices));
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (vec) launch_kernel(sample_kernel<DT, true>, dim3((unsigned)a.rows), dim3(SAMPLE_THREADS), 0, s, a);
-        else launch_kernel(sample_kernel<DT, false>, dim3((unsigned)a.rows), dim3(SAMPLE_THREADS), 0, s, a);
+        auto split = [&](auto sp) {
+            constexpr bool SPLIT = decltype(sp)::value;
+            if (vec) launch_kernel(sample_kernel<DT, true, SPLIT>, grid, dim3(SAMPLE_THREADS), 0, s, a);
+            else launch_kernel(sample_kernel<DT, false, SPLIT>, grid, dim3(SAMPLE_THREADS), 0, s, a);
+        };
+        if (a.slices > 1) split(std::true_type{});
+        else split(std::false_type{});
     };
     if (a.dtype == MVLM_F32) go(std::integral_constant<int, MVLM_F32>{});
     else if (a.dtype == MVLM_F16) go(std::integral_constant<int, MVLM_F16>{});
