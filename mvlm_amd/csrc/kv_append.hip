@@ -191,13 +191,14 @@ __device__ __forceinline__ T over_lanes(T v, int from, int lanes, F&& f) {
     return v;
 }
 
-// XD: type of qkv; VEC: its rows are 16-byte aligned; MX: 8-bit cache; NORM: of q or k heads
-template <int XD, bool VEC, bool MX, bool NORM>
+// XD: type of qkv; VEC: its rows are 16-byte aligned; MX: 8-bit cache; NORM: of q or k heads; LANES: of a head, all with
+// 8 dims, 0: any number; HALVES: rotated pairs are halves of multiples of 8
+template <int XD, bool VEC, bool MX, bool NORM, int LANES, bool HALVES>
 __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const KvAppendArgs a) {
     const int row = (int)blockIdx.x;
     const PagedKv& kv = a.kv;
     const int D = kv.D, half = a.rot / 2, qk = a.heads + kv.kv_heads, all = qk + kv.kv_heads;
-    const int shift = D > 64 ? 4 : D > 32 ? 3 : D > 16 ? 2 : D > 8 ? 1 : 0, lanes = 1 << shift;
+    const int shift = LANES == 16 ? 4 : LANES == 8 ? 3 : D > 64 ? 4 : D > 32 ? 3 : D > 16 ? 2 : D > 8 ? 1 : 0, lanes = 1 << shift;
     const int sub = (int)threadIdx.x & (lanes - 1), d = 8 * sub, step = (int)blockDim.x >> shift;
     const int own = (int)threadIdx.x >> shift;
     const int dl = min(d, D - 8);                          // a lane past the head's end reads its last dims
@@ -230,10 +231,11 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
     // cos and signed sin of this lane's dims: x' = x co + (its pair's other element) si
     float co[8], si[8];
     const bool turns = d < a.rot && slot0 >= 0;
-    const bool whole = (a.interleaved ? a.rot : half) % 8 == 0;   // a chunk turns as a whole
+    const bool whole = HALVES || (a.interleaved ? a.rot : half) % 8 == 0;   // a chunk turns as a whole
+    const bool inter = !HALVES && a.interleaved;
     const float* cs = a.rope + (int64_t)p * a.rot;         // [rot / 2][2]
     if (turns) {
-        if (whole && a.interleaved) {
+        if (whole && inter) {
             const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(cs + d), hi = *reinterpret_cast<const f32x4_any*>(cs + d + 4);
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -253,8 +255,8 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const bool first = a.interleaved ? (e & 1) == 0 : d + e < half;
-                const int i = min(a.interleaved ? (d + e) / 2 : first ? d + e : d + e - half, half - 1);
+                const bool first = inter ? (e & 1) == 0 : d + e < half;
+                const int i = min(inter ? (d + e) / 2 : first ? d + e : d + e - half, half - 1);
                 co[e] = cs[2 * i];
                 si[e] = first ? -cs[2 * i + 1] : cs[2 * i + 1];
             }
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = x.get(e);
-        if (8 * lanes > D) {
+        if (LANES == 0 && 8 * lanes > D) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = d < D ? v[e] : 0.0f;
         }
@@ -291,9 +293,9 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
                 for (int e = 0; e < 8; ++e) v[e] = v[e] * r * wt[e];
             }
         }
-        if (a.rot) {
+        if (HALVES || a.rot) {
             float w[8];                                    // the pairs' other elements
-            if (a.interleaved) {
+            if (inter) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = v[e ^ 1];
             } else if (whole) {                            // a chunk lies in one half, its partner chunk in the other
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
                 out[j] = !MX && kv.dtype == MVLM_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2_t))
                                                      : __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_t));
             }
-            if (d >= D) return;
+            if (LANES == 0 && d >= D) return;
             if (is_q) {
                 if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
                 *reinterpret_cast<u32x4*>(q_to + head * D) = out;
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
             word = over_lanes(word, MX_BLOCK / 8, lanes, [](uint32_t u, uint32_t w) { return u | w; });
             if (slot0 < 0) return;
             const int h = head - (is_k ? a.heads : qk);
-            if (d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + (kv_to + (int64_t)h * kv_step)) = code;
+            if (LANES > 0 || d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + (kv_to + (int64_t)h * kv_step)) = code;
             if (sub == 0) (is_k ? kv.k_scale : kv.v_scale)[slot0 + h * kv.page.div] = word;
         }
     };
@@ -394,8 +396,16 @@ hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a) {
         constexpr int XD = decltype(dt)::value;
         if (by_head) {
             auto heads = [&](auto mx, auto norm) {
-                if (vec) launch_kernel(kv_append_heads_kernel<XD, true, decltype(mx)::value, decltype(norm)::value>, grid, hblock, 0, s, a);
-                else launch_kernel(kv_append_heads_kernel<XD, false, decltype(mx)::value, decltype(norm)::value>, grid, hblock, 0, s, a);
+                constexpr bool MX = decltype(mx)::value, NORM = decltype(norm)::value;
+                auto lanes = [&](auto n) {
+                    constexpr int LANES = decltype(n)::value;
+                    if (a.rot > 0 && !a.interleaved && a.rot % 16 == 0) launch_kernel(kv_append_heads_kernel<XD, true, MX, NORM, LANES, true>, grid, hblock, 0, s, a);
+                    else launch_kernel(kv_append_heads_kernel<XD, true, MX, NORM, LANES, false>, grid, hblock, 0, s, a);
+                };
+                if (!vec) launch_kernel(kv_append_heads_kernel<XD, false, MX, NORM, 0, false>, grid, hblock, 0, s, a);
+                else if (a.kv.D == 128) lanes(std::integral_constant<int, 16>{});
+                else if (a.kv.D == 64) lanes(std::integral_constant<int, 8>{});
+                else lanes(std::integral_constant<int, 0>{});
             };
             const bool norm = a.q_weight || a.k_weight;
             if (a.kv.dtype != MVLM_MXFP8) heads(std::false_type{}, std::true_type{});
