@@ -31,7 +31,7 @@
 namespace mvlm {
 
 constexpr int SAMPLE_THREADS = 1024;
-constexpr int SAMPLE_BATCH = 8;        // 16-byte chunks in flight per thread behind the held ones
+constexpr int SAMPLE_BATCH = 4;        // 16-byte chunks in flight per thread behind the held ones
 constexpr int HOLD = 52;               // words of tokens that a thread keeps: 53248 fp32 tokens of a row, twice as many of 16 bits
 constexpr int CANDIDATES = 8192;       // room for them in LDS
 constexpr int LIST = SAMPLE_THREADS;   // entries that are sorted at once
@@ -169,14 +169,21 @@ struct RowTokens {
     template <class F, class E, class R>
     __device__ __forceinline__ void each_batch(int first, int last, F&& f, E&& end, R&& rest) const {
         const int whole = VEC ? min(last, n / EPC) : last;     // chunks read in one load, but where rows are not aligned
-        for (int base = first; base < whole; base += SAMPLE_THREADS * SAMPLE_BATCH) {
-            u32x4 w[SAMPLE_BATCH];
+        u32x4 next[SAMPLE_BATCH];
+        auto ask = [&](int base) {
 #pragma unroll
             for (int u = 0; u < SAMPLE_BATCH; ++u) {
                 const int c = min(base + (int)threadIdx.x + u * SAMPLE_THREADS, whole - 1);
-                if constexpr (VEC) w[u] = whole_chunk(c);
-                else w[u] = load(c);
+                if constexpr (VEC) next[u] = whole_chunk(c);
+                else next[u] = load(c);
             }
+        };
+        if (first < whole) ask(first);
+        for (int base = first; base < whole; base += SAMPLE_THREADS * SAMPLE_BATCH) {
+            u32x4 w[SAMPLE_BATCH];
+#pragma unroll
+            for (int u = 0; u < SAMPLE_BATCH; ++u) w[u] = next[u];
+            if (base + SAMPLE_THREADS * SAMPLE_BATCH < whole) ask(base + SAMPLE_THREADS * SAMPLE_BATCH);
 #pragma unroll
             for (int u = 0; u < SAMPLE_BATCH; ++u)
                 if (base + (int)threadIdx.x + u * SAMPLE_THREADS < whole)
@@ -356,6 +363,56 @@ __device__ __forceinline__ void sort_list(u64* list, int size) {
     __syncthreads();
     list[tid] = own;
     __syncthreads();
+}
+
+// Up to 128 entries in their order, two to a lane of a wave, with running sums of their weights.
+struct WaveList {
+    u64 entry0, entry1, upto0, upto1;  // of places 2 lane and 2 lane + 1
+    int live;                          // entries that live
+    __device__ __forceinline__ static u64 of_lane(u64 v, int l) {
+        return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+    }
+    __device__ __forceinline__ u64 sum_at(int place) const {
+        const u64 even = of_lane(upto0, place >> 1), odd = of_lane(upto1, place >> 1);
+        return place & 1 ? odd : even;
+    }
+    __device__ __forceinline__ int token_at(int place) const {
+        const u64 even = of_lane(entry0, place >> 1), odd = of_lane(entry1, place >> 1);
+        return (int)(uint32_t)(place & 1 ? odd : even);
+    }
+    // the first place whose running sum is need, which the sum of all is at least
+    __device__ __forceinline__ int reaches(u64 need) const {
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(upto1 >= need);
+        const int l = lanes ? __builtin_ctzll(lanes) : 63;
+        return 2 * l + (of_lane(upto0, l) >= need ? 0 : 1);
+    }
+};
+// from[0 .. size) through to[0 .. size), which may be the same
+__device__ __forceinline__ WaveList wave_list(const u64* from, u64* to, int size, const SampleRow& r, double t_least) {
+    const int lane = (int)threadIdx.x & 63;
+    const u64 e0 = lane < size ? from[lane] : ~0ull, e1 = lane + 64 < size ? from[lane + 64] : ~0ull;
+    int place0 = 0, place1 = 0;
+    for (int j = 0; j < size; ++j) {
+        const u64 other = from[j];
+        place0 += other < e0;
+        place1 += other < e1;
+    }
+    asm_wait_lgkmcnt<0>();
+    if (lane < size) *(volatile u64*)&to[place0] = e0;
+    if (lane + 64 < size) *(volatile u64*)&to[place1] = e1;
+    asm_wait_lgkmcnt<0>();
+    WaveList l;
+    const auto weigh = [&](int place, u64* entry) {
+        *entry = place < size ? *(volatile u64*)&to[place] : 0ull;
+        const double t = place < size ? r.t(key_value(~(uint32_t)(*entry >> 32))) : -INFINITY;
+        return t >= t_least ? t : -INFINITY;
+    };
+    const double t0 = weigh(2 * lane, &l.entry0), t1 = weigh(2 * lane + 1, &l.entry1);
+    const u64 w0 = t0 > -INFINITY ? r.weight(t0) : 0, w1 = t1 > -INFINITY ? r.weight(t1) : 0;
+    l.live = __popcll(__builtin_amdgcn_ballot_w64(t0 > -INFINITY)) + __popcll(__builtin_amdgcn_ballot_w64(t1 > -INFINITY));
+    l.upto1 = scan_wave(w0 + w1);
+    l.upto0 = l.upto1 - w1;
+    return l;
 }
 
 // SPLIT: a row may be made by several blocks
@@ -624,48 +681,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     const auto token_need = [&](u64 kept) { return u < 1.0f ? part_of<false>(u, kept) + 1 : kept; };
     if (compact && candidates <= 128) {                        // a wave's work: two entries to a lane, and no barriers
         if (tid >= 64) return;
-        const int size = candidates;
-        u64 e[2];
-        int place[2] = {0, 0};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) e[q] = tid + 64 * q < size ? s.candidates[tid + 64 * q] : ~0ull;
-        for (int j = 0; j < size; ++j) {
-            const u64 other = s.candidates[j];
-            place[0] += other < e[0];
-            place[1] += other < e[1];
-        }
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-            if (tid + 64 * q < size) *(volatile u64*)&s.list[place[q]] = e[q];
-        asm_wait_lgkmcnt<0>();
-        u64 w[2];
-        bool lives[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            e[q] = 2 * tid + q < size ? *(volatile u64*)&s.list[2 * tid + q] : 0ull;
-            const double t = 2 * tid + q < size ? r.t(key_value(~(uint32_t)(e[q] >> 32))) : -INFINITY;
-            lives[q] = t >= t_least;
-            w[q] = lives[q] ? r.weight(t) : 0;
-        }
-        const u64 upto1 = scan_wave(w[0] + w[1]), upto0 = upto1 - w[1];
-        const auto lane_of = [](u64 v, int l) {
-            return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
-        };
-        const int live = __popcll(__builtin_amdgcn_ballot_w64(lives[0])) + __popcll(__builtin_amdgcn_ballot_w64(lives[1]));
-        const int last = max(top_k > 0 ? min(top_k, live) : live, 1) - 1;
-        u64 kept = lane_of(last & 1 ? upto1 : upto0, last >> 1);
-        // the first entry up to which the sum is need
-        const auto entry = [&](u64 need) {
-            const uint64_t reached = __builtin_amdgcn_ballot_w64(upto1 >= min(need, kept));
-            const int l = reached ? __builtin_ctzll(reached) : 0;
-            return 2 * l + (lane_of(upto0, l) >= min(need, kept) ? 0 : 1);
-        };
-        if (top_p < 1.0f) {
-            const int i = entry(top_p_need(kept));
-            kept = lane_of(i & 1 ? upto1 : upto0, i >> 1);
-        }
-        const int i = entry(token_need(kept));
-        if (tid == 0) a.out[row] = (int)(uint32_t)s.list[i];
+        const WaveList list = wave_list(s.candidates, s.list, candidates, r, t_least);
+        u64 kept = list.sum_at(max(top_k > 0 ? min(top_k, list.live) : list.live, 1) - 1);
+        if (top_p < 1.0f) kept = list.sum_at(list.reaches(top_p_need(kept)));
+        const int token = list.token_at(list.reaches(token_need(kept)));
+        if (tid == 0) a.out[row] = token;
         return;
     }
 
@@ -753,11 +773,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             const u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
             u64 sum = by_count ? all : sum_here;
             SamplePlace p = reaches(bins, by_count, need, sum);
+            const int bin = p.index;
             u64 before = p.before;                             // of the tokens above the range
             uint32_t above = p.above, inside = p.count;
             // the range's keys: from the least with a bin <= this one to the one before the least with a bin below it
-            uint32_t lo = least_where(live, r.top, [&](uint32_t key) { return r.bin(key_value(key)) <= p.index; });
-            uint32_t hi = p.index == 0 ? r.top : least_where(lo, r.top, [&](uint32_t key) { return r.bin(key_value(key)) < p.index; }) - 1;
+            uint32_t lo = least_where(live, r.top, [&](uint32_t key) { return r.bin(key_value(key)) <= bin; });
+            uint32_t hi = bin == 0 ? r.top : least_where(lo, r.top, [&](uint32_t key) { return r.bin(key_value(key)) < bin; }) - 1;
             while (inside > LIST && lo < hi) {
                 const uint32_t span = hi - lo;                 // keys less one
                 int shift = 0;
@@ -794,6 +815,21 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     });
                 __syncthreads();
                 const int size = min((int)s.listed, LIST);
+                if (size <= 128) {                             // a wave's work
+                    if (tid < 64) {
+                        const WaveList list = wave_list(s.list, s.list, size, r, t_least);
+                        const u64 rest = need - (by_count ? (u64)above : before), sum = list.sum_at(size - 1);
+                        const int at = max(by_count ? (int)min(rest, (u64)size) - 1 : list.reaches(min(rest, sum)), 0);
+                        const u64 upto = list.sum_at(at);
+                        const int index = list.token_at(at);
+                        if (tid == 0) s.place[turn] = SamplePlace{upto, 0, 0, 0, index};
+                    }
+                    __syncthreads();
+                    kept = before + s.place[turn].before;
+                    token = s.place[turn].index;
+                    turn ^= 1;
+                    continue;
+                }
                 const Share m = share_list(size, &sum);
                 p = reaches(m, by_count, need - (by_count ? (u64)above : before), by_count ? (u64)size : sum);
                 token = (int)(uint32_t)s.list[p.index];

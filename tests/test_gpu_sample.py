@@ -120,6 +120,92 @@ def test_sample(dev, case):
               ld=n + extra, offset=offset)
 
 
+@pytest.mark.parametrize("case", range(6))
+def test_sample_of_long_rows(dev, case):
+    """rows of more tokens than a block holds, made by one block or by several, by all kinds of settings"""
+    rows, n, dt, std = [(3, 128000, F32, 3.0), (3, 128000, F16, 3.0), (130, 60000, F32, 2.0), (140, 9001, BF16, 2.0),
+                        (3, 120001, BF16, 0.3), (2, 300000, F32, 1.0)][case]
+    print("[sample] long", rows, n, dt, flush=True)
+    rng = np.random.default_rng(160 + case)
+    x = values(rng, (rows, n), dt, std)
+    few = min(rows, 12)                                      # rows that the reference looks at
+    for kw in ({}, {"top_p": 0.9}, {"top_k": 50}, {"top_k": 3000, "top_p": 0.8}, {"min_p": 0.05}, {"min_p": 1e-7, "top_p": 0.95},
+               {"T": 0.0}, {"top_k": n - 5, "top_p": 0.99}):
+        u = rng.random(rows)
+        T = np.full(rows, kw.get("T", 0.9))
+        args = [np.full(rows, kw[k]) if k in kw else None for k in ("top_k", "top_p", "min_p")]
+        got = draw(dev, x, dt, T, *args, u)
+        for r in range(few):
+            f = [None if a is None else float(np.float32(a[r])) for a in args]
+            want, near = pick(from_bits(x[r], dt), float(np.float32(T[r])), int(f[0] or 0), 1.0 if f[1] is None else f[1], f[2] or 0.0,
+                              float(np.float32(u[r])))
+            assert got[r] == want or near < 1e-12, (kw, r, got[r], want, near)
+
+
+@pytest.mark.parametrize("rows", [2, 150])
+def test_sample_of_long_rows_that_are_not_ordinary(dev, rows):
+    """infinities, NaN, values whose products with 1 / T leave no fraction, temperatures at their ends; one block and several"""
+    n = 20000
+    rng = np.random.default_rng(12)
+    base = (2 * rng.standard_normal(n)).astype(np.float32)
+    u = np.full(rows, 0.6, np.float32)
+    def same(x, T=None, top_p=None):  # noqa: E306
+        got = draw(dev, np.repeat(x[None], rows, 0), F32, None if T is None else np.full(rows, T), None,
+                   None if top_p is None else np.full(rows, top_p), None, u)
+        want, near = pick(x.astype(np.float64), 1.0 if T is None else float(np.float32(T)), 0, 1.0 if top_p is None else float(np.float32(top_p)), 0.0,
+                          float(u[0]))
+        assert near < 1e-12 or np.all(got == want), (got[:3], want)
+    x = base.copy()
+    x[[5, 700, 19999]] = np.inf
+    same(x)
+    x = base.copy()
+    x[[11, 12000]] = np.nan
+    same(x, top_p=0.7)
+    x = base.copy()
+    x[3:9000] = np.copysign(np.float32(np.nan), np.float32(-1))
+    same(x, top_p=0.7)
+    x = np.full(n, -np.inf, np.float32)
+    same(x)
+    x[15000] = -7.0
+    same(x)
+    same(base * np.float32(1e30))
+    same(base * np.float32(1e30), T=1e30)
+    same(base + np.float32(3000.0))                          # 4300 octaves: 2^-43 of weights apart
+    same(base, T=1e-30)
+    same(base, T=1e-3, top_p=0.5)
+    same(base, T=np.inf, top_p=0.5)
+    same(np.abs(base) * np.float32(2.0 ** -140))             # subnormals
+
+
+def test_sample_of_long_rows_in_a_graph(dev):
+    """rows made by several blocks, whose parts are counted in the same words, replayed with eager calls between"""
+    rng = np.random.default_rng(18)
+    jobs = []
+    for rows, n in ((3, 50000), (9, 30000)):
+        x, out, eager = dev.alloc(rows * n * 4), dev.alloc(rows * 4), dev.alloc(rows * 4)
+        u = dev.alloc(rows * 4)
+        s = m.Sampling(u, top_p=dev.upload(np.full(rows, 0.9, np.float32)))
+        plan = m.Plan(dev)
+        plan.add_sample(x, F32, rows, n, n, s, out)
+        plan.use_graph(True)
+        jobs.append((rows, n, x, u, s, out, eager, plan))
+    for _ in range(4):
+        host = []
+        for rows, n, x, u, s, out, eager, plan in jobs:
+            host.append(((3 * rng.standard_normal((rows, n))).astype(np.float32), rng.random(rows).astype(np.float32)))
+            x.upload(host[-1][0])
+            u.upload(host[-1][1])
+        for rows, n, x, u, s, out, eager, plan in jobs:
+            plan.run(2)
+        for (xs, us), (rows, n, x, u, s, out, eager, plan) in zip(host, jobs):
+            dev.sample(x, F32, rows, n, n, s, eager)
+            got = out.download(np.int32)
+            assert np.array_equal(eager.download(np.int32), got)
+            for r in range(rows):
+                want, near = pick(xs[r].astype(np.float64), 1.0, 0, float(np.float32(0.9)), 0.0, float(us[r]))
+                assert got[r] == want or near < 1e-12
+
+
 @pytest.mark.parametrize("n", [1, 7, 5000, 40000])
 def test_sample_of_equal_values(dev, n):
     """ties go to the lower index, also where there are more than any list holds"""
