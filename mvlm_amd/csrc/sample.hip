@@ -39,9 +39,7 @@ constexpr int RANKED = 256;            // of which so many by counting
 constexpr int RANKS = 1000;            // of the threads' largest values
 constexpr int RANK_BINS = 256, RANK_STEPS = 8;   // in which they are counted, per factor of two of the weight
 constexpr int BINS = SAMPLE_THREADS;
-constexpr int STEPS = 16;              // bins per factor of two of the weight
-constexpr int MOST_BITS = 51;
-static_assert((MOST_BITS + 2) * STEPS <= BINS, "all live tokens have a bin");
+constexpr int STEPS = 48;              // bins per factor of two of the weight; the last has all that lies 2^21 and more below the first
 
 typedef unsigned long long u64;
 
@@ -80,16 +78,18 @@ __device__ __forceinline__ double exp2_series(double x) {
     return __longlong_as_double((long long)(b + ((u64)(uint32_t)__double_as_longlong(r) << 52)));
 }
 
+// 2^x rounded to an integer, -1 <= x <= 51
+__device__ __forceinline__ u64 integer_power(double x) {
+    return (u64)__double_as_longlong(exp2_series(x) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: its unit is 1
+}
+
 // What a row's block knows of it.
 struct SampleRow {
     uint32_t top;                      // key of the largest value
     double m, c;                       // that value, log2(e) / T; where it is infinite, 0 and 0: its like have t = 0
     double bits;
     __device__ __forceinline__ double t(float v) const { return ((double)fminf(v, 3.402823466e38f) - m) * c; }
-    __device__ __forceinline__ u64 weight(double t) const {
-        const double w = exp2_series(t + bits);                        // at most 2^51
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to an integer
-    }
+    __device__ __forceinline__ u64 weight(double t) const { return integer_power(t + bits); }
     // The bin of a value: how many steps of v log2(e) / T lie between its own and the largest's.
     double steps = STEPS, step0;
     __device__ __forceinline__ double step(float v, double c) const { return __builtin_floor((double)fminf(v, 3.402823466e38f) * c * steps); }
@@ -472,13 +472,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         if (top > -INFINITY && top < INFINITY)
             tokens.each_between(from, to, [&](float v, int) {
                 if (!(v > -INFINITY)) return;                  // a NaN lies below all others here
-                const double steps = r.step(v, c), down = step0 - steps;
-                if (down >= BINS) return;
-                const double octave = __builtin_floor(steps * (1.0 / STEPS));
-                SampleRow one;
-                one.bits = (double)(a.bits - 1);
-                atomicAdd(&s.counts[(int)down], 1u);
-                atomicAdd(&s.sums[(int)down], one.weight((double)v * c - octave));
+                const double steps = fmax(r.step(v, c), step0 - (BINS - 1)), octave = __builtin_floor(steps * (1.0 / STEPS));
+                const double x = (double)v * c - octave + (a.bits - 1);    // below bits, by much in the last bin
+                const int b = (int)(step0 - steps);
+                atomicAdd(&s.counts[b], 1u);
+                if (x >= -1.0) atomicAdd(&s.sums[b], integer_power(x));
             });
         __syncthreads();
         // The slices' parts cross workgroups: device-scope stores and loads, complete before a block counts itself in.
@@ -505,26 +503,34 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         // beyond that the 64 bits of v log2(e) / T leave too few for its fraction
         summed = top > -INFINITY && top < INFINITY && fabs(r.m * c) < 1024.0;
         if (summed) {
-            // 2^(octave - m c), from the slices' unit to the row's
-            const double unit = exp2(__builtin_floor((r.step0 - tid) * (1.0 / STEPS)) - r.m * c + 1.0);
+            s.counts[tid] = 0, s.sums[tid] = 0;
+            __syncthreads();
+            // a part's unit is 2^(octave of its bin), the row's 2^(m c)
+            const double mc = __builtin_floor(r.m * c), unit = exp2(mc - r.m * c);
             constexpr int AHEAD = 8;
             for (int i = 0; i < a.slices; i += AHEAD) {
                 u64 w[AHEAD];
                 uint32_t k[AHEAD];
-                bool has[AHEAD];
 #pragma unroll
                 for (int q = 0; q < AHEAD; ++q) {
-                    const int slice = min(i + q, a.slices - 1);
-                    const double down = r.step0 - r.step(s.tops[slice], c);
-                    has[q] = i + q < a.slices && down <= tid;  // not where the slice holds nothing
-                    const int64_t at = (first + slice) * BINS + (has[q] ? tid - (int)down : 0);
+                    const int64_t at = (first + min(i + q, a.slices - 1)) * BINS + tid;
                     w[q] = __hip_atomic_load(a.slice_sums + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     k[q] = __hip_atomic_load(a.slice_counts + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
 #pragma unroll
-                for (int q = 0; q < AHEAD; ++q)
-                    if (has[q]) slice_sum += (u64)__builtin_rint((double)w[q] * unit), slice_count += k[q];
+                for (int q = 0; q < AHEAD; ++q) {
+                    const float slice_top = s.tops[min(i + q, a.slices - 1)];
+                    if (i + q >= a.slices || k[q] == 0) continue;          // as all are of a slice that holds nothing
+                    const double step0 = r.step(slice_top, c), octave = __builtin_floor((step0 - tid) * (1.0 / STEPS));
+                    const double part = __builtin_rint((double)w[q] * __builtin_ldexp(unit, (int)fmax(octave - mc + 1.0, -200.0)));
+                    const int b = (int)fmin(r.step0 - step0 + tid, BINS - 1.0);
+                    atomicAdd(&s.counts[b], k[q]);
+                    atomicAdd(&s.sums[b], (u64)part);
+                }
             }
+            __syncthreads();
+            slice_sum = s.sums[tid];
+            slice_count = s.counts[tid];
         }
         if (tid == 0) s.word = 0;
         __syncthreads();
