@@ -572,7 +572,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         return;
     }
 
-    double t_least = -(r.bits + 1.0);
+    double t_least = -(r.bits + 1.0) + 0x1p-30;                // what lives has a weight of 1 at least
     if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
     // a finite value that is below those of all tokens with t >= t_to, by a little
     auto value_below = [&](double t_to) {
@@ -704,8 +704,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         turn ^= 1;                                             // the next one is written while this is still read
         return p;
     };
-    // where the running count or sum reaches need, or, where slices' sums were rounded and it just does not, ends
+    // Where the running count or sum reaches need, or ends: bins of slices also have tokens that do not live, and sums that
+    // were rounded otherwise, so that what a search finds in one can be less than it holds, or nothing.
     auto reaches = [&](const Share& m, bool by_count, u64 need, u64 sum) {
+        if (sum == 0) return SamplePlace{};
         need = max(min(need, sum), (u64)1);
         const u64 before = by_count ? (u64)m.above : m.before;
         return announce(before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
@@ -776,10 +778,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         for (int step = 0; step < 3; ++step) {                 // top-k, top-p, the token
             if ((step == 0 && k == all) || (step == 1 && !(top_p < 1.0f))) continue;
             const bool by_count = step == 0;
-            const u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
+            u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
             u64 sum = by_count ? all : sum_here;
             SamplePlace p = reaches(bins, by_count, need, sum);
             const int bin = p.index;
+            if (step == 2 && u >= 1.0f && kept == sum_here) need = ~0ull >> 1;   // the last, whatever the bin is found to hold
             u64 before = p.before;                             // of the tokens above the range
             uint32_t above = p.above, inside = p.count;
             // the range's keys: from the least with a bin <= this one to the one before the least with a bin below it
@@ -807,10 +810,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 hi -= (uint32_t)p.index << shift;
                 lo = max(lo, hi - ((1u << shift) - 1u));
             }
-            if (inside <= LIST) {
+            if (inside <= LIST || lo > hi) {
                 if (tid == 0) s.listed = 0;
                 __syncthreads();
-                if (of_row && top < INFINITY) {                // there is no NaN but below
+                if (lo > hi) {
+                } else if (of_row && top < INFINITY) {         // there is no NaN but below
                     const float low = key_value(lo), high = key_value(hi);
                     tokens.each([&](float v, int i) {
                         if (v >= low && v <= high) to_list(sample_key(v), i);
@@ -821,6 +825,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     });
                 __syncthreads();
                 const int size = min((int)s.listed, LIST);
+                if (size == 0) {                               // where the bin is of slices only
+                    kept = before;
+                    token = -1;
+                    __syncthreads();
+                    continue;
+                }
                 if (size <= 128) {                             // a wave's work
                     if (tid < 64) {
                         const WaveList list = wave_list(s.list, s.list, size, r, t_least);
@@ -843,13 +853,14 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 __syncthreads();
                 continue;
             }
-            // equal values: the rank among them, and its index where the token is asked for
+            // equal values: the rank among them, and its index (or the last one's) where the token is asked for
             const u64 w = r.weight(r.t(key_value(lo)));
             const u64 rank = min(by_count ? need - above : (need - before + w - 1) / max(w, (u64)1), (u64)inside);
             kept = before + rank * w;
             if (step < 2) continue;
             // THREADS tokens at a time, in their order
-            uint32_t seen = 0;
+            uint32_t seen = 0, latest = 0;
+            if (tid == 0) s.word = 0;
             for (int from = 0; from < n; from += SAMPLE_THREADS) {
                 const int i = from + tid;
                 const bool same = i < n && sample_key(tokens.at(i)) == lo;
@@ -861,12 +872,24 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     if (w2 < (tid >> 6)) mine += s.wave_counts[w2];
                     total += s.wave_counts[w2];
                 }
-                if (same && mine + 1 == rank) s.word = (uint32_t)i;
+                if (same && mine < rank) latest = (uint32_t)i;
                 __syncthreads();
                 if (seen + total >= rank) break;
                 seen += total;
             }
+            if (latest) atomicMax(&s.word, latest);
+            __syncthreads();
             token = (int)s.word;
+        }
+        if (token < 0) {                                       // the last token that lives
+            __syncthreads();
+            if (tid == 0) s.list[0] = 0;
+            __syncthreads();
+            u64 last = 0;
+            each_live([&](double, uint32_t key, int i) { last = max(last, (u64)~key << 32 | (uint32_t)i); });
+            if (last) atomicMax(&s.list[0], last);
+            __syncthreads();
+            token = (int)(uint32_t)s.list[0];
         }
         if (tid == 0) a.out[row] = token;
     }
