@@ -265,7 +265,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
     // where the lane's dims of q head 0 and of kv head 0 go; a kv head further on is a page's slots further on
     uint16_t* const q_to = a.q_out + (int64_t)row * a.heads * D + d;
     const int64_t kv_to = (int64_t)max(slot0, 0) * D + d;
-    const int kv_step = kv.page.div * D;                   // below 2^31 2^7 / kv_heads: 64 bits where multiplied
+    const int64_t kv_step = (int64_t)kv.page.div * D;      // past 2^31 in pages of 2^24 positions and more
     const int partner = ((int)threadIdx.x & 63) + (d < half ? half / 8 : -(half / 8));
     auto make = [&](int head, const AppendRaw<XD, VEC>& x) {
         float v[8];
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
                 if (slot0 < 0) out = u32x4{0u, 0u, 0u, 0u};
                 *reinterpret_cast<u32x4*>(q_to + head * D) = out;
             } else if (slot0 >= 0)
-                *reinterpret_cast<u32x4*>((is_k ? kv.k : kv.v) + (kv_to + (int64_t)(head - (is_k ? a.heads : qk)) * kv_step)) = out;
+                *reinterpret_cast<u32x4*>((is_k ? kv.k : kv.v) + (kv_to + (head - (is_k ? a.heads : qk)) * kv_step)) = out;
             return;
         }
         if constexpr (MX) {
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_heads_kernel(const K
             word = over_lanes(word, MX_BLOCK / 8, lanes, [](uint32_t u, uint32_t w) { return u | w; });
             if (slot0 < 0) return;
             const int h = head - (is_k ? a.heads : qk);
-            if (LANES > 0 || d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + (kv_to + (int64_t)h * kv_step)) = code;
+            if (LANES > 0 || d < D) *reinterpret_cast<u32x2*>((uint8_t*)(is_k ? kv.k : kv.v) + (kv_to + h * kv_step)) = code;
             if (sub == 0) (is_k ? kv.k_scale : kv.v_scale)[slot0 + h * kv.page.div] = word;
         }
     };

@@ -436,6 +436,27 @@ def test_over_int32_offsets(dev):
     assert close(o.download(np.float32).reshape(ref.shape).astype(np.float64), ref, tol, F32) <= 1.0
 
 
+@pytest.mark.parametrize("cd", [MX, BF16])
+def test_pages_past_int32(dev, cd):
+    """one page of 2^25 positions: the second head's elements start 2^32 further on"""
+    D, page, kv_heads = 128, 1 << 25, 2
+    rng = np.random.default_rng(6)
+    size = m.paged_kv_bytes(cd, 1, page, kv_heads, D)
+    cache = m.PagedKV(dev.alloc(size), dev.alloc(size), cd, 1, page, kv_heads, D)
+    batch = m.PagedBatch(1, 3, dev.upload(np.array([page], np.int32)), dev.upload(np.zeros(1, np.int32)), 1,
+                         row_start=dev.upload(np.array([0, 3], np.int32)))
+    x = values(rng, (3, 3, kv_heads, D), BF16)
+    norm = m.HeadNorm(dev.upload(np.ones(D, np.float32)), None, 1e-6)
+    q = dev.alloc(3 * kv_heads * D * 2)
+    k, v = (dev.alloc(3 * kv_heads * D * 4) for _ in range(2))
+    say("a page of", page)
+    dev.kv_append_paged_ex(dev.upload(x), BF16, 3 * kv_heads * D, batch, cache, kv_heads, q, None, norm)
+    dev.kv_read_paged(batch, cache, k, v, F32, kv_heads * D)
+    for i, buf in ((1, k), (2, v)):
+        want = from_bits(x[:, i], BF16)
+        assert np.array_equal(buf.download(np.float32).reshape(3, kv_heads, D), mx_ref.decode(*mx_ref.encode(want)) if cd == MX else want)
+
+
 def test_graphs_of_one_device_share_workspaces(dev):
     """two captured graphs with split attention, over 8 and over 16 bits, replayed in turn with eager calls between"""
     rng = np.random.default_rng(31)
