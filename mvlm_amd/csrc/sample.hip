@@ -707,10 +707,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     // Where the running count or sum reaches need, or ends: bins of slices also have tokens that do not live, and sums that
     // were rounded otherwise, so that what a search finds in one can be less than it holds, or nothing.
     auto reaches = [&](const Share& m, bool by_count, u64 need, u64 sum) {
-        if (sum == 0) return SamplePlace{};
         need = max(min(need, sum), (u64)1);
         const u64 before = by_count ? (u64)m.above : m.before;
-        return announce(before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
+        return announce(sum == 0 ? tid == 0 : before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
     };
     // the list sorted, an entry to each thread
     auto share_list = [&](int size, u64* sum) __attribute__((always_inline)) {
@@ -885,9 +884,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             __syncthreads();
             if (tid == 0) s.list[0] = 0;
             __syncthreads();
-            u64 last = 0;
-            each_live([&](double, uint32_t key, int i) { last = max(last, (u64)~key << 32 | (uint32_t)i); });
-            if (last) atomicMax(&s.list[0], last);
+#pragma unroll 1
+            for (int i = tid; i < n; i += SAMPLE_THREADS) {
+                const uint32_t key = sample_key(tokens.at(i));
+                if (key >= live) atomicMax(&s.list[0], (u64)~key << 32 | (uint32_t)i);
+            }
             __syncthreads();
             token = (int)(uint32_t)s.list[0];
         }
