@@ -19,8 +19,9 @@ struct SampleArgs {
     int* out;
     int bits;                      // weights are multiples of 2^-bits
     int slices;                    // blocks per row
-    // where slices > 1: the slices' parts, and the row's finished slices, zero between launches
+    // where slices > 1: what the slices found, and the row's finished slices, zero between launches
     unsigned long long* slice_sums;
+    unsigned long long* part_entries;
     uint32_t* slice_counts;
     float* slice_tops;
     uint32_t* arrived;

@@ -423,9 +423,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     const int tid = (int)threadIdx.x, n = a.n;
     RowTokens<DT, VEC> tokens;
     tokens.x = a.x;
-    tokens.row = (int64_t)row * a.ld;
-    tokens.n = n;
-    tokens.chunks = (n + tokens.EPC - 1) / tokens.EPC;
+    auto whole_row = [&] {
+        tokens.row = (int64_t)row * a.ld;
+        tokens.n = n;
+        tokens.chunks = (n + tokens.EPC - 1) / tokens.EPC;
+    };
+    whole_row();
     if constexpr (!SPLIT) tokens.hold();
     const float T = a.temperature ? a.temperature[row] : 1.0f;
     float min_p = a.min_p ? a.min_p[row] : 0.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
@@ -448,7 +451,24 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     const bool by_rank = top_k > 0 && top_k <= RANKS, closed = by_rank || min_p > 0.0f;
     const double c = 1.4426950408889634074 / (double)T;
     const bool split = SPLIT && T > 0.0f && !closed;
-    if (slice > 0 && !split) return;
+    // Blocks that look for candidates: as many as it takes to hold the row.  1: this one looks at all of it.
+    int parts = 1;
+    if (SPLIT && T > 0.0f && closed) parts = min(a.slices, (tokens.chunks + tokens.CHUNKS * SAMPLE_THREADS - 1) / (tokens.CHUNKS * SAMPLE_THREADS));
+    if (slice >= (split ? a.slices : parts)) return;
+    // Parts cross workgroups: device-scope stores and loads, complete before a block counts itself in.  Whether this is
+    // the last of `blocks`.
+    auto arrive = [&](int blocks) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            const uint32_t before = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (before == (uint32_t)blocks - 1) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.word = before;
+        }
+        __syncthreads();
+        return s.word == (uint32_t)blocks - 1;
+    };
+    const int64_t first_part = (int64_t)row * (SPLIT ? a.slices : 1), own_part = first_part + slice;
     const auto as_number = [](float v) { return v == v ? v : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x7F800000u); };
     float own = -INFINITY, top;                                // the largest of those that this thread holds, of all
     u64 slice_sum = 0;                                         // of this thread's bin, where the slices are added up
@@ -479,23 +499,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 if (x >= -1.0) atomicAdd(&s.sums[b], integer_power(x));
             });
         __syncthreads();
-        // The slices' parts cross workgroups: device-scope stores and loads, complete before a block counts itself in.
-        const int64_t part = (int64_t)row * a.slices + slice;
-        __hip_atomic_store(a.slice_sums + part * BINS + tid, s.sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(a.slice_counts + part * BINS + tid, s.counts[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (tid == 0) __hip_atomic_store(a.slice_tops + part, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tid == 0) {
-            const uint32_t before = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (before == (uint32_t)a.slices - 1) __hip_atomic_store(a.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            s.word = before;
-        }
-        __syncthreads();
-        if (s.word != (uint32_t)a.slices - 1) return;
-        const int64_t first = (int64_t)row * a.slices;
+        __hip_atomic_store(a.slice_sums + own_part * BINS + tid, s.sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.slice_counts + own_part * BINS + tid, s.counts[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) __hip_atomic_store(a.slice_tops + own_part, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!arrive(a.slices)) return;
         for (int i = tid; i < a.slices; i += SAMPLE_THREADS)   // at most a CU each
-            s.tops[i] = __hip_atomic_load(a.slice_tops + first + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.tops[i] = __hip_atomic_load(a.slice_tops + first_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         top = -INFINITY;
         for (int i = 0; i < a.slices; ++i) top = fmaxf(top, s.tops[i]);
@@ -513,7 +522,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 uint32_t k[AHEAD];
 #pragma unroll
                 for (int q = 0; q < AHEAD; ++q) {
-                    const int64_t at = (first + min(i + q, a.slices - 1)) * BINS + tid;
+                    const int64_t at = (first_part + min(i + q, a.slices - 1)) * BINS + tid;
                     w[q] = __hip_atomic_load(a.slice_sums + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     k[q] = __hip_atomic_load(a.slice_counts + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
@@ -534,9 +543,78 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         }
         if (tid == 0) s.word = 0;
         __syncthreads();
-    } else {
+    }
+    const int per_part = (tokens.chunks + parts - 1) / parts;
+    int base = 0;                                              // index of the tokens' first in the row
+    if (parts > 1) {
+        base = slice * per_part * tokens.EPC;
+        tokens.row += base;
+        tokens.n = min(n - base, per_part * tokens.EPC);
+        tokens.chunks = (tokens.n + tokens.EPC - 1) / tokens.EPC;
+    }
+    double t_least = -(r.bits + 1.0) + 0x1p-30;                // what lives has a weight of 1 at least
+    if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
+    // a finite value that is below those of all tokens with t >= t_to, by a little
+    auto value_below = [&](double t_to) {
+        const uint32_t k = sample_key((float)(r.m + t_to / c));
+        return key_value(max(k, KEY_NEG_INF + 9) - 8);
+    };
+    auto to_list = [&](uint32_t key, int i) {
+        const uint32_t to = atomicAdd(&s.listed, 1u);
+        if (to < LIST) s.list[to] = (u64)~key << 32 | (uint32_t)i;
+    };
+    // the indices of marked tokens to the candidates, from place `to` on
+    auto put = [&](u64 marks, uint32_t to, auto&& index) {
+        for (; marks; marks &= marks - 1, ++to)
+            if (to < CANDIDATES) s.candidates[to] = (u64)(uint32_t)index(__builtin_ctzll(marks));
+    };
+    // room for `own` of them from each lane of a wave
+    auto places = [&](uint32_t own) {
+        const uint32_t upto = (uint32_t)scan_wave((u64)own);
+        uint32_t to = 0;
+        if ((tid & 63) == 63) to = atomicAdd(&s.listed, upto);
+        return (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
+    };
+    float least = -3.402823466e38f;                            // the candidates: from this value on
+    int candidates = 0;
+    bool compact = false;                                      // all of them are in LDS
+    // Steps as fine as the bins allow for the candidates, and of many those that top_k may keep.
+    auto refine = [&] {
+        if (!compact) return;
+        const double span = 2.0 - fmax(t_least, r.t(least));
+        r.steps = STEPS;
+        while (r.steps * 2.0 * span < BINS && r.steps < 65536.0) r.steps *= 2.0;
+        with_top();
+        if (!by_rank || candidates <= 128 || candidates <= top_k) return;
+        s.counts[tid] = 0;
+        if (tid == 0) s.word = BINS - 1, s.listed = 0;
+        __syncthreads();
+        for (int i = tid; i < candidates; i += SAMPLE_THREADS) atomicAdd(&s.counts[r.bin(key_value(~(uint32_t)(s.candidates[i] >> 32)))], 1u);
+        __syncthreads();
+        const uint32_t count = s.counts[tid], upto = (uint32_t)scan_wave((u64)count);
+        if ((tid & 63) == 63) s.wave_counts[tid >> 6] = upto;
+        __syncthreads();
+        uint32_t above = upto - count;
+        for (int w = 0; w < tid >> 6; ++w) above += s.wave_counts[w];
+        if (above < (uint32_t)top_k && above + count >= (uint32_t)top_k) s.word = (uint32_t)tid;
+        __syncthreads();
+        const int bin = (int)s.word;
+        for (int i = tid; i < candidates; i += SAMPLE_THREADS)
+            if (const u64 entry = s.candidates[i]; r.bin(key_value(~(uint32_t)(entry >> 32))) <= bin) {
+                const uint32_t to = atomicAdd(&s.listed, 1u);
+                if (to < LIST) s.list[to] = entry;
+            }
+        __syncthreads();
+        if (s.listed > LIST) return;
+        candidates = (int)s.listed;
+        if (tid < candidates) s.candidates[tid] = s.list[tid];
+        if (bin < BINS - 1) least = fmaxf(least, value_below((r.step0 - bin) / r.steps - r.m * r.c));
+        __syncthreads();
+    };
+    if (!split) {
         if constexpr (SPLIT) tokens.hold();
         bool odd = false;
+        own = -INFINITY;
         tokens.each_held([&](float v) {
             own = fmaxf(own, v);                               // a NaN is not taken
             odd |= v != v;
@@ -572,15 +650,13 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         return;
     }
 
-    double t_least = -(r.bits + 1.0) + 0x1p-30;                // what lives has a weight of 1 at least
-    if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
-    // a finite value that is below those of all tokens with t >= t_to, by a little
-    auto value_below = [&](double t_to) {
-        const uint32_t k = sample_key((float)(r.m + t_to / c));
-        return key_value(max(k, KEY_NEG_INF + 9) - 8);
-    };
-    // the candidates: from `least` on
-    float least = -3.402823466e38f;
+    // A bound of many tokens is worth another look at those that are not held: with theirs among the threads' largest
+    // it leaves fewer candidates.
+    if (more && by_rank && top_k > RANKS / 4) {
+        tokens.each_other([&](float x, int) { own = fmaxf(own, as_number(x)); });
+        top = largest(own);
+        with_top();
+    }
     if (closed && top > -INFINITY && top < INFINITY) {
         if (by_rank) {                                         // the step of the k-th of the threads' largest
             if (tid < RANK_BINS) s.counts[tid] = 0;
@@ -607,24 +683,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         }
         if (min_p > 0.0f) least = fmaxf(least, value_below(t_least));
     }
-    auto to_list = [&](uint32_t key, int i) {
-        const uint32_t to = atomicAdd(&s.listed, 1u);
-        if (to < LIST) s.list[to] = (u64)~key << 32 | (uint32_t)i;
-    };
-    int candidates = 0;
-    bool compact = false;                                      // all of them are in LDS
-    // the indices of marked tokens to the candidates, from place `to` on
-    auto put = [&](u64 marks, uint32_t to, auto&& index) {
-        for (; marks; marks &= marks - 1, ++to)
-            if (to < CANDIDATES) s.candidates[to] = (u64)(uint32_t)index(__builtin_ctzll(marks));
-    };
-    // room for `own` of them from each lane of a wave
-    auto places = [&](uint32_t own) {
-        const uint32_t upto = (uint32_t)scan_wave((u64)own);
-        uint32_t to = 0;
-        if ((tid & 63) == 63) to = atomicAdd(&s.listed, upto);
-        return (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
-    };
     if (more) {
         float v = own;
         u64 marks = 0;
@@ -643,11 +701,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         with_top();
         if (min_p > 0.0f && top < INFINITY) least = fmaxf(least, value_below(t_least));
     }
-    if (top == -INFINITY) {
-        if (tid == 0) a.out[row] = 0;
-        return;
-    }
-    if (closed) {
+    if (closed && top > -INFINITY) {
         u64 marks[2] = {0, 0};
         int nth = 0;
         tokens.each_held([&](float v) {
@@ -675,13 +729,55 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 if (tid + q * SAMPLE_THREADS < candidates) s.candidates[tid + q * SAMPLE_THREADS] = (u64)~sample_key(v[q]) << 32 | (uint32_t)at[q];
         }
         __syncthreads();
-        // their steps as fine as the bins allow
-        if (compact) {
-            const double span = 2.0 - fmax(t_least, r.t(least));
-            while (r.steps * 2.0 * span < BINS && r.steps < 65536.0) r.steps *= 2.0;
-            with_top();
-        }
     }
+    if (parts > 1) {
+    // the part's candidates, to the block that ends last
+    refine();
+    const bool fits = top == -INFINITY || compact;
+    if (fits)
+        for (int i = tid; i < candidates; i += SAMPLE_THREADS)
+            __hip_atomic_store(a.part_entries + own_part * CANDIDATES + i, s.candidates[i] + (u64)base, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) {
+        __hip_atomic_store(a.slice_counts + own_part * BINS, fits ? (uint32_t)candidates : CANDIDATES + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.slice_counts + own_part * BINS + 1, __float_as_uint(least), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.slice_tops + own_part, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!arrive(parts)) return;
+    whole_row();
+    bool all_fit = true;
+    top = -INFINITY;
+    for (int i = 0; i < parts; ++i) {
+        const uint32_t count = __hip_atomic_load(a.slice_counts + (first_part + i) * BINS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        all_fit = all_fit && count <= CANDIDATES;
+        // what bounds a part's candidates from below bounds the row's: there are as many above it, or more
+        least = fmaxf(least, __uint_as_float(__hip_atomic_load(a.slice_counts + (first_part + i) * BINS + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)));
+        top = fmaxf(top, __hip_atomic_load(a.slice_tops + first_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    }
+    with_top();
+    if (min_p > 0.0f && top > -INFINITY && top < INFINITY) least = fmaxf(least, value_below(t_least));
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
+    if (all_fit)
+        for (int i = 0; i < parts; ++i) {
+            const int count = (int)__hip_atomic_load(a.slice_counts + (first_part + i) * BINS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll 1
+            for (int from = 0; from < count; from += SAMPLE_THREADS) {
+                const int j = from + tid;
+                const u64 entry = j < count ? __hip_atomic_load(a.part_entries + (first_part + i) * CANDIDATES + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : ~0ull;
+                const bool takes = key_value(~(uint32_t)(entry >> 32)) >= least;   // of none: a NaN
+                const uint32_t to = places(takes ? 1u : 0u);
+                if (takes && to < CANDIDATES) s.candidates[to] = entry;
+            }
+        }
+    __syncthreads();
+    candidates = (int)min(s.listed, CANDIDATES + 1u);
+    compact = all_fit && candidates <= CANDIDATES;
+    }
+    if (top == -INFINITY) {
+        if (tid == 0) a.out[row] = 0;
+        return;
+    }
+    refine();
 
     const auto top_p_need = [&](u64 kept) { return top_p > 0.0f ? max(part_of<true>(top_p, kept), (u64)1) : (u64)1; };
     const auto token_need = [&](u64 kept) { return u < 1.0f ? part_of<false>(u, kept) + 1 : kept; };
@@ -905,12 +1001,13 @@ int sample_slices(int dtype, int rows, int n, int num_cus) {
 
 // Bytes of the slices' parts; placing them.
 size_t sample_workspace_bytes(const SampleArgs& a) {
-    return a.slices == 1 ? 0 : (size_t)a.rows * a.slices * (BINS * (sizeof(u64) + sizeof(uint32_t)) + sizeof(float));
+    return a.slices == 1 ? 0 : (size_t)a.rows * a.slices * ((BINS + CANDIDATES) * sizeof(u64) + BINS * sizeof(uint32_t) + sizeof(float));
 }
 void sample_place(SampleArgs* a, void* workspace) {
     const size_t parts = (size_t)a->rows * a->slices;
     a->slice_sums = (unsigned long long*)workspace;
-    a->slice_counts = (uint32_t*)(a->slice_sums + parts * BINS);
+    a->part_entries = a->slice_sums + parts * BINS;
+    a->slice_counts = (uint32_t*)(a->part_entries + parts * CANDIDATES);
     a->slice_tops = (float*)(a->slice_counts + parts * BINS);
 }
 

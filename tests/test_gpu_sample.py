@@ -136,7 +136,7 @@ def test_sample_of_long_rows(dev, case):
     rng = np.random.default_rng(160 + case)
     x = values(rng, (rows, n), dt, std)
     few = min(rows, 12)                                      # rows that the reference looks at
-    for kw in ({}, {"top_p": 0.9}, {"top_k": 50}, {"top_k": 3000, "top_p": 0.8}, {"min_p": 0.05}, {"min_p": 1e-7, "top_p": 0.95},
+    for kw in ({}, {"top_p": 0.9}, {"top_k": 50}, {"top_k": 1000}, {"top_k": 3000, "top_p": 0.8}, {"min_p": 0.05}, {"min_p": 1e-7, "top_p": 0.95},
                {"T": 0.0}, {"top_k": n - 5, "top_p": 0.99}):
         u = rng.random(rows)
         T = np.full(rows, kw.get("T", 0.9))
@@ -182,6 +182,36 @@ def test_sample_of_long_rows_that_are_not_ordinary(dev, rows):
     same(base, T=1e-3, top_p=0.5)
     same(base, T=np.inf, top_p=0.5)
     same(np.abs(base) * np.float32(2.0 ** -140))             # subnormals
+
+
+@pytest.mark.parametrize("rows,n", [(3, 128000), (100, 120000), (150, 70001)])
+def test_sample_of_parts_that_differ(dev, rows, n):
+    """few tokens kept of a row that more blocks than one look through: nothing in a part, all of them in one, ties across
+    parts, more in a part than it may have, infinities"""
+    rng = np.random.default_rng(30)
+    base = (3 * rng.standard_normal(n)).astype(np.float32)
+    rise = np.linspace(-20, 20, n).astype(np.float32)
+    half = base.copy()
+    half[:n // 2] = -np.inf
+    one = np.full(n, -np.inf, np.float32)
+    one[n - 3] = 1.0
+    ties = np.round(base)
+    inf = base.copy()
+    inf[[17, n - 5]] = np.inf
+    nan = base.copy()
+    nan[[3, n - 2]] = np.nan
+    flat = (1e-3 * base).astype(np.float32)                    # min_p keeps all of them
+    for what, x in (("base", base), ("rise", rise), ("half", half), ("one", one), ("ties", ties), ("inf", inf), ("nan", nan), ("flat", flat),
+                    ("none", np.full(n, -np.inf, np.float32))):
+        for kw in ({"top_k": 1}, {"top_k": 50}, {"top_k": 1000}, {"top_k": 700, "min_p": 0.02, "top_p": 0.9}, {"min_p": 0.3}):
+            args = [np.full(rows, kw[k]) if k in kw else None for k in ("top_k", "top_p", "min_p")]
+            u = rng.random(rows)
+            got = draw(dev, np.repeat(x[None], rows, 0), F32, np.full(rows, 0.8), *args, u)
+            for r in range(2):
+                f = [None if a is None else float(np.float32(a[r])) for a in args]
+                want, near = pick(x.astype(np.float64), float(np.float32(0.8)), int(f[0] or 0), 1.0 if f[1] is None else f[1], f[2] or 0.0,
+                                  float(np.float32(u[r])))
+                assert got[r] == want or near < slack(n), (what, kw, r, got[r], want, near)
 
 
 @pytest.mark.parametrize("rows", [3, 150])
