@@ -254,7 +254,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     }
 
     uint16_t* vt = (uint16_t*)(lds + wave * L::REGION);        // [32 keys][VP]
-    const int cpr = (D + CE - 1) / CE;                         // the last chunk of a row of 8 bits may reach 8 bytes past it,
+    const int cpr = MX ? (D + CE - 1) / CE : D / 8;            // the last chunk of a row of 8 bits may reach 8 bytes past it,
                                                                // which are the next slot's or the scales' behind the last
     int vkey[VI], vdim[VI];                                    // V chunk c = lane + 64 i: key c / cpr, dims CE (c % cpr)
 #pragma unroll
@@ -314,7 +314,7 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
         for (int i = 0; i < VI; ++i) at[i] = __shfl(where, vkey[i] & 31, 64) + (MX ? 0u : (uint32_t)(vdim[i] >> 3));
     };
     auto load_scale = [&](uint32_t where) {
-        if constexpr (MX) scale_next = *(global_u32*)((uintptr_t)(lane < 32 ? a.kv.k_scale : a.kv.v_scale) + ((uint64_t)where << 2));
+        if constexpr (MX) scale_next = *(global_u32*)((uintptr_t)a.kv.scales(lane < 32 ? a.kv.k : a.kv.v) + ((uint64_t)where << 2));
     };
     auto load_k = [&](uint32_t where) {
         if constexpr (STAGED) {

@@ -37,6 +37,12 @@
 // 132 MB: 31.5 us, 4.2 TB/s (a large copy reaches 5.1); 64 sequences of 1000 .. 1500:
 // 121 us, 5.4 TB/s; 4 of 20000 .. 32768, bf16, 32 heads of 128 over 8, 448 MB: 84 us,
 // 5.3 TB/s; one of 512: 7.35 us, the launch and a chain of loads (lengths, table, keys).
+// 8-bit caches (MVLM_MXFP8) take the same path with half the bytes, q and O in bf16: v_cvt_scalef32 makes two bf16
+// of two codes and their block's power of two, exactly, between the loads and the matrix instructions (tiles of 16
+// rows for K, whose fragments are 16 codes, so that two steps share a load) or as a tile is stored in LDS (V, and K of tiles of 32).
+// A key's word of scales is loaded by one lane and handed to the others.  In turn on one machine with the 16-bit
+// cache's: 16 of 30 .. 2047, 32 heads of 64, 70 MB: 19.3 us, 3.6 TB/s, against 31; 4 of 20000 .. 32768, 32 heads of 128
+// over 8, 231 MB: 49.4 us, 4.7 TB/s, against 84 (blocks per CU 1: 60, 3: 51.9, 4: 55.8); one of 512: 7.0 us, as before.
 // Each block walks the lengths of all sequences three times: beyond some 500 that is
 // felt (1024 sequences of 200 .. 400, 32 heads of 128 over 8: 373 us, 3.4 TB/s).
 #include "attention_paged.h"

@@ -29,7 +29,7 @@ __device__ __forceinline__ ReadRaw read_raw(const PagedKv& kv, bool keys, int64_
     if constexpr (MX) {
         const u32x2 c = *reinterpret_cast<const u32x2*>((const uint8_t*)base + slot * kv.D + d);
         r.w[0] = c[0], r.w[1] = c[1];
-        r.scale = (keys ? kv.k_scale : kv.v_scale)[slot];
+        r.scale = kv.scales(base)[slot];
     } else
         r.w = *reinterpret_cast<const u32x4*>(base + slot * kv.D + d);
     return r;

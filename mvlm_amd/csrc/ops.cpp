@@ -343,19 +343,20 @@ int make_paged_kv(mvlm_device* dev, const mvlm_paged_kv* in, const char* fn, Pag
     NEED(in->k, bytes, "K");
     NEED(in->v, bytes, "V");
     REQUIRE(!overlaps(in->k->ptr, bytes, in->v->ptr, bytes), "%s: K and V overlap", fn);
-    const size_t slots = (size_t)in->num_pages * in->page_size * in->kv_heads;
-    const bool mx = in->dtype == MVLM_MXFP8;
     out->k = (uint16_t*)in->k->ptr;
     out->v = (uint16_t*)in->v->ptr;
-    out->k_scale = mx ? (uint32_t*)((char*)in->k->ptr + (bytes - 4 * slots)) : nullptr;
-    out->v_scale = mx ? (uint32_t*)((char*)in->v->ptr + (bytes - 4 * slots)) : nullptr;
-    out->bytes = bytes;
     out->dtype = in->dtype;
     out->num_pages = in->num_pages;
     out->kv_heads = in->kv_heads;
     out->D = in->head_dim;
     out->page = fast_div(in->page_size);
     return MVLM_OK;
+}
+
+// Bytes of K, and of V as much.
+size_t kv_bytes(const PagedKv& kv) {
+    const size_t slots = kv.slots();
+    return kv.dtype == MVLM_MXFP8 ? (size_t)((char*)kv.scales(kv.k) - (char*)kv.k) + 4 * slots : slots * kv.D * 2;
 }
 
 int make_paged_batch(mvlm_device* dev, const mvlm_paged_batch* in, int page_size, const char* fn, PagedSeqs* out) {
@@ -440,7 +441,7 @@ int make_kv_append(mvlm_device* dev, const mvlm_buffer* qkv, int x_dtype, int64_
         a.eps = norm->eps;
         a.per_dim = 1.0f / (float)a.kv.D;
     }
-    const size_t kvb = a.kv.bytes;
+    const size_t kvb = kv_bytes(a.kv);
     const struct { const void* p; size_t bytes; } written[3] = {{a.kv.k, kvb}, {a.kv.v, kvb}, {q_out->ptr, q_bytes}};
     for (const auto& w : written)
         REQUIRE(!overlaps(w.p, w.bytes, qkv->ptr, x_bytes) && !overlaps(w.p, w.bytes, a.rope, rope_bytes) &&
@@ -475,7 +476,7 @@ int make_kv_read(mvlm_device* dev, const mvlm_paged_batch* batch, const mvlm_pag
         if (!out) continue;
         NEED(out, bytes, out == K_out ? "K_out" : "V_out");
         REQUIRE((uintptr_t)out->ptr % es == 0, "%s: an output does not start at a multiple of %zu bytes", fn, es);
-        REQUIRE(!overlaps(out->ptr, bytes, a.kv.k, a.kv.bytes) && !overlaps(out->ptr, bytes, a.kv.v, a.kv.bytes) &&
+        REQUIRE(!overlaps(out->ptr, bytes, a.kv.k, kv_bytes(a.kv)) && !overlaps(out->ptr, bytes, a.kv.v, kv_bytes(a.kv)) &&
                     !holds_batch(out->ptr, bytes, a.batch),
                 "%s: outputs must not overlap what is read", fn);
     }
@@ -513,8 +514,8 @@ int make_attention_paged(mvlm_device* dev, const mvlm_buffer* Q, const mvlm_page
     const size_t o_bytes = elems * dtype_size(o_dtype);
     NEED(Q, elems * 2, "Q");
     NEED(O, o_bytes, "O");
-    REQUIRE(!overlaps(O->ptr, o_bytes, Q->ptr, elems * 2) && !overlaps(O->ptr, o_bytes, a.kv.k, a.kv.bytes) &&
-                !overlaps(O->ptr, o_bytes, a.kv.v, a.kv.bytes) && !holds_batch(O->ptr, o_bytes, a.batch),
+    REQUIRE(!overlaps(O->ptr, o_bytes, Q->ptr, elems * 2) && !overlaps(O->ptr, o_bytes, a.kv.k, kv_bytes(a.kv)) &&
+                !overlaps(O->ptr, o_bytes, a.kv.v, kv_bytes(a.kv)) && !holds_batch(O->ptr, o_bytes, a.batch),
             "%s: O must not overlap what is read", fn);
     a.q = (const uint16_t*)Q->ptr;
     a.o = O->ptr;

@@ -40,9 +40,6 @@ inline FastDiv fast_div(int d) {
 struct PagedKv {
     uint16_t* k;               // elements of 16 bits, or codes of 8 (MVLM_MXFP8)
     uint16_t* v;
-    uint32_t* k_scale;         // MVLM_MXFP8: a word per slot, else null
-    uint32_t* v_scale;
-    size_t bytes;              // of K, and of V
     int dtype;
     int num_pages, kv_heads, D;
     FastDiv page;              // by page_size
@@ -50,6 +47,12 @@ struct PagedKv {
     // elements; below 2^31 (checked on the host)
     MVLM_HD int slot(int page_id, int head, int offset) const {
         return (page_id * kv_heads + head) * page.div + offset;
+    }
+    MVLM_HD uint32_t slots() const { return (uint32_t)num_pages * (uint32_t)kv_heads * (uint32_t)page.div; }
+    // MVLM_MXFP8: a word per slot, behind the codes of K or of V.  Worked out where they are needed, as kernels for 16 bits
+    // started 0.2 us later with more in their arguments (768 rows 12.0 -> 12.25 us).
+    MVLM_HD uint32_t* scales(const uint16_t* codes) const {
+        return (uint32_t*)((uintptr_t)codes + (((uint64_t)slots() * (uint32_t)D + 15) & ~(uint64_t)15));
     }
 };
 
