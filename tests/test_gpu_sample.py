@@ -246,6 +246,27 @@ def test_sample_of_weights_that_round_to_nothing(dev):
             assert list(draw(dev, x, F32, u=[u] * 2, **kw)) == [777, n - 1], (kw, u)
 
 
+@pytest.mark.parametrize("rows,n,dt", [(20, 70001, F32), (20, 120000, F16), (160, 3000, BF16), (160, 70000, F16)])
+def test_sample_of_requests_of_all_kinds(dev, rows, n, dt):
+    """one call whose rows ask for unlike things, with infinite, tiny and no temperatures, masks and NaN among them"""
+    rng = np.random.default_rng(50)
+    x = values(rng, (rows, n), dt, 3.0)
+    x[rng.random((rows, n)) < 0.3] = to_bits(np.float32(-np.inf), dt)
+    x[3, 11:12] = to_bits(np.float32(np.nan), dt)
+    x[7, ::3] = to_bits(np.copysign(np.float32(np.nan), np.float32(-1)), dt)
+    x[11, 1:] = to_bits(np.float32(-np.inf), dt)
+    T = rng.choice([0.7, 1.0, 1.3, 0.0, np.inf, 1e-30, 1e-3], rows).astype(np.float32)
+    top_k = rng.choice([0, 0, 1, 5, 50, 300, 1000, 5000], rows).astype(np.int32)
+    top_p = rng.choice([1.0, 0.95, 0.5, 0.0], rows).astype(np.float32)
+    min_p = rng.choice([0.0, 0.0, 0.01, 0.3, 1.0], rows).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    u[::9] = 1.0
+    got = draw(dev, x, dt, T, top_k, top_p, min_p, u)
+    for r in range(min(rows, 40)):
+        want, near = pick(from_bits(x[r], dt), float(T[r]), int(top_k[r]), float(top_p[r]), float(min_p[r]), float(u[r]))
+        assert got[r] == want or near < slack(n), (r, T[r], top_k[r], top_p[r], min_p[r], u[r], got[r], want, near)
+
+
 def test_sample_of_long_rows_in_a_graph(dev):
     """rows made by several blocks, whose parts are counted in the same words, replayed with eager calls between"""
     rng = np.random.default_rng(18)
