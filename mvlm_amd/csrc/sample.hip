@@ -781,6 +781,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     __syncthreads();
     candidates = (int)min(s.listed, CANDIDATES + 1u);
     compact = all_fit && candidates <= CANDIDATES;
+    __syncthreads();                                           // all have read the count, which refine() starts anew
     }
     if (top == -INFINITY) {
         if (tid == 0) a.out[row] = 0;
