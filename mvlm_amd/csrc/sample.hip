@@ -503,7 +503,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 if (!(v > -INFINITY)) return;                  // a NaN lies below all others here
                 const double steps = fmax(r.step(v, c), step0 - (BINS - 1)), octave = __builtin_floor(steps * (1.0 / STEPS));
                 const double x = (double)v * c - octave + (a.bits - 1);    // below bits, by much in the last bin
-                const int b = (int)(step0 - steps);
+                const int b = (int)fmin(step0 - steps, BINS - 1.0);        // where steps are past 2^53 their differences round
                 atomicAdd(&s.counts[b], 1u);
                 if (x >= -1.0) atomicAdd(&s.sums[b], integer_power(x));
             });

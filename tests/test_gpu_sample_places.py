@@ -34,3 +34,14 @@ def test_candidates_of_several_blocks(dev, rows, n, dt):
         for top_k in (130, 600, 1000):
             for more in ({}, {"top_p": np.full(rows, 0.95), "min_p": np.full(rows, 1e-3)}):
                 check(dev, x, dt, rng.random(rows), range(min(rows, 8)), top_k=np.full(rows, top_k), **more)
+
+
+@pytest.mark.parametrize("rows", [2, 150])
+@pytest.mark.parametrize("T", [1e-10, 1e-13, 1e-14, 1e-16])
+def test_exponents_without_a_fraction(dev, rows, T):
+    """v / T of 1e11 .. 1e17: their bins lie past 2^53, where not every integer is a double"""
+    rng = np.random.default_rng(71)
+    x = (3 * rng.standard_normal((rows, 30000))).astype(np.float32)
+    x[:, 5::7] = x[:, :1].max() + 9                            # the largest, many times
+    check(dev, x, F32, rng.random(rows), range(min(rows, 4)), T=np.full(rows, T))
+    check(dev, x, F32, rng.random(rows), range(min(rows, 4)), T=np.full(rows, T), top_p=np.full(rows, 0.5))
