@@ -565,6 +565,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
     // a finite value that is below those of all tokens with t >= t_to, by a little
     auto value_below = [&](double t_to) {
+        if (!(c > 0.0)) return -3.402823466e38f;               // an infinite temperature: every finite value has t = 0
         const uint32_t k = sample_key((float)(r.m + t_to / c));
         return key_value(max(k, KEY_NEG_INF + 9) - 8);
     };

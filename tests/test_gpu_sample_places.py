@@ -45,3 +45,14 @@ def test_exponents_without_a_fraction(dev, rows, T):
     x[:, 5::7] = x[:, :1].max() + 9                            # the largest, many times
     check(dev, x, F32, rng.random(rows), range(min(rows, 4)), T=np.full(rows, T))
     check(dev, x, F32, rng.random(rows), range(min(rows, 4)), T=np.full(rows, T), top_p=np.full(rows, 0.5))
+
+
+@pytest.mark.parametrize("rows,n", [(4, 500), (3, 70000), (150, 70000)])
+def test_infinite_temperatures_with_the_largest_min_p(dev, rows, n):
+    """every finite value weighs 1, as much as min_p asks for"""
+    rng = np.random.default_rng(72)
+    x = (3 * rng.standard_normal((rows, n))).astype(np.float32)
+    x[:, ::3] = -np.inf
+    u, T, ones = rng.random(rows), np.full(rows, np.inf), np.ones(rows)
+    for kw in ({}, {"top_k": np.full(rows, 40)}, {"top_p": np.full(rows, 0.25)}):
+        check(dev, x, F32, u, range(min(rows, 3)), T=T, min_p=ones, **kw)
