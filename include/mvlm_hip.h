@@ -477,9 +477,10 @@ int mvlm_logits_process(mvlm_device* dev, const mvlm_buffer* x, int dtype, int r
  * largest v), top_k int32 (0 or below: all), top_p fp32 (1, above or NaN: all; 0 or below: one token),
  * min_p fp32 (0, below or NaN: all; above 1 counts as 1).  A row that holds only -inf picks token 0, as mvlm_argmax
  * does.
- * w is computed in 64 bits; sums are of integer multiples of 2^-s or less, s = 62 -
- * ceil(log2 n), at most 51 (what rounds to 0 is never picked unless it is the only
- * one), so that a result does not depend on the order of the work. */
+ * w is computed in 64 bits and rounded to a multiple of 2^-s, s = 62 - ceil(log2 n),
+ * at most 51 (what rounds to 0 is not kept), and sums of these are exact, so that a
+ * row's token depends on the row and its settings, not on the order of the work or on
+ * the rows beside it. */
 typedef struct mvlm_sampling {
     const mvlm_buffer* uniform;          /* fp32 [rows] */
     const mvlm_buffer* temperature;      /* fp32 [rows] or NULL */

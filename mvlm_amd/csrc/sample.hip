@@ -2,7 +2,8 @@
 //
 // With m the row's largest value and t_i = (v_i - m) log2(e) / T <= 0 in 64 bits, a token's weight is
 //   W_i = round(2^(bits + t_i)), an integer: 2^bits for the largest, 0 below 2^-(bits + 1) of it.
-// Integers below 2^62 / n add up exactly in any order.  In the order of falling value (the lower index first among
+// Integers below 2^62 / n add up exactly in any order and in any parts, so that a row's token is the same whichever
+// blocks make it.  In the order of falling value (the lower index first among
 // equals) everything asked for is a start of the row or a place in it:
 //   live     t_i >= max(log2(min_p), -(bits + 1))
 //   top-k    the place of the k-th live token
@@ -21,8 +22,9 @@
 //    again in ranges of keys, down to equal values, of which the index decides.
 // A row whose candidates are enough and that a block can hold is made by one block.  A longer one is looked through by
 // as many as can hold it, and the block that ends last puts their candidates together.  Of the others, whose weights all
-// count, each of `slices` blocks counts a slice, in steps of v log2(e) / T, which need no m, with weights relative to
-// the step's octave, and the block that ends last adds the slices up and searches.  No block waits for another.
+// count, each of `slices` blocks looks for the row's largest value, so that it need not wait to be told the weights' unit, and
+// counts a slice; the block that ends last adds the slices up and searches.  No block waits for another.  A row's blocks
+// are on one XCD where there are 8 rows, whose L2 has the row after the first of them (64 open rows of 128000 82 us, spread 98).
 // Running sums are over THREADS bins or entries, one of each thread's, which then knows whether a place is its own.
 //
 // Its floor is one look at the row, but few rows leave most of the chip without work, and what bounds it are chains of
@@ -59,6 +61,7 @@ __device__ __forceinline__ uint32_t sample_key(float f) {
     if (b == 0x80000000u) b = 0u;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float as_number(float v) { return v == v ? v : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x7F800000u); }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu, KEY_INF = 0xFF800000u;
 
@@ -97,8 +100,17 @@ struct SampleRow {
     uint32_t top;                      // key of the largest value
     double m, c;                       // that value, log2(e) / T; where it is infinite, 0 and 0: its like have t = 0
     double bits;
-    __device__ __forceinline__ double t(float v) const { return ((double)fminf(v, 3.402823466e38f) - m) * c; }
-    __device__ __forceinline__ u64 weight(double t) const { return integer_power(t + bits); }
+    // Each operation rounds by itself: t's product and the sum below made one fma in one place and not in another would make
+    // two weights of a token, and a sum would not be that of its tokens'.
+    __device__ __forceinline__ double t(float v) const {
+#pragma clang fp contract(off)
+        return ((double)fminf(v, 3.402823466e38f) - m) * c;
+    }
+    __device__ __forceinline__ u64 weight(double t) const {
+#pragma clang fp contract(off)
+        const double x = t + bits;
+        return integer_power(x);
+    }
     // The bin of a value: how many steps of v log2(e) / T lie between its own and the largest's.
     double steps = STEPS, step0;
     __device__ __forceinline__ double step(float v, double c) const { return __builtin_floor((double)fminf(v, 3.402823466e38f) * c * steps); }
@@ -225,6 +237,35 @@ struct RowTokens {
         if constexpr (VEC)
             for (int i = max(whole, first) * EPC + (int)threadIdx.x; i < min(last * EPC, n); i += SAMPLE_THREADS) f(at(i), i);
     }
+    // The largest of this thread's tokens of the row, a NaN as as_number takes it.  Nothing else is kept of them, so more
+    // are in flight.
+    __device__ __forceinline__ float most() const {
+        constexpr int FLIGHT = 2 * SAMPLE_BATCH;
+        const int whole = VEC ? n / EPC : chunks;
+        float own = -INFINITY;
+        bool odd = false;
+        for (int base = (int)threadIdx.x; base < whole; base += SAMPLE_THREADS * FLIGHT) {
+            u32x4 w[FLIGHT];
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {                 // those past the end: the last chunk again
+                const int c = min(base + u * SAMPLE_THREADS, whole - 1);
+                if constexpr (VEC) w[u] = whole_chunk(c);
+                else w[u] = load(c);
+            }
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u)
+#pragma unroll
+                for (int e = 0; e < EPC; e += 2) {
+                    const float a = value(w[u][e * 4 / EPC], e), b = value(w[u][(e + 1) * 4 / EPC], e + 1);
+                    own = fmaxf(own, fmaxf(a, b));             // a NaN is not taken
+                    odd |= __builtin_isunordered(a, b);
+                }
+        }
+        if (odd) each([&](float v, int) { own = fmaxf(own, as_number(v)); });
+        else if constexpr (VEC)
+            for (int i = whole * EPC + (int)threadIdx.x; i < n; i += SAMPLE_THREADS) own = fmaxf(own, as_number(at(i)));
+        return own;
+    }
     template <class F>
     __device__ __forceinline__ void each_other(F&& f) const { each_between(CHUNKS * SAMPLE_THREADS, chunks, f); }
     template <class F>
@@ -275,7 +316,6 @@ struct SampleLds {
     uint32_t wave_counts[SAMPLE_THREADS / 64];
     float wave_values[SAMPLE_THREADS / 64];
     SamplePlace place[2];
-    float tops[SAMPLE_SYNC_WORDS];     // of a row's slices
     uint32_t listed, word;
 };
 
@@ -428,7 +468,17 @@ __device__ __forceinline__ WaveList wave_list(const u64* from, u64* to, int size
 template <int DT, bool VEC, bool SPLIT>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs a) {
     __shared__ SampleLds s;
-    const int row = SPLIT ? (int)(blockIdx.x / (uint32_t)a.slices) : (int)blockIdx.x, slice = SPLIT ? (int)blockIdx.x - row * a.slices : 0;
+    int row = (int)blockIdx.x, slice = 0;
+    if constexpr (SPLIT) {                                     // a row's blocks on one XCD (every eighth block's), while rows are left for all
+        const int eight = 8 * a.slices, group = a.rows < 8 ? 0 : row / eight;
+        row -= group * eight;
+        if (8 * group + 8 <= a.rows) slice = row / 8, row %= 8;
+        else {
+            const int of_these = row / a.slices;
+            slice = row - of_these * a.slices, row = of_these;
+        }
+        row += 8 * group;
+    }
     const int tid = (int)threadIdx.x, n = a.n;
     RowTokens<DT, VEC> tokens;
     tokens.x = a.x;
@@ -478,7 +528,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         return s.word == (uint32_t)blocks - 1;
     };
     const int64_t first_part = (int64_t)row * (SPLIT ? a.slices : 1), own_part = first_part + slice;
-    const auto as_number = [](float v) { return v == v ? v : __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x7F800000u); };
     float own = -INFINITY, top;                                // the largest of those that this thread holds, of all
     u64 slice_sum = 0;                                         // of this thread's bin, where the slices are added up
     uint32_t slice_count = 0;
@@ -491,67 +540,45 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         r.c = top < INFINITY ? c : 0.0;
         r.step0 = r.step(top, r.c);
     };
+    double t_least = -(r.bits + 1.0) + 0x1p-30;                // what lives has a weight of 1 at least
+    if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
     if (split) {
+        // each block finds the row's largest value, so that all count in the same unit and the sums are the row's
+        top = largest(tokens.most());
+        with_top();
+        summed = top > -INFINITY && top < INFINITY;
+        if (!summed && slice) return;                          // nothing to count, or infinities only: one block's work
+    }
+    if (summed) {
         const int per = (tokens.chunks + a.slices - 1) / a.slices, from = min(slice * per, tokens.chunks), to = min(from + per, tokens.chunks);
-        tokens.each_between(from, to, [&](float v, int) { own = fmaxf(own, as_number(v)); });
-        top = largest(own);
-        const double step0 = r.step(top, c);
         s.counts[tid] = 0, s.sums[tid] = 0;
         __syncthreads();
-        if (top > -INFINITY && top < INFINITY)
-            tokens.each_between(from, to, [&](float v, int) {
-                if (!(v > -INFINITY)) return;                  // a NaN lies below all others here
-                const double steps = fmax(r.step(v, c), step0 - (BINS - 1)), octave = __builtin_floor(steps * (1.0 / STEPS));
-                const double x = (double)v * c - octave + (a.bits - 1);    // below bits, by much in the last bin
-                const int b = (int)fmin(step0 - steps, BINS - 1.0);        // where steps are past 2^53 their differences round
-                atomicAdd(&s.counts[b], 1u);
-                if (x >= -1.0) atomicAdd(&s.sums[b], integer_power(x));
-            });
+        tokens.each_between(from, to, [&](float v, int) {
+            if (!(v > -INFINITY)) return;                      // a NaN lies below all others here
+            const double t = r.t(v);
+            if (!(t >= t_least)) return;
+            const int b = r.bin(v);
+            atomicAdd(&s.counts[b], 1u);
+            atomicAdd(&s.sums[b], r.weight(t));
+        });
         __syncthreads();
         __hip_atomic_store(a.slice_sums + own_part * BINS + tid, s.sums[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(a.slice_counts + own_part * BINS + tid, s.counts[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (tid == 0) __hip_atomic_store(a.slice_tops + own_part, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (!arrive(a.slices)) return;
-        for (int i = tid; i < a.slices; i += SAMPLE_THREADS)   // at most a CU each
-            s.tops[i] = __hip_atomic_load(a.slice_tops + first_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        top = -INFINITY;
-        for (int i = 0; i < a.slices; ++i) top = fmaxf(top, s.tops[i]);
-        with_top();
-        // beyond that the 64 bits of v log2(e) / T leave too few for its fraction
-        summed = top > -INFINITY && top < INFINITY && fabs(r.m * c) < 1024.0;
-        if (summed) {
-            s.counts[tid] = 0, s.sums[tid] = 0;
-            __syncthreads();
-            // a part's unit is 2^(octave of its bin), the row's 2^(m c)
-            const double mc = __builtin_floor(r.m * c), unit = exp2(mc - r.m * c);
-            constexpr int AHEAD = 8;
-            for (int i = 0; i < a.slices; i += AHEAD) {
-                u64 w[AHEAD];
-                uint32_t k[AHEAD];
+        constexpr int AHEAD = 8;
+        for (int i = 0; i < a.slices; i += AHEAD) {
+            u64 w[AHEAD];
+            uint32_t k[AHEAD];
 #pragma unroll
-                for (int q = 0; q < AHEAD; ++q) {
-                    const int64_t at = (first_part + min(i + q, a.slices - 1)) * BINS + tid;
-                    w[q] = __hip_atomic_load(a.slice_sums + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    k[q] = __hip_atomic_load(a.slice_counts + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-#pragma unroll
-                for (int q = 0; q < AHEAD; ++q) {
-                    const float slice_top = s.tops[min(i + q, a.slices - 1)];
-                    if (i + q >= a.slices || k[q] == 0) continue;          // as all are of a slice that holds nothing
-                    const double step0 = r.step(slice_top, c), octave = __builtin_floor((step0 - tid) * (1.0 / STEPS));
-                    const double part = __builtin_rint((double)w[q] * __builtin_ldexp(unit, (int)fmax(octave - mc + 1.0, -200.0)));
-                    const int b = (int)fmin(r.step0 - step0 + tid, BINS - 1.0);
-                    atomicAdd(&s.counts[b], k[q]);
-                    atomicAdd(&s.sums[b], (u64)part);
-                }
+            for (int q = 0; q < AHEAD; ++q) {
+                const int64_t at = (first_part + min(i + q, a.slices - 1)) * BINS + tid;
+                w[q] = __hip_atomic_load(a.slice_sums + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                k[q] = __hip_atomic_load(a.slice_counts + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            __syncthreads();
-            slice_sum = s.sums[tid];
-            slice_count = s.counts[tid];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q < a.slices) slice_sum += w[q], slice_count += k[q];
         }
-        if (tid == 0) s.word = 0;
-        __syncthreads();
     }
     const int per_part = (tokens.chunks + parts - 1) / parts;
     int base = 0;                                              // index of the tokens' first in the row
@@ -561,8 +588,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         tokens.n = min(n - base, per_part * tokens.EPC);
         tokens.chunks = (tokens.n + tokens.EPC - 1) / tokens.EPC;
     }
-    double t_least = -(r.bits + 1.0) + 0x1p-30;                // what lives has a weight of 1 at least
-    if (min_p > 0.0f) t_least = fmax(t_least, log2((double)fminf(min_p, 1.0f)));
     // a finite value that is below those of all tokens with t >= t_to, by a little
     auto value_below = [&](double t_to) {
         if (!(c > 0.0)) return -3.402823466e38f;               // an infinite temperature: every finite value has t = 0
@@ -811,12 +836,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         turn ^= 1;                                             // the next one is written while this is still read
         return p;
     };
-    // Where the running count or sum reaches need, or ends: bins of slices also have tokens that do not live, and sums that
-    // were rounded otherwise, so that what a search finds in one can be less than it holds, or nothing.
-    auto reaches = [&](const Share& m, bool by_count, u64 need, u64 sum) {
-        need = max(min(need, sum), (u64)1);
+    // Where the running count or sum reaches need, which is 1 at least and the whole at most: a weight is the same integer
+    // wherever it is counted.
+    auto reaches = [&](const Share& m, bool by_count, u64 need) {
         const u64 before = by_count ? (u64)m.above : m.before;
-        return announce(sum == 0 ? tid == 0 : before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
+        return announce(before < need && before + (by_count ? (u64)m.count : m.own) >= need, m);
     };
     // the list sorted, an entry to each thread
     auto share_list = [&](int size, u64* sum) __attribute__((always_inline)) {
@@ -833,8 +857,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         const Share m = share_list(size, &sum);
         const int live = __syncthreads_count(tid < size && r.t(key_value(~(uint32_t)(s.list[tid] >> 32))) >= t_least);
         SamplePlace p = announce(tid == (top_k > 0 ? min(top_k, live) : live) - 1, m);
-        if (top_p < 1.0f) p = reaches(m, false, top_p_need(p.before + p.own), sum);
-        p = reaches(m, false, token_need(p.before + p.own), sum);
+        if (top_p < 1.0f) p = reaches(m, false, top_p_need(p.before + p.own));
+        p = reaches(m, false, token_need(p.before + p.own));
         if (tid == 0) a.out[row] = (int)(uint32_t)s.list[p.index];
         return;
     }
@@ -884,11 +908,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
         for (int step = 0; step < 3; ++step) {                 // top-k, top-p, the token
             if ((step == 0 && k == all) || (step == 1 && !(top_p < 1.0f))) continue;
             const bool by_count = step == 0;
-            u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
-            u64 sum = by_count ? all : sum_here;
-            SamplePlace p = reaches(bins, by_count, need, sum);
+            const u64 need = by_count ? k : step == 1 ? top_p_need(kept) : token_need(kept);
+            u64 sum;
+            SamplePlace p = reaches(bins, by_count, need);
             const int bin = p.index;
-            if (step == 2 && u >= 1.0f && kept == sum_here) need = ~0ull >> 1;   // the last, whatever the bin is found to hold
             u64 before = p.before;                             // of the tokens above the range
             uint32_t above = p.above, inside = p.count;
             // the range's keys: from the least with a bin <= this one to the one before the least with a bin below it
@@ -909,18 +932,17 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                 __syncthreads();
                 uint32_t count;
                 const Share parts = share_out(s.part_sums[tid], s.part_counts[tid], s, &sum, &count);
-                p = reaches(parts, by_count, need - (by_count ? (u64)above : before), by_count ? (u64)count : sum);
+                p = reaches(parts, by_count, need - (by_count ? (u64)above : before));
                 inside = p.count;
                 before += p.before;
                 above += p.above;
                 hi -= (uint32_t)p.index << shift;
                 lo = max(lo, hi - ((1u << shift) - 1u));
             }
-            if (inside <= LIST || lo > hi) {
+            if (inside <= LIST) {
                 if (tid == 0) s.listed = 0;
                 __syncthreads();
-                if (lo > hi) {
-                } else if (of_row && top < INFINITY) {         // there is no NaN but below
+                if (of_row && top < INFINITY) {                // there is no NaN but below
                     const float low = key_value(lo), high = key_value(hi);
                     tokens.each([&](float v, int i) {
                         if (v >= low && v <= high) to_list(sample_key(v), i);
@@ -931,17 +953,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     });
                 __syncthreads();
                 const int size = min((int)s.listed, LIST);
-                if (size == 0) {                               // where the bin is of slices only
-                    kept = before;
-                    token = -1;
-                    __syncthreads();
-                    continue;
-                }
                 if (size <= 128) {                             // a wave's work
                     if (tid < 64) {
                         const WaveList list = wave_list(s.list, s.list, size, r, t_least);
-                        const u64 rest = need - (by_count ? (u64)above : before), sum = list.sum_at(size - 1);
-                        const int at = max(by_count ? (int)min(rest, (u64)size) - 1 : list.reaches(min(rest, sum)), 0);
+                        const u64 rest = need - (by_count ? (u64)above : before);
+                        const int at = by_count ? (int)rest - 1 : list.reaches(rest);
                         const u64 upto = list.sum_at(at);
                         const int index = list.token_at(at);
                         if (tid == 0) s.place[turn] = SamplePlace{upto, 0, 0, 0, index};
@@ -953,7 +969,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
                     continue;
                 }
                 const Share m = share_list(size, &sum);
-                p = reaches(m, by_count, need - (by_count ? (u64)above : before), by_count ? (u64)size : sum);
+                p = reaches(m, by_count, need - (by_count ? (u64)above : before));
                 token = (int)(uint32_t)s.list[p.index];
                 kept = before + p.before + p.own;
                 __syncthreads();
@@ -986,18 +1002,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
             if (latest) atomicMax(&s.word, latest);
             __syncthreads();
             token = (int)s.word;
-        }
-        if (token < 0) {                                       // the last token that lives
-            __syncthreads();
-            if (tid == 0) s.list[0] = 0;
-            __syncthreads();
-#pragma unroll 1
-            for (int i = tid; i < n; i += SAMPLE_THREADS) {
-                const uint32_t key = sample_key(tokens.at(i));
-                if (key >= live) atomicMax(&s.list[0], (u64)~key << 32 | (uint32_t)i);
-            }
-            __syncthreads();
-            token = (int)(uint32_t)s.list[0];
         }
         if (tid == 0) a.out[row] = token;
     }

@@ -3,7 +3,7 @@
 Weights are the interface's integers of 2^-bits, sums of them are exact.  What the library may do otherwise is round a
 weight another way: its exponent (v - m) log2(e) / T takes a subtraction, a constant, a division and a product of 64
 bits, 4 2^-53 of an exponent of 52 at most, 2^-45.3, and here a subtraction and a division, 2 2^-53 of 36 nats, 2^-46.8:
-2^-45.8 and 2^-46.8 of the weight (ln 2 of the first), 2^-45 together, and one unit where that takes the rounding over a half."""
+2^-45.8 and 2^-46.8 of the weight (ln 2 of the first), 2^-45 together."""
 import math
 
 import numpy as np
@@ -38,22 +38,20 @@ class Places:
             least = min(min_p, 1.0)
             live = [min(a, int(np.count_nonzero((w >= least * s) | (w == 1.0)))) for a, s in zip(live, (1 + OFF, 1 - OFF))]
         kept = [min(a, top_k) if top_k > 0 else a for a in live]
-        sums = np.cumsum(np.round(w / unit).astype(np.uint64))
+        sums = [np.cumsum(np.round(w * s / unit).astype(np.uint64)) for s in (1 - OFF, 1 + OFF)]   # they lie between
 
         def place(part, over, limit):
             """the least and the most place, below limit's, at which the sum reaches part of (over: exceeds) the kept's"""
             if part >= 1:
                 return [k - 1 for k in limit]
             found = []
-            for k, sign in zip(limit, (-1, 1)):
-                total = int(sums[k - 1])
+            for i, k in enumerate(limit):
+                total = int(sums[i][k - 1])
                 mant, two = math.frexp(part)                 # exactly: part = mant 2^53 / 2^(53 - two)
                 need = int(mant * 2 ** 53) * total
                 down = 53 - two
                 need = (need >> down) + 1 if over else -(-need >> down)
-                need += sign * (int(total * OFF) + k + 1)
-                need = max(1, min(need, total))
-                found.append(min(int(np.searchsorted(sums, np.uint64(need), "left")), k - 1))
+                found.append(min(int(np.searchsorted(sums[1 - i], np.uint64(max(need, 1)), "left")), k - 1))
             return found
 
         if top_p < 1:                                        # a NaN is none

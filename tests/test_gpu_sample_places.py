@@ -56,3 +56,30 @@ def test_infinite_temperatures_with_the_largest_min_p(dev, rows, n):
     u, T, ones = rng.random(rows), np.full(rows, np.inf), np.ones(rows)
     for kw in ({}, {"top_k": np.full(rows, 40)}, {"top_p": np.full(rows, 0.25)}):
         check(dev, x, F32, u, range(min(rows, 3)), T=T, min_p=ones, **kw)
+
+
+@pytest.mark.parametrize("rows,n,dt", [(2, 51200, F32), (16, 51200, F32), (3, 70001, F16), (150, 51200, F32)])
+def test_one_as_random_number_picks_the_last_kept(dev, rows, n, dt):
+    """many kept tokens whose weights are a unit or two, where a sum of roundings is not the rounding of a sum"""
+    rng = np.random.default_rng(73)
+    x = values(rng, (rows, n), dt, 3.0)
+    looked = range(min(rows, 6))
+    for T in (0.2, 0.3, 0.4):
+        for kw in ({}, {"top_k": rng.integers(1001, 8000, rows)}, {"top_p": np.full(rows, 1 - 2.0 ** -24)},
+                   {"top_k": rng.integers(3000, 8000, rows), "top_p": np.full(rows, 0.999)}):
+            for u in (np.ones(rows), np.full(rows, 1 - 2.0 ** -24), np.zeros(rows)):
+                check(dev, x, dt, u, looked, T=np.full(rows, T), **kw)
+
+
+@pytest.mark.parametrize("n,dt", [(51200, F32), (70001, F16), (128000, BF16)])
+def test_a_row_alone_and_in_a_batch(dev, n, dt):
+    """a row's token depends on the row and its settings, not on the rows beside it, whose number says how many blocks make it"""
+    rng = np.random.default_rng(74)
+    x = values(rng, (3, n), dt, 3.0)
+    for kw in ({}, {"T": 0.25}, {"T": 0.4}, {"T": 0.3, "top_k": 5000}, {"top_p": 0.9}, {"T": 0.2, "top_p": 1 - 2.0 ** -24}, {"T": 0.4, "top_k": 20000, "top_p": 0.999},
+               {"top_k": 300}, {"min_p": 1e-3}):
+        for u in (rng.random(3), np.ones(3), np.full(3, 1 - 2.0 ** -24)):
+            got = [draw(dev, np.tile(x, (b, 1))[:max(3 * b, 1)], dt, u=np.tile(u, b), **{k: np.full(3 * b, v) for k, v in kw.items()})
+                   for b in (1, 8, 50)]
+            alone = [draw(dev, x[r:r + 1], dt, u=u[r:r + 1], **{k: np.full(1, v) for k, v in kw.items()})[0] for r in range(3)]
+            assert all(np.array_equal(np.tile(alone, len(g) // 3), g) for g in got), (kw, u, alone, [g[:3] for g in got])
