@@ -83,3 +83,15 @@ def test_a_row_alone_and_in_a_batch(dev, n, dt):
                    for b in (1, 8, 50)]
             alone = [draw(dev, x[r:r + 1], dt, u=u[r:r + 1], **{k: np.full(1, v) for k, v in kw.items()})[0] for r in range(3)]
             assert all(np.array_equal(np.tile(alone, len(g) // 3), g) for g in got), (kw, u, alone, [g[:3] for g in got])
+
+
+@pytest.mark.parametrize("rows,n,dt,std", [(3, 128000, F32, 3.0), (3, 128000, F16, 3.0), (130, 60000, F32, 2.0), (140, 9001, BF16, 2.0), (2, 300000, F32, 1.0)])
+def test_more_live_tokens_than_candidates(dev, rows, n, dt, std):
+    """a min_p that leaves more tokens than LDS has room for, and rows without any limit"""
+    rng = np.random.default_rng(75)
+    x = values(rng, (rows, n), dt, std)
+    for T in (0.9, 1.6):
+        for kw in ({}, {"min_p": np.full(rows, 1e-7)}, {"min_p": np.full(rows, 1e-7), "top_p": np.full(rows, 0.95)},
+                   {"min_p": np.full(rows, 1e-5), "top_k": np.full(rows, 30000)}, {"min_p": np.full(rows, 1e-5), "top_k": np.full(rows, 900)}):
+            for u in (rng.random(rows), np.ones(rows)):
+                check(dev, x, dt, u, range(min(rows, 6)), T=np.full(rows, T), **kw)
