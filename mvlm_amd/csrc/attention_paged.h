@@ -293,7 +293,8 @@ __device__ __forceinline__ void paged_few_item(const PagedAttnArgs& a, const Pag
     // (768 rows of 32 heads of 80 22.4 us, staged 23.4; 256 and 11 of 96 41.4 and 40.7), and not
     // for 128 inside the kernel for many rows, more of whose registers it would spill (306 -> 330 us;
     // here 3 spill, outside the key loop).
-    // Of 8 bits a tile in LDS is made of the registers' values as it is stored, K's and V's alike.
+    // Of 8 bits a tile in LDS is made of the registers' values as it is stored, K's and V's alike, whatever KS is (768 rows of
+    // 32 heads of 72, 80, 96 22.4, 22.8, 23.2 us, of 16 bits 20.2, 20.7, 21.4).
     constexpr bool STAGED = R == 32 && (MX || (KS != 3 && (KS < 4 || NW == 4)));
     u32x4 kf[U][PAIRS ? S / 2 : S], kr[STAGED ? VI : 1], vf[VI];
     uint32_t scale = 0, scale_next = 0;                        // of key kv0 + lane % 32: K's, in lanes 32.. V's

@@ -43,6 +43,8 @@
 // A key's word of scales is loaded by one lane and handed to the others.  In turn on one machine with the 16-bit
 // cache's: 16 of 30 .. 2047, 32 heads of 64, 70 MB: 19.3 us, 3.6 TB/s, against 31; 4 of 20000 .. 32768, 32 heads of 128
 // over 8, 231 MB: 49.4 us, 4.7 TB/s, against 84 (blocks per CU 1: 60, 3: 51.9, 4: 55.8); one of 512: 7.0 us, as before.
+// Tiles of 32 rows, 8 and 16 bits, bf16 O: 768 rows of 32 heads of 64 12.9 and 12.5 us, of 128 27.5 and 27.3; 256 rows
+// and 11 single tokens on 500 .. 1870 of 32 heads of 64 22.8 and 24.3, of 80 33.1 and 30.8, of 128 39.1 and 42.1.
 // Each block walks the lengths of all sequences three times: beyond some 500 that is
 // felt (1024 sequences of 200 .. 400, 32 heads of 128 over 8: 373 us, 3.4 TB/s).
 #include "attention_paged.h"

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void kv_append_kernel(const KvAppen
 // leave in 8-byte stores, a head's scales in one word.
 // Measured: 16162 bf16 rows of 32 + 2 x 8 heads of 128 with both norms into an 8-bit cache, 303 MB: 84 us, 3.6 TB/s
 // (a wave's chain of lookup, sums over lanes and conversions; the 16-bit append without norms 5.1); 768 fp16 rows
-// of 3 x 32 heads of 64 with norms, 19 MB: 6.4 us; one row 4.0 us, a launch.  Sums over lanes by DPP, loads ahead and
+// of 3 x 32 heads of 64 with norms, 19 MB: 6.5 us; one row 4.0 us, a launch.  Sums over lanes by DPP, loads ahead and
 // weights, cos and sin in registers brought the first from 176 us, halves and lanes known to the compiler from 93.
 constexpr int HEADS_AHEAD = 3;
 
@@ -393,8 +393,9 @@ hipError_t launch_kv_append(hipStream_t s, const KvAppendArgs& a) {
     const bool vec = ((uintptr_t)a.qkv & 15u) == 0 && (a.ld * (int64_t)es) % 16 == 0;
     const dim3 grid((unsigned)a.batch.rows), block(APPEND_THREADS);
     // a row's prologue is paid by each of its waves: two of them where the rows fill the chip (16162 rows of 32 + 2 x 8
-    // heads of 128: 93 us, with four 102, with one 93, all since 9 less), four where they do not (768 of 3 x 32 heads of
-    // 64: 7.3 us, since 6.4, with two 9.0)
+    // heads of 128: 93 us, with four 102, with one 93, all since 9 less), four where they do not.  fp16 rows of 3 x 32 heads
+    // of 64 with two and with four waves: 512 rows 7.2 and 5.7 us, 1024 8.8 and 7.9, 1536 10.9 and 10.7, 2048 11.8 and 13.3, 4096
+    // 19.1 and 21.1; bf16 of 32 + 2 x 8 heads of 128 the same within 6%
     const dim3 hblock(a.batch.rows >= 2048 ? APPEND_THREADS / 2 : APPEND_THREADS);
     const bool by_head = a.kv.dtype == MVLM_MXFP8 || a.q_weight || a.k_weight;
     auto go = [&](auto dt) {

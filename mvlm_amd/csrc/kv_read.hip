@@ -5,7 +5,8 @@
 // Bytes bound it: each is read once and written once.  A thread makes 8 elements of one head, of one row or of
 // four that follow one another.
 // Measured: 65536 bf16 rows of 8 heads of 128 out of an 8-bit cache, 406 MB: 88 us, 4.6 TB/s (a large copy reaches
-// 5.1); 729 fp16 rows of 32 heads of 64, 9 MB: 4.6 us, little more than a launch.
+// 5.1), out of a bf16 cache, 535 MB: 98 us, 5.5 TB/s; 729 fp16 rows of 32 heads of 64, 9 MB: 4.3 us, little more than a
+// launch, out of an fp16 cache 4.2.
 #include "common.h"
 #include "device_math.h"
 #include "paged_ops.h"
@@ -140,7 +141,9 @@ hipError_t launch_kv_read(hipStream_t s, const KvReadArgs& a) {
             else launch_kernel(kv_read_kernel<OD, false, MX, ROWS>, grid, block, 0, s, a);
         };
         // four rows to a block have four times the loads in flight behind one chain of lookups (65536 rows of 8 heads of
-        // 128: 112 -> 88 us), which few rows pay for with CUs that have none (729 of 32 heads of 64: 4.6 -> 5.0)
+        // 128: 112 -> 88 us), which few rows pay for with CUs that have none.  Four and one, 8 bits: 1024 rows of 32 heads of 64
+        // 5.8 and 4.7 us, 1536 6.6 and 6.6, 2048 7.3 and 8.2, 4096 11.6 and 13.4; of 8 heads of 128 4.1 and 4.2, 4.5 and
+        // 4.1, 4.8 and 4.8, 7.1 and 7.8, of 16 bits 3.9 and 4.1, 4.4 and 4.2, 4.8 and 5.0, 8.2 and 8.3
         if (a.batch.rows >= 2048) rows(std::integral_constant<int, 4>{});
         else rows(std::integral_constant<int, 1>{});
     };

@@ -30,8 +30,9 @@
 // Its floor is one look at the row, but few rows leave most of the chip without work, and what bounds it are chains of
 // barriers, LDS atomics and searches.  Measured: one fp32 row of 51200, top_k 50, top_p 0.95: 9.2 us (a launch 3.7,
 // tokens 2, bound and candidates 2, sort and draw 1.5; found one by one 28, in bins 11); 16 bf16 rows, half masked,
-// top_p 0.9: 32 us (slices 8, their sum 4, two searches of 8; by one block each 83, steps of 1/8 octave 38); 128
-// fp32 rows of 128000, 65.5 MB, top_k to 1250, min_p 0.02: 39 us, 1.7 TB/s (tokens 19, as many as greedy rows take; a row
+// top_p 0.9: 32 us (largest value 3.4, slices 9, arrival and their sum 2, two searches 16; by one block each 83, steps of
+// 1/8 octave 38); 128 fp32 rows of 128000, 65.5 MB, top_p 0.9: 138 us, 0.5 TB/s (two blocks a row, which count for 62 of them,
+// and search for 28); the same rows with top_k to 1250, min_p 0.02: 39 us, 1.7 TB/s (tokens 19, as many as greedy rows take; a row
 // to a block 41, candidates counted in bins 86); one row of 128000, top_k 1000: 32 us (its tail read without a bound 216).
 #include "common.h"
 #include "device_math.h"
@@ -686,7 +687,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     }
 
     // A bound of many tokens is worth another look at those that are not held: with theirs among the threads' largest
-    // it leaves fewer candidates.
+    // it leaves fewer candidates, where they might be too many else, which costs far more (160 rows of 128000, with the look and
+    // without: top_k 60 28 and 23 us, 250 35 and 30, 500 39 and 35, 1000 48 and 240; 200 of 60000 17 and 16, 23 and 21, 27 and 26,
+    // 35 and 34).
     if (more && by_rank && top_k > RANKS / 4) {
         tokens.each_other([&](float x, int) { own = fmaxf(own, as_number(x)); });
         top = largest(own);
