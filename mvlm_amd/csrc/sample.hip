@@ -782,6 +782,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_kernel(const SampleArgs
     }
     if (!arrive(parts)) return;
     whole_row();
+    r.steps = STEPS;                                           // those of the part's candidates are too fine for a row
     bool all_fit = true;
     top = -INFINITY;
     for (int i = 0; i < parts; ++i) {

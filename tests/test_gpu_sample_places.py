@@ -95,3 +95,11 @@ def test_more_live_tokens_than_candidates(dev, rows, n, dt, std):
                    {"min_p": np.full(rows, 1e-5), "top_k": np.full(rows, 30000)}, {"min_p": np.full(rows, 1e-5), "top_k": np.full(rows, 900)}):
             for u in (rng.random(rows), np.ones(rows)):
                 check(dev, x, dt, u, range(min(rows, 6)), T=np.full(rows, T), **kw)
+
+
+@pytest.mark.parametrize("rows,n,top_k", [(1, 1 << 24, 50), (2, 1 << 22, 900)])
+def test_candidates_of_too_many_blocks(dev, rows, n, top_k):
+    """each block has few candidates, all of them together are more than one holds"""
+    rng = np.random.default_rng(76)
+    x = (3 * rng.standard_normal((rows, n), dtype=np.float32))
+    check(dev, x, F32, rng.random(rows), top_k=np.full(rows, top_k), top_p=np.full(rows, 0.95))
